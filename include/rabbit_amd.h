@@ -342,6 +342,133 @@ typedef struct {
 int rbt_gqa_step_d(rbt_ctx *ctx, const rbt_gqa_desc *desc, float *k_cache, float *v_cache, size_t cap, size_t pos,
                    const float *qg, const float *k, const float *v, float *ctx_out);
 
+/* ---- several drafted tokens at once (device buffers; no counterpart in the reference) ----------- */
+/* One decode step over a tree of drafted tokens per sequence: rbt_tree_positions_d once; per attention
+ * layer rbt_rope_d (norms, rotary positions, rows for the draft buffers) and rbt_gqa_tree_d; once at the
+ * end rbt_draft_verify_d and rbt_kv_commit_d. With one node per sequence this is plain decoding of a
+ * batch.
+ *  - A step holds n_seq sequences of at most max_nodes (<= 256) nodes; arrays over nodes are
+ *    [n_seq, max_nodes, ...], and nodes from n_nodes[b] on are padding: never read, their outputs left
+ *    as they were. n_nodes, len, parent and the like are int32 device arrays, so a captured graph
+ *    follows them.
+ *  - parent[b, i] is in -1..i-1; -1 hangs node i from the sequence's committed tokens.
+ *  - A sequence whose n_nodes is outside 0..max_nodes, or whose len is outside 0..cap, is skipped and a
+ *    parent outside its range is taken as -1; the next rbt_sync then returns RBT_E_INVALID. Nothing out
+ *    of the arrays' bounds is read or written.
+ *  - Graphs captured on one context share its scratch: replay them one after another. */
+typedef enum { RBT_DT_F32 = 0, RBT_DT_BF16 = 1 } rbt_dtype;
+
+/* Frequencies of rotary positions. theta^(-2j/rope_dim), j < rope_dim/2, changed for long contexts:
+ *   LINEAR      every frequency / factor (positions interpolated)
+ *   BASE        theta * factor^(rope_dim / (rope_dim - 2)) as the base
+ *   YARN        by parts (YaRN): turns over orig_ctx above beta_fast keep theirs, below beta_slow divide
+ *               by factor, a linear ramp over j in between
+ *   WAVELENGTH  wavelengths above orig_ctx / low_freq divide by factor, below orig_ctx / high_freq keep
+ *               theirs, between them the two are mixed linearly in orig_ctx / wavelength
+ * attn_factor multiplies cos and sin; 0 gives 0.1 ln(factor) + 1 for YARN and 1 otherwise. */
+enum { RBT_ROPE_PLAIN = 0, RBT_ROPE_LINEAR = 1, RBT_ROPE_BASE = 2, RBT_ROPE_YARN = 3, RBT_ROPE_WAVELENGTH = 4 };
+typedef struct {
+    int32_t kind;            /* RBT_ROPE_PLAIN .. RBT_ROPE_WAVELENGTH */
+    float factor;            /* >= 1; not used by PLAIN */
+    float orig_ctx;          /* YARN, WAVELENGTH: the context the model was trained for */
+    float beta_fast, beta_slow;   /* YARN */
+    float low_freq, high_freq;    /* WAVELENGTH */
+    float attn_factor;
+    int32_t as_f32;          /* PLAIN: each frequency rounded to f32 as rbt_gqa_step_d forms it */
+} rbt_rope_scaling;
+/* Host only, no context: inv_freq f64 [rope_dim / 2] (host memory; the caller copies it to the device once)
+ * and the factor for rbt_rope_desc. sc NULL = PLAIN. */
+int rbt_rope_freqs(const rbt_rope_scaling *sc, float theta, size_t rope_dim, double *inv_freq, float *factor);
+
+enum { RBT_ROPE_HALF = 0, RBT_ROPE_INTERLEAVED = 1 }; /* pairs (i, i + rope_dim/2) or (2i, 2i + 1) */
+typedef struct {
+    int32_t layout;          /* RBT_ROPE_HALF, RBT_ROPE_INTERLEAVED */
+    size_t head_dim;         /* 1..1024 */
+    size_t rope_start, rope_dim;  /* the rotated entries of a head; rope_dim even, may be 0 */
+    const double *inv_freq;  /* device f64 [rope_dim / 2] (rbt_rope_freqs) */
+    float factor;            /* multiplies cos and sin */
+    int32_t angle_f32;       /* 0: pos * inv_freq in 64 bits; 1: the product rounded to f32, as
+                                rbt_gqa_step_d rounds it (with frequencies made as_f32) */
+    float eps;               /* of the parts' norms */
+} rbt_rope_desc;
+/* One tensor of the call: rows src[t, h, :] to dst[t, h, :], strides in elements, head_dim contiguous.
+ * dst may be src itself where type and strides agree; other overlaps are the caller's mistake, and
+ * dst rows may not overlap each other (RBT_E_INVALID). */
+typedef struct {
+    const void *src;
+    void *dst;
+    int32_t src_dtype, dst_dtype;  /* rbt_dtype; bf16 results are rounded to nearest even once */
+    size_t n_heads;
+    size_t src_token_stride, src_head_stride, dst_token_stride, dst_head_stride;
+    const float *norm;       /* f32 [head_dim]: x * (1 + norm) / sqrt(mean(x^2) + eps) first, or NULL */
+    int32_t rotate;          /* 0: rows are normalised and copied only (values) */
+} rbt_rope_part;
+/* norm_heads and rope_half (qwen38/attention.rs:138-172) for s tokens of up to 8 tensors in one launch:
+ * token t at position pos[t] (device int32); pos[t] < 0 leaves the token's rows as they were. */
+int rbt_rope_d(rbt_ctx *ctx, const rbt_rope_desc *desc, const rbt_rope_part *parts, size_t n_parts, const int32_t *pos,
+               size_t s);
+
+/* pos[b, i] = len[b] + the number of node i's ancestors in the tree; -1 for padding nodes and for
+ * skipped sequences. */
+int rbt_tree_positions_d(rbt_ctx *ctx, size_t n_seq, size_t max_nodes, const int32_t *parent, const int32_t *n_nodes,
+                         const int32_t *len, int32_t *pos);
+
+/* Attention of drafted tokens (attend and apply_output_gate, qwen38/attention.rs:190-226, for a tree):
+ * node i of sequence b attends to the len[b] committed rows of its cache, to itself and to its ancestors
+ * among the drafted rows. q f32 [n_seq, max_nodes, n_heads, head_dim]; k_cache, v_cache
+ * [n_seq, cap, n_kv_heads, head_dim] and k_draft, v_draft [n_seq, max_nodes, n_kv_heads, head_dim] of
+ * kv_dtype; out f32 as q. gate: out is multiplied by sigmoid of
+ * gate[(b * max_nodes + i) * gate_token_stride + h * gate_head_stride + e] (q_proj's [query, gate] rows:
+ * strides n_heads * 2 * head_dim and 2 * head_dim), or NULL. Products are exact and sums f32.
+ * head_dim 1..1024; any number of query heads per KV head. Values that a node does not see never reach
+ * its output, non-finite ones included; a non-finite value that it sees makes the output entries it
+ * reaches non-finite, or drops out, as the order of the sums has it. */
+typedef struct {
+    size_t n_heads, n_kv_heads, head_dim;
+    float attn_scale;
+    int32_t kv_dtype;        /* rbt_dtype of caches and draft rows */
+    size_t cap;              /* rows of a sequence's cache */
+    size_t max_len;          /* a length no sequence is expected to pass (0: cap): the work is split for it */
+    size_t gate_token_stride, gate_head_stride;
+} rbt_gqa_tree_desc;
+int rbt_gqa_tree_d(rbt_ctx *ctx, const rbt_gqa_tree_desc *desc, size_t n_seq, size_t max_nodes, const float *q,
+                   const void *k_cache, const void *v_cache, const void *k_draft, const void *v_draft,
+                   const int32_t *len, const int32_t *n_nodes, const int32_t *parent, const float *gate, float *out);
+
+/* Which drafted tokens stand, and the token after them, by rejection against the target's distribution.
+ * Node 0 holds the token that the previous step ended with and stands. p[b, i, :] (f32, vocab) is the
+ * target's distribution after node i, q[b, i, :] the one that node i's children were drawn from
+ * independently, or NULL where they were not drawn (looked up, or the likeliest); rows sum to 1.
+ * At the current node, with c = 0 and S = 1 at first, its children are taken in index order: child j with
+ * token x stands, and the walk moves to it, if u[b, j] * S * q(x) < max(p(x) - c q(x), 0); otherwise c += S
+ * and S = the sum of max(p - c q, 0). Without q: if u[b, j] * S < p(x), otherwise S -= p(x) and p(x) counts as
+ * 0. When no child is left, next[b] is the least token whose running sum of max(p - c q, 0) (of what is
+ * left of p) passes u[b, 0] times the whole; an empty residual gives way to p. All in 64 bits; entries that are
+ * not above 0 (NaN too) count as 0. u f32 [n_seq, max_nodes] in [0, 1).
+ * path[b, :] gets the standing nodes in order, then -1; n_path[b] their number; next[b] is -1 where
+ * nothing can be drawn (no nodes, or a row without a finite positive sum). tokens int32; a node
+ * whose token is outside 0..vocab-1 is passed over and reported by the next rbt_sync (RBT_E_INVALID).
+ * n_seq <= 1024.
+ * max_children: the most children a node has, where known (1: chains), else 0; it changes only how the
+ * work is launched. */
+int rbt_draft_verify_d(rbt_ctx *ctx, size_t n_seq, size_t max_nodes, size_t vocab, size_t max_children,
+                       const int32_t *tokens, const int32_t *parent, const int32_t *n_nodes, const float *p,
+                       const float *q, const float *u, int32_t *path, int32_t *n_path, int32_t *next);
+
+/* KvCache::push (qwen38/attention.rs:76-82) of the standing nodes, for every layer at once: rows
+ * path[b, j], j < n_path[b], of the layers' draft rows to rows len[b] + j of their caches;
+ * len_out[b] = len[b] + n_path[b]. The four pointer arrays are host memory holding n_layers device
+ * pointers each. len_out must not be len. A sequence that does not fit (len + n_path > cap, or a path entry
+ * outside 0..max_nodes-1) is left as it was with len_out = len, and reported by the next rbt_sync. */
+typedef struct {
+    size_t n_layers, n_kv_heads, head_dim;
+    int32_t kv_dtype;
+    size_t cap;
+} rbt_kv_commit_desc;
+int rbt_kv_commit_d(rbt_ctx *ctx, const rbt_kv_commit_desc *desc, size_t n_seq, size_t max_nodes, void *const *k_caches,
+                    void *const *v_caches, const void *const *k_drafts, const void *const *v_drafts,
+                    const int32_t *path, const int32_t *n_path, const int32_t *len, int32_t *len_out);
+
 /* ---- instrumentation (no counterpart in the reference: benchmark support) -------------------- */
 typedef struct {
     double router_ms;    /* router logits + top-k selection + grouping (one-token MXFP4 calls: the

@@ -27,8 +27,11 @@ from .abi import (ACT_SILU, FAMILY_GLM52, FAMILY_KIMI_K3, FAMILY_QWEN38, QT_F32,
 
 __all__ = ["Context", "QT", "Slot", "Shards", "RbtError", "load", "QT_F32", "QT_I4_GROUPED", "QT_MXFP4",
            "FAMILY_QWEN38", "FAMILY_GLM52", "FAMILY_KIMI_K3", "ACT_SILU", "NAMING_QWEN38_MXFP4",
-           "NAMING_KIMI_K3_MXFP4", "ACT_SITU", "situ"]
+           "NAMING_KIMI_K3_MXFP4", "ACT_SITU", "situ", "DT_F32", "DT_BF16", "ROPE_HALF", "ROPE_INTERLEAVED",
+           "ROPE_PLAIN", "ROPE_LINEAR", "ROPE_BASE", "ROPE_YARN", "ROPE_WAVELENGTH", "rope_freqs", "rope_part"]
 from .abi import NAMING_KIMI_K3_MXFP4, NAMING_QWEN38_MXFP4, ACT_SITU  # noqa: E402
+from .abi import (DT_BF16, DT_F32, ROPE_BASE, ROPE_HALF, ROPE_INTERLEAVED, ROPE_LINEAR, ROPE_PLAIN,  # noqa: E402
+                  ROPE_WAVELENGTH, ROPE_YARN)
 
 
 def situ(beta, linear_beta=None):
@@ -66,6 +69,53 @@ def _ptr(a):
     if isinstance(a, int):
         return a
     raise TypeError(f"unsupported buffer {type(a)}")
+
+
+def _dtype(t) -> int:
+    """The rbt_dtype of a torch tensor."""
+    name = str(t.dtype)
+    if name not in ("torch.float32", "torch.bfloat16"):
+        raise TypeError(f"float32 or bfloat16 tensors only, not {name}")
+    return DT_BF16 if name == "torch.bfloat16" else DT_F32
+
+
+def _dense(name, t, dtype, *shape):
+    """t's device pointer, its type, size and layout checked (None passes)."""
+    if t is None:
+        return None
+    if str(t.dtype) != "torch." + dtype or tuple(t.shape) != shape:
+        raise ValueError(f"{name} is {dtype} {list(shape)}, not {str(t.dtype)[6:]} {list(t.shape)}")
+    return _ptr(t)
+
+
+def rope_freqs(rope_dim: int, theta: float, kind: int = ROPE_PLAIN, factor: float = 1.0, orig_ctx: float = 0.0,
+               beta_fast: float = 32.0, beta_slow: float = 1.0, low_freq: float = 1.0, high_freq: float = 4.0,
+               attn_factor: float = 0.0, as_f32: bool = False):
+    """rbt_rope_freqs: (inverse frequencies as a float64 numpy array [rope_dim / 2], factor of cos and sin).
+    Host only; copy the array to the device once (torch.from_numpy(..).cuda())."""
+    lib = abi.load()
+    sc = abi.RbtRopeScaling(kind, factor, orig_ctx, beta_fast, beta_slow, low_freq, high_freq, attn_factor, int(as_f32))
+    out, f = np.zeros(max(rope_dim // 2, 1), np.float64), C.c_float()
+    st = lib.rbt_rope_freqs(C.byref(sc), theta, rope_dim, out.ctypes.data, C.byref(f))
+    if st != 0:
+        raise RbtError(st, (lib.rbt_last_error(None) or b"").decode())
+    return out[:rope_dim // 2], f.value
+
+
+def rope_part(src, dst, norm=None, rotate: bool = True) -> abi.RbtRopePart:
+    """One tensor of Context.rope: src and dst are [s, n_heads, head_dim] torch tensors on the GPU (float32
+    or bfloat16), strided views allowed as long as head_dim is contiguous."""
+    for name, t in (("src", src), ("dst", dst)):
+        if not t.is_cuda:
+            raise ValueError("torch tensors passed to rabbit_amd must live on the GPU")
+        if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
+            raise ValueError(f"{name} must be [s, n_heads, head_dim] with head_dim contiguous")
+    if src.shape != dst.shape:
+        raise ValueError(f"src {list(src.shape)} and dst {list(dst.shape)} differ")
+    if norm is not None:
+        _dense("norm", norm, "float32", src.shape[2])
+    return abi.RbtRopePart(src.data_ptr(), dst.data_ptr(), _dtype(src), _dtype(dst), src.shape[1], src.stride(0),
+                           src.stride(1), dst.stride(0), dst.stride(1), _ptr(norm), int(rotate))
 
 
 class QT:
@@ -361,6 +411,101 @@ class Context:
         if sync:
             self.sync()
         return out
+
+    # -- drafted tokens (device tensors) ----------------------------------------------------
+    def rope(self, parts, pos, head_dim, inv_freq, rope_dim=None, rope_start=0, layout=ROPE_HALF, factor=1.0,
+             angle_f32=False, eps=1e-6, sync=True):
+        """rbt_rope_d: norms and rotary positions of up to 8 tensors (rope_part) at pos (int32 [s]);
+        inv_freq float64 [rope_dim / 2] on the GPU."""
+        rope_dim = 2 * inv_freq.numel() if rope_dim is None else rope_dim
+        s = pos.numel()
+        if rope_dim > 0:
+            _dense("inv_freq", inv_freq, "float64", rope_dim // 2)
+        d = abi.RbtRopeDesc(layout, head_dim, rope_start, rope_dim, _ptr(inv_freq), factor, int(angle_f32), eps)
+        arr = (abi.RbtRopePart * max(1, len(parts)))(*parts)
+        if sync:
+            self._torch_sync()
+        self.check(self.lib.rbt_rope_d(self.h, C.byref(d), arr, len(parts), _dense("pos", pos, "int32", *pos.shape), s))
+        if sync:
+            self.sync()
+
+    def tree_positions(self, parent, n_nodes, length, pos, sync=True):
+        """rbt_tree_positions_d: pos[b, i] = length[b] + depth of node i (int32 [n_seq, max_nodes]); -1 past
+        n_nodes[b]."""
+        B, T = parent.shape
+        if sync:
+            self._torch_sync()
+        self.check(self.lib.rbt_tree_positions_d(self.h, B, T, _dense("parent", parent, "int32", B, T),
+                                                 _dense("n_nodes", n_nodes, "int32", B),
+                                                 _dense("length", length, "int32", B),
+                                                 _dense("pos", pos, "int32", B, T)))
+        if sync:
+            self.sync()
+        return pos
+
+    def gqa_tree(self, q, k_cache, v_cache, k_draft, v_draft, length, n_nodes, parent, attn_scale, out, gate=None,
+                 max_len=0, sync=True):
+        """rbt_gqa_tree_d: attention of a tree of drafted tokens per sequence. q, out float32
+        [n_seq, max_nodes, n_heads, head_dim]; caches [n_seq, cap, n_kv, head_dim] and draft rows
+        [n_seq, max_nodes, n_kv, head_dim], float32 or bfloat16; gate as q, or a view of [query, gate] rows."""
+        B, T, H, D = q.shape
+        cap, K = k_cache.shape[1:3]
+        kv = "bfloat16" if _dtype(k_cache) == DT_BF16 else "float32"
+        gs = (0, 0)
+        if gate is not None:
+            if not gate.is_cuda or str(gate.dtype) != "torch.float32" or tuple(gate.shape) != (B, T, H, D) or \
+                    (D > 1 and gate.stride(3) != 1) or (B > 1 and gate.stride(0) != T * gate.stride(1)):
+                raise ValueError("gate must be float32 like q, its entries contiguous and its sequences T tokens apart")
+            gs = (gate.stride(1) if T > 1 else gate.stride(0), gate.stride(2))
+        d = abi.RbtGqaTreeDesc(H, K, D, attn_scale, _dtype(k_cache), cap, max_len, *gs)
+        if sync:
+            self._torch_sync()
+        self.check(self.lib.rbt_gqa_tree_d(
+            self.h, C.byref(d), B, T, _dense("q", q, "float32", B, T, H, D), _dense("k_cache", k_cache, kv, B, cap, K, D),
+            _dense("v_cache", v_cache, kv, B, cap, K, D), _dense("k_draft", k_draft, kv, B, T, K, D),
+            _dense("v_draft", v_draft, kv, B, T, K, D), _dense("length", length, "int32", B),
+            _dense("n_nodes", n_nodes, "int32", B), _dense("parent", parent, "int32", B, T),
+            None if gate is None else gate.data_ptr(), _dense("out", out, "float32", B, T, H, D)))
+        if sync:
+            self.sync()
+        return out
+
+    def draft_verify(self, tokens, parent, n_nodes, p, u, path, n_path, next_token, q=None, max_children=0, sync=True):
+        """rbt_draft_verify_d: the standing nodes (path, n_path) and the token after them. tokens, parent, path
+        int32 [n_seq, max_nodes]; p, q float32 [n_seq, max_nodes, vocab] (q None: drafts that were not drawn);
+        u float32 [n_seq, max_nodes] in [0, 1)."""
+        B, T, V = p.shape
+        if sync:
+            self._torch_sync()
+        self.check(self.lib.rbt_draft_verify_d(
+            self.h, B, T, V, max_children, _dense("tokens", tokens, "int32", B, T), _dense("parent", parent, "int32", B, T),
+            _dense("n_nodes", n_nodes, "int32", B), _dense("p", p, "float32", B, T, V), _dense("q", q, "float32", B, T, V),
+            _dense("u", u, "float32", B, T), _dense("path", path, "int32", B, T), _dense("n_path", n_path, "int32", B),
+            _dense("next_token", next_token, "int32", B)))
+        if sync:
+            self.sync()
+        return path, n_path, next_token
+
+    def kv_commit(self, k_caches, v_caches, k_drafts, v_drafts, path, n_path, length, length_out, sync=True):
+        """rbt_kv_commit_d: the standing nodes' draft rows appended to every layer's cache. Lists with one
+        tensor per layer: caches [n_seq, cap, n_kv, head_dim], drafts [n_seq, max_nodes, n_kv, head_dim]."""
+        L = len(k_caches)
+        if not (len(v_caches) == len(k_drafts) == len(v_drafts) == L):
+            raise ValueError("one cache and one draft buffer per side and layer")
+        B, T = path.shape
+        cap, K, D = k_caches[0].shape[1:] if L else (2**31 - 1, 1, 1)
+        kv = "float32" if L == 0 or _dtype(k_caches[0]) == DT_F32 else "bfloat16"
+        arr = [(C.c_void_p * max(1, L))(*[_dense("cache or draft", t, kv, B, rows, K, D) for t in ts])
+               for ts, rows in ((k_caches, cap), (v_caches, cap), (k_drafts, T), (v_drafts, T))]
+        d = abi.RbtKvCommitDesc(L, K, D, DT_F32 if kv == "float32" else DT_BF16, cap)
+        if sync:
+            self._torch_sync()
+        self.check(self.lib.rbt_kv_commit_d(self.h, C.byref(d), B, T, *arr, _dense("path", path, "int32", B, T),
+                                            _dense("n_path", n_path, "int32", B), _dense("length", length, "int32", B),
+                                            _dense("length_out", length_out, "int32", B)))
+        if sync:
+            self.sync()
+        return length_out
 
     # -- instrumentation --------------------------------------------------------------------
     def profile_enable(self, on: bool = True):

@@ -27,6 +27,9 @@ STATUS_NAMES = {0: "RBT_OK", -1: "RBT_E_INVALID", -2: "RBT_E_SHAPE", -3: "RBT_E_
 QT_F32, QT_I4_GROUPED, QT_MXFP4 = 0, 1, 2
 FAMILY_QWEN38, FAMILY_GLM52, FAMILY_KIMI_K3 = 0, 1, 2
 ACT_SILU, ACT_SITU = 0, 1
+DT_F32, DT_BF16 = 0, 1
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_YARN, ROPE_WAVELENGTH = 0, 1, 2, 3, 4
 
 
 class RbtQT(C.Structure):
@@ -77,6 +80,35 @@ class RbtGqaDesc(C.Structure):
     _fields_ = [("n_heads", C.c_size_t), ("n_kv_heads", C.c_size_t), ("head_dim", C.c_size_t),
                 ("rope_dim", C.c_size_t), ("theta", C.c_float), ("attn_scale", C.c_float), ("eps", C.c_float),
                 ("q_norm", C.c_void_p), ("k_norm", C.c_void_p)]
+
+
+class RbtRopeScaling(C.Structure):
+    _fields_ = [("kind", C.c_int32), ("factor", C.c_float), ("orig_ctx", C.c_float), ("beta_fast", C.c_float),
+                ("beta_slow", C.c_float), ("low_freq", C.c_float), ("high_freq", C.c_float),
+                ("attn_factor", C.c_float), ("as_f32", C.c_int32)]
+
+
+class RbtRopeDesc(C.Structure):
+    _fields_ = [("layout", C.c_int32), ("head_dim", C.c_size_t), ("rope_start", C.c_size_t), ("rope_dim", C.c_size_t),
+                ("inv_freq", C.c_void_p), ("factor", C.c_float), ("angle_f32", C.c_int32), ("eps", C.c_float)]
+
+
+class RbtRopePart(C.Structure):
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("src_dtype", C.c_int32), ("dst_dtype", C.c_int32),
+                ("n_heads", C.c_size_t), ("src_token_stride", C.c_size_t), ("src_head_stride", C.c_size_t),
+                ("dst_token_stride", C.c_size_t), ("dst_head_stride", C.c_size_t), ("norm", C.c_void_p),
+                ("rotate", C.c_int32)]
+
+
+class RbtGqaTreeDesc(C.Structure):
+    _fields_ = [("n_heads", C.c_size_t), ("n_kv_heads", C.c_size_t), ("head_dim", C.c_size_t),
+                ("attn_scale", C.c_float), ("kv_dtype", C.c_int32), ("cap", C.c_size_t), ("max_len", C.c_size_t),
+                ("gate_token_stride", C.c_size_t), ("gate_head_stride", C.c_size_t)]
+
+
+class RbtKvCommitDesc(C.Structure):
+    _fields_ = [("n_layers", C.c_size_t), ("n_kv_heads", C.c_size_t), ("head_dim", C.c_size_t),
+                ("kv_dtype", C.c_int32), ("cap", C.c_size_t)]
 
 
 class RbtKernelStat(C.Structure):
@@ -145,6 +177,13 @@ SIGNATURES = {
     "rbt_moe_sublayer_d": (_I, [_CTX, _U32, _P, _S, _P, _F, _P, _P]),
     "rbt_gdn_step_d": (_I, [_CTX, C.POINTER(RbtGdnDesc), _P, _P, _P, _P, _P, _P, _P]),
     "rbt_gqa_step_d": (_I, [_CTX, C.POINTER(RbtGqaDesc), _P, _P, _S, _S, _P, _P, _P, _P]),
+    "rbt_rope_freqs": (_I, [C.POINTER(RbtRopeScaling), _F, _S, _P, C.POINTER(C.c_float)]),
+    "rbt_rope_d": (_I, [_CTX, C.POINTER(RbtRopeDesc), C.POINTER(RbtRopePart), _S, _P, _S]),
+    "rbt_tree_positions_d": (_I, [_CTX, _S, _S, _P, _P, _P, _P]),
+    "rbt_gqa_tree_d": (_I, [_CTX, C.POINTER(RbtGqaTreeDesc), _S, _S, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "rbt_draft_verify_d": (_I, [_CTX, _S, _S, _S, _S, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "rbt_kv_commit_d": (_I, [_CTX, C.POINTER(RbtKvCommitDesc), _S, _S, C.POINTER(_P), C.POINTER(_P), C.POINTER(_P),
+                             C.POINTER(_P), _P, _P, _P, _P]),
     "rbt_profile_enable": (_I, [_CTX, _I]),
     "rbt_profile_read": (_I, [_CTX, C.POINTER(RbtProfile), _I]),
     "rbt_profile_kernels": (_I, [_CTX, _I]),

@@ -191,7 +191,7 @@ bool kernel_events(const Ctx &base, const void *fn, hipEvent_t *start, hipEvent_
 
 namespace {
 
-constexpr int FLAG_ERR = 0, FLAG_AMB = 1, FLAG_UNIQ = 2, FLAG_NR = 3, FLAG_GUP = 4, FLAG_N = 8;
+constexpr int FLAG_ERR = 0, FLAG_AMB = 1, FLAG_UNIQ = 2, FLAG_NR = 3, FLAG_GUP = 4, FLAG_TREE = 5, FLAG_N = 8;
 
 int fail(rbt_ctx *c, int code, const char *fmt, ...) __attribute__((format(printf, 3, 4)));
 int fail(rbt_ctx *c, int code, const char *fmt, ...) {
@@ -390,6 +390,10 @@ int sync_and_check(rbt_ctx *c) {
   if (c->h_flags[FLAG_ERR]) {
     HIP_OK(c, hipMemset(c->d_flags, 0, sizeof(int)));
     return fail(c, RBT_E_NOT_RESIDENT, "a routed expert is not resident in the pool");
+  }
+  if (c->h_flags[FLAG_TREE]) {
+    HIP_OK(c, hipMemset(c->d_flags + FLAG_TREE, 0, sizeof(int)));
+    return fail(c, RBT_E_INVALID, "drafted tokens: a length, node count, parent, token or path did not fit its range");
   }
   return RBT_OK;
 }
@@ -2123,6 +2127,288 @@ int rbt_gqa_step_d(rbt_ctx *c, const rbt_gqa_desc *d, float *k_cache, float *v_c
   RBT_TRY(scratch_t(c, SC_MIXB, rbt::gqa_part_floats((int)nh, (int)nkv, (int)hd, (int)pos + 1), &part));
   HIP_OK(c, rbt::launch_gqa(*c, qg, k, v, (int)nh, (int)nkv, (int)hd, d->q_norm, d->k_norm, d->eps, (int)d->rope_dim,
                             d->theta, d->attn_scale, (int)pos, k_cache, v_cache, qp, part, ctx_out));
+  return RBT_OK;
+}
+
+// ---- drafted tokens. The arguments are checked before the context, so that a refusal needs no GPU; without
+// a context its message is rbt_last_error(NULL)'s.
+static int refuse(rbt_ctx *c, int code, const char *fmt, ...) __attribute__((format(printf, 3, 4)));
+static int refuse(rbt_ctx *c, int code, const char *fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  (c ? c->err : g_init_err) = buf;
+  return code;
+}
+
+static bool bad_dtype(int32_t t) { return t != RBT_DT_F32 && t != RBT_DT_BF16; }
+static size_t dtype_size(int32_t t) { return t == RBT_DT_BF16 ? 2 : 4; }
+static bool misaligned(const void *p, size_t n) { return (uintptr_t)p % n != 0; }
+
+// The context's device made current for a call, and what was current before afterwards.
+struct DeviceScope {
+  int before = -1;
+  explicit DeviceScope(int device) {
+    int now = 0;
+    if (hipGetDevice(&now) == hipSuccess && now != device && hipSetDevice(device) == hipSuccess) before = now;
+  }
+  ~DeviceScope() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+};
+
+// A step's size: sequences and nodes.
+static int tree_size(rbt_ctx *c, size_t n_seq, size_t max_nodes) {
+  if (max_nodes == 0 || n_seq > 65535) return refuse(c, RBT_E_INVALID, "bad step (%zu sequences of %zu nodes)", n_seq, max_nodes);
+  if (max_nodes > rbt::TREE_MAX)
+    return refuse(c, RBT_E_UNSUPPORTED, "%zu nodes per sequence (at most %d)", max_nodes, rbt::TREE_MAX);
+  return RBT_OK;
+}
+
+int rbt_rope_freqs(const rbt_rope_scaling *sc, float theta, size_t rope_dim, double *inv_freq, float *factor) {
+  const rbt_rope_scaling z{};
+  const rbt_rope_scaling &s = sc ? *sc : z;
+  if (!inv_freq || !factor) return refuse(nullptr, RBT_E_INVALID, "null inv_freq or factor");
+  if (rope_dim % 2 || rope_dim > 1024) return refuse(nullptr, RBT_E_INVALID, "rope_dim %zu (even, at most 1024)", rope_dim);
+  if (!(theta > 0.0f) || !std::isfinite(theta)) return refuse(nullptr, RBT_E_INVALID, "theta %g", theta);
+  if (s.kind < RBT_ROPE_PLAIN || s.kind > RBT_ROPE_WAVELENGTH)
+    return refuse(nullptr, RBT_E_INVALID, "scaling kind %d", s.kind);
+  if (s.kind != RBT_ROPE_PLAIN && (!(s.factor >= 1.0f) || !std::isfinite(s.factor)))
+    return refuse(nullptr, RBT_E_INVALID, "scaling factor %g (at least 1)", s.factor);
+  if (s.kind == RBT_ROPE_BASE && rope_dim == 2) return refuse(nullptr, RBT_E_INVALID, "no other base for rope_dim 2");
+  if (s.kind == RBT_ROPE_YARN && (!(s.orig_ctx > 0.0f) || !(s.beta_slow > 0.0f) || !(s.beta_fast > s.beta_slow) ||
+                                  !std::isfinite(s.orig_ctx) || !std::isfinite(s.beta_fast) || !(theta > 1.0f)))
+    return refuse(nullptr, RBT_E_INVALID, "YaRN needs theta > 1, orig_ctx > 0 and beta_fast > beta_slow > 0");
+  if (s.kind == RBT_ROPE_WAVELENGTH && (!(s.orig_ctx > 0.0f) || !(s.low_freq > 0.0f) || !(s.high_freq > s.low_freq) ||
+                                        !std::isfinite(s.orig_ctx) || !std::isfinite(s.high_freq)))
+    return refuse(nullptr, RBT_E_INVALID, "wavelengths need orig_ctx > 0 and high_freq > low_freq > 0");
+  if (!(s.attn_factor >= 0.0f) || !std::isfinite(s.attn_factor))
+    return refuse(nullptr, RBT_E_INVALID, "attn_factor %g", s.attn_factor);
+  if (s.as_f32 && s.kind != RBT_ROPE_PLAIN) return refuse(nullptr, RBT_E_UNSUPPORTED, "as_f32 is for PLAIN frequencies");
+  const double d = (double)rope_dim, two_pi = 6.283185307179586;
+  double base = theta;
+  if (s.kind == RBT_ROPE_BASE && rope_dim) base *= std::pow((double)s.factor, d / (d - 2.0));
+  // YaRN's ramp: the (fractional) pair whose wavelength fits `turns` times into the context
+  const auto pair_of = [&](double turns) { return d * std::log(s.orig_ctx / (turns * two_pi)) / (2.0 * std::log(base)); };
+  double low = 0.0, high = 0.0;
+  if (s.kind == RBT_ROPE_YARN) {
+    low = std::max(std::floor(pair_of(s.beta_fast)), 0.0);
+    high = std::min(std::ceil(pair_of(s.beta_slow)), d - 1.0);
+    if (high <= low) high = low + 0.001;
+  }
+  for (size_t j = 0; j < rope_dim / 2; j++) {
+    double f = std::pow(base, -2.0 * (double)j / d);
+    if (s.as_f32) {
+      const float e = (-2.0f * (float)j) / (float)rope_dim;
+      f = (double)(float)std::pow((double)theta, (double)e);
+    } else if (s.kind == RBT_ROPE_LINEAR) {
+      f /= s.factor;
+    } else if (s.kind == RBT_ROPE_YARN) {
+      const double ramp = std::min(std::max(((double)j - low) / (high - low), 0.0), 1.0);
+      f = f / s.factor * ramp + f * (1.0 - ramp);
+    } else if (s.kind == RBT_ROPE_WAVELENGTH) {
+      const double turns = s.orig_ctx * f / two_pi;
+      const double keep = std::min(std::max((turns - s.low_freq) / ((double)s.high_freq - s.low_freq), 0.0), 1.0);
+      f = f / s.factor * (1.0 - keep) + f * keep;
+    }
+    inv_freq[j] = f;
+  }
+  *factor = s.attn_factor > 0.0f ? s.attn_factor
+            : s.kind == RBT_ROPE_YARN ? (float)(0.1 * std::log((double)s.factor) + 1.0) : 1.0f;
+  return RBT_OK;
+}
+
+int rbt_rope_d(rbt_ctx *c, const rbt_rope_desc *d, const rbt_rope_part *parts, size_t n_parts, const int32_t *pos,
+               size_t s) {
+  if (!d || (n_parts && !parts)) return refuse(c, RBT_E_INVALID, "null descriptor or parts");
+  if (n_parts > 8) return refuse(c, RBT_E_INVALID, "%zu tensors in one call (at most 8)", n_parts);
+  if (d->layout != RBT_ROPE_HALF && d->layout != RBT_ROPE_INTERLEAVED)
+    return refuse(c, RBT_E_INVALID, "rotary layout %d", d->layout);
+  if (d->head_dim == 0 || d->head_dim > 1024) return refuse(c, RBT_E_UNSUPPORTED, "head_dim %zu (1..1024)", d->head_dim);
+  if (d->rope_dim % 2 || d->rope_dim > d->head_dim || d->rope_start > d->head_dim - d->rope_dim)
+    return refuse(c, RBT_E_INVALID, "rotated entries %zu from %zu of %zu", d->rope_dim, d->rope_start, d->head_dim);
+  if (!std::isfinite(d->factor) || !(d->eps >= 0.0f) || !std::isfinite(d->eps))
+    return refuse(c, RBT_E_INVALID, "factor %g, eps %g", d->factor, d->eps);
+  if (s > (size_t)INT32_MAX) return refuse(c, RBT_E_INVALID, "%zu tokens", s);
+  rbt::RopeArgs a{};
+  size_t rows = 0;
+  for (size_t i = 0; i < n_parts; i++) {
+    const rbt_rope_part &p = parts[i];
+    if (bad_dtype(p.src_dtype) || bad_dtype(p.dst_dtype))
+      return refuse(c, RBT_E_INVALID, "part %zu: types %d, %d", i, p.src_dtype, p.dst_dtype);
+    if (p.n_heads == 0 || p.n_heads > 65536) return refuse(c, RBT_E_INVALID, "part %zu: %zu heads", i, p.n_heads);
+    if (s == 0) continue;
+    if (!p.src || !p.dst) return refuse(c, RBT_E_INVALID, "part %zu: null src or dst", i);
+    if (misaligned(p.src, dtype_size(p.src_dtype)) || misaligned(p.dst, dtype_size(p.dst_dtype)) || misaligned(p.norm, 4))
+      return refuse(c, RBT_E_INVALID, "part %zu: a pointer is not aligned to its type", i);
+    if (p.rotate && d->rope_dim && !d->inv_freq) return refuse(c, RBT_E_INVALID, "null inv_freq");
+    const size_t lim = (size_t)1 << 40;
+    if (p.src_token_stride > lim || p.src_head_stride > lim || p.dst_token_stride > lim || p.dst_head_stride > lim)
+      return refuse(c, RBT_E_INVALID, "part %zu: a stride is past 2^40", i);
+    // rows of the result lie apart: heads within tokens, or tokens within heads
+    const size_t hs = p.dst_head_stride, ts = p.dst_token_stride, hd = d->head_dim;
+    const bool heads_in = (p.n_heads == 1 || hs >= hd) && (s == 1 || ts >= (p.n_heads - 1) * hs + hd);
+    const bool tokens_in = (s == 1 || ts >= hd) && (p.n_heads == 1 || hs >= (s - 1) * ts + hd);
+    if (!heads_in && !tokens_in) return refuse(c, RBT_E_INVALID, "part %zu: result rows overlap", i);
+    rbt::RopePartD &o = a.part[i];
+    o.src = p.src;
+    o.dst = p.dst;
+    o.sts = (long)p.src_token_stride;
+    o.shs = (long)p.src_head_stride;
+    o.dts = (long)p.dst_token_stride;
+    o.dhs = (long)p.dst_head_stride;
+    o.norm = p.norm;
+    o.row0 = (int)rows;
+    o.s16 = p.src_dtype == RBT_DT_BF16;
+    o.d16 = p.dst_dtype == RBT_DT_BF16;
+    o.rotate = p.rotate != 0 && d->rope_dim > 0;
+    rows += p.n_heads;
+  }
+  if (s && n_parts && !pos) return refuse(c, RBT_E_INVALID, "null positions");
+  if (!c) return refuse(c, RBT_E_INVALID, "null context");
+  if (s == 0 || n_parts == 0) return RBT_OK;
+  a.n_parts = (int)n_parts;
+  a.n_rows = (int)rows;
+  a.hd = (int)d->head_dim;
+  a.start = (int)d->rope_start;
+  a.rd = d->inv_freq ? (int)d->rope_dim : 0;  // without a table no part rotates
+  a.pairs = d->layout == RBT_ROPE_INTERLEAVED;
+  a.angle_f32 = d->angle_f32 != 0;
+  a.factor = d->factor;
+  a.eps = d->eps;
+  a.inv = d->inv_freq;
+  a.pos = pos;
+  DeviceScope dev(c->device);
+  HIP_OK(c, rbt::launch_rope(*c, a, (int)s));
+  return RBT_OK;
+}
+
+int rbt_tree_positions_d(rbt_ctx *c, size_t n_seq, size_t max_nodes, const int32_t *parent, const int32_t *n_nodes,
+                         const int32_t *len, int32_t *pos) {
+  RBT_TRY(tree_size(c, n_seq, max_nodes));
+  if (n_seq && (!parent || !n_nodes || !len || !pos)) return refuse(c, RBT_E_INVALID, "null tree buffer");
+  if (!c) return refuse(c, RBT_E_INVALID, "null context");
+  if (n_seq == 0) return RBT_OK;
+  DeviceScope dev(c->device);
+  HIP_OK(c, rbt::launch_tree_pos(*c, parent, n_nodes, len, (int)n_seq, (int)max_nodes, pos, c->d_flags + FLAG_TREE));
+  return RBT_OK;
+}
+
+int rbt_gqa_tree_d(rbt_ctx *c, const rbt_gqa_tree_desc *d, size_t n_seq, size_t max_nodes, const float *q,
+                   const void *k_cache, const void *v_cache, const void *k_draft, const void *v_draft,
+                   const int32_t *len, const int32_t *n_nodes, const int32_t *parent, const float *gate, float *out) {
+  if (!d) return refuse(c, RBT_E_INVALID, "null descriptor");
+  RBT_TRY(tree_size(c, n_seq, max_nodes));
+  const size_t nh = d->n_heads, nkv = d->n_kv_heads, hd = d->head_dim;
+  if (nh == 0 || nkv == 0 || nh % nkv || nh > 4096)
+    return refuse(c, RBT_E_INVALID, "bad attention shape (heads %zu over %zu kv heads)", nh, nkv);
+  if (hd == 0 || hd > 1024) return refuse(c, RBT_E_UNSUPPORTED, "head_dim %zu (1..1024)", hd);
+  if (bad_dtype(d->kv_dtype)) return refuse(c, RBT_E_INVALID, "cache type %d", d->kv_dtype);
+  if (!std::isfinite(d->attn_scale)) return refuse(c, RBT_E_INVALID, "attn_scale %g", d->attn_scale);
+  if (d->cap == 0 || d->cap > (size_t)INT32_MAX || d->max_len > d->cap)
+    return refuse(c, RBT_E_INVALID, "cache of %zu rows, max_len %zu", d->cap, d->max_len);
+  if (gate && (d->gate_token_stride > (size_t)1 << 40 || d->gate_head_stride > (size_t)1 << 40))
+    return refuse(c, RBT_E_INVALID, "a gate stride is past 2^40");
+  if (n_seq) {
+    if (!q || !k_cache || !v_cache || !k_draft || !v_draft || !len || !n_nodes || !parent || !out)
+      return refuse(c, RBT_E_INVALID, "null attention buffer");
+    if (misaligned(k_cache, 16) || misaligned(v_cache, 16) || misaligned(k_draft, 16) || misaligned(v_draft, 16) ||
+        misaligned(q, 16) || misaligned(out, 16) || misaligned(gate, 4))
+      return refuse(c, RBT_E_INVALID, "q, out, caches and draft rows must be 16-byte aligned");
+  }
+  if (!c) return refuse(c, RBT_E_INVALID, "null context");
+  if (n_seq == 0) return RBT_OK;
+  DeviceScope dev(c->device);
+  rbt::TreeArgs a{};
+  a.q = q;
+  a.kc = k_cache;
+  a.vc = v_cache;
+  a.kd = k_draft;
+  a.vd = v_draft;
+  a.len = len;
+  a.n_nodes = n_nodes;
+  a.parent = parent;
+  a.gate = gate;
+  a.gts = (long)d->gate_token_stride;
+  a.ghs = (long)d->gate_head_stride;
+  a.out = out;
+  a.B = (int)n_seq;
+  a.T = (int)max_nodes;
+  a.H = (int)nh;
+  a.K = (int)nkv;
+  a.hd = (int)hd;
+  a.cap = (long)d->cap;
+  a.max_len = (long)(d->max_len ? d->max_len : d->cap);
+  a.scale = d->attn_scale;
+  a.kv16 = d->kv_dtype == RBT_DT_BF16;
+  a.bad = c->d_flags + FLAG_TREE;
+  HIP_OK(c, rbt::launch_tree(*c, a));
+  return RBT_OK;
+}
+
+int rbt_draft_verify_d(rbt_ctx *c, size_t n_seq, size_t max_nodes, size_t vocab, size_t max_children,
+                       const int32_t *tokens, const int32_t *parent, const int32_t *n_nodes, const float *p,
+                       const float *q, const float *u, int32_t *path, int32_t *n_path, int32_t *next) {
+  RBT_TRY(tree_size(c, n_seq, max_nodes));
+  if (n_seq > 1024) return refuse(c, RBT_E_UNSUPPORTED, "%zu sequences (at most 1024)", n_seq);
+  if (vocab == 0 || vocab > (size_t)1 << 30) return refuse(c, RBT_E_INVALID, "vocabulary of %zu", vocab);
+  if (n_seq) {
+    if (!tokens || !parent || !n_nodes || !p || !u || !path || !n_path || !next)
+      return refuse(c, RBT_E_INVALID, "null verification buffer");
+    if (misaligned(p, 4) || misaligned(q, 4)) return refuse(c, RBT_E_INVALID, "a pointer is not aligned to its type");
+  }
+  if (!c) return refuse(c, RBT_E_INVALID, "null context");
+  if (n_seq == 0) return RBT_OK;
+  DeviceScope dev(c->device);
+  HIP_OK(c, rbt::launch_verify(*c, tokens, parent, n_nodes, p, q, u, (int)n_seq, (int)max_nodes, (int)vocab, path, n_path,
+                               next, c->d_flags + FLAG_TREE));
+  return RBT_OK;
+}
+
+int rbt_kv_commit_d(rbt_ctx *c, const rbt_kv_commit_desc *d, size_t n_seq, size_t max_nodes, void *const *k_caches,
+                    void *const *v_caches, const void *const *k_drafts, const void *const *v_drafts,
+                    const int32_t *path, const int32_t *n_path, const int32_t *len, int32_t *len_out) {
+  if (!d) return refuse(c, RBT_E_INVALID, "null descriptor");
+  RBT_TRY(tree_size(c, n_seq, max_nodes));
+  if (bad_dtype(d->kv_dtype)) return refuse(c, RBT_E_INVALID, "cache type %d", d->kv_dtype);
+  if (d->n_layers > 4096 || d->n_kv_heads == 0 || d->head_dim == 0 || d->n_kv_heads > 4096 || d->head_dim > 1024 ||
+      d->cap == 0 || d->cap > (size_t)INT32_MAX)
+    return refuse(c, RBT_E_INVALID, "bad caches (%zu layers, %zu kv heads of %zu, %zu rows)", d->n_layers, d->n_kv_heads,
+                  d->head_dim, d->cap);
+  const size_t es = dtype_size(d->kv_dtype), row = d->n_kv_heads * d->head_dim * es;
+  bool al16 = row % 16 == 0;
+  if (n_seq) {
+    if (!path || !n_path || !len || !len_out) return refuse(c, RBT_E_INVALID, "null path or length buffer");
+    if (len == len_out) return refuse(c, RBT_E_INVALID, "len_out must not be len");
+    if (d->n_layers && (!k_caches || !v_caches || !k_drafts || !v_drafts))
+      return refuse(c, RBT_E_INVALID, "null layer pointers");
+    for (size_t l = 0; l < d->n_layers; l++) {
+      const void *ptr[4] = {k_caches[l], v_caches[l], k_drafts[l], v_drafts[l]};
+      for (const void *x : ptr) {
+        if (!x) return refuse(c, RBT_E_INVALID, "layer %zu: null cache or draft rows", l);
+        if (misaligned(x, es)) return refuse(c, RBT_E_INVALID, "layer %zu: a pointer is not aligned to its type", l);
+        al16 = al16 && !misaligned(x, 16);
+      }
+    }
+  }
+  if (!c) return refuse(c, RBT_E_INVALID, "null context");
+  if (n_seq == 0) return RBT_OK;
+  DeviceScope dev(c->device);
+  const int unit = al16 ? 16 : (int)es;
+  size_t l = 0;
+  do {
+    rbt::CommitArgs a{};
+    for (; l < d->n_layers && a.sides < rbt::COMMIT_SIDES; l++) {
+      a.dst[a.sides] = k_caches[l];
+      a.src[a.sides++] = k_drafts[l];
+      a.dst[a.sides] = v_caches[l];
+      a.src[a.sides++] = v_drafts[l];
+    }
+    HIP_OK(c, rbt::launch_commit(*c, a, unit, path, n_path, len, (int)n_seq, (int)max_nodes, (int)d->cap,
+                                 (int)(row / unit), len_out, c->d_flags + FLAG_TREE));
+  } while (l < d->n_layers);
   return RBT_OK;
 }
 

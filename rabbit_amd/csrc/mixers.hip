@@ -223,37 +223,13 @@ __global__ __launch_bounds__(GDN_NT) void k_gdn_head(float *__restrict__ states,
 }
 
 // ---- GQA --------------------------------------------------------------------------------------
-// sin and cos of an fp32 angle (|x| < 2^22) in fp64, light on registers: x minus the nearest
-// multiple k of pi/2 (Cody and Waite's reduction with pi/2 split into three doubles; the first fma
-// is exact since x - k c1 is a multiple of 2^-52 below 1 in magnitude), then the Taylor series of
-// sin and cos on |r| <= pi/4 + ulp to degree 21 and 22 (truncation error below 2e-25), and the
-// quadrant k mod 4. Rounded to fp32, this gives the fp32 rounding of the exact values, as fp64
-// library calls do, without their large-argument paths.
+// sin and cos of an fp32 angle (|x| < 2^22), rounded to fp32: the fp32 rounding of the exact values, as
+// fp64 library calls give.
 __device__ __forceinline__ void mx_sincos(float xf, float &sn, float &cs) {
-  constexpr double c1 = 1.5707963267948966, c2 = 6.123233995736766e-17, c3 = -1.4973849048591698e-33;
-  const double x = xf, k = rint(x * 0.6366197723675814);
-  double r = fma(-k, c1, x);
-  r = fma(-k, c2, r);
-  r = fma(-k, c3, r);
-  const double r2 = r * r;
-  // 1 / n! for n = 0 .. 22 (each factorial is exact in fp64, so each quotient is correctly rounded)
-  constexpr double f[23] = {1.0, 1.0, 1.0 / 2, 1.0 / 6, 1.0 / 24, 1.0 / 120, 1.0 / 720, 1.0 / 5040,
-                            1.0 / 40320, 1.0 / 362880, 1.0 / 3628800, 1.0 / 39916800, 1.0 / 479001600,
-                            1.0 / 6227020800.0, 1.0 / 87178291200.0, 1.0 / 1307674368000.0,
-                            1.0 / 20922789888000.0, 1.0 / 355687428096000.0, 1.0 / 6402373705728000.0,
-                            1.0 / 121645100408832000.0, 1.0 / 2432902008176640000.0,
-                            1.0 / 51090942171709440000.0, 1.0 / 1124000727777607680000.0};
-  // sin r = r sum_{n<=10} (-r^2)^n / (2n+1)!, cos r = sum_{n<=11} (-r^2)^n / (2n)!, by Horner
-  double ps = f[21], pc = -f[22];
-#pragma unroll
-  for (int n = 10; n >= 0; n--) {
-    if (n < 10) ps = (n & 1 ? -f[2 * n + 1] : f[2 * n + 1]) + r2 * ps;
-    pc = (n & 1 ? -f[2 * n] : f[2 * n]) + r2 * pc;
-  }
-  const double sr = r * ps, cr = pc;
-  const int q = (int)((long long)k & 3);
-  sn = (float)(q == 0 ? sr : q == 1 ? cr : q == 2 ? -sr : -cr);
-  cs = (float)(q == 0 ? cr : q == 1 ? -sr : q == 2 ? -cr : sr);
+  double s, c;
+  rbt_sincos_d((double)xf, s, c);
+  sn = (float)s;
+  cs = (float)c;
 }
 
 // One workgroup of 256 threads per head: workgroups [0, n_heads) take the query heads -> qp

@@ -206,6 +206,42 @@ __device__ __forceinline__ void rbt_single_rows(const int32_t *__restrict__ ids,
   if (threadIdx.x == 0) *nr = base;
 }
 
+// sin and cos of an angle |x| < 2^31 in fp64, light on registers: x minus the nearest multiple k of pi/2
+// (Cody and Waite's reduction with pi/2 split into three doubles; the first fma is exact since x - k c1 is a
+// multiple of 2^-52 below 1 in magnitude wherever k is not 0), then the Taylor series of sin and cos on
+// |r| <= pi/4 + ulp to degree 21 and 22 (truncation error below 2e-25), and the quadrant k mod 4. Without the
+// library calls' large-argument paths.
+__device__ __forceinline__ void rbt_sincos_d(double x, double &sn, double &cs) {
+  constexpr double c1 = 1.5707963267948966, c2 = 6.123233995736766e-17, c3 = -1.4973849048591698e-33;
+  const double k = rint(x * 0.6366197723675814);
+  double r = fma(-k, c1, x);
+  r = fma(-k, c2, r);
+  r = fma(-k, c3, r);
+  const double r2 = r * r;
+  // 1 / n! for n = 0 .. 22 (each factorial is exact in fp64, so each quotient is correctly rounded)
+  constexpr double f[23] = {1.0, 1.0, 1.0 / 2, 1.0 / 6, 1.0 / 24, 1.0 / 120, 1.0 / 720, 1.0 / 5040,
+                            1.0 / 40320, 1.0 / 362880, 1.0 / 3628800, 1.0 / 39916800, 1.0 / 479001600,
+                            1.0 / 6227020800.0, 1.0 / 87178291200.0, 1.0 / 1307674368000.0,
+                            1.0 / 20922789888000.0, 1.0 / 355687428096000.0, 1.0 / 6402373705728000.0,
+                            1.0 / 121645100408832000.0, 1.0 / 2432902008176640000.0,
+                            1.0 / 51090942171709440000.0, 1.0 / 1124000727777607680000.0};
+  // sin r = r sum_{n<=10} (-r^2)^n / (2n+1)!, cos r = sum_{n<=11} (-r^2)^n / (2n)!, by Horner
+  double ps = f[21], pc = -f[22];
+#pragma unroll
+  for (int n = 10; n >= 0; n--) {
+    if (n < 10) ps = (n & 1 ? -f[2 * n + 1] : f[2 * n + 1]) + r2 * ps;
+    pc = (n & 1 ? -f[2 * n] : f[2 * n]) + r2 * pc;
+  }
+  const double sr = r * ps, cr = pc;
+  const int q = (int)((long long)k & 3);
+  sn = q == 0 ? sr : q == 1 ? cr : q == 2 ? -sr : -cr;
+  cs = q == 0 ? cr : q == 1 ? -sr : q == 2 ? -cr : sr;
+}
+
+// bf16 bits to fp32, and fp32 to bf16 bits rounded to nearest even (v_cvt_pk_bf16_f32; a NaN stays one).
+__device__ __forceinline__ float rbt_bf16_f32(uint32_t b) { return __uint_as_float(b << 16); }
+__device__ __forceinline__ uint16_t rbt_f32_bf16(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }
+
 // Device view of one expert: gate/up/down as separate (data, scale) pointers. A fused gate_up
 // tensor is presented as two views into the same allocation.
 struct RbtExpertDev {

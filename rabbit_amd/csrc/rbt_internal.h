@@ -421,6 +421,56 @@ hipError_t launch_gqa(const Ctx &c, const float *qg, const float *k, const float
                       const float *qn, const float *kn, float eps, int rope_dim, float theta, float scale, int pos,
                       float *kc, float *vc, float *qp, float *part, float *ctx);
 
+// drafts.hip: several drafted tokens at once.
+constexpr int TREE_MAX = 256;  // nodes per sequence
+struct RopePartD {
+  const void *src;
+  void *dst;
+  long sts, shs, dts, dhs;  // token and head strides in entries
+  const float *norm;
+  int row0;                 // the part's first row among a token's rows
+  int s16, d16, rotate;     // bf16 source, bf16 destination
+};
+struct RopeArgs {
+  RopePartD part[8];
+  int n_parts, n_rows, hd, start, rd, pairs, angle_f32;
+  float factor, eps;
+  const double *inv;
+  const int *pos;
+};
+hipError_t launch_rope(const Ctx &c, const RopeArgs &a, int s);
+// bad: set to 1 by sequences or nodes whose numbers do not fit.
+hipError_t launch_tree_pos(const Ctx &c, const int *parent, const int *n_nodes, const int *len, int B, int T, int *pos,
+                           int *bad);
+hipError_t launch_verify(const Ctx &c, const int *tokens, const int *parent, const int *n_nodes, const float *p,
+                         const float *q, const float *u, int B, int T, int V, int *path, int *n_path, int *next, int *bad);
+constexpr int COMMIT_SIDES = 64;  // K and V of the layers of one launch
+struct CommitArgs {
+  void *dst[COMMIT_SIDES];
+  const void *src[COMMIT_SIDES];
+  int sides;
+};
+// unit: bytes of one copy (16, 4 or 2), row_units of them per row.
+hipError_t launch_commit(const Ctx &c, const CommitArgs &a, int unit, const int *path, const int *n_path, const int *len,
+                         int B, int T, int cap, int row_units, int *len_out, int *bad);
+
+// tree.hip: attention of drafted tokens.
+struct TreeArgs {
+  const float *q;
+  const void *kc, *vc, *kd, *vd;
+  const int *len, *n_nodes, *parent;
+  const float *gate;
+  long gts, ghs;
+  float *out;
+  int B, T, H, K, hd;  // sequences, nodes, query heads, KV heads
+  long cap;
+  long max_len;
+  float scale;
+  int kv16;  // bf16 caches and draft rows
+  int *bad;
+};
+hipError_t launch_tree(const Ctx &c, const TreeArgs &a);
+
 // synth.hip
 hipError_t launch_synth_mxfp4(const Ctx &c, uint8_t *data, uint8_t *scale, size_t rows, size_t cols, uint64_t seed,
                               uint32_t lo, uint32_t hi);
