@@ -468,8 +468,15 @@ struct TreeArgs {
   float scale;
   int kv16;  // bf16 caches and draft rows
   int *bad;
+  // tree_plan: whether the matrix cores take it, row tiles, pieces of the cache (keys per piece), scratch
+  int tiled, tiles, pieces;
+  long per, rows_max;
+  float *part;
+  float2 *part_ml;
 };
-hipError_t launch_tree(const Ctx &c, const TreeArgs &a);
+bool tree_plan(const Ctx &c, TreeArgs &a, int &rw, int &kw);
+size_t tree_part_floats(const TreeArgs &a);
+hipError_t launch_tree(const Ctx &c, const TreeArgs &a, int rw, int kw);
 
 // synth.hip
 hipError_t launch_synth_mxfp4(const Ctx &c, uint8_t *data, uint8_t *scale, size_t rows, size_t cols, uint64_t seed,

@@ -20,6 +20,17 @@ __device__ __forceinline__ bool tree_fits(const TreeArgs &a, int b, int &n, int 
   return false;
 }
 
+// Entries e .. e + 3 of a row: v / l, times sigmoid of the gate.
+__device__ __forceinline__ void tree_store(const TreeArgs &a, int b, int i, int h, int e, float4 v, float l) {
+  float o[4] = {v.x / l, v.y / l, v.z / l, v.w / l};
+  if (a.gate) {
+    const float *g = a.gate + ((long)b * a.T + i) * a.gts + (long)h * a.ghs + e;
+#pragma unroll
+    for (int k = 0; k < 4; k++) o[k] = __fmul_rn(o[k], rbt_sigmoid(g[k]));
+  }
+  *(float4 *)(a.out + (((long)b * a.T + i) * a.H + h) * a.hd + e) = make_float4(o[0], o[1], o[2], o[3]);
+}
+
 // Any shape: one workgroup per (query head, node, sequence), 256 keys at a time with the running maximum and
 // sum. Thread t takes key t's score, then entries t, t + 256, ... of the output; rows that the node does not
 // see are passed over.
@@ -98,8 +109,509 @@ __global__ __launch_bounds__(256) void k_tree_any(TreeArgs a) {
   }
 }
 
-hipError_t launch_tree(const Ctx &c, const TreeArgs &a) {
-  launch_k(c, k_tree_any, dim3(a.H, a.T, a.B), dim3(256), a);
+// ---- on the matrix cores -----------------------------------------------------------------------------
+// The rows of a KV head are its nodes times its query heads (row r = node * n_rep + head), sixteen per wave. With
+// keys on the M side, S^T = K Q^T leaves each lane four keys of one row (column n = lane % 16), which is the B operand
+// that O^T = V^T P^T wants if V's rows are taken in the same order: the probabilities never leave their lane, and
+// the running maximum and sum of a row are the lane's own (joined over the four lanes of a column).
+//   bf16 caches: q and p are split into three bf16 parts that hold their 24 bits exactly (by truncation: 8 bits
+//     each), so every product is exact and only the fp32 sums round, at three times the products.
+//   f32 caches: fp32 MFMAs.
+// A workgroup of RW x KW waves takes RW row tiles and one piece of the keys: KW groups of waves share out each
+// stage's keys (few rows: every wave has its own keys; many rows: every wave has its own rows). Stages of TK keys
+// land in LDS by direct loads (global_load_lds, 16 bytes per lane), two stages in turn: while one is multiplied the
+// next is in flight. LDS rows hold their 16-byte chunks in an order turned by the row's number, so that
+// the columns read at once lie in different banks.
+typedef float tf4 __attribute__((ext_vector_type(4)));
+typedef short ts4 __attribute__((ext_vector_type(4)));
+typedef __bf16 tb8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) ts4 tree_lds_s4;
+
+// 64 lanes' 16 bytes at p (each its own) to LDS at `base` (the wave's) + 16 lane.
+__device__ __forceinline__ void tree_dma(const void *p, uint32_t base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(base), "v"(p) : "memory");
+}
+
+// x = hi + mid + lo, each with its low 16 bits zero (fp32 has 24 significant bits, each part 8).
+__device__ __forceinline__ void tree_split(float x, uint32_t &hi, uint32_t &mid, uint32_t &lo) {
+  hi = __float_as_uint(x) & 0xffff0000u;
+  const float r = x - __uint_as_float(hi);
+  mid = __float_as_uint(r) & 0xffff0000u;
+  lo = __float_as_uint(r - __uint_as_float(mid));
+}
+// The high halves of a and b as two bf16 (a low).
+__device__ __forceinline__ uint32_t tree_pack(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+
+__device__ __forceinline__ float tree_xor_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16, 64));
+  return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float tree_xor_sum(float v) {
+  v = v + __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
+
+template <int HD, bool B16>
+struct TreeTile {
+  static constexpr int ES = B16 ? 2 : 4, ROWB = HD * ES, CH = ROWB / 16;
+  static constexpr int TK = B16 ? 64 : 32;                  // keys per stage
+  static constexpr int SIDE = TK * ROWB, STAGE = 2 * SIDE;  // bytes of one side, of K and V
+  static constexpr int LDS = 2 * STAGE;
+  static constexpr int INSTR = TK * CH / 64;                // 1 KB loads per side
+  static_assert(TK * CH % 64 == 0 && CH % 8 == 0, "whole loads");
+};
+
+template <int HD, bool B16, int KW>
+__global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(TreeArgs a) {
+  using TT = TreeTile<HD, B16>;
+  constexpr int ROWB = TT::ROWB, CH = TT::CH, TK = TT::TK, SK = TK / KW, NT = SK / 16;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  __shared__ int par[TREE_MAX];
+  __shared__ uint32_t vis[128][TREE_MAX / 32];  // per node of the row tile: which drafted rows it sees
+  __shared__ uint32_t dirty[2][2];              // per stage buffer: drafted rows with non-finite values
+  __shared__ float ml[KW > 1 ? 4 : 1][2][16];
+
+  // workgroup -> (row tile, piece, KV head, sequence): consecutive workgroups of an XCD (id % 8) share the keys
+  const int id = blockIdx.x, g = (id / 8 / a.tiles) * 8 + id % 8, rt = id / 8 % a.tiles;
+  if (g >= a.pieces * a.K * a.B) return;
+  const int piece = g / (a.K * a.B), kv = g % a.K, b = g / a.K % a.B;
+  int n, L;
+  if (!tree_fits(a, b, n, L)) return;
+  const int R = a.H / a.K, rows = n * R;
+  const int NW = blockDim.x >> 6, RW = NW / KW;
+  const int row0 = rt * RW * 16;
+  if (row0 >= rows) return;
+  long per = a.per;  // keys of a piece: a sequence longer than expected takes larger ones
+  if (L > per * a.pieces) per = ((L + a.pieces - 1) / a.pieces + TK - 1) / TK * TK;
+  const int np = L > 0 ? (int)((L + per - 1) / per) : 1;
+  if (piece >= np) return;
+  const int k0 = (int)(piece * per), k1 = (int)min((long)L, k0 + per);
+  const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int rg = w % RW, kgp = w / RW, col = lane & 15, kg = lane >> 4;
+  const int node_lo = row0 / R, node_hi = (min(rows, row0 + RW * 16) - 1) / R;
+  const int nd = piece == np - 1 ? node_hi + 1 : 0;  // drafted rows: those up to the last node of the tile
+  const int st_c = (k1 - k0 + TK - 1) / TK, st_n = st_c + (nd + TK - 1) / TK;
+
+  const long seq_row = (long)a.K * HD * TT::ES;  // bytes from a row to the next
+  const char *kc = (const char *)a.kc + ((long)b * a.cap * a.K + kv) * ROWB, *vc = (const char *)a.vc + ((long)b * a.cap * a.K + kv) * ROWB;
+  const char *kd = (const char *)a.kd + ((long)b * a.T * a.K + kv) * ROWB, *vd = (const char *)a.vd + ((long)b * a.T * a.K + kv) * ROWB;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)smem;
+
+  auto issue = [&](int s) {
+    const bool dr = s >= st_c;
+    const char *kp = dr ? kd : kc, *vp = dr ? vd : vc;
+    const int base = dr ? (s - st_c) * TK : k0 + s * TK, last = (dr ? nd : k1) - 1;
+    const uint32_t to = lds0 + (s & 1) * TT::STAGE;
+    for (int i = w; i < TT::INSTR; i += NW) {
+      const int u = i * 64 + lane, r = u / CH, c = u - r * CH;
+      const long at = (long)min(base + r, last) * seq_row;
+      tree_dma(kp + at + (c ^ (r & 7)) * 16, to + i * 1024);
+      tree_dma(vp + at + (B16 ? c ^ ((r & 3) << 1) : c) * 16, to + TT::SIDE + i * 1024);
+    }
+  };
+  issue(0);
+
+  // this lane's row, and its query in the B operand's layout
+  const int row = row0 + rg * 16 + col, rc = min(row, rows - 1);
+  const int node = rc / R, head = kv * R + (rc - node * R);
+  const long qrow = ((long)b * a.T + node) * a.H + head;
+  const float *qp = a.q + qrow * HD;
+  tb8 qb[B16 ? HD / 32 : 1][3];
+  float4 qf[B16 ? 1 : HD / 16];
+  if constexpr (B16) {
+#pragma unroll
+    for (int s = 0; s < HD / 32; s++) {
+      const float4 x = *(const float4 *)(qp + 32 * s + 8 * kg), y = *(const float4 *)(qp + 32 * s + 8 * kg + 4);
+      const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+      uint32_t o[3][8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) tree_split(v[e], o[0][e], o[1][e], o[2][e]);
+#pragma unroll
+      for (int p = 0; p < 3; p++)
+        qb[s][p] = __builtin_bit_cast(tb8, rbt_u4{tree_pack(o[p][0], o[p][1]), tree_pack(o[p][2], o[p][3]),
+                                                  tree_pack(o[p][4], o[p][5]), tree_pack(o[p][6], o[p][7])});
+    }
+  } else {
+#pragma unroll
+    for (int s = 0; s < HD / 16; s++) qf[s] = *(const float4 *)(qp + 16 * s + 4 * kg);
+  }
+  if (nd > 0) {
+    if (t < 4) dirty[t >> 1][t & 1] = 0;
+    for (int j = t; j < n; j += blockDim.x) {
+      int p = a.parent[(long)b * a.T + j];
+      if (p < -1 || p >= j) {
+        *a.bad = 1;
+        p = -1;
+      }
+      par[j] = p;
+    }
+    lds_barrier();
+    for (int i = node_lo + t; i <= node_hi; i += blockDim.x) {
+      for (int x = 0; x < TREE_MAX / 32; x++) vis[i - node_lo][x] = 0;
+      for (int j = i; j >= 0; j = par[j]) vis[i - node_lo][j >> 5] |= 1u << (j & 31);
+    }
+    // (read after the barrier of the first drafted stage)
+  }
+
+  const float c1 = a.scale * 1.44269504088896341f;  // scores in powers of two
+  float m = -INFINITY, l = 0.0f;
+  tf4 o[HD / 16];
+#pragma unroll
+  for (int x = 0; x < HD / 16; x++) o[x] = tf4{0.f, 0.f, 0.f, 0.f};
+
+  for (int s = 0; s < st_n; s++) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    lds_barrier();  // the stage has landed, and the other buffer's readers are done
+    if (s + 1 < st_n) issue(s + 1);
+    const bool dr = s >= st_c;
+    char *kt = smem + (s & 1) * TT::STAGE, *vt = kt + TT::SIDE;
+    uint32_t bad0 = 0, bad1 = 0;
+    const int base = dr ? (s - st_c) * TK : k0 + s * TK, last = dr ? nd : k1;
+    if (dr) {
+      // a value that some rows do not see must not meet their zero probabilities: non-finite ones are taken
+      // out of the tile and added below for the rows that do see them
+      for (int u = t; u < TK * CH; u += blockDim.x) {
+        const int r = u / CH;
+        uint32_t *x = (uint32_t *)(vt + u * 16);
+        bool hit = false;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          uint32_t v = x[e];
+          if constexpr (B16) {
+            if ((v & 0x7f80u) == 0x7f80u) v &= 0xffff0000u, hit = true;
+            if ((v & 0x7f800000u) == 0x7f800000u) v &= 0xffffu, hit = true;
+          } else {
+            if ((v & 0x7f800000u) == 0x7f800000u) v = 0, hit = true;
+          }
+          if (hit) x[e] = v;
+        }
+        if (hit) atomicOr(&dirty[s & 1][r >> 5], 1u << (r & 31));
+      }
+      lds_barrier();
+      bad0 = dirty[s & 1][0];
+      bad1 = dirty[s & 1][1];
+      if (t < 2) dirty[(s & 1) ^ 1][t] = 0;
+    }
+
+    // scores: lane (col, kg) gets keys 16 x + 4 kg + i of its row
+    tf4 sc[NT];
+#pragma unroll
+    for (int x = 0; x < NT; x++) sc[x] = tf4{0.f, 0.f, 0.f, 0.f};
+    const char *kb = kt + (kgp * SK + col) * ROWB;
+    if constexpr (B16) {
+      const int c0 = (kg ^ (col & 7)) * 16, c1_ = ((4 + kg) ^ (col & 7)) * 16;
+#pragma unroll
+      for (int st = 0; st < HD / 32; st++) {
+        tb8 kf[NT];
+#pragma unroll
+        for (int x = 0; x < NT; x++) kf[x] = *(const tb8 *)(kb + x * 16 * ROWB + (st & 1 ? c1_ : c0) + (st >> 1) * 128);
+#pragma unroll
+        for (int p = 2; p >= 0; p--)
+#pragma unroll
+          for (int x = 0; x < NT; x++) sc[x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[x], qb[st][p], sc[x], 0, 0, 0);
+      }
+    } else {
+      const int c0 = (kg ^ (col & 7)) * 16, c1_ = ((4 + kg) ^ (col & 7)) * 16;
+#pragma unroll
+      for (int st = 0; st < HD / 16; st++) {
+        float4 kf[NT];
+#pragma unroll
+        for (int x = 0; x < NT; x++) kf[x] = *(const float4 *)(kb + x * 16 * ROWB + (st & 1 ? c1_ : c0) + (st >> 1) * 128);
+#pragma unroll
+        for (int x = 0; x < NT; x++) sc[x] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[x].x, qf[st].x, sc[x], 0, 0, 0);
+#pragma unroll
+        for (int x = 0; x < NT; x++) sc[x] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[x].y, qf[st].y, sc[x], 0, 0, 0);
+#pragma unroll
+        for (int x = 0; x < NT; x++) sc[x] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[x].z, qf[st].z, sc[x], 0, 0, 0);
+#pragma unroll
+        for (int x = 0; x < NT; x++) sc[x] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[x].w, qf[st].w, sc[x], 0, 0, 0);
+      }
+    }
+    float mt = -INFINITY;
+    const int kfirst = base + kgp * SK + 4 * kg;
+    if (dr || base + TK > last) {
+#pragma unroll
+      for (int x = 0; x < NT; x++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const int j = kfirst + 16 * x + i;
+          bool see = j < last;
+          if (dr) see = see && (vis[node - node_lo][min(j, TREE_MAX - 1) >> 5] >> (j & 31) & 1);
+          sc[x][i] = see ? sc[x][i] * c1 : -INFINITY;
+        }
+    } else {
+#pragma unroll
+      for (int x = 0; x < NT; x++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) sc[x][i] *= c1;
+    }
+#pragma unroll
+    for (int x = 0; x < NT; x++) mt = fmaxf(mt, fmaxf(fmaxf(sc[x][0], sc[x][1]), fmaxf(sc[x][2], sc[x][3])));
+    mt = fmaxf(m, tree_xor_max(mt));
+    if (__any(mt > m)) {
+      const float f = mt == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mt);
+      l *= f;
+#pragma unroll
+      for (int x = 0; x < HD / 16; x++) o[x] *= f;
+      m = mt;
+    }
+    const float ms = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int x = 0; x < NT; x++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        sc[x][i] = __builtin_amdgcn_exp2f(sc[x][i] - ms);
+        l += sc[x][i];
+      }
+
+    // values
+    if constexpr (B16) {
+      const int xr = col >> 2;
+      const char *vb = vt + (kgp * SK + 4 * kg + xr) * ROWB + (col & 1) * 8 + ((col >> 1) & 1) * 16;
+      uint32_t pp[NT][3][2];
+#pragma unroll
+      for (int x = 0; x < NT; x++) {
+        uint32_t h[3][4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) tree_split(sc[x][i], h[0][i], h[1][i], h[2][i]);
+#pragma unroll
+        for (int p = 0; p < 3; p++) {
+          pp[x][p][0] = tree_pack(h[p][0], h[p][1]);
+          pp[x][p][1] = tree_pack(h[p][2], h[p][3]);
+        }
+      }
+#pragma unroll
+      for (int dt = 0; dt < HD / 16; dt++) {
+        const char *vp = vb + (dt >> 2) * 128 + (((dt & 3) ^ xr) * 32);
+        ts4 vf[NT];
+#pragma unroll
+        for (int x = 0; x < NT; x++)
+          vf[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tree_lds_s4 *)(vp + x * 16 * ROWB));
+        if constexpr (NT >= 2) {
+#pragma unroll
+          for (int x = 0; x < NT; x += 2) {
+            struct { ts4 lo, hi; } vv{vf[x], vf[x + 1]};
+#pragma unroll
+            for (int p = 2; p >= 0; p--)
+              o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                  __builtin_bit_cast(tb8, vv),
+                  __builtin_bit_cast(tb8, rbt_u4{pp[x][p][0], pp[x][p][1], pp[x + 1][p][0], pp[x + 1][p][1]}), o[dt], 0, 0, 0);
+          }
+        } else {
+#pragma unroll
+          for (int p = 2; p >= 0; p--) {
+            struct { uint32_t x, y; } pv{pp[0][p][0], pp[0][p][1]};
+            o[dt] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(vf[0], __builtin_bit_cast(ts4, pv), o[dt], 0, 0, 0);
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int x = 0; x < NT; x++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const char *vb = vt + (kgp * SK + 16 * x + 4 * kg + i) * ROWB + col * 16;
+#pragma unroll
+          for (int dt = 0; dt < HD / 64; dt++) {
+            const float4 v = *(const float4 *)(vb + dt * 256);
+            o[4 * dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(v.x, sc[x][i], o[4 * dt], 0, 0, 0);
+            o[4 * dt + 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(v.y, sc[x][i], o[4 * dt + 1], 0, 0, 0);
+            o[4 * dt + 2] = __builtin_amdgcn_mfma_f32_16x16x4f32(v.z, sc[x][i], o[4 * dt + 2], 0, 0, 0);
+            o[4 * dt + 3] = __builtin_amdgcn_mfma_f32_16x16x4f32(v.w, sc[x][i], o[4 * dt + 3], 0, 0, 0);
+          }
+        }
+    }
+    if (bad0 | bad1) {  // never in a healthy step
+#pragma unroll
+      for (int x = 0; x < NT; x++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          for (int k = 0; k < 4; k++) {
+            const int r = kgp * SK + 16 * x + 4 * k + i;
+            if (!((r < 32 ? bad0 >> r : bad1 >> (r - 32)) & 1) || base + r >= last) continue;
+            const float p = __shfl(sc[x][i], k * 16 + col, 64);
+            if (p == 0.0f) continue;
+            const char *src = vd + (long)(base + r) * seq_row;
+#pragma unroll
+            for (int d = 0; d < HD / 16; d++)
+#pragma unroll
+              for (int e = 0; e < 4; e++) {
+                const int at = B16 ? 16 * d + 4 * kg + e : 64 * (d >> 2) + 16 * kg + 4 * e + (d & 3);
+                const float v = tree_ld(src, at, B16);
+                if (!(fabsf(v) < INFINITY)) o[d][e] += p * v;
+              }
+          }
+    }
+  }
+
+  // the column's four lanes hold parts of the row's sum
+  l = tree_xor_sum(l);
+  const bool direct = np == 1;
+  float *po = a.part + ((long)(piece * a.B + b) * a.K + kv) * a.rows_max * HD;
+  float2 *pm = a.part_ml + ((long)(piece * a.B + b) * a.K + kv) * a.rows_max;
+  // entry e of value tile d is entry at(d, e) of the head
+  if constexpr (KW > 1) {
+    // join the key groups in LDS: every group's O and l scaled to the row's largest maximum
+    constexpr int ST = HD + 4;
+    if (kg == 0) {
+      ml[w][0][col] = m;
+      ml[w][1][col] = l;
+    }
+    lds_barrier();
+    float M = -INFINITY;
+    for (int k = 0; k < KW; k++) M = fmaxf(M, ml[k * RW + rg][0][col]);
+    const float Ms = M == -INFINITY ? 0.0f : M;
+    float lt = 0.0f;
+    for (int k = 0; k < KW; k++) lt += ml[k * RW + rg][1][col] * __builtin_amdgcn_exp2f(ml[k * RW + rg][0][col] - Ms);
+    const float f = __builtin_amdgcn_exp2f(m - Ms);
+    float *oj = (float *)smem;
+#pragma unroll
+    for (int d = 0; d < HD / 16; d++) {
+      if constexpr (B16) {
+        *(float4 *)(oj + (w * 16 + col) * ST + 16 * d + 4 * kg) = make_float4(o[d][0] * f, o[d][1] * f, o[d][2] * f, o[d][3] * f);
+      } else {
+        *(float4 *)(oj + (w * 16 + col) * ST + 64 * (d >> 2) + 16 * kg + 4 * (d & 3)) =
+            make_float4(o[d & ~3][d & 3] * f, o[(d & ~3) + 1][d & 3] * f, o[(d & ~3) + 2][d & 3] * f, o[(d & ~3) + 3][d & 3] * f);
+      }
+    }
+    lds_barrier();
+    // the group's waves share its rows' entries
+    constexpr int Q4 = HD / 4;
+    for (int u = kgp * 64 + lane; u < 16 * Q4; u += 64 * KW) {
+      const int r = u / Q4, e = u - r * Q4, rr = row0 + rg * 16 + r;
+      if (rr >= rows) continue;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      float Mr = -INFINITY, lr = 0.0f;
+      for (int k = 0; k < KW; k++) {
+        const float4 x = *(const float4 *)(oj + ((k * RW + rg) * 16 + r) * ST + 4 * e);
+        v = make_float4(v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w);
+        Mr = fmaxf(Mr, ml[k * RW + rg][0][r]);
+      }
+      const float Mrs = Mr == -INFINITY ? 0.0f : Mr;
+      for (int k = 0; k < KW; k++) lr += ml[k * RW + rg][1][r] * __builtin_amdgcn_exp2f(ml[k * RW + rg][0][r] - Mrs);
+      if (direct) {
+        const int nodr = rr / R, hdr = kv * R + (rr - nodr * R);
+        tree_store(a, b, nodr, hdr, 4 * e, v, lr);
+      } else {
+        *(float4 *)(po + (long)rr * HD + 4 * e) = v;
+        if (e == 0) pm[rr] = make_float2(Mr, lr);
+      }
+    }
+    (void)lt;
+  } else {
+    if (row >= rows) return;
+#pragma unroll
+    for (int d = 0; d < HD / 16; d++) {
+      const int at = B16 ? 16 * d + 4 * kg : 64 * (d >> 2) + 16 * kg + 4 * (d & 3);
+      const float4 v = B16 ? make_float4(o[d][0], o[d][1], o[d][2], o[d][3])
+                           : make_float4(o[d & ~3][d & 3], o[(d & ~3) + 1][d & 3], o[(d & ~3) + 2][d & 3], o[(d & ~3) + 3][d & 3]);
+      if (direct)
+        tree_store(a, b, node, head, at, v, l);
+      else
+        *(float4 *)(po + (long)row * HD + at) = v;
+    }
+    if (!direct && kg == 0) pm[row] = make_float2(m, l);
+  }
+}
+
+// The pieces of a row joined, one wave per row: lane j takes entries 4 j .. 4 j + 3.
+__global__ __launch_bounds__(256) void k_tree_join(TreeArgs a, int TK) {
+  __shared__ float wt[4][256];
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const long r = (long)blockIdx.x * 4 + w;
+  const int h = (int)(r % a.H), i = (int)(r / a.H % a.T), b = (int)(r / a.H / a.T);
+  if (b >= a.B) return;
+  const int n = a.n_nodes[b], L = a.len[b];
+  if (n < 0 || n > a.T || L < 0 || L > a.cap || i >= n) return;
+  long per = a.per;
+  if (L > per * a.pieces) per = ((L + a.pieces - 1) / a.pieces + TK - 1) / TK * TK;
+  const int np = L > 0 ? (int)((L + per - 1) / per) : 1;
+  if (np == 1) return;
+  const int R = a.H / a.K, kv = h / R;
+  const long ps = (long)a.B * a.K * a.rows_max, at = ((long)b * a.K + kv) * a.rows_max + (long)i * R + (h - kv * R);
+  float M = -INFINITY;
+  for (int j = lane; j < np; j += 64) M = fmaxf(M, a.part_ml[j * ps + at].x);
+  M = rbt_wave_max_f(M);
+  const float Ms = M == -INFINITY ? 0.0f : M;
+  float l = 0.0f;
+  for (int j = lane; j < np; j += 64) {
+    const float2 x = a.part_ml[j * ps + at];
+    const float f = __builtin_amdgcn_exp2f(x.x - Ms);
+    wt[w][j] = f;
+    l += x.y * f;
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d, 64);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+  if (4 * lane >= a.hd) return;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  const float *po = a.part + at * a.hd + 4 * lane;
+#pragma unroll 8
+  for (int j = 0; j < np; j++) {
+    const float4 x = *(const float4 *)(po + j * ps * a.hd);
+    const float f = wt[w][j];
+    v = make_float4(v.x + x.x * f, v.y + x.y * f, v.z + x.z * f, v.w + x.w * f);
+  }
+  tree_store(a, b, i, h, 4 * lane, v, l);
+}
+
+// Pieces and row tiles for a call on the matrix cores.
+bool tree_plan(const Ctx &c, TreeArgs &a, int &rw, int &kw) {
+  a.tiled = a.hd == 64 || a.hd == 128 || a.hd == 192 || a.hd == 256;
+  if (!a.tiled) return false;
+  const int R = a.H / a.K, t16 = (a.T * R + 15) / 16;
+  const int TK = a.kv16 ? 64 : 32;
+  a.rows_max = (long)a.T * R;
+  if (t16 <= 2) {
+    rw = t16;
+    kw = a.kv16 ? 4 / rw : 2;
+  } else {
+    kw = 1;
+    a.tiles = (t16 + 7) / 8;
+    rw = (t16 + a.tiles - 1) / a.tiles;
+  }
+  a.tiles = (t16 + rw - 1) / rw;
+  const long base = (long)a.tiles * a.K * a.B, want = 2L * c.num_cu;
+  long pieces = std::max(1L, std::min(want / base, (a.max_len + TK - 1) / TK));
+  pieces = std::min(pieces, 256L);
+  a.per = ((a.max_len + pieces - 1) / pieces + TK - 1) / TK * TK;
+  a.pieces = (int)((a.max_len + a.per - 1) / a.per);
+  return true;
+}
+
+size_t tree_part_floats(const TreeArgs &a) {
+  return a.pieces > 1 ? (size_t)a.pieces * a.B * a.K * a.rows_max * (a.hd + 2) : 0;
+}
+
+template <int HD, bool B16, int KW>
+static hipError_t run_tree(const Ctx &c, const TreeArgs &a, int rw) {
+  constexpr int lds = TreeTile<HD, B16>::LDS;
+  static_assert(4 * 16 * (HD + 4) * 4 <= lds || KW == 1, "the key groups' join fits the stages' LDS");
+  const long groups = (long)a.pieces * a.K * a.B;
+  const long blocks = (groups + 7) / 8 * 8 * a.tiles;
+  if (blocks > INT32_MAX) return hipErrorInvalidValue;
+  launch_ks(c, k_tree<HD, B16, KW>, dim3((unsigned)blocks), dim3(64 * rw * KW), (unsigned)lds, a);
+  return hipGetLastError();
+}
+
+template <int HD>
+static hipError_t run_tree_hd(const Ctx &c, const TreeArgs &a, int rw, int kw) {
+  if (a.kv16)
+    return kw == 4 ? run_tree<HD, true, 4>(c, a, rw) : kw == 2 ? run_tree<HD, true, 2>(c, a, rw) : run_tree<HD, true, 1>(c, a, rw);
+  return kw == 2 ? run_tree<HD, false, 2>(c, a, rw) : run_tree<HD, false, 1>(c, a, rw);
+}
+
+hipError_t launch_tree(const Ctx &c, const TreeArgs &a, int rw, int kw) {
+  if (!a.tiled) {
+    launch_k(c, k_tree_any, dim3(a.H, a.T, a.B), dim3(256), a);
+    return hipGetLastError();
+  }
+  hipError_t e = a.hd == 64 ? run_tree_hd<64>(c, a, rw, kw) : a.hd == 128 ? run_tree_hd<128>(c, a, rw, kw)
+                 : a.hd == 192 ? run_tree_hd<192>(c, a, rw, kw) : run_tree_hd<256>(c, a, rw, kw);
+  if (e != hipSuccess || a.pieces == 1) return e;
+  const long rows = (long)a.B * a.T * a.H;
+  if ((rows + 3) / 4 > INT32_MAX) return hipErrorInvalidValue;
+  launch_k(c, k_tree_join, dim3((unsigned)((rows + 3) / 4)), dim3(256), a, a.kv16 ? 64 : 32);
   return hipGetLastError();
 }
 
