@@ -2261,6 +2261,7 @@ int rbt_rope_d(rbt_ctx *c, const rbt_rope_desc *d, const rbt_rope_part *parts, s
     o.dhs = (long)p.dst_head_stride;
     o.norm = p.norm;
     o.row0 = (int)rows;
+    o.heads = (int)p.n_heads;
     o.s16 = p.src_dtype == RBT_DT_BF16;
     o.d16 = p.dst_dtype == RBT_DT_BF16;
     o.rotate = p.rotate != 0 && d->rope_dim > 0;

@@ -428,7 +428,7 @@ struct RopePartD {
   void *dst;
   long sts, shs, dts, dhs;  // token and head strides in entries
   const float *norm;
-  int row0;                 // the part's first row among a token's rows
+  int row0, heads;          // the part's first row among a token's rows, its rows
   int s16, d16, rotate;     // bf16 source, bf16 destination
 };
 struct RopeArgs {
