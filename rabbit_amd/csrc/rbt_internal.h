@@ -470,7 +470,9 @@ struct TreeArgs {
   int *bad;
   // tree_plan: whether the matrix cores take it, row tiles, pieces of the cache (keys per piece), scratch
   int tiled, tiles, pieces;
-  long per, rows_max;
+  unsigned per, magic;
+  int R;  // query heads per KV head
+  long rows_max;
   float *part;
   float2 *part_ml;
 };

@@ -161,6 +161,21 @@ struct TreeTile {
   static_assert(TK * CH % 64 == 0 && CH % 8 == 0, "whole loads");
 };
 
+// A row's node, row / n_rep: magic = ceil(2^32 / n_rep), exact since row * n_rep < 2^32 (at most 2^20 rows, 2^12 heads).
+__device__ __forceinline__ int tree_div(int row, const TreeArgs &a) { return a.R == 1 ? row : (int)__umulhi(row, a.magic); }
+
+// Keys of a piece and pieces of a sequence of L committed rows; one longer than expected takes larger pieces.
+__device__ __forceinline__ void tree_pieces(const TreeArgs &a, int L, int TK, unsigned &per, unsigned &np) {
+  per = a.per;
+  np = 1;
+  if (a.pieces == 1 && L > 0) {
+    per = L;
+  } else if (L > 0) {
+    if ((unsigned)L > (unsigned long long)per * a.pieces) per = (((unsigned)L + a.pieces - 1) / a.pieces + TK - 1) / TK * TK;
+    np = ((unsigned)L + per - 1) / per;
+  }
+}
+
 template <int HD, bool B16, int KW>
 __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(TreeArgs a) {
   using TT = TreeTile<HD, B16>;
@@ -171,49 +186,65 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
   __shared__ uint32_t dirty[2][2];              // per stage buffer: drafted rows with non-finite values
   __shared__ float ml[KW > 1 ? 4 : 1][2][16];
 
-  // workgroup -> (row tile, piece, KV head, sequence): consecutive workgroups of an XCD (id % 8) share the keys
-  const int id = blockIdx.x, g = (id / 8 / a.tiles) * 8 + id % 8, rt = id / 8 % a.tiles;
-  if (g >= a.pieces * a.K * a.B) return;
-  const int piece = g / (a.K * a.B), kv = g % a.K, b = g / a.K % a.B;
+  // workgroup -> (row tile, piece, KV head, sequence); with several row tiles the workgroups that share keys are
+  // consecutive ones of an XCD (id % 8)
+  int piece = blockIdx.x, rt = 0, kv = blockIdx.y, b = blockIdx.z;
+  if (a.tiles > 1) {
+    const unsigned id = blockIdx.x, g = id / 8 / a.tiles * 8 + id % 8, KB = a.K * a.B;
+    if (g >= a.pieces * KB) return;
+    rt = id / 8 % a.tiles;
+    piece = g / KB;
+    const unsigned r = g - piece * KB;
+    b = r / a.K;
+    kv = r - b * a.K;
+  }
   int n, L;
   if (!tree_fits(a, b, n, L)) return;
-  const int R = a.H / a.K, rows = n * R;
+  const int R = a.R, rows = n * R;
   const int NW = blockDim.x >> 6, RW = NW / KW;
   const int row0 = rt * RW * 16;
   if (row0 >= rows) return;
-  long per = a.per;  // keys of a piece: a sequence longer than expected takes larger ones
-  if (L > per * a.pieces) per = ((L + a.pieces - 1) / a.pieces + TK - 1) / TK * TK;
-  const int np = L > 0 ? (int)((L + per - 1) / per) : 1;
-  if (piece >= np) return;
-  const int k0 = (int)(piece * per), k1 = (int)min((long)L, k0 + per);
+  unsigned per, np;
+  tree_pieces(a, L, TK, per, np);
+  if (piece >= (int)np) return;
+  const int k0 = piece * per, nc = min(L - k0, (int)per);  // cache rows k0 .. k0 + nc - 1, then drafted rows
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int rg = w % RW, kgp = w / RW, col = lane & 15, kg = lane >> 4;
-  const int node_lo = row0 / R, node_hi = (min(rows, row0 + RW * 16) - 1) / R;
-  const int nd = piece == np - 1 ? node_hi + 1 : 0;  // drafted rows: those up to the last node of the tile
-  const int st_c = (k1 - k0 + TK - 1) / TK, st_n = st_c + (nd + TK - 1) / TK;
+  const int node_lo = tree_div(row0, a), node_hi = tree_div(min(rows, row0 + RW * 16) - 1, a);
+  const int nd = piece == (int)np - 1 ? node_hi + 1 : 0;  // drafted rows: those up to the last node of the tile
+  const int keys = nc + nd, st_n = (keys + TK - 1) / TK;
 
-  const long seq_row = (long)a.K * HD * TT::ES;  // bytes from a row to the next
-  const char *kc = (const char *)a.kc + ((long)b * a.cap * a.K + kv) * ROWB, *vc = (const char *)a.vc + ((long)b * a.cap * a.K + kv) * ROWB;
-  const char *kd = (const char *)a.kd + ((long)b * a.T * a.K + kv) * ROWB, *vd = (const char *)a.vd + ((long)b * a.T * a.K + kv) * ROWB;
+  const long seq_row = (long)a.K * ROWB;  // bytes from a row to the next
+  const long off_c = (((long)b * a.cap + k0) * a.K + kv) * ROWB, off_d = ((long)b * a.T * a.K + kv) * ROWB;
+  const char *kc = (const char *)a.kc + off_c, *vc = (const char *)a.vc + off_c;
+  const char *kd = (const char *)a.kd + off_d, *vd = (const char *)a.vd + off_d;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)smem;
 
+  // keys s TK .. of the piece into buffer s & 1; rows past the last one repeat it
   auto issue = [&](int s) {
-    const bool dr = s >= st_c;
-    const char *kp = dr ? kd : kc, *vp = dr ? vd : vc;
-    const int base = dr ? (s - st_c) * TK : k0 + s * TK, last = (dr ? nd : k1) - 1;
+    const int base = s * TK;
     const uint32_t to = lds0 + (s & 1) * TT::STAGE;
-    for (int i = w; i < TT::INSTR; i += NW) {
-      const int u = i * 64 + lane, r = u / CH, c = u - r * CH;
-      const long at = (long)min(base + r, last) * seq_row;
-      tree_dma(kp + at + (c ^ (r & 7)) * 16, to + i * 1024);
-      tree_dma(vp + at + (B16 ? c ^ ((r & 3) << 1) : c) * 16, to + TT::SIDE + i * 1024);
+    if (base + TK <= nc) {
+      for (int i = w; i < TT::INSTR; i += NW) {
+        const int u = i * 64 + lane, r = u / CH, c = u - r * CH;
+        const long at = (long)(base + r) * seq_row;
+        tree_dma(kc + at + (c ^ (r & 7)) * 16, to + i * 1024);
+        tree_dma(vc + at + (B16 ? c ^ ((r & 3) << 1) : c) * 16, to + TT::SIDE + i * 1024);
+      }
+    } else {
+      for (int i = w; i < TT::INSTR; i += NW) {
+        const int u = i * 64 + lane, r = u / CH, c = u - r * CH, j = min(base + r, keys - 1);
+        const long at = (long)(j < nc ? j : j - nc) * seq_row;
+        tree_dma((j < nc ? kc : kd) + at + (c ^ (r & 7)) * 16, to + i * 1024);
+        tree_dma((j < nc ? vc : vd) + at + (B16 ? c ^ ((r & 3) << 1) : c) * 16, to + TT::SIDE + i * 1024);
+      }
     }
   };
   issue(0);
 
   // this lane's row, and its query in the B operand's layout
   const int row = row0 + rg * 16 + col, rc = min(row, rows - 1);
-  const int node = rc / R, head = kv * R + (rc - node * R);
+  const int node = tree_div(rc, a), head = kv * R + (rc - node * R);
   const long qrow = ((long)b * a.T + node) * a.H + head;
   const float *qp = a.q + qrow * HD;
   tb8 qb[B16 ? HD / 32 : 1][3];
@@ -263,14 +294,13 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     lds_barrier();  // the stage has landed, and the other buffer's readers are done
     if (s + 1 < st_n) issue(s + 1);
-    const bool dr = s >= st_c;
     char *kt = smem + (s & 1) * TT::STAGE, *vt = kt + TT::SIDE;
     uint32_t bad0 = 0, bad1 = 0;
-    const int base = dr ? (s - st_c) * TK : k0 + s * TK, last = dr ? nd : k1;
-    if (dr) {
+    const int base = s * TK;
+    if (nd > 1 && base + TK > nc) {
       // a value that some rows do not see must not meet their zero probabilities: non-finite ones are taken
-      // out of the tile and added below for the rows that do see them
-      for (int u = t; u < TK * CH; u += blockDim.x) {
+      // out of the tile (its repeated last row too) and added below for the rows that do see them
+      for (int u = t + max(nc - base, 0) * CH; u < TK * CH; u += blockDim.x) {
         const int r = u / CH;
         uint32_t *x = (uint32_t *)(vt + u * 16);
         bool hit = false;
@@ -328,15 +358,14 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
       }
     }
     float mt = -INFINITY;
-    const int kfirst = base + kgp * SK + 4 * kg;
-    if (dr || base + TK > last) {
+    if (base + TK > nc) {
+      const int kfirst = base + kgp * SK + 4 * kg - nc;  // drafted row of the lane's first key, below 0 in the cache
 #pragma unroll
       for (int x = 0; x < NT; x++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           const int j = kfirst + 16 * x + i;
-          bool see = j < last;
-          if (dr) see = see && (vis[node - node_lo][min(j, TREE_MAX - 1) >> 5] >> (j & 31) & 1);
+          const bool see = j < 0 || (j < nd && (vis[node - node_lo][min(j, TREE_MAX - 1) >> 5] >> (j & 31) & 1));
           sc[x][i] = see ? sc[x][i] * c1 : -INFINITY;
         }
     } else {
@@ -428,10 +457,10 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
         for (int i = 0; i < 4; i++)
           for (int k = 0; k < 4; k++) {
             const int r = kgp * SK + 16 * x + 4 * k + i;
-            if (!((r < 32 ? bad0 >> r : bad1 >> (r - 32)) & 1) || base + r >= last) continue;
+            if (!((r < 32 ? bad0 >> r : bad1 >> (r - 32)) & 1) || base + r >= keys) continue;
             const float p = __shfl(sc[x][i], k * 16 + col, 64);
             if (p == 0.0f) continue;
-            const char *src = vd + (long)(base + r) * seq_row;
+            const char *src = vd + (long)(base + r - nc) * seq_row;
 #pragma unroll
             for (int d = 0; d < HD / 16; d++)
 #pragma unroll
@@ -490,7 +519,7 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
       const float Mrs = Mr == -INFINITY ? 0.0f : Mr;
       for (int k = 0; k < KW; k++) lr += ml[k * RW + rg][1][r] * __builtin_amdgcn_exp2f(ml[k * RW + rg][0][r] - Mrs);
       if (direct) {
-        const int nodr = rr / R, hdr = kv * R + (rr - nodr * R);
+        const int nodr = tree_div(rr, a), hdr = kv * R + (rr - nodr * R);
         tree_store(a, b, nodr, hdr, 4 * e, v, lr);
       } else {
         *(float4 *)(po + (long)rr * HD + 4 * e) = v;
@@ -514,45 +543,74 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
   }
 }
 
-// The pieces of a row joined, one wave per row: lane j takes entries 4 j .. 4 j + 3.
+// The pieces of a row joined by WR waves, a row's lane j taking entries 4 j .. 4 j + 3; each wave's pieces are summed in
+// order, then the waves' sums.
+template <int WR>
 __global__ __launch_bounds__(256) void k_tree_join(TreeArgs a, int TK) {
-  __shared__ float wt[4][256];
-  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const long r = (long)blockIdx.x * 4 + w;
-  const int h = (int)(r % a.H), i = (int)(r / a.H % a.T), b = (int)(r / a.H / a.T);
-  if (b >= a.B) return;
-  const int n = a.n_nodes[b], L = a.len[b];
-  if (n < 0 || n > a.T || L < 0 || L > a.cap || i >= n) return;
-  long per = a.per;
-  if (L > per * a.pieces) per = ((L + a.pieces - 1) / a.pieces + TK - 1) / TK * TK;
-  const int np = L > 0 ? (int)((L + per - 1) / per) : 1;
-  if (np == 1) return;
-  const int R = a.H / a.K, kv = h / R;
-  const long ps = (long)a.B * a.K * a.rows_max, at = ((long)b * a.K + kv) * a.rows_max + (long)i * R + (h - kv * R);
+  __shared__ __attribute__((aligned(16))) float wt[4][256], sum[WR > 1 ? 4 : 1][256];
+  __shared__ float red[2][4];
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, wr = w % WR, tr = wr * 64 + lane;
+  // (rows of the kernels' tiling: row = node * n_rep + head of the group)
+  const int row = blockIdx.x * (4 / WR) + w / WR, kv = blockIdx.y, b = blockIdx.z;
+  const int n = a.n_nodes[b], L = a.len[b], i = tree_div(row, a);
+  const bool live = n >= 0 && n <= a.T && L >= 0 && L <= a.cap && i < n;
+  if (WR > 1 && !live) return;  // (the workgroup's only row)
+  unsigned per, np = 0;
+  if (live) tree_pieces(a, L, TK, per, np);
+  if (np <= 1) return;
+  const long ps = (long)a.B * a.K * a.rows_max, at = ((long)b * a.K + kv) * a.rows_max + row;
   float M = -INFINITY;
-  for (int j = lane; j < np; j += 64) M = fmaxf(M, a.part_ml[j * ps + at].x);
+  float2 x[4 / WR];
+#pragma unroll
+  for (int k = 0; k < 4 / WR; k++) {
+    const unsigned j = tr + 64 * WR * k;
+    x[k] = j < np ? a.part_ml[j * ps + at] : make_float2(-INFINITY, 0.0f);
+    M = fmaxf(M, x[k].x);
+  }
   M = rbt_wave_max_f(M);
+  if constexpr (WR > 1) {
+    if (lane == 0) red[0][w] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  }
   const float Ms = M == -INFINITY ? 0.0f : M;
   float l = 0.0f;
-  for (int j = lane; j < np; j += 64) {
-    const float2 x = a.part_ml[j * ps + at];
-    const float f = __builtin_amdgcn_exp2f(x.x - Ms);
-    wt[w][j] = f;
-    l += x.y * f;
+#pragma unroll
+  for (int k = 0; k < 4 / WR; k++) {
+    const float f = __builtin_amdgcn_exp2f(x[k].x - Ms);
+    wt[WR > 1 ? 0 : w][tr + 64 * WR * k] = f;
+    l += x[k].y * f;
   }
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d, 64);
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
-  if (4 * lane >= a.hd) return;
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  const float *po = a.part + at * a.hd + 4 * lane;
-#pragma unroll 8
-  for (int j = 0; j < np; j++) {
-    const float4 x = *(const float4 *)(po + j * ps * a.hd);
-    const float f = wt[w][j];
-    v = make_float4(v.x + x.x * f, v.y + x.y * f, v.z + x.z * f, v.w + x.w * f);
+  if constexpr (WR > 1) {
+    if (lane == 0) red[1][w] = l;
+    __syncthreads();
+    l = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+  } else {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
   }
-  tree_store(a, b, i, h, 4 * lane, v, l);
+  const bool mine = 4 * lane < a.hd;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  const float *po = a.part + at * a.hd + 4 * (mine ? lane : 0);
+  const float *wp = wt[WR > 1 ? 0 : w];
+#pragma unroll 8
+  for (unsigned j = wr; j < np; j += WR) {
+    const float4 y = *(const float4 *)(po + j * ps * a.hd);
+    const float f = wp[j];
+    v = make_float4(v.x + y.x * f, v.y + y.y * f, v.z + y.z * f, v.w + y.w * f);
+  }
+  if constexpr (WR > 1) {
+    *(float4 *)(sum[w] + 4 * lane) = v;
+    __syncthreads();
+    if (w) return;
+#pragma unroll
+    for (int k = 1; k < 4; k++) {
+      const float4 y = *(const float4 *)(sum[k] + 4 * lane);
+      v = make_float4(v.x + y.x, v.y + y.y, v.z + y.z, v.w + y.w);
+    }
+  }
+  if (mine) tree_store(a, b, i, kv * a.R + (row - i * a.R), 4 * lane, v, l);
 }
 
 // Pieces and row tiles for a call on the matrix cores.
@@ -562,6 +620,8 @@ bool tree_plan(const Ctx &c, TreeArgs &a, int &rw, int &kw) {
   const int R = a.H / a.K, t16 = (a.T * R + 15) / 16;
   const int TK = a.kv16 ? 64 : 32;
   a.rows_max = (long)a.T * R;
+  a.R = R;
+  a.magic = R == 1 ? 0 : (unsigned)((0x100000000ull + R - 1) / R);
   if (t16 <= 2) {
     rw = t16;
     kw = a.kv16 ? 4 / rw : 2;
@@ -574,7 +634,7 @@ bool tree_plan(const Ctx &c, TreeArgs &a, int &rw, int &kw) {
   const long base = (long)a.tiles * a.K * a.B, want = 2L * c.num_cu;
   long pieces = std::max(1L, std::min(want / base, (a.max_len + TK - 1) / TK));
   pieces = std::min(pieces, 256L);
-  a.per = ((a.max_len + pieces - 1) / pieces + TK - 1) / TK * TK;
+  a.per = (unsigned)(((a.max_len + pieces - 1) / pieces + TK - 1) / TK * TK);
   a.pieces = (int)((a.max_len + a.per - 1) / a.per);
   return true;
 }
@@ -590,7 +650,8 @@ static hipError_t run_tree(const Ctx &c, const TreeArgs &a, int rw) {
   const long groups = (long)a.pieces * a.K * a.B;
   const long blocks = (groups + 7) / 8 * 8 * a.tiles;
   if (blocks > INT32_MAX) return hipErrorInvalidValue;
-  launch_ks(c, k_tree<HD, B16, KW>, dim3((unsigned)blocks), dim3(64 * rw * KW), (unsigned)lds, a);
+  const dim3 grid = a.tiles > 1 ? dim3((unsigned)blocks) : dim3(a.pieces, a.K, a.B);
+  launch_ks(c, k_tree<HD, B16, KW>, grid, dim3(64 * rw * KW), (unsigned)lds, a);
   return hipGetLastError();
 }
 
@@ -609,9 +670,11 @@ hipError_t launch_tree(const Ctx &c, const TreeArgs &a, int rw, int kw) {
   hipError_t e = a.hd == 64 ? run_tree_hd<64>(c, a, rw, kw) : a.hd == 128 ? run_tree_hd<128>(c, a, rw, kw)
                  : a.hd == 192 ? run_tree_hd<192>(c, a, rw, kw) : run_tree_hd<256>(c, a, rw, kw);
   if (e != hipSuccess || a.pieces == 1) return e;
-  const long rows = (long)a.B * a.T * a.H;
-  if ((rows + 3) / 4 > INT32_MAX) return hipErrorInvalidValue;
-  launch_k(c, k_tree_join, dim3((unsigned)((rows + 3) / 4)), dim3(256), a, a.kv16 ? 64 : 32);
+  const unsigned rows = (unsigned)a.rows_max, TK = a.kv16 ? 64 : 32;
+  if (a.pieces > 4)
+    launch_k(c, k_tree_join<4>, dim3(rows, a.K, a.B), dim3(256), a, (int)TK);
+  else
+    launch_k(c, k_tree_join<1>, dim3((rows + 3) / 4, a.K, a.B), dim3(256), a, (int)TK);
   return hipGetLastError();
 }
 
