@@ -5,6 +5,8 @@
 #include "rbt_device.h"
 #include "rbt_internal.h"
 
+#include <cmath>
+
 namespace rbt {
 
 __device__ __forceinline__ float tree_ld(const void *p, long i, int b16) {
@@ -243,6 +245,7 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
   issue(0);
 
   // this lane's row, and its query in the B operand's layout
+  const bool active = row0 + rg * 16 < rows;  // a wave without rows only loads
   const int row = row0 + rg * 16 + col, rc = min(row, rows - 1);
   const int node = tree_div(rc, a), head = kv * R + (rc - node * R);
   const long qrow = ((long)b * a.T + node) * a.H + head;
@@ -322,6 +325,8 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
       bad1 = dirty[s & 1][1];
       if (t < 2) dirty[(s & 1) ^ 1][t] = 0;
     }
+
+    if (!active) continue;
 
     // scores: lane (col, kg) gets keys 16 x + 4 kg + i of its row
     tf4 sc[NT];
@@ -631,11 +636,30 @@ bool tree_plan(const Ctx &c, TreeArgs &a, int &rw, int &kw) {
     rw = (t16 + a.tiles - 1) / a.tiles;
   }
   a.tiles = (t16 + rw - 1) / rw;
-  const long base = (long)a.tiles * a.K * a.B, want = 2L * c.num_cu;
-  long pieces = std::max(1L, std::min(want / base, (a.max_len + TK - 1) / TK));
-  pieces = std::min(pieces, 256L);
-  a.per = (unsigned)(((a.max_len + pieces - 1) / pieces + TK - 1) / TK * TK);
-  a.pieces = (int)((a.max_len + a.per - 1) / a.per);
+  // Pieces by the time they should take, in microseconds: a workgroup (one per CU: its stages fill the LDS) starts
+  // and ends in 7, takes `stage` per stage (measured at head_dim 256; it goes with the head dim), and several pieces
+  // cost a second launch and a write and read of their rows' partial sums. Equal sequences end together, so their
+  // workgroups count by whole rounds of the chip; those of a batch are of any length: past one round they fill it
+  // evenly, at about 0.8 of the longest each, and the last ones are waited for. Measured over bf16 and head_dim 256: one node over 4096 rows 113 us in one piece,
+  // 27 in 8, 17 in 32, 17 in 64; 64 nodes over 32749 rows 527 in 4, 311 in 8, 326 in 16, 368 in 32.
+  const double base = (double)a.tiles * a.K * a.B, most = std::ceil((double)(a.max_len + a.T) / TK), ncu = c.num_cu;
+  const double stage = (kw > 1 ? (a.kv16 ? 1.6 : 2.6) : a.kv16 ? (rw > 4 ? 4.4 : 2.6) : (rw > 4 ? 8.5 : 4.5)) * a.hd / 256.0;
+  const double bytes = (double)a.B * a.K * a.rows_max * a.hd * 8.0;
+  double best = 0.0;
+  long pieces = 1;
+  auto consider = [&](long p) {
+    if (p < 1 || p > 256 || (p > 1 && p > most)) return;
+    const double one = 7.0 + stage * std::ceil(most / p);
+    const double rounds = base * p / ncu;
+    const double t = (rounds <= 1.0 ? one : a.B == 1 ? std::ceil(rounds) * one : (0.8 * rounds + 0.4) * one) +
+                     (p > 1 ? 4.0 + bytes * p / 1.2e7 : 0.0);
+    if (best == 0.0 || t < best) best = t, pieces = p;
+  };
+  consider(1);
+  for (long p = 2; p <= 256; p += p < 16 ? 1 : p / 8) consider(p);
+  for (int k = 1; k <= 4; k++) consider((long)(k * ncu / base));
+  a.per = (unsigned)((long)((most + pieces - 1) / pieces) * TK);
+  a.pieces = (int)std::max(1L, (a.max_len + a.per - 1) / (long)a.per);
   return true;
 }
 
