@@ -2369,8 +2369,22 @@ int rbt_draft_verify_d(rbt_ctx *c, size_t n_seq, size_t max_nodes, size_t vocab,
   if (!c) return refuse(c, RBT_E_INVALID, "null context");
   if (n_seq == 0) return RBT_OK;
   DeviceScope dev(c->device);
-  HIP_OK(c, rbt::launch_verify(*c, tokens, parent, n_nodes, p, q, u, (int)n_seq, (int)max_nodes, (int)vocab, path, n_path,
-                               next, c->d_flags + FLAG_TREE));
+  rbt::VerifyArgs a{};
+  a.tokens = tokens;
+  a.parent = parent;
+  a.n_nodes = n_nodes;
+  a.p = p;
+  a.q = q;
+  a.u = u;
+  a.T = (int)max_nodes;
+  a.V = (int)vocab;
+  a.path = path;
+  a.n_path = n_path;
+  a.next = next;
+  a.bad = c->d_flags + FLAG_TREE;
+  void *work;
+  RBT_TRY(scratch(c, SC_MIXA, rbt::verify_scratch((int)n_seq), &work));
+  HIP_OK(c, rbt::launch_verify(*c, a, (int)n_seq, (int)std::min<size_t>(max_children, 256), work));
   return RBT_OK;
 }
 

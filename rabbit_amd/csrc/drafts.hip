@@ -264,198 +264,351 @@ hipError_t launch_tree_pos(const Ctx &c, const int *parent, const int *n_nodes, 
 }
 
 // ---- verification --------------------------------------------------------------------------------
-// One workgroup per sequence. The walk needs p and q of each node's token under the node's parent, gathered
-// once; a rejected child needs the mass of the residual, one pass over the vocabulary.
-constexpr int VF_NT = 1024, VF_W = VF_NT / 64;
+// The walk reads p and q of every node's token under the node's parent, gathered once, and takes a step per test;
+// only a rejected child (given q) and the draw need a pass over the vocabulary. A launch holds G workgroups per
+// sequence: each takes the walk to its first pass by itself (the same numbers in the same order: the same walk),
+// sums its chunk of the residual, and the last one to arrive goes on: it adds the chunks in order, continues the
+// walk, and either draws from the chunks at hand or leaves the state for the next launch's pass. In the last
+// launch it makes whatever passes are left by itself. No workgroup waits for another.
+// Chains, and drafts without q, need one pass and so one launch. Sums are in 64 bits, and as their order is fixed
+// the drawn token is too. Bound by trips to memory that follow one another (count, tokens, their p and q, the
+// pass, the arrival, the sums, the draw), not by bytes: a chain of five over 32000 entries takes 12.7 us, one over
+// 131072 entries 13, sixteen of them 21; sixteen trees of 32 nodes 80 in six launches, of which most end at once (one
+// workgroup per sequence for all of it: 26 and, for the trees, 191).
+constexpr int VF_NT = 256, VF_G = 64, VF_ROUNDS = 6;  // threads per workgroup, chunks and launches at most
 
 struct VerifyRow {
   const float *p, *q;  // the current node's rows (q may be null)
   double c;
   const int *gone;  // without q: tokens that count as 0
   int n_gone;
-  __device__ double at(int i) const {
-    double r = (double)p[i];
-    if (q) r = r - c * (double)q[i];
+  __device__ __forceinline__ double of(float pv, float qv, int i) const {
+    double r = (double)pv;
+    if (q) r = r - c * (double)qv;
     for (int k = 0; k < n_gone; k++)
       if (gone[k] == i) return 0.0;
     return r > 0.0 ? r : 0.0;
   }
+  __device__ __forceinline__ double at(int i) const { return of(p[i], q ? q[i] : 0.0f, i); }
 };
 
-// Sums of [lo, hi) in VF_W contiguous segments (seg entries each) into sums; every thread returns the whole.
-__device__ double vf_sums(const VerifyRow &row, int lo, int hi, int seg, double *sums) {
-  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int s0 = lo + w * seg, s1 = min(hi, s0 + seg);
+// The workgroup's sum of [lo, hi), in every thread; quads: rows and lo are aligned to 16 bytes.
+__device__ double vf_sum(const VerifyRow &row, int lo, int hi, bool quads, double *red) {
+  const int t = threadIdx.x, w = t >> 6, lane = t & 63;
   double acc = 0.0;
-  for (int i = s0 + lane; i < s1; i += 64) acc += row.at(i);
+  if (quads) {
+    constexpr int UN = 4;
+    const int he = lo + ((hi - lo) & ~3);
+    for (int i0 = lo + 4 * t; i0 < he; i0 += UN * 4 * VF_NT) {
+      float4 pv[UN], qv[UN];
+#pragma unroll
+      for (int k = 0; k < UN; k++) pv[k] = *(const float4 *)(row.p + min(i0 + k * 4 * VF_NT, he - 4));
+#pragma unroll
+      for (int k = 0; k < UN; k++)
+        qv[k] = row.q ? *(const float4 *)(row.q + min(i0 + k * 4 * VF_NT, he - 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < UN; k++) {
+        const int i = i0 + k * 4 * VF_NT;
+        if (i < he)
+          acc += (row.of(pv[k].x, qv[k].x, i) + row.of(pv[k].y, qv[k].y, i + 1)) +
+                 (row.of(pv[k].z, qv[k].z, i + 2) + row.of(pv[k].w, qv[k].w, i + 3));
+      }
+    }
+    lo = he;
+  }
+  constexpr int UN = 8;
+  for (int i0 = lo + t; i0 < hi; i0 += UN * VF_NT) {
+    float pv[UN], qv[UN];
+#pragma unroll
+    for (int k = 0; k < UN; k++) pv[k] = row.p[min(i0 + k * VF_NT, hi - 1)];
+#pragma unroll
+    for (int k = 0; k < UN; k++) qv[k] = row.q ? row.q[min(i0 + k * VF_NT, hi - 1)] : 0.0f;
+#pragma unroll
+    for (int k = 0; k < UN; k++)
+      if (i0 + k * VF_NT < hi) acc += row.of(pv[k], qv[k], i0 + k * VF_NT);
+  }
   acc = rbt_wave_sum_d(acc);
   __syncthreads();
-  if (lane == 0) sums[w] = acc;
+  if (lane == 0) red[w] = acc;
   __syncthreads();
-  double tot = 0.0;
-  for (int k = 0; k < VF_W; k++) tot += sums[k];
-  return tot;
+  return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-__global__ __launch_bounds__(VF_NT) void k_verify(const int *__restrict__ tokens, const int *__restrict__ parent,
-                                                  const int *__restrict__ n_nodes, const float *__restrict__ p,
-                                                  const float *__restrict__ q, const float *__restrict__ u, int T, int V,
-                                                  int *__restrict__ path, int *__restrict__ n_path,
-                                                  int *__restrict__ next, int *__restrict__ bad) {
+__device__ __forceinline__ void vf_put(double *p, double v) {
+  __hip_atomic_store((unsigned long long *)p, (unsigned long long)__double_as_longlong(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ double vf_get(double *p) {
+  return __longlong_as_double(
+      (long long)__hip_atomic_load((unsigned long long *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
+__global__ __launch_bounds__(VF_NT) void k_verify(VerifyArgs a, int round, int last_round) {
   __shared__ int par[TREE_MAX], tok[TREE_MAX], way[TREE_MAX], gone[TREE_MAX];
   __shared__ float px[TREE_MAX], qx[TREE_MAX], us[TREE_MAX];
-  __shared__ double sums[VF_W], st_c, st_s;
-  __shared__ int st_cur, st_i, st_need, st_np, st_gone, found;
-  const int b = blockIdx.x, t = threadIdx.x;
-  int n = n_nodes[b];
-  if (n < 0 || n > T) {
-    if (t == 0) *bad = 1;
+  __shared__ double red[4], sums[VF_G];
+  __shared__ VerifyState st;
+  __shared__ int n_gone, found, is_last;
+  const int b = blockIdx.y, ch = blockIdx.x, G = gridDim.x, t = threadIdx.x, lane = t & 63, V = a.V;
+  int n = a.n_nodes[b];
+  if (n < 0 || n > a.T) {
+    if (t == 0) *a.bad = 1;
     n = 0;
   }
-  const float *pb = p + (long)b * T * V, *qb = q ? q + (long)b * T * V : nullptr;
-  if (t < n) {
-    int pr = parent[(long)b * T + t], x = tokens[(long)b * T + t];
-    if (pr < -1 || pr >= t) {
-      *bad = 1;
-      pr = -1;
-    }
-    if (t > 0 && (x < 0 || x >= V)) {
-      *bad = 1;
-      x = -1;
-    }
-    par[t] = t == 0 ? -1 : pr;
-    tok[t] = x;
-    us[t] = u[(long)b * T + t];
-    const bool ok = t > 0 && pr >= 0 && x >= 0;
-    px[t] = ok ? pb[(long)pr * V + x] : 0.0f;
-    qx[t] = ok && qb ? qb[(long)pr * V + x] : ok ? 1.0f : 0.0f;
+  if (n == 0) {
+    if (ch || round) return;
+    for (int j = t; j < a.T; j += VF_NT) a.path[(long)b * a.T + j] = -1;
+    if (t == 0) a.n_path[b] = 0, a.next[b] = -1;
+    return;
   }
   if (t == 0) {
-    st_cur = 0;
-    st_c = 0.0;
-    st_s = 1.0;
-    st_i = 1;
-    st_np = n > 0;
-    st_gone = 0;
+    if (round)
+      st = a.state[b];
+    else
+      st = VerifyState{0.0, 1.0, 0, 0, 1, 1, 0};
+    n_gone = 0;
     way[0] = 0;
   }
   __syncthreads();
-  for (;;) {
-    if (t == 0) {
-      int i = st_i, cur = st_cur;
-      st_need = 0;
-      for (; i < n; i++) {
-        if (par[i] != cur) continue;
-        const double c = st_c, S = st_s;
+  if (st.done) return;
+  const int np0 = round ? st.np : 0;  // standing nodes that an earlier launch wrote
+  const float *pb = a.p + (long)b * a.T * V, *qb = a.q ? a.q + (long)b * a.T * V : nullptr;
+  auto tables = [&]() {
+    if (t < n) {
+      int pr = a.parent[(long)b * a.T + t], x = a.tokens[(long)b * a.T + t];
+      us[t] = a.u[(long)b * a.T + t];
+      if (pr < -1 || pr >= t) {
+        *a.bad = 1;
+        pr = -1;
+      }
+      if (t > 0 && (x < 0 || x >= V)) {
+        *a.bad = 1;
+        x = -1;
+      }
+      const bool ok = t > 0 && pr >= 0 && x >= 0;
+      par[t] = ok ? pr : -1;  // a node without a token of the vocabulary is nobody's child
+      tok[t] = x;
+      px[t] = ok ? pb[(long)pr * V + x] : 0.0f;
+      qx[t] = ok && qb ? qb[(long)pr * V + x] : 1.0f;
+    }
+    __syncthreads();
+  };
+  // wave 0: tests children until one is rejected (st.need = 1) or none is left (0)
+  auto walk = [&]() {
+    if (t < 64) {
+      int pk[TREE_MAX / 64], cur = st.cur, at = st.at, np = st.np, ng = n_gone, nd = 0;
+      double c = st.c, S = st.mass;
+#pragma unroll
+      for (int k = 0; k < TREE_MAX / 64; k++) pk[k] = lane + 64 * k < n ? par[lane + 64 * k] : -1;
+      for (;;) {
+        int i = -1;
+#pragma unroll
+        for (int k = TREE_MAX / 64 - 1; k >= 0; k--) {
+          const unsigned long long m = __ballot(pk[k] == cur && lane + 64 * k > at);
+          if (m) i = 64 * k + __ffsll((long long)m) - 1;
+        }
+        if (i < 0) break;
+        at = i;
+        const double q = (double)qx[i];
         double r = (double)px[i];
-        if (q) {
-          r = r - c * (double)qx[i];
+        if (qb) {
+          r = r - c * q;
         } else {
-          for (int k = 0; k < st_gone; k++)
+          for (int k = 0; k < ng; k++)
             if (gone[k] == tok[i]) r = 0.0;
         }
         r = r > 0.0 ? r : 0.0;
-        if ((double)us[i] * (S * (double)qx[i]) < r) {
+        if ((double)us[i] * (S * q) < r) {
           cur = i;
-          way[st_np++] = i;
-          st_c = 0.0;
-          st_s = 1.0;
-          st_gone = 0;
-        } else if (tok[i] < 0) {
-          // a token outside the vocabulary leaves the residual as it is
-        } else if (q) {
-          st_c = c + S;
-          st_need = 1;
-          i++;
+          if (lane == 0) way[np - np0] = i;
+          np++;
+          c = 0.0;
+          S = 1.0;
+          ng = 0;
+        } else if (qb) {
+          c = c + S;
+          nd = 1;
           break;
         } else {
-          st_s = S - r;
-          gone[st_gone++] = tok[i];
+          S = S - r;
+          if (lane == 0) gone[ng] = tok[i];
+          ng++;
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
         }
       }
-      st_i = i;
-      st_cur = cur;
+      if (lane == 0) {
+        st = VerifyState{c, S, cur, at, np, nd, 0};
+        n_gone = ng;
+      }
     }
     __syncthreads();
-    const int need = st_need;
-    if (!need) break;
-    const VerifyRow row{pb + (long)st_cur * V, qb + (long)st_cur * V, st_c, gone, 0};
-    const double S = vf_sums(row, 0, V, (V + VF_W - 1) / VF_W, sums);
-    __syncthreads();
-    if (t == 0) st_s = S;
-    __syncthreads();
+  };
+  if (!round) {
+    tables();
+    walk();
   }
-  const int np = st_np;
-  for (int j = t; j < T; j += VF_NT) path[(long)b * T + j] = j < np ? way[j] : -1;
-  if (t == 0) n_path[b] = np;
-  if (n == 0) {
-    if (t == 0) next[b] = -1;
-    return;
+  const bool quads = V % 4 == 0 && (((uintptr_t)a.p | (uintptr_t)a.q) & 15) == 0;
+  const int len = ((V + G - 1) / G + 3) & ~3, lo = min(V, ch * len), hi = min(V, lo + len);
+  auto row_of = [&]() {
+    return VerifyRow{pb + (long)st.cur * V, st.c > 0.0 ? qb + (long)st.cur * V : nullptr, st.c, gone, n_gone};
+  };
+  VerifyRow row = row_of();
+  double s = lo < hi ? vf_sum(row, lo, hi, quads, red) : 0.0;
+  if (t == 0) {
+    is_last = 1;
+    if (G > 1) {
+      vf_put(a.part + b * VF_G + ch, s);
+      __builtin_amdgcn_s_waitcnt(0);  // the sum is at the device's coherence point before its announcement
+      const unsigned old = __hip_atomic_fetch_add(a.cnt + b, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      is_last = old + 1 == (unsigned)G;
+      if (is_last) __hip_atomic_store(a.cnt + b, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    } else {
+      sums[0] = s;
+    }
   }
-  // the draw: the segment, then the entry, where the running sum passes u times the whole
-  const int cur = st_cur;
-  VerifyRow row{pb + (long)cur * V, qb && st_c > 0.0 ? qb + (long)cur * V : nullptr, st_c, gone, st_gone};
-  int lo = 0, hi = V, seg = (V + VF_W - 1) / VF_W;
-  double tot = vf_sums(row, lo, hi, seg, sums);
-  if (!(tot > 0.0)) {
-    row = VerifyRow{pb + (long)cur * V, nullptr, 0.0, gone, 0};
-    tot = vf_sums(row, lo, hi, seg, sums);
+  __syncthreads();
+  if (!is_last) return;
+  if (G > 1 && t < G) sums[t] = vf_get(a.part + b * VF_G + t);
+  if (round) tables();
+  __syncthreads();
+  for (;;) {
+    double S = 0.0;
+    for (int k = 0; k < G; k++) S += sums[k];
+    if (st.need) {  // the pass was for a rejected child
+      const int cur0 = st.cur;
+      const double c0 = st.c;
+      __syncthreads();
+      if (t == 0) st.mass = S;
+      __syncthreads();
+      walk();
+      if (!st.need && st.cur == cur0 && st.c == c0) break;  // no child is left: the draw is from this residual
+    } else {
+      break;
+    }
+    // another residual
+    if (!last_round) {
+      for (int j = np0 + t; j < st.np; j += VF_NT) a.path[(long)b * a.T + j] = way[j - np0];
+      if (t == 0) a.state[b] = st;
+      return;
+    }
+    row = row_of();
+    for (int k = 0; k < G; k++) {
+      const int l0 = min(V, k * len), h0 = min(V, l0 + len);
+      const double x = l0 < h0 ? vf_sum(row, l0, h0, quads, red) : 0.0;
+      if (t == 0) sums[k] = x;
+    }
+    __syncthreads();
+    if (!st.need) break;
+  }
+  const int np = st.np;
+  for (int j = np0 + t; j < a.T; j += VF_NT) a.path[(long)b * a.T + j] = j < np ? way[j - np0] : -1;
+  if (t == 0) {
+    a.n_path[b] = np;
+    if (!last_round) a.state[b].done = 1;
+  }
+  // the draw: the chunk, then the entry, where the running sum passes u times the whole
+  row = row_of();
+  double tot = 0.0;
+  for (int k = 0; k < G; k++) tot += sums[k];
+  if (!(tot > 0.0)) {  // an empty residual: p itself
+    row = VerifyRow{row.p, nullptr, 0.0, gone, 0};
+    tot = 0.0;
+    for (int k = 0; k < G; k++) {
+      const int l0 = min(V, k * len), h0 = min(V, l0 + len);
+      const double x = l0 < h0 ? vf_sum(row, l0, h0, quads, red) : 0.0;
+      if (t == 0) sums[k] = x;
+      tot += x;
+    }
+    __syncthreads();
   }
   if (!(tot > 0.0) || tot > 1.7e308) {
-    if (t == 0) next[b] = -1;
+    if (t == 0) a.next[b] = -1;
     return;
   }
   double left = (double)us[0] * tot;
-  for (;;) {
-    // the first segment whose end passes `left`; rounding may leave none: then the last one with any mass
-    int k = -1, last = 0;
-    double before = 0.0, lb = 0.0, run = 0.0;
-    for (int j = 0; j < VF_W; j++) {
-      if (sums[j] > 0.0) {
-        last = j;
-        lb = run;
-      }
-      if (k < 0 && run + sums[j] > left) {
-        k = j;
-        before = run;
-      }
-      run += sums[j];
+  int k = -1, last = 0;
+  double before = 0.0, lb = 0.0, run = 0.0;
+  for (int j = 0; j < G; j++) {
+    const double x = sums[j];
+    if (x > 0.0) {
+      last = j;
+      lb = run;
     }
-    if (k < 0) {
-      k = last;
-      before = lb;
+    if (k < 0 && run + x > left) {
+      k = j;
+      before = run;
     }
-    left -= before;
-    lo = lo + k * seg;
-    hi = min(hi, lo + seg);
-    if (hi - lo <= VF_NT) break;
-    seg = (hi - lo + VF_W - 1) / VF_W;
-    vf_sums(row, lo, hi, seg, sums);
+    run += x;
   }
-  const int i = lo + t, w = t >> 6, lane = t & 63;
-  const double r = i < hi ? row.at(i) : 0.0;
-  const double in = rbt_wave_scan_d(r);
-  __syncthreads();
-  if (lane == 63) sums[w] = in;
-  if (t == 0) found = INT32_MAX;
-  __syncthreads();
-  double run = in;
-  for (int k = 0; k < w; k++) run += sums[k];
-  if (r > 0.0 && run > left) atomicMin(&found, i);
-  __syncthreads();
-  if (found == INT32_MAX) {  // rounding: the last entry with any mass
+  if (k < 0) {  // rounding left none: the last one with any mass
+    k = last;
+    before = lb;
+  }
+  left -= before;
+  // blocks of eight entries a thread, in order
+  constexpr int E = 8;
+  const int l0 = k * len, h0 = min(V, l0 + len), w = t >> 6;
+  int tail = -1;  // this thread's last entry with any mass
+  for (int b0 = l0; b0 < h0; b0 += E * VF_NT) {
+    const int i0 = b0 + t * E;
+    float pv[E], qv[E];
+    double r[E], mine = 0.0;
+#pragma unroll
+    for (int e = 0; e < E; e++) pv[e] = row.p[min(i0 + e, V - 1)];
+#pragma unroll
+    for (int e = 0; e < E; e++) qv[e] = row.q ? row.q[min(i0 + e, V - 1)] : 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      r[e] = i0 + e < h0 ? row.of(pv[e], qv[e], i0 + e) : 0.0;
+      mine += r[e];
+      if (r[e] > 0.0) tail = i0 + e;
+    }
+    const double in = rbt_wave_scan_d(mine), up = __shfl_up(in, 1, 64);
+    __syncthreads();
+    if (lane == 63) red[w] = in;
+    if (t == 0) found = INT32_MAX;
+    __syncthreads();
+    double base = lane ? up : 0.0;
+    for (int j = 0; j < w; j++) base += red[j];
+    if (mine > 0.0 && base + mine > left) {
+      int at = -1;  // (the thread's last entry with any mass where rounding lets none pass)
+#pragma unroll
+      for (int e = E - 1; e >= 0; e--)
+        if (at < 0 && r[e] > 0.0) at = i0 + e;
+      double sum = base;
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        sum += r[e];
+        if (r[e] > 0.0 && sum > left && at > i0 + e) at = i0 + e;
+      }
+      atomicMin(&found, at);
+    }
+    __syncthreads();
+    if (found != INT32_MAX) break;
+    left -= (red[0] + red[1]) + (red[2] + red[3]);
+  }
+  if (found == INT32_MAX) {  // rounding: the chunk's last entry with any mass
     __syncthreads();
     if (t == 0) found = -1;
     __syncthreads();
-    if (r > 0.0) atomicMax(&found, i);
+    if (tail >= 0) atomicMax(&found, tail);
     __syncthreads();
   }
-  if (t == 0) next[b] = found;
+  if (t == 0) a.next[b] = found;
 }
 
-hipError_t launch_verify(const Ctx &c, const int *tokens, const int *parent, const int *n_nodes, const float *p,
-                         const float *q, const float *u, int B, int T, int V, int *path, int *n_path, int *next, int *bad) {
-  launch_k(c, k_verify, dim3(B), dim3(VF_NT), tokens, parent, n_nodes, p, q, u, T, V, path, n_path, next, bad);
+int verify_chunks(const Ctx &c, int B, int V) {
+  // 4096 entries each: sixteen trees over 131072 entries take 80 us so, 90 with 2048 (the arrivals queue on their
+  // counter), 95 with 8192 and 133 with 16384 (the pass itself)
+  return std::max(1, std::min({VF_G, (V + 4095) / 4096, 8 * c.num_cu / B}));
+}
+size_t verify_scratch(int B) { return (size_t)B * (VF_G * sizeof(double) + sizeof(VerifyState)); }
+
+hipError_t launch_verify(const Ctx &c, VerifyArgs a, int B, int max_children, void *scratch) {
+  a.part = (double *)scratch;
+  a.state = (VerifyState *)(a.part + (size_t)B * VF_G);
+  a.cnt = c.d_cnt;
+  const int G = verify_chunks(c, B, a.V), rounds = !a.q || max_children == 1 ? 1 : VF_ROUNDS;
+  for (int r = 0; r < rounds; r++) launch_k(c, k_verify, dim3(G, B), dim3(VF_NT), a, r, (int)(r == rounds - 1));
   return hipGetLastError();
 }
 

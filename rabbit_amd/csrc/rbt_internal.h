@@ -442,8 +442,22 @@ hipError_t launch_rope(const Ctx &c, const RopeArgs &a, int s);
 // bad: set to 1 by sequences or nodes whose numbers do not fit.
 hipError_t launch_tree_pos(const Ctx &c, const int *parent, const int *n_nodes, const int *len, int B, int T, int *pos,
                            int *bad);
-hipError_t launch_verify(const Ctx &c, const int *tokens, const int *parent, const int *n_nodes, const float *p,
-                         const float *q, const float *u, int B, int T, int V, int *path, int *n_path, int *next, int *bad);
+struct VerifyState {
+  double c, mass;
+  int cur, at, np;  // current node, last node looked at, standing nodes
+  int need, done;   // whether the pass to make is for a rejected child (else for the draw)
+};
+struct VerifyArgs {
+  const int *tokens, *parent, *n_nodes;
+  const float *p, *q, *u;
+  int T, V;
+  int *path, *n_path, *next, *bad;
+  double *part;        // scratch: the chunks' sums
+  VerifyState *state;  // scratch: the walk between launches
+  unsigned *cnt;       // arrival counters, one per sequence (at most CNT_N), left at 0
+};
+size_t verify_scratch(int B);
+hipError_t launch_verify(const Ctx &c, VerifyArgs a, int B, int max_children, void *scratch);
 constexpr int COMMIT_SIDES = 64;  // K and V of the layers of one launch
 struct CommitArgs {
   void *dst[COMMIT_SIDES];
