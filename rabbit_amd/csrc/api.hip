@@ -2345,13 +2345,12 @@ int rbt_gqa_tree_d(rbt_ctx *c, const rbt_gqa_tree_desc *d, size_t n_seq, size_t 
   a.scale = d->attn_scale;
   a.kv16 = d->kv_dtype == RBT_DT_BF16;
   a.bad = c->d_flags + FLAG_TREE;
-  int rw = 1, kw = 1;
-  rbt::tree_plan(*c, a, rw, kw);
+  rbt::tree_plan(*c, a);
   if (const size_t n = a.tiled ? rbt::tree_part_floats(a) : 0) {
     RBT_TRY(scratch_t(c, SC_MIXB, n, &a.part));
     a.part_ml = (float2 *)(a.part + n / (hd + 2) * hd);
   }
-  HIP_OK(c, rbt::launch_tree(*c, a, rw, kw));
+  HIP_OK(c, rbt::launch_tree(*c, a));
   return RBT_OK;
 }
 

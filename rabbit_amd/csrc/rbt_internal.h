@@ -485,14 +485,15 @@ struct TreeArgs {
   // tree_plan: whether the matrix cores take it, row tiles, pieces of the cache (keys per piece), scratch
   int tiled, tiles, pieces;
   unsigned per, magic;
-  int R;  // query heads per KV head
+  int R;       // query heads per KV head
+  int rw, kw;  // waves of a workgroup: row tiles, groups of keys
   long rows_max;
   float *part;
   float2 *part_ml;
 };
-bool tree_plan(const Ctx &c, TreeArgs &a, int &rw, int &kw);
+bool tree_plan(const Ctx &c, TreeArgs &a);
 size_t tree_part_floats(const TreeArgs &a);
-hipError_t launch_tree(const Ctx &c, const TreeArgs &a, int rw, int kw);
+hipError_t launch_tree(const Ctx &c, const TreeArgs &a);
 
 // synth.hip
 hipError_t launch_synth_mxfp4(const Ctx &c, uint8_t *data, uint8_t *scale, size_t rows, size_t cols, uint64_t seed,

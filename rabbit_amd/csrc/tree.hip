@@ -153,13 +153,18 @@ __device__ __forceinline__ float tree_xor_sum(float v) {
   return v + __shfl_xor(v, 32, 64);
 }
 
-template <int HD, bool B16>
+// How keys and values reach the matrix cores: bf16 as they are, f32 as they are, f32 in three bf16 parts.
+enum { KV_BF16 = 0, KV_F32 = 1, KV_PARTS = 2 };
+constexpr int TREE_PARTS_NT = 512;  // threads of the workgroups that split f32 rows
+
+template <int HD, int KV>
 struct TreeTile {
-  static constexpr int ES = B16 ? 2 : 4, ROWB = HD * ES, CH = ROWB / 16;
-  static constexpr int TK = B16 ? 64 : 32;                  // keys per stage
-  static constexpr int SIDE = TK * ROWB, STAGE = 2 * SIDE;  // bytes of one side, of K and V
-  static constexpr int LDS = 2 * STAGE;
-  static constexpr int INSTR = TK * CH / 64;                // 1 KB loads per side
+  static constexpr int ROWB = HD * (KV == KV_F32 ? 4 : 2), CH = ROWB / 16;  // bytes and chunks of a row in LDS
+  static constexpr int GROW = HD * (KV == KV_BF16 ? 2 : 4);                 // bytes of a row of the cache
+  static constexpr int TK = KV == KV_BF16 ? 64 : 32;                        // keys per stage
+  static constexpr int PART = TK * ROWB, SIDE = PART * (KV == KV_PARTS ? 3 : 1), STAGE = 2 * SIDE;  // K, then V
+  static constexpr int LDS = KV == KV_PARTS ? STAGE : 2 * STAGE;
+  static constexpr int INSTR = TK * CH / 64;                                // 1 KB loads per side
   static_assert(TK * CH % 64 == 0 && CH % 8 == 0, "whole loads");
 };
 
@@ -178,14 +183,16 @@ __device__ __forceinline__ void tree_pieces(const TreeArgs &a, int L, int TK, un
   }
 }
 
-template <int HD, bool B16, int KW>
+template <int HD, int KV, int KW>
 __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(TreeArgs a) {
-  using TT = TreeTile<HD, B16>;
+  using TT = TreeTile<HD, KV>;
+  constexpr bool B16 = KV != KV_F32, PARTS = KV == KV_PARTS;  // bf16 products; of split rows
   constexpr int ROWB = TT::ROWB, CH = TT::CH, TK = TT::TK, SK = TK / KW, NT = SK / 16;
+  static_assert(!PARTS || KW == 1, "one group of waves");
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   __shared__ int par[TREE_MAX];
   __shared__ uint32_t vis[128][TREE_MAX / 32];  // per node of the row tile: which drafted rows it sees
-  __shared__ uint32_t dirty[2][2];              // per stage buffer: drafted rows with non-finite values
+  __shared__ uint32_t dirty[TREE_MAX / 32];     // drafted rows with non-finite values
   __shared__ float ml[KW > 1 ? 4 : 1][2][16];
 
   // workgroup -> (row tile, piece, KV head, sequence); with several row tiles the workgroups that share keys are
@@ -203,7 +210,7 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
   int n, L;
   if (!tree_fits(a, b, n, L)) return;
   const int R = a.R, rows = n * R;
-  const int NW = blockDim.x >> 6, RW = NW / KW;
+  const int NW = blockDim.x >> 6, RW = a.rw;
   const int row0 = rt * RW * 16;
   if (row0 >= rows) return;
   unsigned per, np;
@@ -211,13 +218,13 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
   if (piece >= (int)np) return;
   const int k0 = piece * per, nc = min(L - k0, (int)per);  // cache rows k0 .. k0 + nc - 1, then drafted rows
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int rg = w % RW, kgp = w / RW, col = lane & 15, kg = lane >> 4;
+  const int rg = KW == 1 ? w : w % RW, kgp = KW == 1 ? 0 : w / RW, col = lane & 15, kg = lane >> 4;
   const int node_lo = tree_div(row0, a), node_hi = tree_div(min(rows, row0 + RW * 16) - 1, a);
   const int nd = piece == (int)np - 1 ? node_hi + 1 : 0;  // drafted rows: those up to the last node of the tile
   const int keys = nc + nd, st_n = (keys + TK - 1) / TK;
 
-  const long seq_row = (long)a.K * ROWB;  // bytes from a row to the next
-  const long off_c = (((long)b * a.cap + k0) * a.K + kv) * ROWB, off_d = ((long)b * a.T * a.K + kv) * ROWB;
+  const long seq_row = (long)a.K * TT::GROW;  // bytes from a row to the next
+  const long off_c = (((long)b * a.cap + k0) * a.K + kv) * TT::GROW, off_d = ((long)b * a.T * a.K + kv) * TT::GROW;
   const char *kc = (const char *)a.kc + off_c, *vc = (const char *)a.vc + off_c;
   const char *kd = (const char *)a.kd + off_d, *vd = (const char *)a.vd + off_d;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)smem;
@@ -242,10 +249,54 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
       }
     }
   };
-  issue(0);
+  // key i of the piece holds a non-finite value (one past the last repeats it)
+  auto mark = [&](int i) { atomicOr(&dirty[(min(i, keys - 1) - nc) >> 5], 1u << ((min(i, keys - 1) - nc) & 31)); };
+
+  // split rows: a thread's quads of the stage, K's then V's, on their way
+  constexpr int UN = PARTS ? HD / 64 : 1;
+  static_assert(!PARTS || TK * HD / 4 == UN * TREE_PARTS_NT, "whole quads");
+  float4 raw[2][UN];
+  auto fetch = [&](int s) {
+#pragma unroll
+    for (int k = 0; k < UN; k++) {
+      const int u = k * TREE_PARTS_NT + t, r = u / (HD / 4), j = min(s * TK + r, keys - 1);
+      const long at = (long)(j < nc ? j : j - nc) * seq_row + (u - r * (HD / 4)) * 16;
+      raw[0][k] = *(const float4 *)((j < nc ? kc : kd) + at);
+      raw[1][k] = *(const float4 *)((j < nc ? vc : vd) + at);
+    }
+  };
+  // the quads in three parts to LDS; non-finite drafted values are taken out (see below)
+  auto split = [&](int s) {
+#pragma unroll
+    for (int k = 0; k < UN; k++) {
+      const int u = k * TREE_PARTS_NT + t, r = u / (HD / 4), c = u - r * (HD / 4);
+#pragma unroll
+      for (int side = 0; side < 2; side++) {
+        float v[4] = {raw[side][k].x, raw[side][k].y, raw[side][k].z, raw[side][k].w};
+        if (side && nd > 1 && s * TK + r >= nc) {
+          bool hit = false;
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            if (!(fabsf(v[e]) < INFINITY)) v[e] = 0.0f, hit = true;
+          if (hit) mark(s * TK + r);
+        }
+        uint32_t o[3][4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) tree_split(v[e], o[0][e], o[1][e], o[2][e]);
+        char *to = smem + side * TT::SIDE + r * ROWB + (((c >> 1) ^ (side ? (r & 3) << 1 : r & 7)) * 16) + (c & 1) * 8;
+#pragma unroll
+        for (int p = 0; p < 3; p++)
+          *(uint2 *)(to + p * TT::PART) = make_uint2(tree_pack(o[p][0], o[p][1]), tree_pack(o[p][2], o[p][3]));
+      }
+    }
+  };
+  if constexpr (PARTS)
+    fetch(0);
+  else
+    issue(0);
 
   // this lane's row, and its query in the B operand's layout
-  const bool active = row0 + rg * 16 < rows;  // a wave without rows only loads
+  const bool active = rg < RW && row0 + rg * 16 < rows;  // a wave without rows only loads
   const int row = row0 + rg * 16 + col, rc = min(row, rows - 1);
   const int node = tree_div(rc, a), head = kv * R + (rc - node * R);
   const long qrow = ((long)b * a.T + node) * a.H + head;
@@ -270,7 +321,7 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
     for (int s = 0; s < HD / 16; s++) qf[s] = *(const float4 *)(qp + 16 * s + 4 * kg);
   }
   if (nd > 0) {
-    if (t < 4) dirty[t >> 1][t & 1] = 0;
+    if (t < TREE_MAX / 32) dirty[t] = 0;
     for (int j = t; j < n; j += blockDim.x) {
       int p = a.parent[(long)b * a.T + j];
       if (p < -1 || p >= j) {
@@ -294,15 +345,21 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
   for (int x = 0; x < HD / 16; x++) o[x] = tf4{0.f, 0.f, 0.f, 0.f};
 
   for (int s = 0; s < st_n; s++) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    lds_barrier();  // the stage has landed, and the other buffer's readers are done
-    if (s + 1 < st_n) issue(s + 1);
-    char *kt = smem + (s & 1) * TT::STAGE, *vt = kt + TT::SIDE;
-    uint32_t bad0 = 0, bad1 = 0;
+    char *kt = smem + (PARTS ? 0 : (s & 1) * TT::STAGE), *vt = kt + TT::SIDE;
     const int base = s * TK;
-    if (nd > 1 && base + TK > nc) {
+    if constexpr (PARTS) {
+      lds_barrier();  // the last stage's readers are done
+      split(s);
+      if (s + 1 < st_n) fetch(s + 1);
+      lds_barrier();
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      lds_barrier();  // the stage has landed, and the other buffer's readers are done
+      if (s + 1 < st_n) issue(s + 1);
+    }
+    if (!PARTS && nd > 1 && base + TK > nc) {
       // a value that some rows do not see must not meet their zero probabilities: non-finite ones are taken
-      // out of the tile (its repeated last row too) and added below for the rows that do see them
+      // out of the tile (its repeated last row too) and make NaNs at the end of the rows that do see them
       for (int u = t + max(nc - base, 0) * CH; u < TK * CH; u += blockDim.x) {
         const int r = u / CH;
         uint32_t *x = (uint32_t *)(vt + u * 16);
@@ -318,12 +375,9 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
           }
           if (hit) x[e] = v;
         }
-        if (hit) atomicOr(&dirty[s & 1][r >> 5], 1u << (r & 31));
+        if (hit) mark(base + r);
       }
       lds_barrier();
-      bad0 = dirty[s & 1][0];
-      bad1 = dirty[s & 1][1];
-      if (t < 2) dirty[(s & 1) ^ 1][t] = 0;
     }
 
     if (!active) continue;
@@ -337,13 +391,19 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
       const int c0 = (kg ^ (col & 7)) * 16, c1_ = ((4 + kg) ^ (col & 7)) * 16;
 #pragma unroll
       for (int st = 0; st < HD / 32; st++) {
-        tb8 kf[NT];
+        constexpr int NP = PARTS ? 3 : 1;
+        // the small parts first; products of two parts below 2^-24 of the whole are left out
 #pragma unroll
-        for (int x = 0; x < NT; x++) kf[x] = *(const tb8 *)(kb + x * 16 * ROWB + (st & 1 ? c1_ : c0) + (st >> 1) * 128);
+        for (int f = NP - 1; f >= 0; f--) {
+          tb8 kf[NT];
 #pragma unroll
-        for (int p = 2; p >= 0; p--)
+          for (int x = 0; x < NT; x++)
+            kf[x] = *(const tb8 *)(kb + f * TT::PART + x * 16 * ROWB + (st & 1 ? c1_ : c0) + (st >> 1) * 128);
 #pragma unroll
-          for (int x = 0; x < NT; x++) sc[x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[x], qb[st][p], sc[x], 0, 0, 0);
+          for (int p = 2 - f; p >= 0; p--)
+#pragma unroll
+            for (int x = 0; x < NT; x++) sc[x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[x], qb[st][p], sc[x], 0, 0, 0);
+        }
       }
     } else {
       const int c0 = (kg ^ (col & 7)) * 16, c1_ = ((4 + kg) ^ (col & 7)) * 16;
@@ -417,25 +477,29 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
 #pragma unroll
       for (int dt = 0; dt < HD / 16; dt++) {
         const char *vp = vb + (dt >> 2) * 128 + (((dt & 3) ^ xr) * 32);
-        ts4 vf[NT];
+        constexpr int NP = PARTS ? 3 : 1;
 #pragma unroll
-        for (int x = 0; x < NT; x++)
-          vf[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tree_lds_s4 *)(vp + x * 16 * ROWB));
-        if constexpr (NT >= 2) {
+        for (int f = NP - 1; f >= 0; f--) {
+          ts4 vf[NT];
 #pragma unroll
-          for (int x = 0; x < NT; x += 2) {
-            struct { ts4 lo, hi; } vv{vf[x], vf[x + 1]};
+          for (int x = 0; x < NT; x++)
+            vf[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tree_lds_s4 *)(vp + f * TT::PART + x * 16 * ROWB));
+          if constexpr (NT >= 2) {
 #pragma unroll
-            for (int p = 2; p >= 0; p--)
-              o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                  __builtin_bit_cast(tb8, vv),
-                  __builtin_bit_cast(tb8, rbt_u4{pp[x][p][0], pp[x][p][1], pp[x + 1][p][0], pp[x + 1][p][1]}), o[dt], 0, 0, 0);
-          }
-        } else {
+            for (int x = 0; x < NT; x += 2) {
+              struct { ts4 lo, hi; } vv{vf[x], vf[x + 1]};
 #pragma unroll
-          for (int p = 2; p >= 0; p--) {
-            struct { uint32_t x, y; } pv{pp[0][p][0], pp[0][p][1]};
-            o[dt] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(vf[0], __builtin_bit_cast(ts4, pv), o[dt], 0, 0, 0);
+              for (int p = 2 - f; p >= 0; p--)
+                o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                    __builtin_bit_cast(tb8, vv),
+                    __builtin_bit_cast(tb8, rbt_u4{pp[x][p][0], pp[x][p][1], pp[x + 1][p][0], pp[x + 1][p][1]}), o[dt], 0, 0, 0);
+            }
+          } else {
+#pragma unroll
+            for (int p = 2; p >= 0; p--) {
+              struct { uint32_t x, y; } pv{pp[0][p][0], pp[0][p][1]};
+              o[dt] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(vf[0], __builtin_bit_cast(ts4, pv), o[dt], 0, 0, 0);
+            }
           }
         }
       }
@@ -455,27 +519,22 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
           }
         }
     }
-    if (bad0 | bad1) {  // never in a healthy step
+  }
+
+  if (nd > 1) {  // the non-finite values that were taken out, for the rows that see them; none in a healthy step
+    for (int x = 0; x < TREE_MAX / 32; x++)
+      for (uint32_t bits = dirty[x]; bits; bits &= bits - 1) {
+        const int j = 32 * x + __ffs(bits) - 1;
+        if (!active || !(vis[node - node_lo][x] >> (j & 31) & 1)) continue;
 #pragma unroll
-      for (int x = 0; x < NT; x++)
+        for (int d = 0; d < HD / 16; d++)
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-          for (int k = 0; k < 4; k++) {
-            const int r = kgp * SK + 16 * x + 4 * k + i;
-            if (!((r < 32 ? bad0 >> r : bad1 >> (r - 32)) & 1) || base + r >= keys) continue;
-            const float p = __shfl(sc[x][i], k * 16 + col, 64);
-            if (p == 0.0f) continue;
-            const char *src = vd + (long)(base + r - nc) * seq_row;
-#pragma unroll
-            for (int d = 0; d < HD / 16; d++)
-#pragma unroll
-              for (int e = 0; e < 4; e++) {
-                const int at = B16 ? 16 * d + 4 * kg + e : 64 * (d >> 2) + 16 * kg + 4 * e + (d & 3);
-                const float v = tree_ld(src, at, B16);
-                if (!(fabsf(v) < INFINITY)) o[d][e] += p * v;
-              }
+          for (int e = 0; e < 4; e++) {
+            const int at = B16 ? 16 * d + 4 * kg + e : 64 * (d >> 2) + 16 * kg + 4 * e + (d & 3);
+            const float v = tree_ld(vd + j * seq_row, at, KV == KV_BF16);
+            o[d][e] += fabsf(v) < INFINITY ? 0.0f : v - v;
           }
-    }
+      }
   }
 
   // the column's four lanes hold parts of the row's sum
@@ -533,7 +592,7 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
     }
     (void)lt;
   } else {
-    if (row >= rows) return;
+    if (!active || row >= rows) return;
 #pragma unroll
     for (int d = 0; d < HD / 16; d++) {
       const int at = B16 ? 16 * d + 4 * kg : 64 * (d >> 2) + 16 * kg + 4 * (d & 3);
@@ -619,7 +678,8 @@ __global__ __launch_bounds__(256) void k_tree_join(TreeArgs a, int TK) {
 }
 
 // Pieces and row tiles for a call on the matrix cores.
-bool tree_plan(const Ctx &c, TreeArgs &a, int &rw, int &kw) {
+bool tree_plan(const Ctx &c, TreeArgs &a) {
+  int rw = 1, kw = 1;
   a.tiled = a.hd == 64 || a.hd == 128 || a.hd == 192 || a.hd == 256;
   if (!a.tiled) return false;
   const int R = a.H / a.K, t16 = (a.T * R + 15) / 16;
@@ -636,6 +696,8 @@ bool tree_plan(const Ctx &c, TreeArgs &a, int &rw, int &kw) {
     rw = (t16 + a.tiles - 1) / a.tiles;
   }
   a.tiles = (t16 + rw - 1) / rw;
+  a.rw = rw;
+  a.kw = kw;
   // Pieces by the time they should take, in microseconds: a workgroup (one per CU: its stages fill the LDS) starts
   // and ends in 7, takes `stage` per stage (measured at head_dim 256; it goes with the head dim), and several pieces
   // cost a second launch and a write and read of their rows' partial sums. Equal sequences end together, so their
@@ -667,32 +729,32 @@ size_t tree_part_floats(const TreeArgs &a) {
   return a.pieces > 1 ? (size_t)a.pieces * a.B * a.K * a.rows_max * (a.hd + 2) : 0;
 }
 
-template <int HD, bool B16, int KW>
-static hipError_t run_tree(const Ctx &c, const TreeArgs &a, int rw) {
-  constexpr int lds = TreeTile<HD, B16>::LDS;
+template <int HD, int KV, int KW>
+static hipError_t run_tree(const Ctx &c, const TreeArgs &a) {
+  constexpr int lds = TreeTile<HD, KV>::LDS;
   static_assert(4 * 16 * (HD + 4) * 4 <= lds || KW == 1, "the key groups' join fits the stages' LDS");
   const long groups = (long)a.pieces * a.K * a.B;
   const long blocks = (groups + 7) / 8 * 8 * a.tiles;
   if (blocks > INT32_MAX) return hipErrorInvalidValue;
   const dim3 grid = a.tiles > 1 ? dim3((unsigned)blocks) : dim3(a.pieces, a.K, a.B);
-  launch_ks(c, k_tree<HD, B16, KW>, grid, dim3(64 * rw * KW), (unsigned)lds, a);
+  launch_ks(c, k_tree<HD, KV, KW>, grid, dim3(KV == KV_PARTS ? TREE_PARTS_NT : 64 * a.rw * KW), (unsigned)lds, a);
   return hipGetLastError();
 }
 
 template <int HD>
-static hipError_t run_tree_hd(const Ctx &c, const TreeArgs &a, int rw, int kw) {
+static hipError_t run_tree_hd(const Ctx &c, const TreeArgs &a) {
   if (a.kv16)
-    return kw == 4 ? run_tree<HD, true, 4>(c, a, rw) : kw == 2 ? run_tree<HD, true, 2>(c, a, rw) : run_tree<HD, true, 1>(c, a, rw);
-  return kw == 2 ? run_tree<HD, false, 2>(c, a, rw) : run_tree<HD, false, 1>(c, a, rw);
+    return a.kw == 4 ? run_tree<HD, KV_BF16, 4>(c, a) : a.kw == 2 ? run_tree<HD, KV_BF16, 2>(c, a) : run_tree<HD, KV_BF16, 1>(c, a);
+  return a.kw == 2 ? run_tree<HD, KV_F32, 2>(c, a) : run_tree<HD, KV_PARTS, 1>(c, a);
 }
 
-hipError_t launch_tree(const Ctx &c, const TreeArgs &a, int rw, int kw) {
+hipError_t launch_tree(const Ctx &c, const TreeArgs &a) {
   if (!a.tiled) {
     launch_k(c, k_tree_any, dim3(a.H, a.T, a.B), dim3(256), a);
     return hipGetLastError();
   }
-  hipError_t e = a.hd == 64 ? run_tree_hd<64>(c, a, rw, kw) : a.hd == 128 ? run_tree_hd<128>(c, a, rw, kw)
-                 : a.hd == 192 ? run_tree_hd<192>(c, a, rw, kw) : run_tree_hd<256>(c, a, rw, kw);
+  hipError_t e = a.hd == 64 ? run_tree_hd<64>(c, a) : a.hd == 128 ? run_tree_hd<128>(c, a)
+                 : a.hd == 192 ? run_tree_hd<192>(c, a) : run_tree_hd<256>(c, a);
   if (e != hipSuccess || a.pieces == 1) return e;
   const unsigned rows = (unsigned)a.rows_max, TK = a.kv16 ? 64 : 32;
   if (a.pieces > 4)
