@@ -487,7 +487,7 @@ struct TreeArgs {
   unsigned per, magic;
   int R;       // query heads per KV head
   int rw, kw;  // waves of a workgroup: row tiles, groups of keys
-  long rows_max;
+  int t16;     // 16-row tiles of a KV head
   float *part;
   float2 *part_ml;
 };

@@ -540,8 +540,11 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
   // the column's four lanes hold parts of the row's sum
   l = tree_xor_sum(l);
   const bool direct = np == 1;
-  float *po = a.part + ((long)(piece * a.B + b) * a.K + kv) * a.rows_max * HD;
-  float2 *pm = a.part_ml + ((long)(piece * a.B + b) * a.K + kv) * a.rows_max;
+  // partial sums lie by 16-row tiles in the order of the lanes: quad 64 d + lane holds row col's entries
+  // 16 d + 4 kg .. + 3, so that they are written and read in whole lines
+  const long unit = (((long)piece * a.B + b) * a.K + kv) * a.t16 + rt * RW + rg;
+  float *po = a.part + unit * 16 * HD;
+  float2 *pm = a.part_ml + unit * 16;
   // entry e of value tile d is entry at(d, e) of the head
   if constexpr (KW > 1) {
     // join the key groups in LDS: every group's O and l scaled to the row's largest maximum
@@ -586,95 +589,100 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
         const int nodr = tree_div(rr, a), hdr = kv * R + (rr - nodr * R);
         tree_store(a, b, nodr, hdr, 4 * e, v, lr);
       } else {
-        *(float4 *)(po + (long)rr * HD + 4 * e) = v;
-        if (e == 0) pm[rr] = make_float2(Mr, lr);
+        *(float4 *)(po + ((e >> 2) * 64 + (e & 3) * 16 + r) * 4) = v;
+        if (e == 0) pm[r] = make_float2(Mr, lr);
       }
     }
     (void)lt;
   } else {
-    if (!active || row >= rows) return;
+    static_assert(B16, "the values' tiles are 16 entries wide");
+    if (!active) return;
 #pragma unroll
     for (int d = 0; d < HD / 16; d++) {
-      const int at = B16 ? 16 * d + 4 * kg : 64 * (d >> 2) + 16 * kg + 4 * (d & 3);
-      const float4 v = B16 ? make_float4(o[d][0], o[d][1], o[d][2], o[d][3])
-                           : make_float4(o[d & ~3][d & 3], o[(d & ~3) + 1][d & 3], o[(d & ~3) + 2][d & 3], o[(d & ~3) + 3][d & 3]);
-      if (direct)
-        tree_store(a, b, node, head, at, v, l);
-      else
-        *(float4 *)(po + (long)row * HD + at) = v;
+      const float4 v = make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
+      if (!direct)
+        *(float4 *)(po + (d * 64 + lane) * 4) = v;
+      else if (row < rows)
+        tree_store(a, b, node, head, 16 * d + 4 * kg, v, l);
     }
-    if (!direct && kg == 0) pm[row] = make_float2(m, l);
+    if (!direct && kg == 0) pm[col] = make_float2(m, l);
   }
 }
 
-// The pieces of a row joined by WR waves, a row's lane j taking entries 4 j .. 4 j + 3; each wave's pieces are summed in
-// order, then the waves' sums.
-template <int WR>
+// The pieces of 16 rows joined. WP = 1: a workgroup takes 64 entries of the rows, 16 per wave; WP = 4: 16 entries, its
+// waves take every fourth piece each and their sums are added in order. Lane by lane as the partial sums lie.
+template <int WP>
 __global__ __launch_bounds__(256) void k_tree_join(TreeArgs a, int TK) {
-  __shared__ __attribute__((aligned(16))) float wt[4][256], sum[WR > 1 ? 4 : 1][256];
-  __shared__ float red[2][4];
-  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, wr = w % WR, tr = wr * 64 + lane;
-  // (rows of the kernels' tiling: row = node * n_rep + head of the group)
-  const int row = blockIdx.x * (4 / WR) + w / WR, kv = blockIdx.y, b = blockIdx.z;
-  const int n = a.n_nodes[b], L = a.len[b], i = tree_div(row, a);
-  const bool live = n >= 0 && n <= a.T && L >= 0 && L <= a.cap && i < n;
-  if (WR > 1 && !live) return;  // (the workgroup's only row)
-  unsigned per, np = 0;
-  if (live) tree_pieces(a, L, TK, per, np);
+  __shared__ float wt[256][16], red[16][16];
+  __shared__ float4 sum[WP > 1 ? 4 : 1][64];
+  const int t = threadIdx.x, w = t >> 6, lane = t & 63, col = lane & 15, kv = blockIdx.y, b = blockIdx.z;
+  const int nd = a.hd / 16, tile = WP > 1 ? blockIdx.x / nd : blockIdx.x * 4 / nd;
+  const int d = WP > 1 ? blockIdx.x - tile * nd : blockIdx.x * 4 - tile * nd + w;
+  const int n = a.n_nodes[b], L = a.len[b];
+  if (n < 0 || n > a.T || L < 0 || L > a.cap || tile * 16 >= n * a.R) return;
+  unsigned per, np;
+  tree_pieces(a, L, TK, per, np);
   if (np <= 1) return;
-  const long ps = (long)a.B * a.K * a.rows_max, at = ((long)b * a.K + kv) * a.rows_max + row;
-  float M = -INFINITY;
-  float2 x[4 / WR];
+  const long ps = (long)a.B * a.K * a.t16, unit = ((long)b * a.K + kv) * a.t16 + tile;
+  // the rows' largest maximum, then each piece's weight and the rows' sums: thread t takes row t % 16 (of up to 256
+  // pieces: all are loaded at once, and so are this wave's first sums)
+  const int r = t & 15, j0 = t >> 4;
+  float2 x[16];
 #pragma unroll
-  for (int k = 0; k < 4 / WR; k++) {
-    const unsigned j = tr + 64 * WR * k;
-    x[k] = j < np ? a.part_ml[j * ps + at] : make_float2(-INFINITY, 0.0f);
-    M = fmaxf(M, x[k].x);
-  }
-  M = rbt_wave_max_f(M);
-  if constexpr (WR > 1) {
-    if (lane == 0) red[0][w] = M;
-    __syncthreads();
-    M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-  }
+  for (int k = 0; k < 16; k++)
+    if (16 * k < (int)np) x[k] = a.part_ml[(min(j0 + 16 * k, (int)np - 1) * ps + unit) * 16 + r];
+  constexpr int PF = 8;
+  const unsigned first = WP > 1 ? w : 0;
+  const float *po = a.part + unit * 16 * a.hd + (d * 64 + lane) * 4;
+  float4 y[PF];
+#pragma unroll
+  for (int k = 0; k < PF; k++) y[k] = *(const float4 *)(po + min(first + k * WP, np - 1) * ps * 16 * a.hd);
+  float M = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < 16; k++)
+    if (16 * k < (int)np) M = fmaxf(M, x[k].x);
+  red[j0][r] = M;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 16; k++) M = fmaxf(M, red[k][r]);
   const float Ms = M == -INFINITY ? 0.0f : M;
   float l = 0.0f;
 #pragma unroll
-  for (int k = 0; k < 4 / WR; k++) {
+  for (int k = 0; k < 16; k++) {
+    const int j = j0 + 16 * k;
+    if (j >= (int)np) break;
     const float f = __builtin_amdgcn_exp2f(x[k].x - Ms);
-    wt[WR > 1 ? 0 : w][tr + 64 * WR * k] = f;
+    wt[j][r] = f;
     l += x[k].y * f;
   }
+  __syncthreads();
+  red[j0][r] = l;
+  __syncthreads();
+  l = 0.0f;
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d, 64);
-  if constexpr (WR > 1) {
-    if (lane == 0) red[1][w] = l;
-    __syncthreads();
-    l = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
-  } else {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
-  }
-  const bool mine = 4 * lane < a.hd;
+  for (int k = 0; k < 16; k++) l += red[k][col];
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  const float *po = a.part + at * a.hd + 4 * (mine ? lane : 0);
-  const float *wp = wt[WR > 1 ? 0 : w];
-#pragma unroll 8
-  for (unsigned j = wr; j < np; j += WR) {
-    const float4 y = *(const float4 *)(po + j * ps * a.hd);
-    const float f = wp[j];
+  auto add = [&](float4 y, unsigned j) {
+    const float f = wt[j][col];
     v = make_float4(v.x + y.x * f, v.y + y.y * f, v.z + y.z * f, v.w + y.w * f);
-  }
-  if constexpr (WR > 1) {
-    *(float4 *)(sum[w] + 4 * lane) = v;
+  };
+#pragma unroll
+  for (int k = 0; k < PF; k++)
+    if (first + k * WP < np) add(y[k], first + k * WP);
+#pragma unroll 8
+  for (unsigned j = first + PF * WP; j < np; j += WP) add(*(const float4 *)(po + j * ps * 16 * a.hd), j);
+  if constexpr (WP > 1) {
+    sum[w][lane] = v;
     __syncthreads();
     if (w) return;
 #pragma unroll
     for (int k = 1; k < 4; k++) {
-      const float4 y = *(const float4 *)(sum[k] + 4 * lane);
+      const float4 y = sum[k][lane];
       v = make_float4(v.x + y.x, v.y + y.y, v.z + y.z, v.w + y.w);
     }
   }
-  if (mine) tree_store(a, b, i, kv * a.R + (row - i * a.R), 4 * lane, v, l);
+  const int row = tile * 16 + col, i = tree_div(row, a);
+  if (i < n) tree_store(a, b, i, kv * a.R + (row - i * a.R), 16 * d + 4 * (lane >> 4), v, l);
 }
 
 // Pieces and row tiles for a call on the matrix cores.
@@ -684,7 +692,7 @@ bool tree_plan(const Ctx &c, TreeArgs &a) {
   if (!a.tiled) return false;
   const int R = a.H / a.K, t16 = (a.T * R + 15) / 16;
   const int TK = a.kv16 ? 64 : 32;
-  a.rows_max = (long)a.T * R;
+  a.t16 = t16;
   a.R = R;
   a.magic = R == 1 ? 0 : (unsigned)((0x100000000ull + R - 1) / R);
   if (t16 <= 2) {
@@ -706,7 +714,7 @@ bool tree_plan(const Ctx &c, TreeArgs &a) {
   // 27 in 8, 17 in 32, 17 in 64; 64 nodes over 32749 rows 527 in 4, 311 in 8, 326 in 16, 368 in 32.
   const double base = (double)a.tiles * a.K * a.B, most = std::ceil((double)(a.max_len + a.T) / TK), ncu = c.num_cu;
   const double stage = (kw > 1 ? (a.kv16 ? 1.6 : 2.6) : a.kv16 ? (rw > 4 ? 4.4 : 2.6) : (rw > 4 ? 8.5 : 4.5)) * a.hd / 256.0;
-  const double bytes = (double)a.B * a.K * a.rows_max * a.hd * 8.0;
+  const double bytes = (double)a.B * a.K * a.t16 * 16 * a.hd * 8.0;
   double best = 0.0;
   long pieces = 1;
   auto consider = [&](long p) {
@@ -726,7 +734,7 @@ bool tree_plan(const Ctx &c, TreeArgs &a) {
 }
 
 size_t tree_part_floats(const TreeArgs &a) {
-  return a.pieces > 1 ? (size_t)a.pieces * a.B * a.K * a.rows_max * (a.hd + 2) : 0;
+  return a.pieces > 1 ? (size_t)a.pieces * a.B * a.K * a.t16 * 16 * (a.hd + 2) : 0;
 }
 
 template <int HD, int KV, int KW>
@@ -756,11 +764,12 @@ hipError_t launch_tree(const Ctx &c, const TreeArgs &a) {
   hipError_t e = a.hd == 64 ? run_tree_hd<64>(c, a) : a.hd == 128 ? run_tree_hd<128>(c, a)
                  : a.hd == 192 ? run_tree_hd<192>(c, a) : run_tree_hd<256>(c, a);
   if (e != hipSuccess || a.pieces == 1) return e;
-  const unsigned rows = (unsigned)a.rows_max, TK = a.kv16 ? 64 : 32;
-  if (a.pieces > 4)
-    launch_k(c, k_tree_join<4>, dim3(rows, a.K, a.B), dim3(256), a, (int)TK);
+  const int TK = a.kv16 ? 64 : 32;
+  // few rows, many pieces: the pieces too over the waves
+  if (a.pieces > 4 && (long)a.t16 * a.K * a.B <= 256)
+    launch_k(c, k_tree_join<4>, dim3(a.t16 * (a.hd / 16), a.K, a.B), dim3(256), a, TK);
   else
-    launch_k(c, k_tree_join<1>, dim3((rows + 3) / 4, a.K, a.B), dim3(256), a, (int)TK);
+    launch_k(c, k_tree_join<1>, dim3(a.t16 * (a.hd / 64), a.K, a.B), dim3(256), a, TK);
   return hipGetLastError();
 }
 
