@@ -166,6 +166,13 @@ struct TreeTile {
   static constexpr int LDS = KV == KV_PARTS ? STAGE : 2 * STAGE;
   static constexpr int INSTR = TK * CH / 64;                                // 1 KB loads per side
   static_assert(TK * CH % 64 == 0 && CH % 8 == 0, "whole loads");
+  // Where chunk c of row r lies in its row: c ^ k_turn(r), c ^ v_turn(r). The LDS serves 256 bytes a cycle from 64
+  // banks, to lanes 0-3, 12-15, 20-23 and 24-27 of a 16-byte read (four such sets) or to half a wave of an 8-byte
+  // one; the turns spread the rows of each set over all banks. (Turns within 128 bytes made every read take
+  // two cycles: half of the LDS's cycles at 64 nodes over 32749 rows.)
+  static constexpr bool WIDE = CH % 16 == 0;  // rows of whole 256 bytes; others begin half a cycle apart
+  static __device__ __forceinline__ int k_turn(int r) { return WIDE ? r & 15 : r & 7; }
+  static __device__ __forceinline__ int v_turn(int r) { return KV == KV_F32 ? 0 : WIDE ? (r & 7) << 1 : (r >> 1 & 3) << 1; }
 };
 
 // A row's node, row / n_rep: magic = ceil(2^32 / n_rep), exact since row * n_rep < 2^32 (at most 2^20 rows, 2^12 heads).
@@ -237,15 +244,15 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
       for (int i = w; i < TT::INSTR; i += NW) {
         const int u = i * 64 + lane, r = u / CH, c = u - r * CH;
         const long at = (long)(base + r) * seq_row;
-        tree_dma(kc + at + (c ^ (r & 7)) * 16, to + i * 1024);
-        tree_dma(vc + at + (B16 ? c ^ ((r & 3) << 1) : c) * 16, to + TT::SIDE + i * 1024);
+        tree_dma(kc + at + (c ^ TT::k_turn(r)) * 16, to + i * 1024);
+        tree_dma(vc + at + (c ^ TT::v_turn(r)) * 16, to + TT::SIDE + i * 1024);
       }
     } else {
       for (int i = w; i < TT::INSTR; i += NW) {
         const int u = i * 64 + lane, r = u / CH, c = u - r * CH, j = min(base + r, keys - 1);
         const long at = (long)(j < nc ? j : j - nc) * seq_row;
-        tree_dma((j < nc ? kc : kd) + at + (c ^ (r & 7)) * 16, to + i * 1024);
-        tree_dma((j < nc ? vc : vd) + at + (B16 ? c ^ ((r & 3) << 1) : c) * 16, to + TT::SIDE + i * 1024);
+        tree_dma((j < nc ? kc : kd) + at + (c ^ TT::k_turn(r)) * 16, to + i * 1024);
+        tree_dma((j < nc ? vc : vd) + at + (c ^ TT::v_turn(r)) * 16, to + TT::SIDE + i * 1024);
       }
     }
   };
@@ -283,7 +290,7 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
         uint32_t o[3][4];
 #pragma unroll
         for (int e = 0; e < 4; e++) tree_split(v[e], o[0][e], o[1][e], o[2][e]);
-        char *to = smem + side * TT::SIDE + r * ROWB + (((c >> 1) ^ (side ? (r & 3) << 1 : r & 7)) * 16) + (c & 1) * 8;
+        char *to = smem + side * TT::SIDE + r * ROWB + (((c >> 1) ^ (side ? TT::v_turn(r) : TT::k_turn(r))) * 16) + (c & 1) * 8;
 #pragma unroll
         for (int p = 0; p < 3; p++)
           *(uint2 *)(to + p * TT::PART) = make_uint2(tree_pack(o[p][0], o[p][1]), tree_pack(o[p][2], o[p][3]));
@@ -387,8 +394,10 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
 #pragma unroll
     for (int x = 0; x < NT; x++) sc[x] = tf4{0.f, 0.f, 0.f, 0.f};
     const char *kb = kt + (kgp * SK + col) * ROWB;
+    // byte of chunk 4 st + kg in the lane's rows (rows 16 apart turn alike): a few offsets per lane and a constant
+    constexpr int KP = TT::WIDE ? 4 : 2;
+    auto kc_at = [&](int st) { return ((4 * (st % KP) + kg) ^ TT::k_turn(col)) * 16 + st / KP * KP * 64; };
     if constexpr (B16) {
-      const int c0 = (kg ^ (col & 7)) * 16, c1_ = ((4 + kg) ^ (col & 7)) * 16;
 #pragma unroll
       for (int st = 0; st < HD / 32; st++) {
         constexpr int NP = PARTS ? 3 : 1;
@@ -398,7 +407,7 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
           tb8 kf[NT];
 #pragma unroll
           for (int x = 0; x < NT; x++)
-            kf[x] = *(const tb8 *)(kb + f * TT::PART + x * 16 * ROWB + (st & 1 ? c1_ : c0) + (st >> 1) * 128);
+            kf[x] = *(const tb8 *)(kb + f * TT::PART + x * 16 * ROWB + kc_at(st));
 #pragma unroll
           for (int p = 2 - f; p >= 0; p--)
 #pragma unroll
@@ -406,12 +415,11 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
         }
       }
     } else {
-      const int c0 = (kg ^ (col & 7)) * 16, c1_ = ((4 + kg) ^ (col & 7)) * 16;
 #pragma unroll
       for (int st = 0; st < HD / 16; st++) {
         float4 kf[NT];
 #pragma unroll
-        for (int x = 0; x < NT; x++) kf[x] = *(const float4 *)(kb + x * 16 * ROWB + (st & 1 ? c1_ : c0) + (st >> 1) * 128);
+        for (int x = 0; x < NT; x++) kf[x] = *(const float4 *)(kb + x * 16 * ROWB + kc_at(st));
 #pragma unroll
         for (int x = 0; x < NT; x++) sc[x] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[x].x, qf[st].x, sc[x], 0, 0, 0);
 #pragma unroll
@@ -462,6 +470,8 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
     if constexpr (B16) {
       const int xr = col >> 2;
       const char *vb = vt + (kgp * SK + 4 * kg + xr) * ROWB + (col & 1) * 8 + ((col >> 1) & 1) * 16;
+      constexpr int VP = TT::WIDE ? 8 : 4;
+      const int turn = TT::v_turn(4 * kg + xr) >> 1;
       uint32_t pp[NT][3][2];
 #pragma unroll
       for (int x = 0; x < NT; x++) {
@@ -476,7 +486,7 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
       }
 #pragma unroll
       for (int dt = 0; dt < HD / 16; dt++) {
-        const char *vp = vb + (dt >> 2) * 128 + (((dt & 3) ^ xr) * 32);
+        const char *vp = vb + dt / VP * VP * 32 + ((dt % VP) ^ turn) * 32;
         constexpr int NP = PARTS ? 3 : 1;
 #pragma unroll
         for (int f = NP - 1; f >= 0; f--) {
