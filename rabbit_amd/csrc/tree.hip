@@ -397,22 +397,28 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
     // byte of chunk 4 st + kg in the lane's rows (rows 16 apart turn alike): a few offsets per lane and a constant
     constexpr int KP = TT::WIDE ? 4 : 2;
     auto kc_at = [&](int st) { return ((4 * (st % KP) + kg) ^ TT::k_turn(col)) * 16 + st / KP * KP * 64; };
+    constexpr int NP = PARTS ? 3 : 1;  // parts of a key or value
     if constexpr (B16) {
+      // a step: 32 entries of one part for up to two tiles of keys, the next step's read while this one's multiply.
+      // Small parts first; products of two parts below 2^-24 of the whole are left out.
+      constexpr int XS = NT > 1 ? 2 : 1, QS = HD / 32 * NP * (NT / XS);
+      tb8 kf[2][XS];
+      auto read = [&](int i, tb8(&to)[XS]) {
+        const int st = i / (NP * (NT / XS)), f = NP - 1 - i / (NT / XS) % NP, x = i % (NT / XS) * XS;
 #pragma unroll
-      for (int st = 0; st < HD / 32; st++) {
-        constexpr int NP = PARTS ? 3 : 1;
-        // the small parts first; products of two parts below 2^-24 of the whole are left out
+        for (int e = 0; e < XS; e++) to[e] = *(const tb8 *)(kb + f * TT::PART + (x + e) * 16 * ROWB + kc_at(st));
+      };
+      read(0, kf[0]);
 #pragma unroll
-        for (int f = NP - 1; f >= 0; f--) {
-          tb8 kf[NT];
+      for (int i = 0; i < QS; i++) {
+        if (i + 1 < QS) read(i + 1, kf[(i + 1) & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+        const int st = i / (NP * (NT / XS)), f = NP - 1 - i / (NT / XS) % NP, x = i % (NT / XS) * XS;
 #pragma unroll
-          for (int x = 0; x < NT; x++)
-            kf[x] = *(const tb8 *)(kb + f * TT::PART + x * 16 * ROWB + kc_at(st));
+        for (int p = 2 - f; p >= 0; p--)
 #pragma unroll
-          for (int p = 2 - f; p >= 0; p--)
-#pragma unroll
-            for (int x = 0; x < NT; x++) sc[x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[x], qb[st][p], sc[x], 0, 0, 0);
-        }
+          for (int e = 0; e < XS; e++)
+            sc[x + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i & 1][e], qb[st][p], sc[x + e], 0, 0, 0);
       }
     } else {
 #pragma unroll
@@ -484,34 +490,38 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
           pp[x][p][1] = tree_pack(h[p][2], h[p][3]);
         }
       }
+      // a step: one part of 32 keys (16 where the wave has no more) for two tiles of entries
+      constexpr int XS = NT > 1 ? 2 : 1, VS = HD / 32 * (NT / XS) * NP;
+      ts4 vf[2][2][XS];
+      auto read = [&](int i, ts4(&to)[2][XS]) {
+        const int dt = i / (NP * (NT / XS)) * 2, x = i / NP % (NT / XS) * XS, f = NP - 1 - i % NP;
 #pragma unroll
-      for (int dt = 0; dt < HD / 16; dt++) {
-        const char *vp = vb + dt / VP * VP * 32 + ((dt % VP) ^ turn) * 32;
-        constexpr int NP = PARTS ? 3 : 1;
+        for (int d = 0; d < 2; d++)
 #pragma unroll
-        for (int f = NP - 1; f >= 0; f--) {
-          ts4 vf[NT];
+          for (int e = 0; e < XS; e++)
+            to[d][e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (tree_lds_s4 *)(vb + (dt + d) / VP * VP * 32 + (((dt + d) % VP) ^ turn) * 32 + f * TT::PART + (x + e) * 16 * ROWB));
+      };
+      read(0, vf[0]);
 #pragma unroll
-          for (int x = 0; x < NT; x++)
-            vf[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tree_lds_s4 *)(vp + f * TT::PART + x * 16 * ROWB));
-          if constexpr (NT >= 2) {
+      for (int i = 0; i < VS; i++) {
+        if (i + 1 < VS) read(i + 1, vf[(i + 1) & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+        const int dt = i / (NP * (NT / XS)) * 2, x = i / NP % (NT / XS) * XS, f = NP - 1 - i % NP;
 #pragma unroll
-            for (int x = 0; x < NT; x += 2) {
-              struct { ts4 lo, hi; } vv{vf[x], vf[x + 1]};
+        for (int p = 2 - f; p >= 0; p--)
 #pragma unroll
-              for (int p = 2 - f; p >= 0; p--)
-                o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                    __builtin_bit_cast(tb8, vv),
-                    __builtin_bit_cast(tb8, rbt_u4{pp[x][p][0], pp[x][p][1], pp[x + 1][p][0], pp[x + 1][p][1]}), o[dt], 0, 0, 0);
-            }
-          } else {
-#pragma unroll
-            for (int p = 2; p >= 0; p--) {
+          for (int d = 0; d < 2; d++) {
+            if constexpr (XS == 2) {
+              struct { ts4 lo, hi; } vv{vf[i & 1][d][0], vf[i & 1][d][1]};
+              o[dt + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                  __builtin_bit_cast(tb8, vv),
+                  __builtin_bit_cast(tb8, rbt_u4{pp[x][p][0], pp[x][p][1], pp[x + 1][p][0], pp[x + 1][p][1]}), o[dt + d], 0, 0, 0);
+            } else {
               struct { uint32_t x, y; } pv{pp[0][p][0], pp[0][p][1]};
-              o[dt] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(vf[0], __builtin_bit_cast(ts4, pv), o[dt], 0, 0, 0);
+              o[dt + d] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(vf[i & 1][d][0], __builtin_bit_cast(ts4, pv), o[dt + d], 0, 0, 0);
             }
           }
-        }
       }
     } else {
 #pragma unroll
