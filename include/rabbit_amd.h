@@ -404,7 +404,7 @@ typedef struct {
     int32_t rotate;          /* 0: rows are normalised and copied only (values) */
 } rbt_rope_part;
 /* norm_heads and rope_half (qwen38/attention.rs:138-172) for s tokens of up to 8 tensors in one launch:
- * token t at position pos[t] (device int32); pos[t] < 0 leaves the token's rows as they were. */
+ * token t at position pos[t] (device int32); pos[t] < 0 leaves the token's rows as they were. s < 2^24. */
 int rbt_rope_d(rbt_ctx *ctx, const rbt_rope_desc *desc, const rbt_rope_part *parts, size_t n_parts, const int32_t *pos,
                size_t s);
 
@@ -419,10 +419,11 @@ int rbt_tree_positions_d(rbt_ctx *ctx, size_t n_seq, size_t max_nodes, const int
  * [n_seq, cap, n_kv_heads, head_dim] and k_draft, v_draft [n_seq, max_nodes, n_kv_heads, head_dim] of
  * kv_dtype; out f32 as q. gate: out is multiplied by sigmoid of
  * gate[(b * max_nodes + i) * gate_token_stride + h * gate_head_stride + e] (q_proj's [query, gate] rows:
- * strides n_heads * 2 * head_dim and 2 * head_dim), or NULL. Products are exact and sums f32.
- * head_dim 1..1024; any number of query heads per KV head. Values that a node does not see never reach
- * its output, non-finite ones included; a non-finite value that it sees makes the output entries it
- * reaches non-finite, or drops out, as the order of the sums has it. */
+ * strides n_heads * 2 * head_dim and 2 * head_dim), or NULL. Products are exact (to 2^-24) and sums f32.
+ * head_dim 1..1024, fastest at 64, 128, 192 and 256; any number of query heads per KV head. q, out, caches
+ * and draft rows are 16-byte aligned, and out overlaps none of the others. Values that a node does not see never reach
+ * its output, non-finite ones included; a non-finite key or value that it sees makes the output entries
+ * it reaches non-finite (an infinite value may give a NaN). */
 typedef struct {
     size_t n_heads, n_kv_heads, head_dim;
     float attn_scale;

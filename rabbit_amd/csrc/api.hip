@@ -2231,7 +2231,7 @@ int rbt_rope_d(rbt_ctx *c, const rbt_rope_desc *d, const rbt_rope_part *parts, s
     return refuse(c, RBT_E_INVALID, "rotated entries %zu from %zu of %zu", d->rope_dim, d->rope_start, d->head_dim);
   if (!std::isfinite(d->factor) || !(d->eps >= 0.0f) || !std::isfinite(d->eps))
     return refuse(c, RBT_E_INVALID, "factor %g, eps %g", d->factor, d->eps);
-  if (s > (size_t)INT32_MAX) return refuse(c, RBT_E_INVALID, "%zu tokens", s);
+  if (s >= (size_t)1 << 24) return refuse(c, RBT_E_UNSUPPORTED, "%zu tokens (fewer than 2^24)", s);
   rbt::RopeArgs a{};
   size_t rows = 0;
   for (size_t i = 0; i < n_parts; i++) {
@@ -2307,7 +2307,7 @@ int rbt_gqa_tree_d(rbt_ctx *c, const rbt_gqa_tree_desc *d, size_t n_seq, size_t 
     return refuse(c, RBT_E_INVALID, "bad attention shape (heads %zu over %zu kv heads)", nh, nkv);
   if (hd == 0 || hd > 1024) return refuse(c, RBT_E_UNSUPPORTED, "head_dim %zu (1..1024)", hd);
   if (bad_dtype(d->kv_dtype)) return refuse(c, RBT_E_INVALID, "cache type %d", d->kv_dtype);
-  if (!std::isfinite(d->attn_scale)) return refuse(c, RBT_E_INVALID, "attn_scale %g", d->attn_scale);
+  if (!std::isfinite(1.5f * d->attn_scale)) return refuse(c, RBT_E_INVALID, "attn_scale %g", d->attn_scale);
   if (d->cap == 0 || d->cap > (size_t)INT32_MAX || d->max_len > d->cap)
     return refuse(c, RBT_E_INVALID, "cache of %zu rows, max_len %zu", d->cap, d->max_len);
   if (gate && (d->gate_token_stride > (size_t)1 << 40 || d->gate_head_stride > (size_t)1 << 40))
@@ -2345,7 +2345,8 @@ int rbt_gqa_tree_d(rbt_ctx *c, const rbt_gqa_tree_desc *d, size_t n_seq, size_t 
   a.scale = d->attn_scale;
   a.kv16 = d->kv_dtype == RBT_DT_BF16;
   a.bad = c->d_flags + FLAG_TREE;
-  rbt::tree_plan(*c, a);
+  if (!rbt::tree_plan(*c, a))
+    return refuse(c, RBT_E_UNSUPPORTED, "%zu sequences of %zu nodes are too many for one call", n_seq, max_nodes);
   if (const size_t n = a.tiled ? rbt::tree_part_floats(a) : 0) {
     RBT_TRY(scratch_t(c, SC_MIXB, n, &a.part));
     a.part_ml = (float2 *)(a.part + n / (hd + 2) * hd);

@@ -707,9 +707,10 @@ __global__ __launch_bounds__(256) void k_tree_join(TreeArgs a, int TK) {
 
 // Pieces and row tiles for a call on the matrix cores.
 bool tree_plan(const Ctx &c, TreeArgs &a) {
+  a.rw = a.kw = a.tiles = a.pieces = 1;
   int rw = 1, kw = 1;
   a.tiled = a.hd == 64 || a.hd == 128 || a.hd == 192 || a.hd == 256;
-  if (!a.tiled) return false;
+  if (!a.tiled) return true;
   const int R = a.H / a.K, t16 = (a.T * R + 15) / 16;
   const int TK = a.kv16 ? 64 : 32;
   a.t16 = t16;
@@ -738,7 +739,8 @@ bool tree_plan(const Ctx &c, TreeArgs &a) {
   double best = 0.0;
   long pieces = 1;
   auto consider = [&](long p) {
-    if (p < 1 || p > 256 || (p > 1 && p > most)) return;
+    // (partial sums of at most 256 MiB)
+    if (p < 1 || p > 256 || (p > 1 && (p > most || bytes * p > 2.0 * (256u << 20)))) return;
     const double one = 7.0 + stage * std::ceil(most / p);
     const double rounds = base * p / ncu;
     const double t = (rounds <= 1.0 ? one : a.B == 1 ? std::ceil(rounds) * one : (0.8 * rounds + 0.4) * one) +
@@ -750,6 +752,8 @@ bool tree_plan(const Ctx &c, TreeArgs &a) {
   for (int k = 1; k <= 4; k++) consider((long)(k * ncu / base));
   a.per = (unsigned)((long)((most + pieces - 1) / pieces) * TK);
   a.pieces = (int)std::max(1L, (a.max_len + a.per - 1) / (long)a.per);
+  // a launch holds fewer than 2^32 threads in x
+  if (a.tiles > 1 && ((long)a.pieces * a.K * a.B + 7) / 8 * 8 * a.tiles > (1L << 23) - 1) return false;
   return true;
 }
 
@@ -763,7 +767,6 @@ static hipError_t run_tree(const Ctx &c, const TreeArgs &a) {
   static_assert(4 * 16 * (HD + 4) * 4 <= lds || KW == 1, "the key groups' join fits the stages' LDS");
   const long groups = (long)a.pieces * a.K * a.B;
   const long blocks = (groups + 7) / 8 * 8 * a.tiles;
-  if (blocks > INT32_MAX) return hipErrorInvalidValue;
   const dim3 grid = a.tiles > 1 ? dim3((unsigned)blocks) : dim3(a.pieces, a.K, a.B);
   launch_ks(c, k_tree<HD, KV, KW>, grid, dim3(KV == KV_PARTS ? TREE_PARTS_NT : 64 * a.rw * KW), (unsigned)lds, a);
   return hipGetLastError();

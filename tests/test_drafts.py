@@ -123,14 +123,14 @@ def test_rope_accepts(rbt_lib):
     _refused(rbt_lib, rbt_lib.rbt_rope_d(None, C.byref(d), C.byref(p), 1, None, 3), RBT_E_INVALID, "positions")
     _refused(rbt_lib, rbt_lib.rbt_rope_d(None, C.byref(d), C.byref(p), 9, A, 3), RBT_E_INVALID, "tensors")
     _refused(rbt_lib, rbt_lib.rbt_rope_d(None, None, C.byref(p), 1, A, 3), RBT_E_INVALID, "null descriptor")
-    _refused(rbt_lib, rbt_lib.rbt_rope_d(None, C.byref(d), C.byref(p), 1, A, 1 << 31), RBT_E_INVALID, "tokens")
+    _refused(rbt_lib, rbt_lib.rbt_rope_d(None, C.byref(d), C.byref(p), 1, A, 1 << 24), RBT_E_UNSUPPORTED, "tokens")
 
 
 @pytest.mark.parametrize("desc,args,status,text", [
     (dict(n_heads=6), {}, RBT_E_INVALID, "shape"), (dict(n_kv_heads=0), {}, RBT_E_INVALID, "shape"),
     (dict(n_heads=0), {}, RBT_E_INVALID, "shape"), (dict(head_dim=0), {}, RBT_E_UNSUPPORTED, "head_dim"),
     (dict(head_dim=1088), {}, RBT_E_UNSUPPORTED, "head_dim"), (dict(kv_dtype=3), {}, RBT_E_INVALID, "type"),
-    (dict(attn_scale=float("nan")), {}, RBT_E_INVALID, "attn_scale"), (dict(cap=0), {}, RBT_E_INVALID, "rows"),
+    (dict(attn_scale=float("nan")), {}, RBT_E_INVALID, "attn_scale"), (dict(attn_scale=3e38), {}, RBT_E_INVALID, "attn_scale"), (dict(cap=0), {}, RBT_E_INVALID, "rows"),
     (dict(max_len=101), {}, RBT_E_INVALID, "max_len"), (dict(gate_head_stride=1 << 41), dict(gate=A), RBT_E_INVALID, "stride"),
     ({}, dict(T=0), RBT_E_INVALID, "step"), ({}, dict(T=257), RBT_E_UNSUPPORTED, "nodes"), ({}, dict(B=65536), RBT_E_INVALID, "step"),
     ({}, dict(q=None), RBT_E_INVALID, "null"), ({}, dict(kd=None), RBT_E_INVALID, "null"), ({}, dict(out=None), RBT_E_INVALID, "null"),

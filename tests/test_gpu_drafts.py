@@ -264,6 +264,14 @@ def test_tree_attention_lengths(ctx, L, kv16):
     _attend(ctx, 2, 3, 8, 2, 128, [L, L // 2], [3, 2], kv16=kv16)
 
 
+@pytest.mark.parametrize("kv16", [False, True])
+@pytest.mark.parametrize("H,K,D,N", [(16, 1, 64, 33), (16, 1, 256, 20), (48, 3, 192, 9), (8, 1, 128, 70), (1, 1, 64, 256)])
+def test_tree_attention_ragged(ctx, H, K, D, N, kv16):
+    """Row tiles over several workgroups and waves without rows: counts from none to all, several pieces of the
+    cache beside none."""
+    _attend(ctx, 4, N, H, K, D, [700, 90, 0, 1300], [N, N // 2 + 1, 1, 0], kv16=kv16, gate=True)
+
+
 @pytest.mark.parametrize("kv16,N", [(False, 1), (True, 1), (False, 6), (True, 20)])
 def test_tree_attention_qwen(ctx, kv16, N):
     """Qwen 3.8's heads with the gate inside q_proj's rows; max_len below and at the lengths."""
@@ -272,13 +280,13 @@ def test_tree_attention_qwen(ctx, kv16, N):
         assert rel_l2(g, got[0]) < 2e-6
 
 
-@pytest.mark.parametrize("D", [64, 80])
+@pytest.mark.parametrize("D,H", [(64, 4), (80, 4), (64, 32), (256, 32), (128, 2)])
 @pytest.mark.parametrize("kv16", [False, True])
-def test_tree_attention_masked_values(ctx, D, kv16):
+def test_tree_attention_masked_values(ctx, D, H, kv16):
     """NaN, infinities and the largest values in nodes that others do not see; a node that sees one has it."""
     import torch
     rng = np.random.default_rng(3)
-    N, H, K, L = 12, 4, 2, 40
+    N, K, L = 12, 2, 40
     big = float(np.finfo(np.float32).max) if not kv16 else 3.0e38
 
     def edit(q, kc, vc, kd, vd, par):
@@ -385,6 +393,18 @@ def test_verify(ctx, B, N, V, shape, children, drawn):
     u = rng.random((B, N), dtype=np.float32)
     path, n_path, _ = _verify(ctx, tok, par, n, p, q if drawn else None, u, children)
     assert n_path.max() <= N
+
+
+def test_verify_children_past_the_hint(ctx):
+    """max_children changes only how the work is launched: a tree of many children called a chain."""
+    rng = np.random.default_rng(3)
+    B, N, V = 3, 40, 9000
+    p, q = (_softmax(rng.standard_normal((B, N, V)) * 3) for _ in range(2))
+    par = np.where(np.arange(N) == 0, -1, 0)[None].repeat(B, 0).astype(np.int32)
+    tok = rng.integers(0, V, (B, N)).astype(np.int32)
+    u = (0.5 + 0.5 * rng.random((B, N))).astype(np.float32).clip(0, np.float32(1 - 2.0 ** -24))
+    for hint in (1, 2, 0, 1 << 40):
+        _verify(ctx, tok, par, [N] * B, p, q, u, hint)
 
 
 def test_verify_borders(ctx):
