@@ -64,7 +64,8 @@ __global__ __launch_bounds__(256) void k_rope_any(RopeArgs a) {
         const bool first = a.pairs ? !(k & 1) : k < half;
         const int d = a.pairs ? 1 : half;
         const float y = x[first ? i + d : i - d];
-        v = first ? __fsub_rn(__fmul_rn(v, cs[j]), __fmul_rn(y, sn[j])) : __fadd_rn(__fmul_rn(v, cs[j]), __fmul_rn(y, sn[j]));
+        const float vc = __fmul_rn(v, cs[j]), ys = __fmul_rn(y, sn[j]);
+        v = first ? __fsub_rn(vc, ys) : __fadd_rn(vc, ys);
       }
       if (p.d16)
         ((uint16_t *)p.dst)[dof + i] = rbt_f32_bf16(v);
@@ -133,7 +134,8 @@ __global__ __launch_bounds__(256) void k_rope(RopeArgs a, int G) {
       }
       if (h >= p.heads) q[u][0] = q[u][1] = -1;
 #pragma unroll
-      for (int e = 0; e < 2; e++) x[u][e] = q[u][e] >= 0 ? rope_ld(p, so + 4 * q[u][e]) : make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int e = 0; e < 2; e++)
+        x[u][e] = q[u][e] >= 0 ? rope_ld(p, so + 4 * q[u][e]) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     return true;
   };
@@ -151,7 +153,8 @@ __global__ __launch_bounds__(256) void k_rope(RopeArgs a, int G) {
 #pragma unroll
         for (int e = 0; e < 2; e++) {
           const float4 v = x[u][e];
-          ss += ((double)v.x * (double)v.x + (double)v.y * (double)v.y) + ((double)v.z * (double)v.z + (double)v.w * (double)v.w);
+          ss += ((double)v.x * (double)v.x + (double)v.y * (double)v.y) +
+                ((double)v.z * (double)v.z + (double)v.w * (double)v.w);
         }
       for (int d = 1; d < G; d <<= 1) ss += __shfl_xor(ss, d, 64);
       const float rr = __fdiv_rn(1.0f, rbt_sqrt_rn(__fadd_rn((float)(ss / (double)a.hd), a.eps)));
@@ -162,8 +165,10 @@ __global__ __launch_bounds__(256) void k_rope(RopeArgs a, int G) {
           if (q[u][e] < 0) continue;
           const float *w = p.norm + 4 * q[u][e];
           float4 &v = x[u][e];
-          v = make_float4(__fmul_rn(v.x, __fmul_rn(rr, __fadd_rn(1.0f, w[0]))), __fmul_rn(v.y, __fmul_rn(rr, __fadd_rn(1.0f, w[1]))),
-                          __fmul_rn(v.z, __fmul_rn(rr, __fadd_rn(1.0f, w[2]))), __fmul_rn(v.w, __fmul_rn(rr, __fadd_rn(1.0f, w[3]))));
+          v.x = __fmul_rn(v.x, __fmul_rn(rr, __fadd_rn(1.0f, w[0])));
+          v.y = __fmul_rn(v.y, __fmul_rn(rr, __fadd_rn(1.0f, w[1])));
+          v.z = __fmul_rn(v.z, __fmul_rn(rr, __fadd_rn(1.0f, w[2])));
+          v.w = __fmul_rn(v.w, __fmul_rn(rr, __fadd_rn(1.0f, w[3])));
         }
     }
     if (p.rotate && !a.pairs) {
@@ -172,10 +177,15 @@ __global__ __launch_bounds__(256) void k_rope(RopeArgs a, int G) {
         if (gl + G * u < a.rd / 8) {
           const float4 c = *(const float4 *)(cs + 4 * (gl + G * u)), s = *(const float4 *)(sn + 4 * (gl + G * u));
           const float4 v = x[u][0], y = x[u][1];
-          x[u][0] = make_float4(__fsub_rn(__fmul_rn(v.x, c.x), __fmul_rn(y.x, s.x)), __fsub_rn(__fmul_rn(v.y, c.y), __fmul_rn(y.y, s.y)),
-                                __fsub_rn(__fmul_rn(v.z, c.z), __fmul_rn(y.z, s.z)), __fsub_rn(__fmul_rn(v.w, c.w), __fmul_rn(y.w, s.w)));
-          x[u][1] = make_float4(__fadd_rn(__fmul_rn(y.x, c.x), __fmul_rn(v.x, s.x)), __fadd_rn(__fmul_rn(y.y, c.y), __fmul_rn(v.y, s.y)),
-                                __fadd_rn(__fmul_rn(y.z, c.z), __fmul_rn(v.z, s.z)), __fadd_rn(__fmul_rn(y.w, c.w), __fmul_rn(v.w, s.w)));
+          float4 &a0 = x[u][0], &a1 = x[u][1];
+          a0.x = __fsub_rn(__fmul_rn(v.x, c.x), __fmul_rn(y.x, s.x));
+          a0.y = __fsub_rn(__fmul_rn(v.y, c.y), __fmul_rn(y.y, s.y));
+          a0.z = __fsub_rn(__fmul_rn(v.z, c.z), __fmul_rn(y.z, s.z));
+          a0.w = __fsub_rn(__fmul_rn(v.w, c.w), __fmul_rn(y.w, s.w));
+          a1.x = __fadd_rn(__fmul_rn(y.x, c.x), __fmul_rn(v.x, s.x));
+          a1.y = __fadd_rn(__fmul_rn(y.y, c.y), __fmul_rn(v.y, s.y));
+          a1.z = __fadd_rn(__fmul_rn(y.z, c.z), __fmul_rn(v.z, s.z));
+          a1.w = __fadd_rn(__fmul_rn(y.w, c.w), __fmul_rn(v.w, s.w));
         }
     } else if (p.rotate) {
 #pragma unroll
@@ -204,8 +214,8 @@ static bool rope_quads(const RopeArgs &a) {
   if (a.hd % 4 || a.start % 4 || a.rd % (a.pairs ? 4 : 8)) return false;
   for (int i = 0; i < a.n_parts; i++) {
     const RopePartD &p = a.part[i];
-    if ((p.sts | p.shs | p.dts | p.dhs) % 4 || (uintptr_t)p.src % (p.s16 ? 8 : 16) || (uintptr_t)p.dst % (p.d16 ? 8 : 16))
-      return false;
+    if ((p.sts | p.shs | p.dts | p.dhs) % 4) return false;
+    if ((uintptr_t)p.src % (p.s16 ? 8 : 16) || (uintptr_t)p.dst % (p.d16 ? 8 : 16)) return false;
   }
   return true;
 }
@@ -335,7 +345,8 @@ __device__ double vf_sum(const VerifyRow &row, int lo, int hi, bool quads, doubl
 }
 
 __device__ __forceinline__ void vf_put(double *p, double v) {
-  __hip_atomic_store((unsigned long long *)p, (unsigned long long)__double_as_longlong(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __hip_atomic_store((unsigned long long *)p, (unsigned long long)__double_as_longlong(v), __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
 }
 __device__ __forceinline__ double vf_get(double *p) {
   return __longlong_as_double(
@@ -613,7 +624,9 @@ hipError_t launch_verify(const Ctx &c, VerifyArgs a, int B, int max_children, vo
 }
 
 // ---- commit --------------------------------------------------------------------------------------
-// grid (sequences, sides of the launch's layers); U: the unit of the copy.
+// grid (sequences, sides of the launch's layers); U: the unit of the copy. The K and V rows of up to 32 layers go in
+// one launch: three rows of 23 layers 3-4 us (the launch), 32 sequences' (28 MB in and out) 6-7 us, against one launch
+// per layer and side.
 template <typename U>
 __global__ __launch_bounds__(256) void k_commit(CommitArgs a, const int *__restrict__ path, const int *__restrict__ n_path,
                                                 const int *__restrict__ len, int T, int cap, int row_units,

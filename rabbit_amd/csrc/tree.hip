@@ -2,6 +2,20 @@
 //
 // Node i of sequence b sees the len[b] committed rows, itself and its ancestors: with s_j = scale q . k_j over
 // those, out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m), times sigmoid(gate) (qwen38/attention.rs:190-226).
+//
+//   k_tree       head dims 64, 128, 192, 256: one pass over a piece of the cache and the drafted rows on the matrix
+//                cores, with the running maximum and sum; writes the output, or the piece's partial sums
+//   k_tree_join  the pieces' partial sums joined
+//   k_tree_any   any head dim: fp32 multiply-adds, one workgroup per query head and node
+//
+// Bounds and times (64 query heads over 4 KV heads of 256, one MI355X):
+//   64 nodes over 32749 bf16 rows: 302-314 us, of them 280-290 in k_tree: 412 GFLOP of bf16 products, 1.4 PFLOP/s (a
+//     large library product reaches 1.2); the matrix cores are busy 61% of the cycles, at a clock that the load holds
+//     near 2 GHz.
+//   16 trees of 12 to 24 nodes over 4096 to 8192 bf16 rows: 361-368 us, k_tree 329-337; the products as above, and
+//     row tiles and pieces that do not fill every CU to the end.
+//   one node over 32768 bf16 rows: 35 us, k_tree 26 (134 MB: 5.1 TB/s); over 513 rows: 13.5 us, two launches of one
+//     trip to memory each; five nodes over 4096 f32 rows: 35 us.
 #include "rbt_device.h"
 #include "rbt_internal.h"
 
@@ -118,12 +132,16 @@ __global__ __launch_bounds__(256) void k_tree_any(TreeArgs a) {
 // the running maximum and sum of a row are the lane's own (joined over the four lanes of a column).
 //   bf16 caches: q and p are split into three bf16 parts that hold their 24 bits exactly (by truncation: 8 bits
 //     each), so every product is exact and only the fp32 sums round, at three times the products.
-//   f32 caches: fp32 MFMAs.
+//   f32 caches, one or two row tiles: fp32 MFMAs, which keep up with memory there (32 rows: 128 cycles a key of
+//     the 157 that its 2 KB take a CU's share of the bandwidth).
+//   f32 caches, more row tiles: keys and values are split too, once per workgroup on their way into LDS, at six
+//     products (those below 2^-24 of the whole left out): 64 nodes over 8192 rows 202 us, 307 with fp32 MFMAs.
 // A workgroup of RW x KW waves takes RW row tiles and one piece of the keys: KW groups of waves share out each
-// stage's keys (few rows: every wave has its own keys; many rows: every wave has its own rows). Stages of TK keys
-// land in LDS by direct loads (global_load_lds, 16 bytes per lane), two stages in turn: while one is multiplied the
-// next is in flight. LDS rows hold their 16-byte chunks in an order turned by the row's number, so that
-// the columns read at once lie in different banks.
+// stage's keys (few rows: every wave has its own keys; many rows: every wave has its own rows, up to eight waves: with
+// four, two workgroups per CU, 64 nodes over 32749 rows took 348 us against 311). Stages of TK keys land in LDS by
+// direct loads (global_load_lds, 16 bytes per lane), two stages in turn: while one is multiplied the next is in
+// flight. (Split rows pass through registers, and have one buffer: its 96 KB at head_dim 256 leave no room.)
+// Wave priorities that let one wave of a SIMD run ahead of the other changed nothing (297 us either way).
 typedef float tf4 __attribute__((ext_vector_type(4)));
 typedef short ts4 __attribute__((ext_vector_type(4)));
 typedef __bf16 tb8 __attribute__((ext_vector_type(8)));
@@ -142,7 +160,9 @@ __device__ __forceinline__ void tree_split(float x, uint32_t &hi, uint32_t &mid,
   lo = __float_as_uint(r - __uint_as_float(mid));
 }
 // The high halves of a and b as two bf16 (a low).
-__device__ __forceinline__ uint32_t tree_pack(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+__device__ __forceinline__ uint32_t tree_pack(uint32_t a, uint32_t b) {
+  return __builtin_amdgcn_perm(b, a, 0x07060302u);
+}
 
 __device__ __forceinline__ float tree_xor_max(float v) {
   v = fmaxf(v, __shfl_xor(v, 16, 64));
@@ -172,11 +192,16 @@ struct TreeTile {
   // two cycles: half of the LDS's cycles at 64 nodes over 32749 rows.)
   static constexpr bool WIDE = CH % 16 == 0;  // rows of whole 256 bytes; others begin half a cycle apart
   static __device__ __forceinline__ int k_turn(int r) { return WIDE ? r & 15 : r & 7; }
-  static __device__ __forceinline__ int v_turn(int r) { return KV == KV_F32 ? 0 : WIDE ? (r & 7) << 1 : (r >> 1 & 3) << 1; }
+  static __device__ __forceinline__ int v_turn(int r) {
+    return KV == KV_F32 ? 0 : WIDE ? (r & 7) << 1 : (r >> 1 & 3) << 1;
+  }
 };
 
-// A row's node, row / n_rep: magic = ceil(2^32 / n_rep), exact since row * n_rep < 2^32 (at most 2^20 rows, 2^12 heads).
-__device__ __forceinline__ int tree_div(int row, const TreeArgs &a) { return a.R == 1 ? row : (int)__umulhi(row, a.magic); }
+// A row's node, row / n_rep: magic = ceil(2^32 / n_rep), exact since row * n_rep < 2^32 (at most 2^20 rows and 2^12
+// query heads).
+__device__ __forceinline__ int tree_div(int row, const TreeArgs &a) {
+  return a.R == 1 ? row : (int)__umulhi(row, a.magic);
+}
 
 // Keys of a piece and pieces of a sequence of L committed rows; one longer than expected takes larger pieces.
 __device__ __forceinline__ void tree_pieces(const TreeArgs &a, int L, int TK, unsigned &per, unsigned &np) {
@@ -185,7 +210,8 @@ __device__ __forceinline__ void tree_pieces(const TreeArgs &a, int L, int TK, un
   if (a.pieces == 1 && L > 0) {
     per = L;
   } else if (L > 0) {
-    if ((unsigned)L > (unsigned long long)per * a.pieces) per = (((unsigned)L + a.pieces - 1) / a.pieces + TK - 1) / TK * TK;
+    if ((unsigned)L > (unsigned long long)per * a.pieces)
+      per = (((unsigned)L + a.pieces - 1) / a.pieces + TK - 1) / TK * TK;
     np = ((unsigned)L + per - 1) / per;
   }
 }
@@ -290,7 +316,8 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
         uint32_t o[3][4];
 #pragma unroll
         for (int e = 0; e < 4; e++) tree_split(v[e], o[0][e], o[1][e], o[2][e]);
-        char *to = smem + side * TT::SIDE + r * ROWB + (((c >> 1) ^ (side ? TT::v_turn(r) : TT::k_turn(r))) * 16) + (c & 1) * 8;
+        const int at = (c >> 1) ^ (side ? TT::v_turn(r) : TT::k_turn(r));
+        char *to = smem + side * TT::SIDE + r * ROWB + at * 16 + (c & 1) * 8;
 #pragma unroll
         for (int p = 0; p < 3; p++)
           *(uint2 *)(to + p * TT::PART) = make_uint2(tree_pack(o[p][0], o[p][1]), tree_pack(o[p][2], o[p][3]));
@@ -303,7 +330,7 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
     issue(0);
 
   // this lane's row, and its query in the B operand's layout
-  const bool active = rg < RW && row0 + rg * 16 < rows;  // a wave without rows only loads
+  const bool active = rg < RW && kgp < KW && row0 + rg * 16 < rows;  // a wave without rows or keys only loads
   const int row = row0 + rg * 16 + col, rc = min(row, rows - 1);
   const int node = tree_div(rc, a), head = kv * R + (rc - node * R);
   const long qrow = ((long)b * a.T + node) * a.H + head;
@@ -498,9 +525,11 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
 #pragma unroll
         for (int d = 0; d < 2; d++)
 #pragma unroll
-          for (int e = 0; e < XS; e++)
+          for (int e = 0; e < XS; e++) {
+            const int tile = (dt + d) / VP * VP + (((dt + d) % VP) ^ turn);
             to[d][e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (tree_lds_s4 *)(vb + (dt + d) / VP * VP * 32 + (((dt + d) % VP) ^ turn) * 32 + f * TT::PART + (x + e) * 16 * ROWB));
+                (tree_lds_s4 *)(vb + tile * 32 + f * TT::PART + (x + e) * 16 * ROWB));
+          }
       };
       read(0, vf[0]);
 #pragma unroll
@@ -514,12 +543,13 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
           for (int d = 0; d < 2; d++) {
             if constexpr (XS == 2) {
               struct { ts4 lo, hi; } vv{vf[i & 1][d][0], vf[i & 1][d][1]};
-              o[dt + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                  __builtin_bit_cast(tb8, vv),
-                  __builtin_bit_cast(tb8, rbt_u4{pp[x][p][0], pp[x][p][1], pp[x + 1][p][0], pp[x + 1][p][1]}), o[dt + d], 0, 0, 0);
+              const rbt_u4 pv{pp[x][p][0], pp[x][p][1], pp[x + 1][p][0], pp[x + 1][p][1]};
+              o[dt + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(tb8, vv),
+                                                                  __builtin_bit_cast(tb8, pv), o[dt + d], 0, 0, 0);
             } else {
               struct { uint32_t x, y; } pv{pp[0][p][0], pp[0][p][1]};
-              o[dt + d] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(vf[i & 1][d][0], __builtin_bit_cast(ts4, pv), o[dt + d], 0, 0, 0);
+              o[dt + d] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(vf[i & 1][d][0], __builtin_bit_cast(ts4, pv),
+                                                                    o[dt + d], 0, 0, 0);
             }
           }
       }
@@ -569,7 +599,7 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
   if constexpr (KW > 1) {
     // join the key groups in LDS: every group's O and l scaled to the row's largest maximum
     constexpr int ST = HD + 4;
-    if (kg == 0) {
+    if (kgp < KW && kg == 0) {
       ml[w][0][col] = m;
       ml[w][1][col] = l;
     }
@@ -577,23 +607,24 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
     float M = -INFINITY;
     for (int k = 0; k < KW; k++) M = fmaxf(M, ml[k * RW + rg][0][col]);
     const float Ms = M == -INFINITY ? 0.0f : M;
-    float lt = 0.0f;
-    for (int k = 0; k < KW; k++) lt += ml[k * RW + rg][1][col] * __builtin_amdgcn_exp2f(ml[k * RW + rg][0][col] - Ms);
     const float f = __builtin_amdgcn_exp2f(m - Ms);
     float *oj = (float *)smem;
 #pragma unroll
     for (int d = 0; d < HD / 16; d++) {
+      if (kgp >= KW) break;
+      float *to = oj + (w * 16 + col) * ST;
       if constexpr (B16) {
-        *(float4 *)(oj + (w * 16 + col) * ST + 16 * d + 4 * kg) = make_float4(o[d][0] * f, o[d][1] * f, o[d][2] * f, o[d][3] * f);
+        *(float4 *)(to + 16 * d + 4 * kg) = make_float4(o[d][0] * f, o[d][1] * f, o[d][2] * f, o[d][3] * f);
       } else {
-        *(float4 *)(oj + (w * 16 + col) * ST + 64 * (d >> 2) + 16 * kg + 4 * (d & 3)) =
-            make_float4(o[d & ~3][d & 3] * f, o[(d & ~3) + 1][d & 3] * f, o[(d & ~3) + 2][d & 3] * f, o[(d & ~3) + 3][d & 3] * f);
+        const int g = d & ~3, e = d & 3;
+        *(float4 *)(to + 16 * g + 16 * kg + 4 * e) =
+            make_float4(o[g][e] * f, o[g + 1][e] * f, o[g + 2][e] * f, o[g + 3][e] * f);
       }
     }
     lds_barrier();
-    // the group's waves share its rows' entries
+    // the waves of a row tile (those that only loaded too) share its rows' entries
     constexpr int Q4 = HD / 4;
-    for (int u = kgp * 64 + lane; u < 16 * Q4; u += 64 * KW) {
+    for (int u = kgp * 64 + lane; u < 16 * Q4; u += 64 * (NW / RW)) {
       const int r = u / Q4, e = u - r * Q4, rr = row0 + rg * 16 + r;
       if (rr >= rows) continue;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -613,7 +644,6 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
         if (e == 0) pm[r] = make_float2(Mr, lr);
       }
     }
-    (void)lt;
   } else {
     static_assert(B16, "the values' tiles are 16 entries wide");
     if (!active) return;
@@ -731,10 +761,13 @@ bool tree_plan(const Ctx &c, TreeArgs &a) {
   // and ends in 7, takes `stage` per stage (measured at head_dim 256; it goes with the head dim), and several pieces
   // cost a second launch and a write and read of their rows' partial sums. Equal sequences end together, so their
   // workgroups count by whole rounds of the chip; those of a batch are of any length: past one round they fill it
-  // evenly, at about 0.8 of the longest each, and the last ones are waited for. Measured over bf16 and head_dim 256: one node over 4096 rows 113 us in one piece,
-  // 27 in 8, 17 in 32, 17 in 64; 64 nodes over 32749 rows 527 in 4, 311 in 8, 326 in 16, 368 in 32.
+  // evenly, at about 0.8 of the longest each, and the last ones are waited for. Measured over bf16 rows at head_dim
+  // 256: one node over 4096 rows 113 us in one piece, 27 in 8, 17 in 32, 17 in 64; 64 nodes over 32749 rows 527 in
+  // 4, 311 in 8, 326 in 16, 368 in 32; 16 sequences of one node over 3000 to 6000 rows 186 in 1, 65 in 4, 74 in 8,
+  // 86 in 16.
   const double base = (double)a.tiles * a.K * a.B, most = std::ceil((double)(a.max_len + a.T) / TK), ncu = c.num_cu;
-  const double stage = (kw > 1 ? (a.kv16 ? 1.6 : 2.6) : a.kv16 ? (rw > 4 ? 4.4 : 2.6) : (rw > 4 ? 8.5 : 4.5)) * a.hd / 256.0;
+  const double us = kw > 1 ? (a.kv16 ? 1.6 : 2.6) : a.kv16 ? (rw > 4 ? 4.4 : 2.6) : (rw > 4 ? 6.5 : 4.0);
+  const double stage = us * a.hd / 256.0;
   const double bytes = (double)a.B * a.K * a.t16 * 16 * a.hd * 8.0;
   double best = 0.0;
   long pieces = 1;
@@ -768,14 +801,17 @@ static hipError_t run_tree(const Ctx &c, const TreeArgs &a) {
   const long groups = (long)a.pieces * a.K * a.B;
   const long blocks = (groups + 7) / 8 * 8 * a.tiles;
   const dim3 grid = a.tiles > 1 ? dim3((unsigned)blocks) : dim3(a.pieces, a.K, a.B);
-  launch_ks(c, k_tree<HD, KV, KW>, grid, dim3(KV == KV_PARTS ? TREE_PARTS_NT : 64 * a.rw * KW), (unsigned)lds, a);
+  const int threads = KV == KV_PARTS ? TREE_PARTS_NT : KW > 1 ? 256 : 64 * a.rw;
+  launch_ks(c, k_tree<HD, KV, KW>, grid, dim3(threads), (unsigned)lds, a);
   return hipGetLastError();
 }
 
 template <int HD>
 static hipError_t run_tree_hd(const Ctx &c, const TreeArgs &a) {
   if (a.kv16)
-    return a.kw == 4 ? run_tree<HD, KV_BF16, 4>(c, a) : a.kw == 2 ? run_tree<HD, KV_BF16, 2>(c, a) : run_tree<HD, KV_BF16, 1>(c, a);
+    return a.kw == 4   ? run_tree<HD, KV_BF16, 4>(c, a)
+           : a.kw == 2 ? run_tree<HD, KV_BF16, 2>(c, a)
+                       : run_tree<HD, KV_BF16, 1>(c, a);
   return a.kw == 2 ? run_tree<HD, KV_F32, 2>(c, a) : run_tree<HD, KV_PARTS, 1>(c, a);
 }
 
