@@ -14,8 +14,8 @@
 //     near 2 GHz.
 //   16 trees of 12 to 24 nodes over 4096 to 8192 bf16 rows: 361-368 us, k_tree 329-337; the products as above, and
 //     row tiles and pieces that do not fill every CU to the end.
-//   one node over 32768 bf16 rows: 35 us, k_tree 26 (134 MB: 5.1 TB/s); over 513 rows: 13.5 us, two launches of one
-//     trip to memory each; five nodes over 4096 f32 rows: 35 us.
+//   one node over 32768 bf16 rows: 35 us, k_tree 26 (134 MB: 5.1 TB/s); over 513 rows: 13.3 us, two launches of one
+//     trip to memory each; five nodes over 4096 f32 rows: 34 us.
 #include "rbt_device.h"
 #include "rbt_internal.h"
 
@@ -668,29 +668,31 @@ __global__ __launch_bounds__(256) void k_tree_join(TreeArgs a, int TK) {
   const int t = threadIdx.x, w = t >> 6, lane = t & 63, col = lane & 15, kv = blockIdx.y, b = blockIdx.z;
   const int nd = a.hd / 16, tile = WP > 1 ? blockIdx.x / nd : blockIdx.x * 4 / nd;
   const int d = WP > 1 ? blockIdx.x - tile * nd : blockIdx.x * 4 - tile * nd + w;
-  const int n = a.n_nodes[b], L = a.len[b];
-  if (n < 0 || n > a.T || L < 0 || L > a.cap || tile * 16 >= n * a.R) return;
-  unsigned per, np;
-  tree_pieces(a, L, TK, per, np);
-  if (np <= 1) return;
   const long ps = (long)a.B * a.K * a.t16, unit = ((long)b * a.K + kv) * a.t16 + tile;
-  // the rows' largest maximum, then each piece's weight and the rows' sums: thread t takes row t % 16 (of up to 256
-  // pieces: all are loaded at once, and so are this wave's first sums)
-  const int r = t & 15, j0 = t >> 4;
+  // Thread t takes row t % 16's maxima and sums (of up to 256 pieces: all are loaded at once, and so are this wave's
+  // first partial outputs), ahead of the sequence's own numbers: pieces that it does not have are read, not used (one
+  // node over 513 rows 13.6 -> 13.3 us, 64 over 32749 330 -> 328, on one MI355X in turn).
+  const int r = t & 15, j0 = t >> 4, most = a.pieces - 1;
   float2 x[16];
 #pragma unroll
   for (int k = 0; k < 16; k++)
-    if (16 * k < (int)np) x[k] = a.part_ml[(min(j0 + 16 * k, (int)np - 1) * ps + unit) * 16 + r];
+    if (16 * k <= most) x[k] = a.part_ml[(min(j0 + 16 * k, most) * ps + unit) * 16 + r];
   constexpr int PF = 8;
-  const unsigned first = WP > 1 ? w : 0;
+  const int first = WP > 1 ? w : 0;
   const float *po = a.part + unit * 16 * a.hd + (d * 64 + lane) * 4;
   float4 y[PF];
 #pragma unroll
-  for (int k = 0; k < PF; k++) y[k] = *(const float4 *)(po + min(first + k * WP, np - 1) * ps * 16 * a.hd);
+  for (int k = 0; k < PF; k++) y[k] = *(const float4 *)(po + min(first + k * WP, most) * ps * 16 * a.hd);
+  const int n = a.n_nodes[b], L = a.len[b];
+  if (n < 0 || n > a.T || L < 0 || L > a.cap || tile * 16 >= n * a.R) return;
+  unsigned per, pieces;
+  tree_pieces(a, L, TK, per, pieces);
+  const int np = (int)pieces;
+  if (np <= 1) return;
   float M = -INFINITY;
 #pragma unroll
   for (int k = 0; k < 16; k++)
-    if (16 * k < (int)np) M = fmaxf(M, x[k].x);
+    if (j0 + 16 * k < np) M = fmaxf(M, x[k].x);
   red[j0][r] = M;
   __syncthreads();
 #pragma unroll
@@ -700,7 +702,7 @@ __global__ __launch_bounds__(256) void k_tree_join(TreeArgs a, int TK) {
 #pragma unroll
   for (int k = 0; k < 16; k++) {
     const int j = j0 + 16 * k;
-    if (j >= (int)np) break;
+    if (j >= np) break;
     const float f = __builtin_amdgcn_exp2f(x[k].x - Ms);
     wt[j][r] = f;
     l += x[k].y * f;
@@ -712,7 +714,7 @@ __global__ __launch_bounds__(256) void k_tree_join(TreeArgs a, int TK) {
 #pragma unroll
   for (int k = 0; k < 16; k++) l += red[k][col];
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto add = [&](float4 y, unsigned j) {
+  auto add = [&](float4 y, int j) {
     const float f = wt[j][col];
     v = make_float4(v.x + y.x * f, v.y + y.y * f, v.z + y.z * f, v.w + y.w * f);
   };
@@ -720,7 +722,7 @@ __global__ __launch_bounds__(256) void k_tree_join(TreeArgs a, int TK) {
   for (int k = 0; k < PF; k++)
     if (first + k * WP < np) add(y[k], first + k * WP);
 #pragma unroll 8
-  for (unsigned j = first + PF * WP; j < np; j += WP) add(*(const float4 *)(po + j * ps * 16 * a.hd), j);
+  for (int j = first + PF * WP; j < np; j += WP) add(*(const float4 *)(po + j * ps * 16 * a.hd), j);
   if constexpr (WP > 1) {
     sum[w][lane] = v;
     __syncthreads();
