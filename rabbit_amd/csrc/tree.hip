@@ -19,6 +19,7 @@
 #include "rbt_device.h"
 #include "rbt_internal.h"
 
+#include <atomic>
 #include <cmath>
 
 namespace rbt {
@@ -737,6 +738,36 @@ __global__ __launch_bounds__(256) void k_tree_join(TreeArgs a, int TK) {
   if (i < n) tree_store(a, b, i, kv * a.R + (row - i * a.R), 16 * d + 4 * (lane >> 4), v, l);
 }
 
+// Workgroups of `threads` that a CU holds at once (their LDS and registers), asked once per kernel and size.
+template <int HD, int KV, int KW>
+static int tree_per_cu(int threads) {
+  static std::atomic<int> known[9];  // by waves, up to 8
+  std::atomic<int> &k = known[threads / 64];
+  int n = k.load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, k_tree<HD, KV, KW>, threads, TreeTile<HD, KV>::LDS) !=
+        hipSuccess) {
+      (void)hipGetLastError();
+      n = 1;
+    }
+    n = std::max(n, 1);
+    k.store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+template <int KV, int KW>
+static int tree_per_cu(int hd, int threads) {
+  return hd == 64    ? tree_per_cu<64, KV, KW>(threads)
+         : hd == 128 ? tree_per_cu<128, KV, KW>(threads)
+         : hd == 192 ? tree_per_cu<192, KV, KW>(threads)
+                     : tree_per_cu<256, KV, KW>(threads);
+}
+
+// Threads of a workgroup.
+static int tree_threads(const TreeArgs &a) {
+  return a.kw > 1 ? 256 : a.kv16 ? 64 * a.rw : TREE_PARTS_NT;
+}
+
 // Pieces and row tiles for a call on the matrix cores.
 bool tree_plan(const Ctx &c, TreeArgs &a) {
   a.rw = a.kw = a.tiles = a.pieces = 1;
@@ -759,32 +790,56 @@ bool tree_plan(const Ctx &c, TreeArgs &a) {
   a.tiles = (t16 + rw - 1) / rw;
   a.rw = rw;
   a.kw = kw;
-  // Pieces by the time they should take, in microseconds: a workgroup (one per CU: its stages fill the LDS) starts
-  // and ends in 7, takes `stage` per stage (measured at head_dim 256; it goes with the head dim), and several pieces
-  // cost a second launch and a write and read of their rows' partial sums. Equal sequences end together, so their
-  // workgroups count by whole rounds of the chip; those of a batch are of any length: past one round they fill it
-  // evenly, at about 0.8 of the longest each, and the last ones are waited for. Measured over bf16 rows at head_dim
-  // 256: one node over 4096 rows 113 us in one piece, 27 in 8, 17 in 32, 17 in 64; 64 nodes over 32749 rows 527 in
-  // 4, 311 in 8, 326 in 16, 368 in 32; 16 sequences of one node over 3000 to 6000 rows 186 in 1, 65 in 4, 74 in 8,
-  // 86 in 16.
-  const double base = (double)a.tiles * a.K * a.B, most = std::ceil((double)(a.max_len + a.T) / TK), ncu = c.num_cu;
-  const double us = kw > 1 ? (a.kv16 ? 1.6 : 2.6) : a.kv16 ? (rw > 4 ? 4.4 : 2.6) : (rw > 4 ? 6.5 : 4.0);
-  const double stage = us * a.hd / 256.0;
+  // Pieces by the time they should take, in microseconds. A workgroup starts and ends in 7 and takes `stage` per stage
+  // (measured at head_dim 256, where a CU holds one; it goes with the head dim), and several pieces cost a second
+  // launch and a write and read of their rows' partial sums. Equal sequences end together, so their workgroups count
+  // by whole rounds of the chip; those of a batch are of any length: past one round they fill it evenly, at about
+  // 0.8 of the longest each, and the last ones are waited for. A batch at a smaller head dim runs `hold` workgroups
+  // beside each other on a CU: a stage is then mostly waiting, all but `busy` of it, and grows less with the head
+  // dim, until the caches pass at 5.0 TB/s (sequences taken at three quarters of the longest; a sixth less with one
+  // workgroup per CU, and evenly only where every CU has as many). Measured over bf16 rows at head_dim 256: one node
+  // over 4096 rows 113 us in one piece, 27 in 8, 17 in 32, 17 in 64; 64 nodes over 32749 rows 527 in 4, 311 in 8, 326
+  // in 16, 368 in 32; 16 sequences of one node over 3000 to 6000 rows 186 in 1, 65 in 4, 74 in 8, 86 in 16. And with
+  // 32 query heads over 8 KV heads, 32 sequences of up to 4096 rows (one piece fills every CU once): one node over
+  // f32 rows of 128 254 in 1, 189 in 2, 212 in 8, of 64 183 in 1, 88 in 3, 102 in 8; 12 nodes over bf16 rows of 128
+  // 133 in 1, 113 in 2, 124 in 8, of 64 90 in 1, 60 in 3, 66 in 8.
+  const bool wide = rw > 4;  // two waves on a SIMD
+  const double ncu = c.num_cu, base = (double)a.tiles * a.K * a.B, most = std::ceil((double)(a.max_len + a.T) / TK);
+  const double part = a.hd / 256.0;
+  double stage, busy = 1.0, hold = 1.0;
+  if (a.B == 1) {
+    stage = (kw > 1 ? (a.kv16 ? 1.6 : 2.6) : a.kv16 ? (wide ? 4.4 : 2.6) : (wide ? 6.5 : 4.0)) * part;
+  } else if (kw > 1) {
+    stage = (a.kv16 ? 1.6 : 2.6) * (0.3 + 0.7 * part);
+    busy = 0.25;
+    hold = a.kv16 ? (kw == 4 ? tree_per_cu<KV_BF16, 4>(a.hd, 256) : tree_per_cu<KV_BF16, 2>(a.hd, 256))
+                  : tree_per_cu<KV_F32, 2>(a.hd, 256);
+  } else if (a.kv16) {
+    stage = (wide ? 4.4 : 2.6) * (0.3 + 0.7 * part);
+    busy = wide ? 0.9 : 0.4;
+    hold = tree_per_cu<KV_BF16, 1>(a.hd, tree_threads(a));
+  } else {
+    stage = (a.hd == 256 ? (wide ? 6.5 : 4.0) : (wide ? 4.4 : 3.6)) * (0.1 + 0.9 * part);
+    busy = wide ? 0.9 : 0.65;
+    hold = tree_per_cu<KV_PARTS, 1>(a.hd, tree_threads(a));
+  }
   const double bytes = (double)a.B * a.K * a.t16 * 16 * a.hd * 8.0;
+  const double pass = a.B > 1 ? 0.75 * a.B * a.K * a.max_len * a.hd * (a.kv16 ? 4.0 : 8.0) / 5.0e6 : 0.0;
   double best = 0.0;
   long pieces = 1;
   auto consider = [&](long p) {
     // (partial sums of at most 256 MiB)
     if (p < 1 || p > 256 || (p > 1 && (p > most || bytes * p > 2.0 * (256u << 20)))) return;
-    const double one = 7.0 + stage * std::ceil(most / p);
-    const double rounds = base * p / ncu;
-    const double t = (rounds <= 1.0 ? one : a.B == 1 ? std::ceil(rounds) * one : (0.8 * rounds + 0.4) * one) +
-                     (p > 1 ? 4.0 + bytes * p / 1.2e7 : 0.0);
+    const double groups = base * p, rounds = groups / (ncu * hold), beside = std::min(hold, std::ceil(groups / ncu));
+    const double one = 7.0 + stage * std::max(1.0, beside * busy) * std::ceil(most / p);
+    double t = rounds <= 1.0 ? one : a.B == 1 ? std::ceil(rounds) * one : (0.8 * rounds + 0.4) * one;
+    t = std::max(t, pass * (rounds > 1.0 ? 1.0 : groups > ncu ? beside * ncu / groups : hold > 1.0 ? 1.2 : 1.0));
+    if (p > 1) t += 4.0 + bytes * p / 1.2e7;
     if (best == 0.0 || t < best) best = t, pieces = p;
   };
   consider(1);
   for (long p = 2; p <= 256; p += p < 16 ? 1 : p / 8) consider(p);
-  for (int k = 1; k <= 4; k++) consider((long)(k * ncu / base));
+  for (int k = 1; k <= 4; k++) consider((long)(k * ncu * hold / base));
   a.per = (unsigned)((long)((most + pieces - 1) / pieces) * TK);
   a.pieces = (int)std::max(1L, (a.max_len + a.per - 1) / (long)a.per);
   // a launch holds fewer than 2^32 threads in x
@@ -803,8 +858,7 @@ static hipError_t run_tree(const Ctx &c, const TreeArgs &a) {
   const long groups = (long)a.pieces * a.K * a.B;
   const long blocks = (groups + 7) / 8 * 8 * a.tiles;
   const dim3 grid = a.tiles > 1 ? dim3((unsigned)blocks) : dim3(a.pieces, a.K, a.B);
-  const int threads = KV == KV_PARTS ? TREE_PARTS_NT : KW > 1 ? 256 : 64 * a.rw;
-  launch_ks(c, k_tree<HD, KV, KW>, grid, dim3(threads), (unsigned)lds, a);
+  launch_ks(c, k_tree<HD, KV, KW>, grid, dim3(tree_threads(a)), (unsigned)lds, a);
   return hipGetLastError();
 }
 

@@ -315,6 +315,47 @@ def test_tree_attention_masked_values(ctx, D, H, kv16):
                 assert np.isnan(got[0, i]).all(), i
 
 
+@pytest.mark.parametrize("kv16", [False, True])
+@pytest.mark.parametrize("B,N,H,K,D,lens,counts,cap", [
+    (9, 12, 32, 4, 64, [4100, 0, 63, 2049, 1, 4096, 700, 64, 4099], [12, 12, 0, 5, 1, 12, 7, 12, 3], 4100),
+    (8, 40, 16, 1, 256, [3400, 100, 3333, 0, 65, 2000, 1500, 3399], [40, 17, 39, 40, 1, 0, 25, 9], 3400),
+    (6, 12, 16, 1, 64, [3, 0, 70, 1, 5, 2], [12, 3, 12, 1, 9, 12], 12000),
+    (6, 12, 16, 1, 192, [11999, 0, 70, 1, 5, 2], [12, 3, 12, 1, 9, 12], 12000),
+    (70, 6, 8, 1, 128, [37 * i % 1900 for i in range(70)], [i % 7 for i in range(70)], 1900),
+    (64, 6, 8, 1, 128, [1900] + [0] * 63, [6] * 64, 1900)])
+def test_tree_attention_batches(ctx, B, N, H, K, D, lens, counts, cap, kv16):
+    """Larger batches: lengths from none to all, several row tiles, caches far longer than what they hold, more
+    than a wave of sequences, one long sequence among empty ones."""
+    _attend(ctx, B, N, H, K, D, lens, counts, kv16=kv16, gate=True, cap=cap)
+
+
+@pytest.mark.parametrize("kv16", [False, True])
+def test_tree_attention_many_short(ctx, kv16):
+    """Many short sequences; non-finite values of one stay out of the others' rows."""
+    import torch
+    B, N, H, K, D, cap = 300, 12, 32, 8, 64, 200
+    rng = np.random.default_rng(17)
+    lens, counts = rng.integers(0, cap + 1, B), rng.integers(0, N + 1, B)
+    _attend(ctx, B, N, H, K, D, lens.tolist(), counts.tolist(), kv16=kv16, cap=cap)
+    dt = torch.bfloat16 if kv16 else torch.float32
+    q = rng.standard_normal((B, N, H, D)).astype(np.float32)
+    kc, vc = (_bf(rng.standard_normal((B, cap, K, D))) for _ in range(2))
+    kd, vd = (_bf(rng.standard_normal((B, N, K, D))) for _ in range(2))
+    par = np.tile(np.array([[-1] + [0] * (N - 1)], np.int32), (B, 1))  # node 1 is seen by itself only
+    outs = []
+    for bad in (False, True):
+        if bad:
+            vd[::2, 1] = np.inf
+        out = torch.zeros(B, N, H, D, device="cuda")
+        ctx.gqa_tree(_t(q), _t(kc, dt), _t(vc, dt), _t(kd, dt), _t(vd, dt), _i(lens), _i(counts), _i(par), 0.125, out)
+        outs.append(_np(out))
+    keep = np.ones((B, N), bool)
+    keep[::2, 1] = False
+    assert np.array_equal(outs[0][keep], outs[1][keep])
+    hit = [b for b in range(0, B, 2) if counts[b] > 1]
+    assert not np.isfinite(outs[1][hit, 1]).any()
+
+
 def test_tree_attention_extreme_scores(ctx):
     """Scores past a hundred, all equal ones, and a scale of 0 and below it."""
     def scaled(f):
