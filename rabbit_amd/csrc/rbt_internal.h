@@ -488,6 +488,7 @@ struct TreeArgs {
   int R;       // query heads per KV head
   int rw, kw;  // waves of a workgroup: row tiles, groups of keys
   int t16;     // 16-row tiles of a KV head
+  int four;    // f32 rows split by workgroups of four waves
   float *part;
   float2 *part_ml;
 };

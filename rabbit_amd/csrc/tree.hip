@@ -175,16 +175,19 @@ __device__ __forceinline__ float tree_xor_sum(float v) {
 }
 
 // How keys and values reach the matrix cores: bf16 as they are, f32 as they are, f32 in three bf16 parts.
-enum { KV_BF16 = 0, KV_F32 = 1, KV_PARTS = 2 };
-constexpr int TREE_PARTS_NT = 512;  // threads of the workgroups that split f32 rows
+// KV_PARTS4: by workgroups of four waves, several of them on a CU, for batches of up to four row tiles at head dims 64
+// and 128. 12 nodes of 32 query heads over 8 KV heads of 128: 32 sequences of up to 4096 rows 243 us with eight waves,
+// 208 with four, but one of 8192 rows (16 nodes) 27.5 and 31.4, where loading a stage is what it waits for.
+enum { KV_BF16 = 0, KV_F32 = 1, KV_PARTS = 2, KV_PARTS4 = 3 };
+constexpr bool tree_parts(int kv) { return kv >= KV_PARTS; }
 
 template <int HD, int KV>
 struct TreeTile {
   static constexpr int ROWB = HD * (KV == KV_F32 ? 4 : 2), CH = ROWB / 16;  // bytes and chunks of a row in LDS
   static constexpr int GROW = HD * (KV == KV_BF16 ? 2 : 4);                 // bytes of a row of the cache
   static constexpr int TK = KV == KV_BF16 ? 64 : 32;                        // keys per stage
-  static constexpr int PART = TK * ROWB, SIDE = PART * (KV == KV_PARTS ? 3 : 1), STAGE = 2 * SIDE;  // K, then V
-  static constexpr int LDS = KV == KV_PARTS ? STAGE : 2 * STAGE;
+  static constexpr int PART = TK * ROWB, SIDE = PART * (tree_parts(KV) ? 3 : 1), STAGE = 2 * SIDE;  // K, then V
+  static constexpr int LDS = tree_parts(KV) ? STAGE : 2 * STAGE;
   static constexpr int INSTR = TK * CH / 64;                                // 1 KB loads per side
   static_assert(TK * CH % 64 == 0 && CH % 8 == 0, "whole loads");
   // Where chunk c of row r lies in its row: c ^ k_turn(r), c ^ v_turn(r). The LDS serves 256 bytes a cycle from 64
@@ -218,9 +221,9 @@ __device__ __forceinline__ void tree_pieces(const TreeArgs &a, int L, int TK, un
 }
 
 template <int HD, int KV, int KW>
-__global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(TreeArgs a) {
+__global__ __launch_bounds__(KW == 1 && KV != KV_PARTS4 ? 512 : 256, KW == 1 && KV != KV_PARTS4 ? 1 : 2) void k_tree(TreeArgs a) {
   using TT = TreeTile<HD, KV>;
-  constexpr bool B16 = KV != KV_F32, PARTS = KV == KV_PARTS;  // bf16 products; of split rows
+  constexpr bool B16 = KV != KV_F32, PARTS = tree_parts(KV);  // bf16 products; of split rows
   constexpr int ROWB = TT::ROWB, CH = TT::CH, TK = TT::TK, SK = TK / KW, NT = SK / 16;
   static_assert(!PARTS || KW == 1, "one group of waves");
   extern __shared__ __attribute__((aligned(1024))) char smem[];
@@ -287,13 +290,13 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
   auto mark = [&](int i) { atomicOr(&dirty[(min(i, keys - 1) - nc) >> 5], 1u << ((min(i, keys - 1) - nc) & 31)); };
 
   // split rows: a thread's quads of the stage, K's then V's, on their way
-  constexpr int UN = PARTS ? HD / 64 : 1;
-  static_assert(!PARTS || TK * HD / 4 == UN * TREE_PARTS_NT, "whole quads");
+  constexpr int PNT = KV == KV_PARTS4 ? 256 : 512, UN = PARTS ? TK * HD / 4 / PNT : 1;
+  static_assert(!PARTS || TK * HD / 4 == UN * PNT, "whole quads");
   float4 raw[2][UN];
   auto fetch = [&](int s) {
 #pragma unroll
     for (int k = 0; k < UN; k++) {
-      const int u = k * TREE_PARTS_NT + t, r = u / (HD / 4), j = min(s * TK + r, keys - 1);
+      const int u = k * PNT + t, r = u / (HD / 4), j = min(s * TK + r, keys - 1);
       const long at = (long)(j < nc ? j : j - nc) * seq_row + (u - r * (HD / 4)) * 16;
       raw[0][k] = *(const float4 *)((j < nc ? kc : kd) + at);
       raw[1][k] = *(const float4 *)((j < nc ? vc : vd) + at);
@@ -303,7 +306,7 @@ __global__ __launch_bounds__(KW == 1 ? 512 : 256, KW == 1 ? 1 : 2) void k_tree(T
   auto split = [&](int s) {
 #pragma unroll
     for (int k = 0; k < UN; k++) {
-      const int u = k * TREE_PARTS_NT + t, r = u / (HD / 4), c = u - r * (HD / 4);
+      const int u = k * PNT + t, r = u / (HD / 4), c = u - r * (HD / 4);
 #pragma unroll
       for (int side = 0; side < 2; side++) {
         float v[4] = {raw[side][k].x, raw[side][k].y, raw[side][k].z, raw[side][k].w};
@@ -765,12 +768,13 @@ static int tree_per_cu(int hd, int threads) {
 
 // Threads of a workgroup.
 static int tree_threads(const TreeArgs &a) {
-  return a.kw > 1 ? 256 : a.kv16 ? 64 * a.rw : TREE_PARTS_NT;
+  return a.kw > 1 || a.four ? 256 : a.kv16 ? 64 * a.rw : 512;
 }
 
 // Pieces and row tiles for a call on the matrix cores.
 bool tree_plan(const Ctx &c, TreeArgs &a) {
   a.rw = a.kw = a.tiles = a.pieces = 1;
+  a.four = 0;
   int rw = 1, kw = 1;
   a.tiled = a.hd == 64 || a.hd == 128 || a.hd == 192 || a.hd == 256;
   if (!a.tiled) return true;
@@ -806,6 +810,9 @@ bool tree_plan(const Ctx &c, TreeArgs &a) {
   const bool wide = rw > 4;  // two waves on a SIMD
   const double ncu = c.num_cu, base = (double)a.tiles * a.K * a.B, most = std::ceil((double)(a.max_len + a.T) / TK);
   const double part = a.hd / 256.0;
+  // (from eight stages a CU on; three sequences of 1001 rows, one and a half a CU: 14.5 us with eight waves, 15.3 with
+  // four; eight of 4096, 32 a CU: 74 and 67)
+  a.four = !a.kv16 && kw == 1 && a.hd <= 128 && rw <= 4 && a.B > 1 && base * most >= 8 * ncu;
   double stage, busy = 1.0, hold = 1.0;
   if (a.B == 1) {
     stage = (kw > 1 ? (a.kv16 ? 1.6 : 2.6) : a.kv16 ? (wide ? 4.4 : 2.6) : (wide ? 6.5 : 4.0)) * part;
@@ -821,7 +828,9 @@ bool tree_plan(const Ctx &c, TreeArgs &a) {
   } else {
     stage = (a.hd == 256 ? (wide ? 6.5 : 4.0) : (wide ? 4.4 : 3.6)) * (0.1 + 0.9 * part);
     busy = wide ? 0.9 : 0.65;
-    hold = tree_per_cu<KV_PARTS, 1>(a.hd, tree_threads(a));
+    hold = !a.four      ? tree_per_cu<KV_PARTS, 1>(a.hd, 512)
+           : a.hd == 64 ? tree_per_cu<64, KV_PARTS4, 1>(256)
+                        : tree_per_cu<128, KV_PARTS4, 1>(256);
   }
   const double bytes = (double)a.B * a.K * a.t16 * 16 * a.hd * 8.0;
   const double pass = a.B > 1 ? 0.75 * a.B * a.K * a.max_len * a.hd * (a.kv16 ? 4.0 : 8.0) / 5.0e6 : 0.0;
@@ -868,6 +877,8 @@ static hipError_t run_tree_hd(const Ctx &c, const TreeArgs &a) {
     return a.kw == 4   ? run_tree<HD, KV_BF16, 4>(c, a)
            : a.kw == 2 ? run_tree<HD, KV_BF16, 2>(c, a)
                        : run_tree<HD, KV_BF16, 1>(c, a);
+  if constexpr (HD <= 128)
+    if (a.four) return run_tree<HD, KV_PARTS4, 1>(c, a);
   return a.kw == 2 ? run_tree<HD, KV_F32, 2>(c, a) : run_tree<HD, KV_PARTS, 1>(c, a);
 }
 
