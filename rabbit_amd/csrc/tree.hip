@@ -9,11 +9,13 @@
 //   k_tree_any   any head dim: fp32 multiply-adds, one workgroup per query head and node
 //
 // Bounds and times (64 query heads over 4 KV heads of 256, one MI355X):
-//   64 nodes over 32749 bf16 rows: 302-314 us, of them 280-290 in k_tree: 412 GFLOP of bf16 products, 1.4 PFLOP/s (a
+//   64 nodes over 32749 bf16 rows: 292-314 us, of them 280-290 in k_tree: 412 GFLOP of bf16 products, 1.4 PFLOP/s (a
 //     large library product reaches 1.2); the matrix cores are busy 61% of the cycles, at a clock that the load holds
 //     near 2 GHz.
-//   16 trees of 12 to 24 nodes over 4096 to 8192 bf16 rows: 361-368 us, k_tree 329-337; the products as above, and
-//     row tiles and pieces that do not fill every CU to the end.
+//   16 trees of 12 to 24 nodes over 4096 to 8192 bf16 rows: 353-368 us, k_tree 324-337; the products as above, and
+//     row tiles that a sequence fills in part.
+//   32 sequences of one node over 2048 to 4096 rows, 32 query heads over 8 KV heads: 41 us for bf16 rows of 64, 90 for
+//     bf16 of 128, 86 and 189 for f32: the caches at 4.3 to 4.9 TB/s.
 //   one node over 32768 bf16 rows: 35 us, k_tree 26 (134 MB: 5.1 TB/s); over 513 rows: 13.3 us, two launches of one
 //     trip to memory each; five nodes over 4096 f32 rows: 34 us.
 #include "rbt_device.h"
