@@ -658,6 +658,35 @@ def test_captured_step_replays(own_ctx, kv):
                 assert torch.equal(got[k], getattr(s, k)), (rep, n, k)
 
 
+@pytest.mark.parametrize("D,H,N", [(64, 8, 3), (128, 16, 5), (192, 8, 2)])
+def test_captured_before_any_call_of_its_kind(own_ctx, D, H, N):
+    """The first call of a shape stands in a capture (its split is chosen there); scratch is there from a larger one."""
+    import torch
+    from helpers import HipGraph
+    ctx, B, K, cap = own_ctx, 12, 2, 900
+    g = torch.Generator(device="cuda").manual_seed(D)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    big = [r(8, 40, 32, 256), r(8, 1000, 2, 256), r(8, 1000, 2, 256), r(8, 40, 2, 256), r(8, 40, 2, 256)]
+    ctx.gqa_tree(*big, _i([1000] * 8), _i([40] * 8), _i(np.tile(np.arange(-1, 39), (8, 1))), 0.1, torch.empty_like(big[0]))
+    q, kc, vc, kd, vd = r(B, N, H, D), r(B, cap, K, D), r(B, cap, K, D), r(B, N, K, D), r(B, N, K, D)
+    par, n = _i(np.tile(np.arange(-1, N - 1), (B, 1))), _i([N] * B)
+    ln, out = _i([0] * B), torch.zeros_like(q)
+    torch.cuda.synchronize()
+    gr = HipGraph(ctx.stream)
+    gr.begin()
+    ctx.gqa_tree(q, kc, vc, kd, vd, ln, n, par, 0.1, out, sync=False)
+    gr.end()
+    for rep in range(3):
+        ln.copy_(_i([(rep * 311 + 97 * b) % (cap + 1) for b in range(B)]))
+        out.zero_()
+        torch.cuda.synchronize()
+        gr.launch()
+        ctx.sync()
+        want = torch.zeros_like(q)
+        ctx.gqa_tree(q, kc, vc, kd, vd, ln, n, par, 0.1, want)
+        assert torch.equal(out, want), rep
+
+
 def test_results_do_not_change_from_run_to_run(ctx):
     """The same call twice gives the same bits."""
     import torch
