@@ -223,7 +223,8 @@ __device__ __forceinline__ void tree_pieces(const TreeArgs &a, int L, int TK, un
 }
 
 template <int HD, int KV, int KW>
-__global__ __launch_bounds__(KW == 1 && KV != KV_PARTS4 ? 512 : 256, KW == 1 && KV != KV_PARTS4 ? 1 : 2) void k_tree(TreeArgs a) {
+__global__ __launch_bounds__(KW == 1 && KV != KV_PARTS4 ? 512 : 256, KW == 1 && KV != KV_PARTS4 ? 1 : 2)
+void k_tree(TreeArgs a) {
   using TT = TreeTile<HD, KV>;
   constexpr bool B16 = KV != KV_F32, PARTS = tree_parts(KV);  // bf16 products; of split rows
   constexpr int ROWB = TT::ROWB, CH = TT::CH, TK = TT::TK, SK = TK / KW, NT = SK / 16;
