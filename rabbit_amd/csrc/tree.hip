@@ -845,7 +845,8 @@ bool tree_plan(const Ctx &c, TreeArgs &a) {
     const double groups = base * p, rounds = groups / (ncu * hold), beside = std::min(hold, std::ceil(groups / ncu));
     const double one = 7.0 + stage * std::max(1.0, beside * busy) * std::ceil(most / p);
     double t = rounds <= 1.0 ? one : a.B == 1 ? std::ceil(rounds) * one : (0.8 * rounds + 0.4) * one;
-    t = std::max(t, pass * (rounds > 1.0 ? 1.0 : groups > ncu ? beside * ncu / groups : hold > 1.0 ? 1.2 : 1.0));
+    const double uneven = rounds > 1.0 ? 1.0 : beside * ncu / groups;
+    t = std::max(t, pass * uneven * (hold > 1.0 && groups <= ncu ? 1.2 : 1.0));
     if (p > 1) t += 4.0 + bytes * p / 1.2e7;
     if (best == 0.0 || t < best) best = t, pieces = p;
   };
