@@ -419,7 +419,8 @@ int rbt_tree_positions_d(rbt_ctx *ctx, size_t n_seq, size_t max_nodes, const int
  * [n_seq, cap, n_kv_heads, head_dim] and k_draft, v_draft [n_seq, max_nodes, n_kv_heads, head_dim] of
  * kv_dtype; out f32 as q. gate: out is multiplied by sigmoid of
  * gate[(b * max_nodes + i) * gate_token_stride + h * gate_head_stride + e] (q_proj's [query, gate] rows:
- * strides n_heads * 2 * head_dim and 2 * head_dim), or NULL. Products are exact (to 2^-24) and sums f32.
+ * strides n_heads * 2 * head_dim and 2 * head_dim), or NULL. Products are exact (over f32 caches to 2^-24, numbers
+ * from 2^-110 on) and sums f32.
  * head_dim 1..1024, fastest at 64, 128, 192 and 256; any number of query heads per KV head. q, out, caches
  * and draft rows are 16-byte aligned, and out overlaps none of the others. Values that a node does not see never reach
  * its output, non-finite ones included; a non-finite key or value that it sees makes the output entries

@@ -138,7 +138,10 @@ __global__ __launch_bounds__(256) void k_tree_any(TreeArgs a) {
 //   f32 caches, one or two row tiles: fp32 MFMAs, which keep up with memory there (32 rows: 128 cycles a key of
 //     the 157 that its 2 KB take a CU's share of the bandwidth).
 //   f32 caches, more row tiles: keys and values are split too, once per workgroup on their way into LDS, at six
-//     products (those below 2^-24 of the whole left out): 64 nodes over 8192 rows 202 us, 307 with fp32 MFMAs.
+//     products. All four are rounded to nearest part by part, so that the middle part is at most 2^-8 of the whole and
+//     the last 2^-17, and the three products left out come to 2^-24 of theirs at most, of either sign (parts by
+//     truncation are of one sign and twice and four times as long: 2^-21, always towards zero). 64 nodes over 8192 rows
+//     187 us, 307 with fp32 MFMAs.
 // A workgroup of RW x KW waves takes RW row tiles and one piece of the keys: KW groups of waves share out each
 // stage's keys (few rows: every wave has its own keys; many rows: every wave has its own rows, up to eight waves: with
 // four, two workgroups per CU, 64 nodes over 32749 rows took 348 us against 311). Stages of TK keys land in LDS by
@@ -155,7 +158,8 @@ __device__ __forceinline__ void tree_dma(const void *p, uint32_t base) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(base), "v"(p) : "memory");
 }
 
-// x = hi + mid + lo, each with its low 16 bits zero (fp32 has 24 significant bits, each part 8).
+// x = hi + mid + lo, each with its low 16 bits zero (fp32 has 24 significant bits, each part 8): for products with bf16
+// rows, of which all three are kept.
 __device__ __forceinline__ void tree_split(float x, uint32_t &hi, uint32_t &mid, uint32_t &lo) {
   hi = __float_as_uint(x) & 0xffff0000u;
   const float r = x - __uint_as_float(hi);
@@ -165,6 +169,27 @@ __device__ __forceinline__ void tree_split(float x, uint32_t &hi, uint32_t &mid,
 // The high halves of a and b as two bf16 (a low).
 __device__ __forceinline__ uint32_t tree_pack(uint32_t a, uint32_t b) {
   return __builtin_amdgcn_perm(b, a, 0x07060302u);
+}
+
+// a and b rounded to the nearest bf16 (a low).
+typedef float tf2 __attribute__((ext_vector_type(2)));
+typedef __bf16 tb2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t tree_cvt(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((tf2{a, b}), tb2));
+}
+// a and b each as the sum of three bf16, the first two rounded to nearest: exact from 2^-110 on, since the first leaves
+// 16 significant bits and the second 7. WIDE: a first part that would round to infinity stays the largest bf16, which
+// leaves no more bits; infinities and NaN give a NaN. (Rounding by integers instead of conversions: 8 sequences of 16
+// nodes 329 us, 321 with conversions. A check of the stage for numbers that large instead of WIDE: 325.)
+template <bool WIDE>
+__device__ __forceinline__ void tree_round(float a, float b, uint32_t &hi, uint32_t &mid, uint32_t &lo) {
+  constexpr float top = 0x1.fep127f;
+  hi = WIDE ? tree_cvt(__builtin_amdgcn_fmed3f(a, -top, top), __builtin_amdgcn_fmed3f(b, -top, top)) : tree_cvt(a, b);
+  a -= __uint_as_float(hi << 16);
+  b -= __uint_as_float(hi & 0xffff0000u);
+  mid = tree_cvt(a, b);
+  lo = tree_pack(__float_as_uint(a - __uint_as_float(mid << 16)),
+                 __float_as_uint(b - __uint_as_float(mid & 0xffff0000u)));
 }
 
 __device__ __forceinline__ float tree_xor_max(float v) {
@@ -296,10 +321,30 @@ void k_tree(TreeArgs a) {
   constexpr int PNT = KV == KV_PARTS4 ? 256 : 512, UN = PARTS ? TK * HD / 4 / PNT : 1;
   static_assert(!PARTS || TK * HD / 4 == UN * PNT, "whole quads");
   float4 raw[2][UN];
+  // Lane numbers formed anew in every stage of split rows of 256: kept from stage to stage, the addresses made of them
+  // push queries out of the registers, and the reloads wait for the rows on their way.
+  auto again = [](int x) {
+    if constexpr (PARTS && HD == 256) asm volatile("" : "+v"(x));
+    return x;
+  };
   auto fetch = [&](int s) {
+    if ((s + 1) * TK <= nc) {  // 32 rows are at most 2^27 bytes: a 32-bit offset per lane from the stage's first row
+      const char *k0 = kc + (long)s * TK * seq_row, *v0 = vc + (long)s * TK * seq_row;
+#pragma unroll
+      for (int k = 0; k < UN; k++) {
+        constexpr int Q = HD / 4, whole = PNT % Q == 0;
+        const unsigned u = whole ? t : k * PNT + t, r = u / Q;
+        const unsigned at = r * (unsigned)seq_row + (u - r * Q) * 16;
+        const long up = whole ? k * (PNT / Q) * seq_row : 0;
+        raw[0][k] = *(const float4 *)(k0 + up + at);
+        raw[1][k] = *(const float4 *)(v0 + up + at);
+      }
+      return;
+    }
+    const int t0 = again(t);
 #pragma unroll
     for (int k = 0; k < UN; k++) {
-      const int u = k * PNT + t, r = u / (HD / 4), j = min(s * TK + r, keys - 1);
+      const int u = k * PNT + t0, r = u / (HD / 4), j = min(s * TK + r, keys - 1);
       const long at = (long)(j < nc ? j : j - nc) * seq_row + (u - r * (HD / 4)) * 16;
       raw[0][k] = *(const float4 *)((j < nc ? kc : kd) + at);
       raw[1][k] = *(const float4 *)((j < nc ? vc : vd) + at);
@@ -307,27 +352,28 @@ void k_tree(TreeArgs a) {
   };
   // the quads in three parts to LDS; non-finite drafted values are taken out (see below)
   auto split = [&](int s) {
+    const int t0 = again(t);
+    const bool drafted = nd > 1 && (s + 1) * TK > nc;
 #pragma unroll
     for (int k = 0; k < UN; k++) {
-      const int u = k * PNT + t, r = u / (HD / 4), c = u - r * (HD / 4);
+      const int u = k * PNT + t0, r = u / (HD / 4), c = u - r * (HD / 4);
 #pragma unroll
       for (int side = 0; side < 2; side++) {
         float v[4] = {raw[side][k].x, raw[side][k].y, raw[side][k].z, raw[side][k].w};
-        if (side && nd > 1 && s * TK + r >= nc) {
+        if (side && drafted && s * TK + r >= nc) {
           bool hit = false;
 #pragma unroll
           for (int e = 0; e < 4; e++)
             if (!(fabsf(v[e]) < INFINITY)) v[e] = 0.0f, hit = true;
           if (hit) mark(s * TK + r);
         }
-        uint32_t o[3][4];
+        uint32_t o[3][2];
 #pragma unroll
-        for (int e = 0; e < 4; e++) tree_split(v[e], o[0][e], o[1][e], o[2][e]);
+        for (int e = 0; e < 2; e++) tree_round<true>(v[2 * e], v[2 * e + 1], o[0][e], o[1][e], o[2][e]);
         const int at = (c >> 1) ^ (side ? TT::v_turn(r) : TT::k_turn(r));
         char *to = smem + side * TT::SIDE + r * ROWB + at * 16 + (c & 1) * 8;
 #pragma unroll
-        for (int p = 0; p < 3; p++)
-          *(uint2 *)(to + p * TT::PART) = make_uint2(tree_pack(o[p][0], o[p][1]), tree_pack(o[p][2], o[p][3]));
+        for (int p = 0; p < 3; p++) *(uint2 *)(to + p * TT::PART) = make_uint2(o[p][0], o[p][1]);
       }
     }
   };
@@ -349,13 +395,21 @@ void k_tree(TreeArgs a) {
     for (int s = 0; s < HD / 32; s++) {
       const float4 x = *(const float4 *)(qp + 32 * s + 8 * kg), y = *(const float4 *)(qp + 32 * s + 8 * kg + 4);
       const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-      uint32_t o[3][8];
+      if constexpr (PARTS) {
+        uint32_t o[3][4];
 #pragma unroll
-      for (int e = 0; e < 8; e++) tree_split(v[e], o[0][e], o[1][e], o[2][e]);
+        for (int e = 0; e < 4; e++) tree_round<true>(v[2 * e], v[2 * e + 1], o[0][e], o[1][e], o[2][e]);
 #pragma unroll
-      for (int p = 0; p < 3; p++)
-        qb[s][p] = __builtin_bit_cast(tb8, rbt_u4{tree_pack(o[p][0], o[p][1]), tree_pack(o[p][2], o[p][3]),
-                                                  tree_pack(o[p][4], o[p][5]), tree_pack(o[p][6], o[p][7])});
+        for (int p = 0; p < 3; p++) qb[s][p] = __builtin_bit_cast(tb8, rbt_u4{o[p][0], o[p][1], o[p][2], o[p][3]});
+      } else {
+        uint32_t o[3][8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) tree_split(v[e], o[0][e], o[1][e], o[2][e]);
+#pragma unroll
+        for (int p = 0; p < 3; p++)
+          qb[s][p] = __builtin_bit_cast(tb8, rbt_u4{tree_pack(o[p][0], o[p][1]), tree_pack(o[p][2], o[p][3]),
+                                                    tree_pack(o[p][4], o[p][5]), tree_pack(o[p][6], o[p][7])});
+      }
     }
   } else {
 #pragma unroll
@@ -434,7 +488,7 @@ void k_tree(TreeArgs a) {
     constexpr int NP = PARTS ? 3 : 1;  // parts of a key or value
     if constexpr (B16) {
       // a step: 32 entries of one part for up to two tiles of keys, the next step's read while this one's multiply.
-      // Small parts first; products of two parts below 2^-24 of the whole are left out.
+      // Small parts first; of two split operands the three products that come to 2^-24 at most are left out.
       constexpr int XS = NT > 1 ? 2 : 1, QS = HD / 32 * NP * (NT / XS);
       tb8 kf[2][XS];
       auto read = [&](int i, tb8(&to)[XS]) {
@@ -508,20 +562,26 @@ void k_tree(TreeArgs a) {
 
     // values
     if constexpr (B16) {
-      const int xr = col >> 2;
-      const char *vb = vt + (kgp * SK + 4 * kg + xr) * ROWB + (col & 1) * 8 + ((col >> 1) & 1) * 16;
+      const int cv = again(lane) & 15, xr = cv >> 2;
+      const char *vb = vt + (kgp * SK + 4 * kg + xr) * ROWB + (cv & 1) * 8 + ((cv >> 1) & 1) * 16;
       constexpr int VP = TT::WIDE ? 8 : 4;
       const int turn = TT::v_turn(4 * kg + xr) >> 1;
       uint32_t pp[NT][3][2];
 #pragma unroll
       for (int x = 0; x < NT; x++) {
-        uint32_t h[3][4];
+        if constexpr (PARTS) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) tree_split(sc[x][i], h[0][i], h[1][i], h[2][i]);
+          for (int i = 0; i < 2; i++)
+            tree_round<false>(sc[x][2 * i], sc[x][2 * i + 1], pp[x][0][i], pp[x][1][i], pp[x][2][i]);
+        } else {
+          uint32_t h[3][4];
 #pragma unroll
-        for (int p = 0; p < 3; p++) {
-          pp[x][p][0] = tree_pack(h[p][0], h[p][1]);
-          pp[x][p][1] = tree_pack(h[p][2], h[p][3]);
+          for (int i = 0; i < 4; i++) tree_split(sc[x][i], h[0][i], h[1][i], h[2][i]);
+#pragma unroll
+          for (int p = 0; p < 3; p++) {
+            pp[x][p][0] = tree_pack(h[p][0], h[p][1]);
+            pp[x][p][1] = tree_pack(h[p][2], h[p][3]);
+          }
         }
       }
       // a step: one part of 32 keys (16 where the wave has no more) for two tiles of entries

@@ -125,3 +125,25 @@ def random_parents(rng, B, T, shape="tree"):
     for i in range(1, T):
         par[:, i] = i - 1 if shape == "chain" else rng.integers(-1 if shape == "forest" else 0, i, B)
     return par
+
+
+def _bf16_bits(x):
+    """float32 rounded to the nearest bf16, as float32."""
+    b = np.asarray(x, np.float32).view(np.uint32).astype(np.uint64)
+    return ((b + 0x7fff + (b >> 16 & 1)) & 0xffff0000).astype(np.uint32).view(np.float32)
+
+
+def bf16_parts(x):
+    """float32 as the sum of three bf16 rounded to nearest; a first part past the largest bf16 stays that."""
+    x = np.asarray(x, np.float32)
+    top = np.array(0x7f7f0000, np.uint32).view(np.float32)
+    hi = _bf16_bits(np.clip(x, -top, top))
+    mid = _bf16_bits(x - hi)
+    return hi, mid, _bf16_bits(x - hi - mid)
+
+
+def six_products(x, y):
+    """The products of parts that the matrix cores take for x y, summed in float64: hi hi, hi mid, mid hi, mid mid,
+    hi lo and lo hi. With |mid| <= 2^-8 and |lo| <= 2^-17 of the whole, the rest is at most 2^-24 + 2^-34 of it."""
+    a, b = (np.asarray(bf16_parts(v), np.float64) for v in (x, y))
+    return sum(a[i] * b[j] for i in range(3) for j in range(3) if i + j <= 2)

@@ -198,3 +198,26 @@ def test_truth_forms_agree_with_closed_cases():
     for i in range(3):
         s = np.exp(qq[0, i] @ k[0, :6 + i, 0].T * 0.5)
         assert np.allclose(o[0, i], s / s.sum(-1, keepdims=True) @ v[0, :6 + i, 0])
+
+
+def test_bf16_parts_of_f32_products():
+    """An fp32 number is its three parts; a product of two by six of the parts' nine products is off by 2^-24 (1 + 2^-6) of
+    it at most, at the mantissas whose parts are longest and at the largest numbers too, and as much to either side."""
+    import draft_truth as T
+    rng = np.random.default_rng(0)
+    man, few = rng.integers(0, 1 << 23, (2, 1 << 20)), rng.integers(0, 1 << 7, (2, 1 << 17)) << 16
+    man[:, :1 << 16] = few[:, :1 << 16] | 0xffff        # parts by truncation are longest here
+    man[:, 1 << 16:1 << 17] = few[:, 1 << 16:] | 0x7f80  # and rounded ones here
+    for ex in (127, 17, 254):  # (below 2^-110 the last part is finer than bf16's subnormals)
+        x, y = (((e << 23) | m).astype(np.uint32).view(np.float32) for e, m in zip((ex, 127), man))
+        for v in (x, y):
+            hi, mid, lo = (np.asarray(p, np.float64) for p in T.bf16_parts(v))
+            v = v.astype(np.float64)
+            assert np.array_equal(hi + mid + lo, v) and np.isfinite(hi).all()
+            # (the factors: numbers past the largest bf16, whose first part is not the nearest)
+            assert (np.abs(mid) <= 2.0 ** -8 * (1 + 2.0 ** -16) * v).all()
+            assert (np.abs(lo) <= 2.0 ** -17 * (1 + 2.0 ** -7) * v).all()
+        exact = x.astype(np.float64) * y.astype(np.float64)
+        off = (T.six_products(x, y) - exact) / exact
+        assert np.abs(off).max() <= T.U32 * (1 + 2.0 ** -6)
+        assert abs(off.mean()) < 0.02 * T.U32

@@ -701,3 +701,56 @@ def test_results_do_not_change_from_run_to_run(ctx):
         ctx.gqa_tree(q, kc, vc, kd, vd, _i([2999, 1777]), _i([9, 8]), par, 0.1, out)
         outs.append(out)
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+# ---- products of split f32 rows ----------------------------------------------------------------------
+def _one_row(ctx, B, N, H, K, D, cap, q, kc, vc, kd, vd, scale):
+    """One committed row, and nodes that see it and themselves; every head and node has the same numbers, given by
+    their first entries. -> (out [D], the 64-bit form's)."""
+    import torch
+    full = lambda head, *sh: np.broadcast_to(np.pad(np.asarray(head, np.float32), (0, D - len(head))), (*sh, D)).copy()  # noqa: E731
+    a = [full(q, B, N, H), full(kc, B, cap, K), full(vc, B, cap, K), full(kd, B, N, K), full(vd, B, N, K)]
+    par = np.full((B, N), -1, np.int32)
+    out = torch.zeros(B, N, H, D, device="cuda")
+    ctx.gqa_tree(*(_t(x) for x in a), _i([1] * B), _i([N] * B), _i(par), scale, out)
+    got = _np(out).astype(np.float64)
+    assert (got == got[0, 0, 0]).all()
+    want, _, _ = T.tree_attention(a[0][:1, :1, :K], *(x[:1, :1] for x in a[1:]), [1], [1], par[:1, :1], scale)
+    return got[0, 0, 0], want[0, 0, 0]
+
+
+# 48 rows of one KV head (three row tiles) by eight waves, and in a batch with room for 600 rows by four
+SPLIT = [(1, 1, 48, 1, 64, 1), (1, 4, 48, 4, 192, 9), (2, 1, 48, 1, 256, 1), (16, 4, 96, 8, 64, 600), (16, 4, 96, 8, 128, 600)]
+LONG = np.array(0x3f80ffff, np.uint32).view(np.float32)  # 1 + 2^-7 - 2^-23
+LN2 = np.float32(np.log(2.0))                            # times log2(e) in f32 it rounds to 1: scores are exact powers of two
+
+
+@pytest.mark.parametrize("B,N,H,K,D,cap", SPLIT)
+def test_split_keys_products(ctx, B, N, H, K, D, cap):
+    """The product of two long mantissas against its fp32 rounding times a power of two (all parts kept, their sum exact).
+    Their difference of scores, near 2^14 in powers of two, is off by the last addition (2u at most, whichever way it
+    rounds) and by the products left out (for these two numbers 2^-38); the output's slope over it is ln 2 / 4."""
+    t = np.float32(2.0 ** 14)
+    got, want = _one_row(ctx, B, N, H, K, D, cap, [LONG, LONG * LONG], [LONG * t], [1.0], [0.0, t], [0.0], LN2)
+    assert abs(got[0] - want[0]) <= np.log(2) / 4 * 2.1 * T.U32 * float(t) * 1.02 + 2.0 ** -22, (got[0], want[0])
+    got, want = _one_row(ctx, B, N, H, K, D, cap, [-LONG, LONG * LONG], [LONG * t], [1.0], [0.0, -t], [0.0], LN2)
+    assert abs(got[0] - want[0]) <= np.log(2) / 4 * 2.1 * T.U32 * float(t) * 1.02 + 2.0 ** -22, (got[0], want[0])
+
+
+@pytest.mark.parametrize("B,N,H,K,D,cap", SPLIT)
+def test_split_values_products(ctx, B, N, H, K, D, cap):
+    """A probability with a long middle and last part times 1 and times a long mantissa: their quotient is that mantissa but
+    for the last addition (2u at most), two divisions (u each) and the products left out (2^-38)."""
+    s = np.float32(np.log2(0.5 * (1.0 + 2.0 ** -7 - 2.0 ** -21)))
+    got, _ = _one_row(ctx, B, N, H, K, D, cap, [1.0], [s], [1.0, LONG, -LONG], [0.0], [0.0], LN2)
+    for g, w in ((got[1], float(LONG)), (got[2], -float(LONG))):
+        assert abs(g / got[0] / w - 1.0) <= 4.1 * T.U32, (g / got[0] / w - 1.0) / T.U32
+
+
+def test_split_rows_of_the_largest_numbers(ctx):
+    """Finite numbers that would round to an infinite bf16 keep their products."""
+    top = np.float32(np.finfo(np.float32).max)
+    got, want = _one_row(ctx, 1, 1, 48, 1, 64, 1, [2.0 ** -126, 0.0], [top], [top, -top], [0.0, top], [0.0], 1.0)
+    assert np.isfinite(got).all() and (np.abs(got[:2] / want[:2] - 1.0) <= 2.0 ** -19).all()
+    got, want = _one_row(ctx, 1, 1, 48, 1, 64, 1, [top], [2.0 ** -126], [1.0], [0.0], [0.0], 1.0)
+    assert abs(got[0] - want[0]) <= 2.0 ** -20
