@@ -102,9 +102,13 @@ def rope_freqs(rope_dim: int, theta: float, kind: int = ROPE_PLAIN, factor: floa
     return out[:rope_dim // 2], f.value
 
 
+class _RopePart(abi.RbtRopePart):
+    """An RbtRopePart with the tensors that it points to (held) and their size."""
+
+
 def rope_part(src, dst, norm=None, rotate: bool = True) -> abi.RbtRopePart:
     """One tensor of Context.rope: src and dst are [s, n_heads, head_dim] torch tensors on the GPU (float32
-    or bfloat16), strided views allowed as long as head_dim is contiguous."""
+    or bfloat16), strided views allowed as long as head_dim is contiguous. The part holds them and norm."""
     for name, t in (("src", src), ("dst", dst)):
         if not t.is_cuda:
             raise ValueError("torch tensors passed to rabbit_amd must live on the GPU")
@@ -114,8 +118,10 @@ def rope_part(src, dst, norm=None, rotate: bool = True) -> abi.RbtRopePart:
         raise ValueError(f"src {list(src.shape)} and dst {list(dst.shape)} differ")
     if norm is not None:
         _dense("norm", norm, "float32", src.shape[2])
-    return abi.RbtRopePart(src.data_ptr(), dst.data_ptr(), _dtype(src), _dtype(dst), src.shape[1], src.stride(0),
-                           src.stride(1), dst.stride(0), dst.stride(1), _ptr(norm), int(rotate))
+    p = _RopePart(src.data_ptr(), dst.data_ptr(), _dtype(src), _dtype(dst), src.shape[1], src.stride(0),
+                  src.stride(1), dst.stride(0), dst.stride(1), _ptr(norm), int(rotate))
+    p.tensors, p.tokens, p.head_dim = (src, dst, norm), src.shape[0], src.shape[2]
+    return p
 
 
 class QT:
@@ -415,10 +421,15 @@ class Context:
     # -- drafted tokens (device tensors) ----------------------------------------------------
     def rope(self, parts, pos, head_dim, inv_freq, rope_dim=None, rope_start=0, layout=ROPE_HALF, factor=1.0,
              angle_f32=False, eps=1e-6, sync=True):
-        """rbt_rope_d: norms and rotary positions of up to 8 tensors (rope_part) at pos (int32 [s]);
-        inv_freq float64 [rope_dim / 2] on the GPU."""
+        """rbt_rope_d: norms and rotary positions of up to 8 tensors (rope_part) at pos (int32, one per token of
+        theirs); inv_freq float64 [rope_dim / 2] on the GPU."""
         rope_dim = 2 * inv_freq.numel() if rope_dim is None else rope_dim
         s = pos.numel()
+        for i, p in enumerate(parts):
+            if not isinstance(p, _RopePart):
+                raise TypeError("the parts of a call are made by rope_part")
+            if (p.tokens, p.head_dim) != (s, head_dim):
+                raise ValueError(f"part {i} has {p.tokens} tokens of head_dim {p.head_dim}, not {s} of {head_dim}")
         if rope_dim > 0:
             _dense("inv_freq", inv_freq, "float64", rope_dim // 2)
         d = abi.RbtRopeDesc(layout, head_dim, rope_start, rope_dim, _ptr(inv_freq), factor, int(angle_f32), eps)

@@ -221,3 +221,61 @@ def test_bf16_parts_of_f32_products():
         off = (T.six_products(x, y) - exact) / exact
         assert np.abs(off).max() <= T.U32 * (1 + 2.0 ** -6)
         assert abs(off.mean()) < 0.02 * T.U32
+
+
+class _Tensor:
+    """What the Python calls ask a device tensor, without a device."""
+
+    is_cuda = True
+
+    def __init__(self, *shape, dtype="float32", stride=None):
+        self.shape, self.dtype = shape, "torch." + dtype
+        self.strides = stride or tuple(int(np.prod(shape[i + 1:])) for i in range(len(shape)))
+
+    def dim(self):
+        return len(self.shape)
+
+    def stride(self, i):
+        return self.strides[i]
+
+    def numel(self):
+        return int(np.prod(self.shape))
+
+    def is_contiguous(self):
+        return True
+
+    def data_ptr(self):
+        return A
+
+
+def _no_gpu(lib):
+    """A Context whose calls reach the library's checks and are refused there for want of a context."""
+    import rabbit_amd as R
+    c = R.Context.__new__(R.Context)
+    c.lib, c.h, c._keep = lib, None, []
+    return c
+
+
+def test_rope_call_fits_its_parts(rbt_lib):
+    """pos and head_dim agree with the tensors of every part; parts hold the tensors they point to."""
+    import gc
+    import weakref
+    import rabbit_amd as R
+    ctx, inv = _no_gpu(rbt_lib), _Tensor(16, dtype="float64")
+    part = lambda s, hd: R.rope_part(_Tensor(s, 2, hd), _Tensor(s, 2, hd), norm=_Tensor(hd))  # noqa: E731
+    pos = lambda *sh: _Tensor(*sh, dtype="int32")  # noqa: E731
+    for parts, p, hd in (([part(5, 64)], pos(6), 64), ([part(5, 64)], pos(4), 64), ([part(5, 64), part(4, 64)], pos(5), 64),
+                         ([part(5, 64)], pos(5), 128), ([part(5, 64)], pos(5), 32), ([part(5, 64), part(5, 32)], pos(5), 64)):
+        with pytest.raises(ValueError):
+            ctx.rope(parts, p, hd, inv, sync=False)
+    with pytest.raises(TypeError):  # nothing is known of a bare struct's rows
+        ctx.rope([_part()], pos(3), 64, inv, sync=False)
+    for p in (pos(6), pos(2, 3)):  # right calls reach the library
+        with pytest.raises(R.RbtError, match="null context"):
+            ctx.rope([part(6, 64), part(6, 64)], p, 64, inv, sync=False)
+    ts = [_Tensor(3, 2, 64), _Tensor(3, 2, 64), _Tensor(64)]
+    p, refs = R.rope_part(ts[0], ts[1], norm=ts[2]), [weakref.ref(t) for t in ts]
+    del ts
+    gc.collect()
+    assert all(r() is not None for r in refs)
+    assert p.src == p.norm == A
