@@ -465,7 +465,7 @@ class Context:
         gs = (0, 0)
         if gate is not None:
             if not gate.is_cuda or str(gate.dtype) != "torch.float32" or tuple(gate.shape) != (B, T, H, D) or \
-                    (D > 1 and gate.stride(3) != 1) or (B > 1 and gate.stride(0) != T * gate.stride(1)):
+                    (D > 1 and gate.stride(3) != 1) or (B > 1 and T > 1 and gate.stride(0) != T * gate.stride(1)):
                 raise ValueError("gate must be float32 like q, its entries contiguous and its sequences T tokens apart")
             gs = (gate.stride(1) if T > 1 else gate.stride(0), gate.stride(2))
         d = abi.RbtGqaTreeDesc(H, K, D, attn_scale, _dtype(k_cache), cap, max_len, *gs)

@@ -279,3 +279,22 @@ def test_rope_call_fits_its_parts(rbt_lib):
     gc.collect()
     assert all(r() is not None for r in refs)
     assert p.src == p.norm == A
+
+
+def _attend_args(B, N, H, K, D, gate):
+    i32 = lambda *sh: _Tensor(*sh, dtype="int32")  # noqa: E731
+    return (_Tensor(B, N, H, D), _Tensor(B, 9, K, D), _Tensor(B, 9, K, D), _Tensor(B, N, K, D), _Tensor(B, N, K, D), i32(B),
+            i32(B), i32(B, N), 0.125, _Tensor(B, N, H, D), gate)
+
+
+@pytest.mark.parametrize("B,N,stride,ok", [
+    (3, 1, (1024, 512, 128, 1), True),   # the first node's gates of q_proj rows with two nodes
+    (3, 1, (512, 7, 128, 1), True),      # one node: the step from node to node is nobody's
+    (1, 4, (7, 512, 128, 1), True),      # one sequence
+    (3, 4, (2048, 512, 128, 1), True), (3, 4, (4096, 512, 128, 1), False), (3, 1, (512, 512, 128, 2), False)])
+def test_gate_views(rbt_lib, B, N, stride, ok):
+    """Gates inside wider rows: every view that two strides describe, no other."""
+    import rabbit_amd as R
+    ctx = _no_gpu(rbt_lib)
+    with pytest.raises(R.RbtError if ok else ValueError, match="null context" if ok else "gate"):
+        ctx.gqa_tree(*_attend_args(B, N, 4, 2, 64, _Tensor(B, N, 4, 64, stride=stride)), sync=False)
