@@ -423,8 +423,9 @@ int rbt_tree_positions_d(rbt_ctx *ctx, size_t n_seq, size_t max_nodes, const int
  * from 2^-110 on) and sums f32.
  * head_dim 1..1024, fastest at 64, 128, 192 and 256; any number of query heads per KV head. q, out, caches
  * and draft rows are 16-byte aligned, and out overlaps none of the others. Values that a node does not see never reach
- * its output, non-finite ones included; a non-finite key or value that it sees makes the output entries
- * it reaches non-finite (an infinite value may give a NaN). */
+ * its output, non-finite ones included. A non-finite value that it sees makes its entry of the output non-finite (an
+ * infinite one may give a NaN), a NaN key all entries. An infinite key counts for nothing where its score is -inf, as in
+ * the formula, or makes all entries non-finite: which of the two is not specified. */
 typedef struct {
     size_t n_heads, n_kv_heads, head_dim;
     float attn_scale;

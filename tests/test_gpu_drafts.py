@@ -754,3 +754,78 @@ def test_split_rows_of_the_largest_numbers(ctx):
     assert np.isfinite(got).all() and (np.abs(got[:2] / want[:2] - 1.0) <= 2.0 ** -19).all()
     got, want = _one_row(ctx, 1, 1, 48, 1, 64, 1, [top], [2.0 ** -126], [1.0], [0.0], [0.0], 1.0)
     assert abs(got[0] - want[0]) <= 2.0 ** -20
+
+
+# ---- non-finite keys and values that are seen ----------------------------------------------------------
+# one to 24 row tiles of a KV head, one sequence and batches; caches of several pieces (the last: one)
+SEEN = [(1, 12, 4, 2, 64, 5000), (1, 24, 32, 2, 256, 3000), (1, 9, 4, 2, 192, 4000), (16, 12, 32, 8, 64, 1500),
+        (16, 12, 32, 4, 128, 1500), (2, 12, 4, 2, 80, 300), (2, 12, 8, 2, 128, 40)]
+
+
+def _seen_case(B, N, H, K, D, L, kv16, rng):
+    q = rng.standard_normal((B, N, H, D)).astype(np.float32)
+    kc, vc = (_bf(rng.standard_normal((B, L, K, D))) for _ in range(2))
+    kd, vd = (_bf(rng.standard_normal((B, N, K, D))) for _ in range(2))
+    par = np.broadcast_to(np.array([-1, 0, 0, 0, 0, 0, 2, 3, 4, 0] + [0] * (N - 10) if N > 9 else [-1, 0, 0, 0, 0, 0, 2, 3, 4]), (B, N))
+    return q, kc, vc, kd, vd, par.astype(np.int32).copy()
+
+
+def _seen_call(ctx, q, kc, vc, kd, vd, par, kv16):
+    import torch
+    B, N, _, D = q.shape
+    dt = torch.bfloat16 if kv16 else torch.float32
+    out = torch.zeros(q.shape, device="cuda")
+    ctx.gqa_tree(_t(q), _t(kc, dt), _t(vc, dt), _t(kd, dt), _t(vd, dt), _i([kc.shape[1]] * B), _i([N] * B), _i(par), D ** -0.5, out)
+    return _np(out)
+
+
+@pytest.mark.parametrize("kv16", [False, True])
+@pytest.mark.parametrize("B,N,H,K,D,L", SEEN)
+def test_seen_values_reach_their_entries(ctx, B, N, H, K, D, L, kv16):
+    """A non-finite value makes its entry of the nodes that see it non-finite and nothing else; a NaN key all entries."""
+    q, kc, vc, kd, vd, par = _seen_case(B, N, H, K, D, L, kv16, np.random.default_rng(D + L))
+    vals = [x.copy() for x in (vc, kd, vd)]
+    R, hit = H // K, np.zeros(q.shape, bool)
+    sees = np.array([[j in T.ancestors(par[0], i) for j in range(N)] for i in range(N)])
+
+    def put(where, j, entry, value, heads=slice(None)):
+        where[:, j, heads, entry] = value
+        rows = slice(None) if where is vals[0] else sees[:, j]
+        h = [x for x in range(H) if x // R in range(K)[heads]]
+        e = slice(None) if where is vals[1] else entry
+        hit[np.ix_(range(B), np.arange(N)[rows], h, np.arange(D)[e] if isinstance(e, slice) else [e])] = True
+
+    put(vals[0], L // 3, 9, np.inf, slice(1, 2))       # committed, seen by every node of one KV head
+    put(vals[0], L - 1, D - 1, np.nan, slice(0, 1))
+    put(vals[2], 2, 3, np.inf)
+    put(vals[2], 3, 17, np.nan)
+    put(vals[2], 4, 40, -np.inf)
+    put(vals[2], 1, 5, np.inf)                          # a leaf
+    put(vals[1], 5, 8, np.nan)                          # a NaN key
+    got = _seen_call(ctx, q, kc, vals[0], vals[1], vals[2], par, kv16)
+    want, mag, qk = T.tree_attention(q, kc, vc, kd, vd, [L] * B, [N] * B, par, D ** -0.5)
+    ok = np.abs(got - want) <= T.tree_attention_bound(mag, qk, L + N, D)
+    assert not np.isfinite(got[hit]).any(), np.argwhere(hit & np.isfinite(got))[:5]
+    assert ok[~hit].all(), np.argwhere(~hit & ~ok)[:5]
+
+
+@pytest.mark.parametrize("kv16", [False, True])
+@pytest.mark.parametrize("B,N,H,K,D,L", SEEN)
+def test_seen_infinite_keys(ctx, B, N, H, K, D, L, kv16):
+    """An infinite key has no weight where its score is -inf, or makes the output non-finite; nodes that do not see it have
+    theirs."""
+    q, kc, vc, kd, vd, par = _seen_case(B, N, H, K, D, L, kv16, np.random.default_rng(D + L + 1))
+    want, mag, qk = T.tree_attention(q, kc, vc, kd, vd, [L] * B, [N] * B, par, D ** -0.5)
+    gone, mag2, qk2 = T.tree_attention(q, np.delete(kc, L // 2, 1), np.delete(vc, L // 2, 1), kd, vd, [L - 1] * B, [N] * B, par, D ** -0.5)
+    bad = kd.copy()
+    bad[:, 2, :, 11] = np.inf
+    sees = np.array([2 in T.ancestors(par[0], i) for i in range(N)])
+    got = _seen_call(ctx, q, kc, vc, bad, vd, par, kv16)
+    assert (np.abs(got - want) <= T.tree_attention_bound(mag, qk, L + N, D))[:, ~sees].all()
+    assert not np.isfinite(got[:, sees][q[:, sees][..., 11] > 0]).any()  # score inf
+    bad = kc.copy()
+    bad[:, L // 2, :, 11] = -np.inf
+    got = _seen_call(ctx, q, bad, vc, kd, vd, par, kv16)
+    rows = np.isfinite(got).all(-1)
+    assert not np.isfinite(got[~rows]).any() and not rows[q[..., 11] < 0].any()
+    assert (np.abs(got - gone) <= T.tree_attention_bound(mag2, qk2, L + N, D))[rows].all()
