@@ -409,7 +409,7 @@ int rbt_rope_d(rbt_ctx *ctx, const rbt_rope_desc *desc, const rbt_rope_part *par
                size_t s);
 
 /* pos[b, i] = len[b] + the number of node i's ancestors in the tree; -1 for padding nodes and for
- * skipped sequences. */
+ * skipped sequences, those too whose len + n_nodes - 1 passes 2^31 - 1. pos overlaps none of the others. */
 int rbt_tree_positions_d(rbt_ctx *ctx, size_t n_seq, size_t max_nodes, const int32_t *parent, const int32_t *n_nodes,
                          const int32_t *len, int32_t *pos);
 

@@ -247,7 +247,7 @@ __global__ __launch_bounds__(256) void k_tree_pos(const int *__restrict__ parent
   __shared__ int par[TREE_MAX];
   const int b = blockIdx.x, t = threadIdx.x;
   int n = n_nodes[b], L = len[b];
-  if (n < 0 || n > T || L < 0) {
+  if (n < 0 || n > T || L < 0 || L > INT32_MAX - max(n - 1, 0)) {
     if (t == 0) *bad = 1;
     n = 0;
   }

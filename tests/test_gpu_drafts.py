@@ -829,3 +829,18 @@ def test_seen_infinite_keys(ctx, B, N, H, K, D, L, kv16):
     rows = np.isfinite(got).all(-1)
     assert not np.isfinite(got[~rows]).any() and not rows[q[..., 11] < 0].any()
     assert (np.abs(got - gone) <= T.tree_attention_bound(mag2, qk2, L + N, D))[rows].all()
+
+
+def test_positions_up_to_the_largest(ctx):
+    """Positions up to 2^31 - 1; a sequence whose nodes could pass it is skipped and reported, not wrapped around."""
+    import torch
+    import rabbit_amd as R
+    top = (1 << 31) - 1
+    par = _i([[-1, 0, 1]] * 4)
+    pos = torch.full((4, 3), 9, dtype=torch.int32, device="cuda")
+    ctx.tree_positions(par, _i([3, 1, 0, 2]), _i([top - 2, top, top, 5]), pos)
+    assert _np(pos).tolist() == [[top - 2, top - 1, top], [top, -1, -1], [-1] * 3, [5, 6, -1]]
+    ctx.tree_positions(par, _i([3, 2, 3, 2]), _i([top - 1, top, 4, 5]), pos, sync=False)
+    with pytest.raises(R.RbtError):
+        ctx.sync()
+    assert _np(pos).tolist() == [[-1] * 3, [-1] * 3, [4, 5, 6], [5, 6, -1]]
