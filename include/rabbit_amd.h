@@ -451,7 +451,7 @@ int rbt_gqa_tree_d(rbt_ctx *ctx, const rbt_gqa_tree_desc *desc, size_t n_seq, si
  * path[b, :] gets the standing nodes in order, then -1; n_path[b] their number; next[b] is -1 where
  * nothing can be drawn (no nodes, or a row without a finite positive sum). tokens int32; a node
  * whose token is outside 0..vocab-1 is passed over and reported by the next rbt_sync (RBT_E_INVALID).
- * n_seq <= 1024.
+ * n_seq <= 1024. path, n_path and next overlap none of the other arrays.
  * max_children: the most children a node has, where known (1: chains), else 0; it changes only how the
  * work is launched. */
 int rbt_draft_verify_d(rbt_ctx *ctx, size_t n_seq, size_t max_nodes, size_t vocab, size_t max_children,
@@ -461,7 +461,7 @@ int rbt_draft_verify_d(rbt_ctx *ctx, size_t n_seq, size_t max_nodes, size_t voca
 /* KvCache::push (qwen38/attention.rs:76-82) of the standing nodes, for every layer at once: rows
  * path[b, j], j < n_path[b], of the layers' draft rows to rows len[b] + j of their caches;
  * len_out[b] = len[b] + n_path[b]. The four pointer arrays are host memory holding n_layers device
- * pointers each. len_out must not be len. A sequence that does not fit (len + n_path > cap, or a path entry
+ * pointers each. len_out overlaps none of len, path and n_path (RBT_E_INVALID). A sequence that does not fit (len + n_path > cap, or a path entry
  * outside 0..max_nodes-1) is left as it was with len_out = len, and reported by the next rbt_sync. */
 typedef struct {
     size_t n_layers, n_kv_heads, head_dim;

@@ -2146,6 +2146,9 @@ static int refuse(rbt_ctx *c, int code, const char *fmt, ...) {
 static bool bad_dtype(int32_t t) { return t != RBT_DT_F32 && t != RBT_DT_BF16; }
 static size_t dtype_size(int32_t t) { return t == RBT_DT_BF16 ? 2 : 4; }
 static bool misaligned(const void *p, size_t n) { return (uintptr_t)p % n != 0; }
+static bool overlap(const void *a, size_t na, const void *b, size_t nb) {
+  return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+}
 
 // The context's device made current for a call, and what was current before afterwards.
 struct DeviceScope {
@@ -2402,7 +2405,9 @@ int rbt_kv_commit_d(rbt_ctx *c, const rbt_kv_commit_desc *d, size_t n_seq, size_
   bool al16 = row % 16 == 0;
   if (n_seq) {
     if (!path || !n_path || !len || !len_out) return refuse(c, RBT_E_INVALID, "null path or length buffer");
-    if (len == len_out) return refuse(c, RBT_E_INVALID, "len_out must not be len");
+    const size_t nb = n_seq * sizeof(int32_t);
+    if (overlap(len_out, nb, len, nb) || overlap(len_out, nb, n_path, nb) || overlap(len_out, nb, path, nb * max_nodes))
+      return refuse(c, RBT_E_INVALID, "len_out overlaps len, path or n_path");
     if (d->n_layers && (!k_caches || !v_caches || !k_drafts || !v_drafts))
       return refuse(c, RBT_E_INVALID, "null layer pointers");
     for (size_t l = 0; l < d->n_layers; l++) {

@@ -298,3 +298,18 @@ def test_gate_views(rbt_lib, B, N, stride, ok):
     ctx = _no_gpu(rbt_lib)
     with pytest.raises(R.RbtError if ok else ValueError, match="null context" if ok else "gate"):
         ctx.gqa_tree(*_attend_args(B, N, 4, 2, 64, _Tensor(B, N, 4, 64, stride=stride)), sync=False)
+
+
+@pytest.mark.parametrize("B,args", [
+    (2, dict(n_path=2 * A, path=3 * A, len=4 * A, len_out=2 * A)), (2, dict(n_path=2 * A, path=3 * A, len=4 * A, len_out=3 * A)),
+    (2, dict(n_path=2 * A, path=3 * A, len=4 * A, len_out=3 * A + 20)), (2, dict(n_path=2 * A, path=3 * A, len=4 * A, len_out=4 * A - 4)),
+    (2, dict(n_path=2 * A, path=3 * A, len=4 * A, len_out=4 * A + 4))])
+def test_commit_refuses_lengths_over_its_inputs(rbt_lib, B, args):
+    """len_out is written while other workgroups, and the launches of further layers, still read path, n_path and len."""
+    d = abi.RbtKvCommitDesc(2, 4, 64, 0, 100)
+    ptr = (C.c_void_p * 2)(A, A)
+    call = lambda a: rbt_lib.rbt_kv_commit_d(None, C.byref(d), B, 3, ptr, ptr, ptr, ptr, a["path"], a["n_path"], a["len"],  # noqa: E731
+                                             a["len_out"])
+    _refused(rbt_lib, call(args), RBT_E_INVALID, "len_out")
+    for free in (3 * A + 24, 3 * A - 8, 2 * A + 8, 4 * A + 8, 5 * A):  # beside them
+        _refused(rbt_lib, call({**args, "len_out": free}), RBT_E_INVALID, "null context")
