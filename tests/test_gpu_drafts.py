@@ -844,3 +844,19 @@ def test_positions_up_to_the_largest(ctx):
     with pytest.raises(R.RbtError):
         ctx.sync()
     assert _np(pos).tolist() == [[-1] * 3, [-1] * 3, [4, 5, 6], [5, 6, -1]]
+
+
+@pytest.mark.parametrize("N,V,children", [(2, 5000, 0), (2, 70001, 0), (12, 70001, 0), (12, 40000, 11), (200, 20000, 0)])
+def test_verify_rejections(ctx, N, V, children):
+    """One child, and more rejections at one node than the call has launches: each residual is the last one's, and the draw is
+    from what the last leaves."""
+    rng = np.random.default_rng(N + V)
+    B = 3
+    p, q = (_softmax(rng.standard_normal((B, N, V)) * 2) for _ in range(2))
+    par = np.where(np.arange(N) == 0, -1, 0)[None].repeat(B, 0).astype(np.int32)
+    tok = np.stack([rng.choice(V, N, p=q[b, 0].astype(np.float64) / q[b, 0].astype(np.float64).sum()) for b in range(B)])
+    u = rng.random((B, N), dtype=np.float32)
+    u[:2, 1:] = np.float32(1.0) - np.float32(2.0 ** -24)  # rejected unless the residual passes q
+    p[1, 0, tok[1, 1:]] = 0.0                              # none can stand
+    path, n_path, _ = _verify(ctx, tok.astype(np.int32), par, [N] * B, p, q, u, children)
+    assert n_path[1] == 1
