@@ -385,7 +385,7 @@ typedef struct {
     int32_t layout;          /* RBT_ROPE_HALF, RBT_ROPE_INTERLEAVED */
     size_t head_dim;         /* 1..1024 */
     size_t rope_start, rope_dim;  /* the rotated entries of a head; rope_dim even, may be 0 */
-    const double *inv_freq;  /* device f64 [rope_dim / 2] (rbt_rope_freqs) */
+    const double *inv_freq;  /* device f64 [rope_dim / 2] (rbt_rope_freqs); pos * inv_freq below 2^31 */
     float factor;            /* multiplies cos and sin */
     int32_t angle_f32;       /* 0: pos * inv_freq in 64 bits; 1: the product rounded to f32, as
                                 rbt_gqa_step_d rounds it (with frequencies made as_f32) */
@@ -423,9 +423,9 @@ int rbt_tree_positions_d(rbt_ctx *ctx, size_t n_seq, size_t max_nodes, const int
  * from 2^-110 on) and sums f32.
  * head_dim 1..1024, fastest at 64, 128, 192 and 256; any number of query heads per KV head. q, out, caches
  * and draft rows are 16-byte aligned, and out overlaps none of the others. Values that a node does not see never reach
- * its output, non-finite ones included. A non-finite value that it sees makes its entry of the output non-finite (an
- * infinite one may give a NaN), a NaN key all entries. An infinite key counts for nothing where its score is -inf, as in
- * the formula, or makes all entries non-finite: which of the two is not specified. */
+ * its output, non-finite ones included. A non-finite value that it sees makes its entry of the output
+ * non-finite (an infinite one may give a NaN), a NaN key all entries. An infinite key counts for nothing where
+ * its score is -inf, as in the formula, or makes all entries non-finite: which of the two is not specified. */
 typedef struct {
     size_t n_heads, n_kv_heads, head_dim;
     float attn_scale;
@@ -461,8 +461,9 @@ int rbt_draft_verify_d(rbt_ctx *ctx, size_t n_seq, size_t max_nodes, size_t voca
 /* KvCache::push (qwen38/attention.rs:76-82) of the standing nodes, for every layer at once: rows
  * path[b, j], j < n_path[b], of the layers' draft rows to rows len[b] + j of their caches;
  * len_out[b] = len[b] + n_path[b]. The four pointer arrays are host memory holding n_layers device
- * pointers each. len_out overlaps none of len, path and n_path (RBT_E_INVALID). A sequence that does not fit (len + n_path > cap, or a path entry
- * outside 0..max_nodes-1) is left as it was with len_out = len, and reported by the next rbt_sync. */
+ * pointers each. len_out overlaps none of len, path and n_path (RBT_E_INVALID). A sequence that does not
+ * fit (len + n_path > cap, or a path entry outside 0..max_nodes-1) is left as it was with len_out = len, and
+ * reported by the next rbt_sync. */
 typedef struct {
     size_t n_layers, n_kv_heads, head_dim;
     int32_t kv_dtype;

@@ -2193,7 +2193,8 @@ int rbt_rope_freqs(const rbt_rope_scaling *sc, float theta, size_t rope_dim, dou
   const double d = (double)rope_dim, two_pi = 6.283185307179586;
   double base = theta;
   if (s.kind == RBT_ROPE_BASE && rope_dim) base *= std::pow((double)s.factor, d / (d - 2.0));
-  // YaRN's ramp: the (fractional) pair whose wavelength fits `turns` times into the context
+  // The larger base, and YaRN's parts and factor, as published (Peng et al., "YaRN: Efficient Context Window Extension of
+  // Large Language Models", 2023). The ramp: the (fractional) pair whose wavelength fits `turns` times into the context
   const auto pair_of = [&](double turns) { return d * std::log(s.orig_ctx / (turns * two_pi)) / (2.0 * std::log(base)); };
   double low = 0.0, high = 0.0;
   if (s.kind == RBT_ROPE_YARN) {

@@ -283,8 +283,8 @@ hipError_t launch_tree_pos(const Ctx &c, const int *parent, const int *n_nodes, 
 // Chains, and drafts without q, need one pass and so one launch. Sums are in 64 bits, and as their order is fixed
 // the drawn token is too. Bound by trips to memory that follow one another (count, tokens, their p and q, the
 // pass, the arrival, the sums, the draw), not by bytes: a chain of five over 32000 entries takes 12.7 us, one over
-// 131072 entries 13, sixteen of them 21; sixteen trees of 32 nodes 80 in six launches, of which most end at once (one
-// workgroup per sequence for all of it: 26 and, for the trees, 191).
+// 131072 entries 13, sixteen of them 21; sixteen trees of 32 nodes 66 to 84 by their walks in six launches, of
+// which most end at once (one workgroup per sequence for all of it: 26 and, for the trees, 191 where six launches take 80).
 constexpr int VF_NT = 256, VF_G = 64, VF_ROUNDS = 6;  // threads per workgroup, chunks and launches at most
 
 struct VerifyRow {

@@ -10,14 +10,14 @@
 //
 // Bounds and times (64 query heads over 4 KV heads of 256, one MI355X):
 //   64 nodes over 32749 bf16 rows: 292-314 us, of them 280-290 in k_tree: 412 GFLOP of bf16 products, 1.4 PFLOP/s (a
-//     large library product reaches 1.2); the matrix cores are busy 61% of the cycles, at a clock that the load holds
+//     large library product reaches 1.2); the matrix cores are busy 63% of the cycles, at a clock that the load holds
 //     near 2 GHz.
 //   16 trees of 12 to 24 nodes over 4096 to 8192 bf16 rows: 353-368 us, k_tree 324-337; the products as above, and
 //     row tiles that a sequence fills in part.
 //   32 sequences of one node over 2048 to 4096 rows, 32 query heads over 8 KV heads: 41 us for bf16 rows of 64, 90 for
-//     bf16 of 128, 86 and 189 for f32: the caches at 4.3 to 4.9 TB/s.
+//     bf16 of 128, 88 and 189 for f32: the caches at 4.3 to 4.9 TB/s.
 //   one node over 32768 bf16 rows: 35 us, k_tree 26 (134 MB: 5.1 TB/s); over 513 rows: 13.3 us, two launches of one
-//     trip to memory each; five nodes over 4096 f32 rows: 34 us.
+//     trip to memory each; five nodes over 4096 f32 rows: 32 us.
 #include "rbt_device.h"
 #include "rbt_internal.h"
 
@@ -153,7 +153,8 @@ typedef short ts4 __attribute__((ext_vector_type(4)));
 typedef __bf16 tb8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) ts4 tree_lds_s4;
 
-// 64 lanes' 16 bytes at p (each its own) to LDS at `base` (the wave's) + 16 lane.
+// 64 lanes' 16 bytes at p (each its own) to LDS at `base` (the wave's) + 16 lane. m0 is a register that the compiler
+// reserves: it keeps nothing there from one statement to the next, and warns of it in a list of clobbers.
 __device__ __forceinline__ void tree_dma(const void *p, uint32_t base) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(base), "v"(p) : "memory");
 }
@@ -203,8 +204,8 @@ __device__ __forceinline__ float tree_xor_sum(float v) {
 
 // How keys and values reach the matrix cores: bf16 as they are, f32 as they are, f32 in three bf16 parts.
 // KV_PARTS4: by workgroups of four waves, several of them on a CU, for batches of up to four row tiles at head dims 64
-// and 128. 12 nodes of 32 query heads over 8 KV heads of 128: 32 sequences of up to 4096 rows 243 us with eight waves,
-// 208 with four, but one of 8192 rows (16 nodes) 27.5 and 31.4, where loading a stage is what it waits for.
+// and 128. 12 nodes of 32 query heads over 8 KV heads of 128: 32 sequences of up to 4096 rows 246 us with eight waves,
+// 207 with four, but one of 8192 rows (16 nodes) 27.6 and 30.9, where loading a stage is what it waits for.
 enum { KV_BF16 = 0, KV_F32 = 1, KV_PARTS = 2, KV_PARTS4 = 3 };
 constexpr bool tree_parts(int kv) { return kv >= KV_PARTS; }
 
@@ -864,7 +865,8 @@ bool tree_plan(const Ctx &c, TreeArgs &a) {
   // 0.8 of the longest each, and the last ones are waited for. A batch at a smaller head dim runs `hold` workgroups
   // beside each other on a CU: a stage is then mostly waiting, all but `busy` of it, and grows less with the head
   // dim, until the caches pass at 5.0 TB/s (sequences taken at three quarters of the longest; a sixth less with one
-  // workgroup per CU, and evenly only where every CU has as many). Measured over bf16 rows at head_dim 256: one node
+  // workgroup per CU, and evenly only where every CU has as many). One sequence keeps the first model, whatever its
+  // head dim: with the batches' it took 5 to 13% longer. Measured over bf16 rows at head_dim 256: one node
   // over 4096 rows 113 us in one piece, 27 in 8, 17 in 32, 17 in 64; 64 nodes over 32749 rows 527 in 4, 311 in 8, 326
   // in 16, 368 in 32; 16 sequences of one node over 3000 to 6000 rows 186 in 1, 65 in 4, 74 in 8, 86 in 16. And with
   // 32 query heads over 8 KV heads, 32 sequences of up to 4096 rows (one piece fills every CU once): one node over
@@ -873,8 +875,8 @@ bool tree_plan(const Ctx &c, TreeArgs &a) {
   const bool wide = rw > 4;  // two waves on a SIMD
   const double ncu = c.num_cu, base = (double)a.tiles * a.K * a.B, most = std::ceil((double)(a.max_len + a.T) / TK);
   const double part = a.hd / 256.0;
-  // (from eight stages a CU on; three sequences of 1001 rows, one and a half a CU: 14.5 us with eight waves, 15.3 with
-  // four; eight of 4096, 32 a CU: 74 and 67)
+  // (from eight stages a CU on, a point between two measured ones: three sequences of 1001 rows, one and a half a CU,
+  // 15.2 us with eight waves, 15.6 with four; eight of 4096, 32 a CU, 72 and 63)
   a.four = !a.kv16 && kw == 1 && a.hd <= 128 && rw <= 4 && a.B > 1 && base * most >= 8 * ncu;
   double stage, busy = 1.0, hold = 1.0;
   if (a.B == 1) {
