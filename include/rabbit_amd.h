@@ -356,7 +356,11 @@ int rbt_gqa_step_d(rbt_ctx *ctx, const rbt_gqa_desc *desc, float *k_cache, float
  *    parent outside its range is taken as -1; the next rbt_sync then returns RBT_E_INVALID. Nothing out
  *    of the arrays' bounds is read or written.
  *  - Graphs captured on one context share its scratch: replay them one after another. */
-typedef enum { RBT_DT_F32 = 0, RBT_DT_BF16 = 1 } rbt_dtype;
+typedef enum {
+    RBT_DT_F32 = 0,
+    RBT_DT_BF16 = 1,
+    RBT_DT_I8 = 8  /* rows of a cache only: int8 entries, one f32 scale per row and KV head (rbt_kv_quant_d) */
+} rbt_dtype;
 
 /* Frequencies of rotary positions. theta^(-2j/rope_dim), j < rope_dim/2, changed for long contexts:
  *   LINEAR      every frequency / factor (positions interpolated)
@@ -472,6 +476,90 @@ typedef struct {
 int rbt_kv_commit_d(rbt_ctx *ctx, const rbt_kv_commit_desc *desc, size_t n_seq, size_t max_nodes, void *const *k_caches,
                     void *const *v_caches, const void *const *k_drafts, const void *const *v_drafts,
                     const int32_t *path, const int32_t *n_path, const int32_t *len, int32_t *len_out);
+
+/* ---- a batch's decode step: 8-bit caches, shared prefixes, sampling (device buffers; no counterpart in
+ * the reference) ----
+ * A server that decodes many sequences calls, per attention layer, rbt_rope_d, rbt_kv_quant_d where the cache is
+ * held in 8 bits, and rbt_gqa_prefix_d; and once per step rbt_sample_d. Lengths and counts are int32 device arrays, so a
+ * captured graph follows them. A sequence (or row of logits) whose numbers do not fit is skipped and
+ * reported by the next rbt_sync (RBT_E_INVALID). Graphs captured on one context share its scratch: replay them
+ * one after another. */
+
+/* An 8-bit cache holds, per row and KV head, head_dim int8 entries and one f32 scale: with a = max |x|,
+ * scale = a / 127 and entry = x / scale, the quotients rounded to f32 and the entry then to the nearest whole number
+ * (ties to even, within -127..127). It stands for entry * scale: off by half a step, a / 254, at most (where a / 127 is a normal
+ * f32). A row of zeros has scale 0; a row with a non-finite entry has scale NaN and entries 0: it reads back
+ * as NaN. Entries lie [n_seq, cap, n_kv_heads, head_dim], scales [n_seq, cap, n_kv_heads]. rbt_kv_commit_d moves
+ * such rows with kv_dtype RBT_DT_I8, and their scales as RBT_DT_F32 rows of head_dim 1. */
+typedef struct {
+    const void *k, *v;            /* the rows' entries */
+    const float *k_scale, *v_scale;  /* RBT_DT_I8 only, else not used */
+} rbt_kv_rows;                   /* a host struct of device pointers; rbt_kv_quant_d writes through them */
+typedef struct {
+    size_t n_kv_heads, head_dim;  /* head_dim 1..1024 */
+    size_t cap;                  /* rows of a sequence's cache */
+    int32_t dtype;               /* RBT_DT_F32 or RBT_DT_BF16: the rows outside the cache */
+    size_t seq_stride, row_stride, head_stride;  /* theirs, in entries, of both k and v; head_dim contiguous */
+} rbt_kv_quant_desc;
+/* KvCache::push (qwen38/attention.rs:76-82) for a batch, into 8 bits: rows j < n_rows[b] (NULL: max_rows) of k and v
+ * to rows len[b] + j (NULL: j) of sequence b's cache. cache->k, v and scales are written; other rows stay as they
+ * were. k, v and the cache do not overlap. A sequence with n_rows outside 0..max_rows, or that does not fit
+ * its cache, is skipped and reported. n_seq <= 65535. */
+int rbt_kv_quant_d(rbt_ctx *ctx, const rbt_kv_quant_desc *desc, size_t n_seq, size_t max_rows, const void *k, const void *v,
+                   const int32_t *len, const int32_t *n_rows, const rbt_kv_rows *cache);
+/* The other way: rows len[b] + j (NULL: j), j < n_rows[b] (NULL: max_rows), of the cache to rows j of k and v,
+ * rounded once to their type. Rows of k and v may not overlap each other (RBT_E_INVALID); rows past n_rows[b] stay as
+ * they were. */
+int rbt_kv_dequant_d(rbt_ctx *ctx, const rbt_kv_quant_desc *desc, size_t n_seq, size_t max_rows, const rbt_kv_rows *cache,
+                     const int32_t *len, const int32_t *n_rows, void *k, void *v);
+
+/* rbt_gqa_tree_d for sequences that share prefixes, over f32, bf16 or 8-bit rows: sequences prefix_first[g] ..
+ * prefix_first[g + 1] - 1 also attend to the prefix_len[g] first rows of prefix g, ahead of their own len[b] rows. A
+ * prefix's rows are read once for all of its sequences. prefix [n_prefix, prefix_cap, n_kv_heads, head_dim];
+ * prefix_first int32 [n_prefix + 1], each at least the one before it and all within 0..n_seq (sequences outside have
+ * no prefix; else every sequence is skipped and reported); prefix_len int32 [n_prefix] in 0..prefix_cap (else
+ * its sequences are skipped and reported). The caches' len[b] are rows after the prefix, and so are positions for
+ * rbt_rope_d: pos = prefix_len + len + depth (rbt_tree_positions_d with the sum as len).
+ *  - draft NULL: the nodes' own rows are in the cache, node i's at row len[b] + i (len + n_nodes <= cap): plain decoding
+ *    whose new row has been written, or a chain. Else as rbt_gqa_tree_d's draft rows, of the cache's type.
+ *  - parent NULL: chains (node i hangs from node i - 1).
+ *  - n_prefix 0: prefix, prefix_len and prefix_first are not used.
+ * Everything else as rbt_gqa_tree_d; entries 16-byte aligned, scales 4-byte. Over 8-bit rows q and the
+ * probabilities are taken to 2^-22 of their row's largest (of 64 or 128 keys at a time), products and
+ * their sums are exact in whole numbers, and sums over all keys f32. n_prefix <= 1024 and
+ * n_seq * max_nodes * (query heads per KV head) <= 2^20 (RBT_E_UNSUPPORTED). A row with scale NaN
+ * makes every entry NaN of the nodes that see it, and of no other. */
+typedef struct {
+    size_t n_heads, n_kv_heads, head_dim;
+    float attn_scale;
+    int32_t kv_dtype;            /* RBT_DT_F32, RBT_DT_BF16, RBT_DT_I8: prefixes, caches and draft rows */
+    size_t cap, max_len;         /* rows of a sequence's cache; a length no sequence is expected to pass (0: cap) */
+    size_t prefix_cap, max_prefix;  /* rows of a prefix's cache; a length none is expected to pass (0: prefix_cap) */
+    size_t gate_token_stride, gate_head_stride;
+} rbt_gqa_prefix_desc;
+int rbt_gqa_prefix_d(rbt_ctx *ctx, const rbt_gqa_prefix_desc *desc, size_t n_seq, size_t max_nodes, size_t n_prefix,
+                     const float *q, const rbt_kv_rows *prefix, const rbt_kv_rows *cache, const rbt_kv_rows *draft,
+                     const int32_t *prefix_len, const int32_t *prefix_first, const int32_t *len, const int32_t *n_nodes,
+                     const int32_t *parent, const float *gate, float *out);
+
+/* The next tokens of n rows of logits, from given random numbers. Per row, with x the logits, t the
+ * temperature and m = max x: w_i = exp((x_i - m) / t), in 64 bits. The entries' order is the larger logit first, of equal ones the
+ * lower index. Of these are kept: the first top_k (0: all); of what is left, the shortest run from the front whose
+ * sum of w reaches top_p of theirs (1: all; at least one); and those with w >= min_p. p_i = w_i / (the sum of
+ * what is kept), 0 elsewhere. tokens[r] is the least index whose running sum of p passes u[r]. t = 0 takes the
+ * first of the order alone (greedy). w and its sums are exact to 2^-45 of the largest w (vocabularies up to 2^17; one bit less
+ * for each doubling).
+ * logits [n, vocab] of logits_dtype, row_stride entries apart. temperature, top_p, min_p f32 [n] and top_k
+ * int32 [n] may be NULL: 1, 1, 0 and 0. u f32 [n] in [0, 1). NaN and -inf entries are never drawn; a row
+ * without an entry above -inf, or with +inf, gives token -1 and zeros. So does one whose settings are out of range
+ * (t negative or not finite, top_k < 0, top_p or min_p outside 0..1, u outside [0, 1)), and the next rbt_sync reports it.
+ * probs f32 [n, vocab] gets p (what rbt_draft_verify_d takes), or is NULL. vocab <= 2^24; n <= 65535. */
+typedef struct {
+    size_t vocab, row_stride;
+    int32_t logits_dtype;        /* RBT_DT_F32, RBT_DT_BF16 */
+} rbt_sample_desc;
+int rbt_sample_d(rbt_ctx *ctx, const rbt_sample_desc *desc, size_t n, const void *logits, const float *temperature,
+                 const int32_t *top_k, const float *top_p, const float *min_p, const float *u, int32_t *tokens, float *probs);
 
 /* ---- instrumentation (no counterpart in the reference: benchmark support) -------------------- */
 typedef struct {

@@ -27,11 +27,11 @@ from .abi import (ACT_SILU, FAMILY_GLM52, FAMILY_KIMI_K3, FAMILY_QWEN38, QT_F32,
 
 __all__ = ["Context", "QT", "Slot", "Shards", "RbtError", "load", "QT_F32", "QT_I4_GROUPED", "QT_MXFP4",
            "FAMILY_QWEN38", "FAMILY_GLM52", "FAMILY_KIMI_K3", "ACT_SILU", "NAMING_QWEN38_MXFP4",
-           "NAMING_KIMI_K3_MXFP4", "ACT_SITU", "situ", "DT_F32", "DT_BF16", "ROPE_HALF", "ROPE_INTERLEAVED",
+           "NAMING_KIMI_K3_MXFP4", "ACT_SITU", "situ", "DT_F32", "DT_BF16", "DT_I8", "ROPE_HALF", "ROPE_INTERLEAVED",
            "ROPE_PLAIN", "ROPE_LINEAR", "ROPE_BASE", "ROPE_YARN", "ROPE_WAVELENGTH", "rope_freqs", "rope_part"]
 from .abi import NAMING_KIMI_K3_MXFP4, NAMING_QWEN38_MXFP4, ACT_SITU  # noqa: E402
-from .abi import (DT_BF16, DT_F32, ROPE_BASE, ROPE_HALF, ROPE_INTERLEAVED, ROPE_LINEAR, ROPE_PLAIN,  # noqa: E402
-                  ROPE_WAVELENGTH, ROPE_YARN)
+from .abi import (DT_BF16, DT_F32, DT_I8, ROPE_BASE, ROPE_HALF, ROPE_INTERLEAVED, ROPE_LINEAR,  # noqa: E402
+                  ROPE_PLAIN, ROPE_WAVELENGTH, ROPE_YARN)
 
 
 def situ(beta, linear_beta=None):
@@ -79,6 +79,14 @@ def _dtype(t) -> int:
     return DT_BF16 if name == "torch.bfloat16" else DT_F32
 
 
+_KV_NAMES = {DT_F32: "float32", DT_BF16: "bfloat16", DT_I8: "int8"}
+
+
+def _kv_dtype(t) -> int:
+    """The rbt_dtype of a cache's rows."""
+    return DT_I8 if str(t.dtype) == "torch.int8" else _dtype(t)
+
+
 def _dense(name, t, dtype, *shape):
     """t's device pointer, its type, size and layout checked (None passes)."""
     if t is None:
@@ -86,6 +94,27 @@ def _dense(name, t, dtype, *shape):
     if str(t.dtype) != "torch." + dtype or tuple(t.shape) != shape:
         raise ValueError(f"{name} is {dtype} {list(shape)}, not {str(t.dtype)[6:]} {list(t.shape)}")
     return _ptr(t)
+
+
+def _kv_rows(name, rows, kv, *shape):
+    """Rows of a cache, (k, v) or (k, v, k_scale, v_scale) tensors of [.., n_kv, head_dim] and [.., n_kv], as an
+    RbtKvRows (None passes)."""
+    if rows is None:
+        return None
+    if len(rows) != (4 if kv == "int8" else 2):
+        raise ValueError(f"{name}: k and v, and the scales of both where they are int8")
+    return abi.RbtKvRows(*[_dense(name, t, kv, *shape) for t in rows[:2]],
+                         *[_dense(name + " scale", t, "float32", *shape[:-1]) for t in rows[2:]])
+
+
+def _gate_strides(gate, B, T, H, D):
+    """Token and head strides of a gate like q [B, T, H, D], or of a view of [query, gate] rows."""
+    if gate is None:
+        return 0, 0
+    if not gate.is_cuda or str(gate.dtype) != "torch.float32" or tuple(gate.shape) != (B, T, H, D) or \
+            (D > 1 and gate.stride(3) != 1) or (B > 1 and T > 1 and gate.stride(0) != T * gate.stride(1)):
+        raise ValueError("gate must be float32 like q, its entries contiguous and its sequences T tokens apart")
+    return gate.stride(1) if T > 1 else gate.stride(0), gate.stride(2)
 
 
 def rope_freqs(rope_dim: int, theta: float, kind: int = ROPE_PLAIN, factor: float = 1.0, orig_ctx: float = 0.0,
@@ -462,12 +491,7 @@ class Context:
         B, T, H, D = q.shape
         cap, K = k_cache.shape[1:3]
         kv = "bfloat16" if _dtype(k_cache) == DT_BF16 else "float32"
-        gs = (0, 0)
-        if gate is not None:
-            if not gate.is_cuda or str(gate.dtype) != "torch.float32" or tuple(gate.shape) != (B, T, H, D) or \
-                    (D > 1 and gate.stride(3) != 1) or (B > 1 and T > 1 and gate.stride(0) != T * gate.stride(1)):
-                raise ValueError("gate must be float32 like q, its entries contiguous and its sequences T tokens apart")
-            gs = (gate.stride(1) if T > 1 else gate.stride(0), gate.stride(2))
+        gs = _gate_strides(gate, B, T, H, D)
         d = abi.RbtGqaTreeDesc(H, K, D, attn_scale, _dtype(k_cache), cap, max_len, *gs)
         if sync:
             self._torch_sync()
@@ -499,16 +523,17 @@ class Context:
 
     def kv_commit(self, k_caches, v_caches, k_drafts, v_drafts, path, n_path, length, length_out, sync=True):
         """rbt_kv_commit_d: the standing nodes' draft rows appended to every layer's cache. Lists with one
-        tensor per layer: caches [n_seq, cap, n_kv, head_dim], drafts [n_seq, max_nodes, n_kv, head_dim]."""
+        tensor per layer: caches [n_seq, cap, n_kv, head_dim], drafts [n_seq, max_nodes, n_kv, head_dim]. int8 rows'
+        scales go by a second call, as float32 rows of head_dim 1 (t.unsqueeze(-1))."""
         L = len(k_caches)
         if not (len(v_caches) == len(k_drafts) == len(v_drafts) == L):
             raise ValueError("one cache and one draft buffer per side and layer")
         B, T = path.shape
         cap, K, D = k_caches[0].shape[1:] if L else (2**31 - 1, 1, 1)
-        kv = "float32" if L == 0 or _dtype(k_caches[0]) == DT_F32 else "bfloat16"
+        kv = _KV_NAMES[_kv_dtype(k_caches[0]) if L else DT_F32]
         arr = [(C.c_void_p * max(1, L))(*[_dense("cache or draft", t, kv, B, rows, K, D) for t in ts])
                for ts, rows in ((k_caches, cap), (v_caches, cap), (k_drafts, T), (v_drafts, T))]
-        d = abi.RbtKvCommitDesc(L, K, D, DT_F32 if kv == "float32" else DT_BF16, cap)
+        d = abi.RbtKvCommitDesc(L, K, D, _kv_dtype(k_caches[0]) if L else DT_F32, cap)
         if sync:
             self._torch_sync()
         self.check(self.lib.rbt_kv_commit_d(self.h, C.byref(d), B, T, *arr, _dense("path", path, "int32", B, T),
@@ -517,6 +542,87 @@ class Context:
         if sync:
             self.sync()
         return length_out
+
+    # -- a batch's decode step (device tensors) -----------------------------------------------
+    def _kv_call(self, name, fn, k, v, cache, length, n_rows, write, sync):
+        # (a step that nothing takes, in a size of one, may be any number)
+        steps = lambda t: [t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)]  # noqa: E731
+        if k.dim() != 4 or tuple(k.shape) != tuple(v.shape) or steps(k) != steps(v) or _dtype(k) != _dtype(v) or \
+                any(t.shape[3] > 1 and t.stride(3) != 1 for t in (k, v)) or not (k.is_cuda and v.is_cuda):
+            raise ValueError(f"{name}: k and v are [n_seq, max_rows, n_kv, head_dim] of one type and layout on the GPU, "
+                             "head_dim contiguous")
+        B, T, K, D = k.shape
+        cap = cache[0].shape[1]
+        rows = _kv_rows("cache", cache, "int8", B, cap, K, D)
+        d = abi.RbtKvQuantDesc(K, D, cap, _dtype(k), *steps(k))
+        at = (_dense("length", length, "int32", B), _dense("n_rows", n_rows, "int32", B))
+        if sync:
+            self._torch_sync()
+        if write:
+            self.check(fn(self.h, C.byref(d), B, T, k.data_ptr(), v.data_ptr(), *at, C.byref(rows)))
+        else:
+            self.check(fn(self.h, C.byref(d), B, T, C.byref(rows), *at, k.data_ptr(), v.data_ptr()))
+        if sync:
+            self.sync()
+
+    def kv_quant(self, k, v, cache, length=None, n_rows=None, sync=True):
+        """rbt_kv_quant_d: rows k, v [n_seq, max_rows, n_kv, head_dim] (float32 or bfloat16, strided views allowed) to
+        rows length[b] + j of an 8-bit cache (k, v, k_scale, v_scale): int8 [n_seq, cap, n_kv, head_dim] and
+        float32 [n_seq, cap, n_kv]. length None: from row 0; n_rows None: all of them."""
+        self._kv_call("kv_quant", self.lib.rbt_kv_quant_d, k, v, cache, length, n_rows, True, sync)
+        return cache
+
+    def kv_dequant(self, cache, k, v, length=None, n_rows=None, sync=True):
+        """rbt_kv_dequant_d: rows length[b] + j of an 8-bit cache to rows j of k and v, float32 or bfloat16."""
+        self._kv_call("kv_dequant", self.lib.rbt_kv_dequant_d, k, v, cache, length, n_rows, False, sync)
+        return k, v
+
+    def gqa_prefix(self, q, cache, length, n_nodes, attn_scale, out, draft=None, parent=None, prefix=None, prefix_len=None,
+                   prefix_first=None, gate=None, max_len=0, max_prefix=0, sync=True):
+        """rbt_gqa_prefix_d: attention of a batch over shared prefixes and own caches. q, out float32 [n_seq,
+        max_nodes, n_heads, head_dim]; cache, draft and prefix (k, v) of [n_seq, cap or max_nodes, or n_prefix,
+        prefix_cap, n_kv, head_dim], float32 or bfloat16, or (k, v, k_scale, v_scale) of int8 rows. draft None: the
+        nodes' rows are in the cache; parent None: chains; gate as gqa_tree's."""
+        B, T, H, D = q.shape
+        cap, K = cache[0].shape[1:3]
+        kind = _kv_dtype(cache[0])
+        kv = _KV_NAMES[kind]
+        G, pcap = prefix[0].shape[:2] if prefix is not None else (0, 0)
+        gs = _gate_strides(gate, B, T, H, D)
+        d = abi.RbtGqaPrefixDesc(H, K, D, attn_scale, kind, cap, max_len, pcap, max_prefix, *gs)
+        rows = [_kv_rows("cache", cache, kv, B, cap, K, D), _kv_rows("draft", draft, kv, B, T, K, D),
+                _kv_rows("prefix", prefix, kv, G, pcap, K, D) if G else None]
+        c, dr, p = [None if r is None else C.byref(r) for r in rows]
+        plen, first = (_dense("prefix_len", prefix_len, "int32", G), _dense("prefix_first", prefix_first, "int32", G + 1)) \
+            if G else (None, None)
+        if sync:
+            self._torch_sync()
+        self.check(self.lib.rbt_gqa_prefix_d(
+            self.h, C.byref(d), B, T, G, _dense("q", q, "float32", B, T, H, D), p, c, dr, plen, first,
+            _dense("length", length, "int32", B), _dense("n_nodes", n_nodes, "int32", B),
+            _dense("parent", parent, "int32", B, T), None if gate is None else gate.data_ptr(),
+            _dense("out", out, "float32", B, T, H, D)))
+        if sync:
+            self.sync()
+        return out
+
+    def sample(self, logits, u, tokens, temperature=None, top_k=None, top_p=None, min_p=None, probs=None, sync=True):
+        """rbt_sample_d: tokens (int32 [n]) from logits [n, vocab] (float32 or bfloat16, rows any distance apart) and
+        uniform numbers u [n]; temperature, top_p, min_p float32 [n] and top_k int32 [n] or None (1, 1, 0, 0: off); probs float32
+        [n, vocab] gets the probabilities that were drawn from."""
+        n, V = logits.shape
+        if not logits.is_cuda or (V > 1 and logits.stride(1) != 1):
+            raise ValueError("logits are [n, vocab] on the GPU, their rows contiguous")
+        d = abi.RbtSampleDesc(V, logits.stride(0) if n > 1 else V, _dtype(logits))
+        if sync:
+            self._torch_sync()
+        self.check(self.lib.rbt_sample_d(
+            self.h, C.byref(d), n, logits.data_ptr(), _dense("temperature", temperature, "float32", n),
+            _dense("top_k", top_k, "int32", n), _dense("top_p", top_p, "float32", n), _dense("min_p", min_p, "float32", n),
+            _dense("u", u, "float32", n), _dense("tokens", tokens, "int32", n), _dense("probs", probs, "float32", n, V)))
+        if sync:
+            self.sync()
+        return tokens
 
     # -- instrumentation --------------------------------------------------------------------
     def profile_enable(self, on: bool = True):

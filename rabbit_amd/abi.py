@@ -27,7 +27,7 @@ STATUS_NAMES = {0: "RBT_OK", -1: "RBT_E_INVALID", -2: "RBT_E_SHAPE", -3: "RBT_E_
 QT_F32, QT_I4_GROUPED, QT_MXFP4 = 0, 1, 2
 FAMILY_QWEN38, FAMILY_GLM52, FAMILY_KIMI_K3 = 0, 1, 2
 ACT_SILU, ACT_SITU = 0, 1
-DT_F32, DT_BF16 = 0, 1
+DT_F32, DT_BF16, DT_I8 = 0, 1, 8
 ROPE_HALF, ROPE_INTERLEAVED = 0, 1
 ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_YARN, ROPE_WAVELENGTH = 0, 1, 2, 3, 4
 
@@ -111,6 +111,26 @@ class RbtKvCommitDesc(C.Structure):
                 ("kv_dtype", C.c_int32), ("cap", C.c_size_t)]
 
 
+class RbtKvRows(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p)]
+
+
+class RbtKvQuantDesc(C.Structure):
+    _fields_ = [("n_kv_heads", C.c_size_t), ("head_dim", C.c_size_t), ("cap", C.c_size_t), ("dtype", C.c_int32),
+                ("seq_stride", C.c_size_t), ("row_stride", C.c_size_t), ("head_stride", C.c_size_t)]
+
+
+class RbtGqaPrefixDesc(C.Structure):
+    _fields_ = [("n_heads", C.c_size_t), ("n_kv_heads", C.c_size_t), ("head_dim", C.c_size_t),
+                ("attn_scale", C.c_float), ("kv_dtype", C.c_int32), ("cap", C.c_size_t), ("max_len", C.c_size_t),
+                ("prefix_cap", C.c_size_t), ("max_prefix", C.c_size_t), ("gate_token_stride", C.c_size_t),
+                ("gate_head_stride", C.c_size_t)]
+
+
+class RbtSampleDesc(C.Structure):
+    _fields_ = [("vocab", C.c_size_t), ("row_stride", C.c_size_t), ("logits_dtype", C.c_int32)]
+
+
 class RbtKernelStat(C.Structure):
     _fields_ = [("name", C.c_char * 160), ("launches", C.c_uint64), ("total_ms", C.c_double)]
 
@@ -184,6 +204,11 @@ SIGNATURES = {
     "rbt_draft_verify_d": (_I, [_CTX, _S, _S, _S, _S, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "rbt_kv_commit_d": (_I, [_CTX, C.POINTER(RbtKvCommitDesc), _S, _S, C.POINTER(_P), C.POINTER(_P), C.POINTER(_P),
                              C.POINTER(_P), _P, _P, _P, _P]),
+    "rbt_kv_quant_d": (_I, [_CTX, C.POINTER(RbtKvQuantDesc), _S, _S, _P, _P, _P, _P, C.POINTER(RbtKvRows)]),
+    "rbt_kv_dequant_d": (_I, [_CTX, C.POINTER(RbtKvQuantDesc), _S, _S, C.POINTER(RbtKvRows), _P, _P, _P, _P]),
+    "rbt_gqa_prefix_d": (_I, [_CTX, C.POINTER(RbtGqaPrefixDesc), _S, _S, _S, _P, C.POINTER(RbtKvRows), C.POINTER(RbtKvRows),
+                              C.POINTER(RbtKvRows), _P, _P, _P, _P, _P, _P, _P]),
+    "rbt_sample_d": (_I, [_CTX, C.POINTER(RbtSampleDesc), _S, _P, _P, _P, _P, _P, _P, _P, _P]),
     "rbt_profile_enable": (_I, [_CTX, _I]),
     "rbt_profile_read": (_I, [_CTX, C.POINTER(RbtProfile), _I]),
     "rbt_profile_kernels": (_I, [_CTX, _I]),

@@ -191,7 +191,7 @@ bool kernel_events(const Ctx &base, const void *fn, hipEvent_t *start, hipEvent_
 
 namespace {
 
-constexpr int FLAG_ERR = 0, FLAG_AMB = 1, FLAG_UNIQ = 2, FLAG_NR = 3, FLAG_GUP = 4, FLAG_TREE = 5, FLAG_N = 8;
+constexpr int FLAG_ERR = 0, FLAG_AMB = 1, FLAG_UNIQ = 2, FLAG_NR = 3, FLAG_GUP = 4, FLAG_TREE = 5, FLAG_BATCH = 6, FLAG_N = 8;
 
 int fail(rbt_ctx *c, int code, const char *fmt, ...) __attribute__((format(printf, 3, 4)));
 int fail(rbt_ctx *c, int code, const char *fmt, ...) {
@@ -394,6 +394,10 @@ int sync_and_check(rbt_ctx *c) {
   if (c->h_flags[FLAG_TREE]) {
     HIP_OK(c, hipMemset(c->d_flags + FLAG_TREE, 0, sizeof(int)));
     return fail(c, RBT_E_INVALID, "drafted tokens: a length, node count, parent, token or path did not fit its range");
+  }
+  if (c->h_flags[FLAG_BATCH]) {
+    HIP_OK(c, hipMemset(c->d_flags + FLAG_BATCH, 0, sizeof(int)));
+    return fail(c, RBT_E_INVALID, "batch step: a length, count, parent, prefix or sampling setting did not fit its range");
   }
   return RBT_OK;
 }
@@ -2144,7 +2148,7 @@ static int refuse(rbt_ctx *c, int code, const char *fmt, ...) {
 }
 
 static bool bad_dtype(int32_t t) { return t != RBT_DT_F32 && t != RBT_DT_BF16; }
-static size_t dtype_size(int32_t t) { return t == RBT_DT_BF16 ? 2 : 4; }
+static size_t dtype_size(int32_t t) { return t == RBT_DT_I8 ? 1 : t == RBT_DT_BF16 ? 2 : 4; }
 static bool misaligned(const void *p, size_t n) { return (uintptr_t)p % n != 0; }
 static bool overlap(const void *a, size_t na, const void *b, size_t nb) {
   return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
@@ -2397,7 +2401,7 @@ int rbt_kv_commit_d(rbt_ctx *c, const rbt_kv_commit_desc *d, size_t n_seq, size_
                     const int32_t *path, const int32_t *n_path, const int32_t *len, int32_t *len_out) {
   if (!d) return refuse(c, RBT_E_INVALID, "null descriptor");
   RBT_TRY(tree_size(c, n_seq, max_nodes));
-  if (bad_dtype(d->kv_dtype)) return refuse(c, RBT_E_INVALID, "cache type %d", d->kv_dtype);
+  if (bad_dtype(d->kv_dtype) && d->kv_dtype != RBT_DT_I8) return refuse(c, RBT_E_INVALID, "cache type %d", d->kv_dtype);
   if (d->n_layers > 4096 || d->n_kv_heads == 0 || d->head_dim == 0 || d->n_kv_heads > 4096 || d->head_dim > 1024 ||
       d->cap == 0 || d->cap > (size_t)INT32_MAX)
     return refuse(c, RBT_E_INVALID, "bad caches (%zu layers, %zu kv heads of %zu, %zu rows)", d->n_layers, d->n_kv_heads,
@@ -2436,6 +2440,201 @@ int rbt_kv_commit_d(rbt_ctx *c, const rbt_kv_commit_desc *d, size_t n_seq, size_
     HIP_OK(c, rbt::launch_commit(*c, a, unit, path, n_path, len, (int)n_seq, (int)max_nodes, (int)d->cap,
                                  (int)(row / unit), len_out, c->d_flags + FLAG_TREE));
   } while (l < d->n_layers);
+  return RBT_OK;
+}
+
+// ---- a batch's decode step: 8-bit caches, shared prefixes, sampling -------------------------------
+static int kvq_call(rbt_ctx *c, const rbt_kv_quant_desc *d, size_t n_seq, size_t max_rows, const void *k, const void *v,
+                    const int32_t *len, const int32_t *n_rows, const rbt_kv_rows *cache, bool read) {
+  if (!d) return refuse(c, RBT_E_INVALID, "null descriptor");
+  if (n_seq > 65535) return refuse(c, RBT_E_INVALID, "%zu sequences (at most 65535)", n_seq);
+  if (bad_dtype(d->dtype)) return refuse(c, RBT_E_INVALID, "row type %d", d->dtype);
+  if (d->n_kv_heads == 0 || d->n_kv_heads > 4096) return refuse(c, RBT_E_INVALID, "%zu kv heads", d->n_kv_heads);
+  if (d->head_dim == 0 || d->head_dim > 1024) return refuse(c, RBT_E_UNSUPPORTED, "head_dim %zu (1..1024)", d->head_dim);
+  if (d->cap == 0 || d->cap > (size_t)INT32_MAX) return refuse(c, RBT_E_INVALID, "cache of %zu rows", d->cap);
+  if (max_rows > d->cap || max_rows * d->n_kv_heads > (size_t)INT32_MAX)
+    return refuse(c, RBT_E_INVALID, "%zu rows of %zu kv heads into a cache of %zu", max_rows, d->n_kv_heads, d->cap);
+  const size_t lim = (size_t)1 << 40, hs = d->head_stride, rs = d->row_stride, ss = d->seq_stride, hd = d->head_dim;
+  if (hs > lim || rs > lim || ss > lim) return refuse(c, RBT_E_INVALID, "a stride is past 2^40");
+  if (n_seq && max_rows) {
+    if (!k || !v || !cache || !cache->k || !cache->v || !cache->k_scale || !cache->v_scale)
+      return refuse(c, RBT_E_INVALID, "null rows, cache or scales");
+    if (misaligned(k, dtype_size(d->dtype)) || misaligned(v, dtype_size(d->dtype)) || misaligned(cache->k_scale, 4) ||
+        misaligned(cache->v_scale, 4) || misaligned(len, 4) || misaligned(n_rows, 4))
+      return refuse(c, RBT_E_INVALID, "a pointer is not aligned to its type");
+    if (read) {
+      // result rows lie apart: sorted by stride, each reaches past what the smaller ones span
+      size_t n[3] = {d->n_kv_heads, max_rows, n_seq}, st[3] = {hs, rs, ss}, span = hd;
+      int o[3] = {0, 1, 2};
+      std::sort(o, o + 3, [&](int x, int y) { return st[x] < st[y]; });
+      for (int i : o) {
+        if (n[i] <= 1) continue;
+        if (st[i] < span) return refuse(c, RBT_E_INVALID, "result rows overlap");
+        span += (n[i] - 1) * st[i];
+      }
+    }
+  }
+  if (!c) return refuse(c, RBT_E_INVALID, "null context");
+  if (n_seq == 0 || max_rows == 0) return RBT_OK;
+  DeviceScope dev(c->device);
+  rbt::KvqArgs a{};
+  a.k = k;
+  a.v = v;
+  a.ko = const_cast<void *>(k);
+  a.vo = const_cast<void *>(v);
+  a.x16 = d->dtype == RBT_DT_BF16;
+  a.seq = (long)ss;
+  a.row = (long)rs;
+  a.head = (long)hs;
+  a.kc = (int8_t *)const_cast<void *>(cache->k);
+  a.vc = (int8_t *)const_cast<void *>(cache->v);
+  a.ks = const_cast<float *>(cache->k_scale);
+  a.vs = const_cast<float *>(cache->v_scale);
+  a.len = len;
+  a.n_rows = n_rows;
+  a.T = (int)max_rows;
+  a.K = (int)d->n_kv_heads;
+  a.hd = (int)hd;
+  a.cap = (long)d->cap;
+  a.bad = c->d_flags + FLAG_BATCH;
+  HIP_OK(c, rbt::launch_kvq(*c, a, (int)n_seq, read));
+  return RBT_OK;
+}
+
+int rbt_kv_quant_d(rbt_ctx *c, const rbt_kv_quant_desc *d, size_t n_seq, size_t max_rows, const void *k, const void *v,
+                   const int32_t *len, const int32_t *n_rows, const rbt_kv_rows *cache) {
+  return kvq_call(c, d, n_seq, max_rows, k, v, len, n_rows, cache, false);
+}
+
+int rbt_kv_dequant_d(rbt_ctx *c, const rbt_kv_quant_desc *d, size_t n_seq, size_t max_rows, const rbt_kv_rows *cache,
+                     const int32_t *len, const int32_t *n_rows, void *k, void *v) {
+  return kvq_call(c, d, n_seq, max_rows, k, v, len, n_rows, cache, true);
+}
+
+// Rows of a cache: both sides, aligned, with scales where they are 8-bit.
+static int kv_rows_ok(rbt_ctx *c, const char *what, const rbt_kv_rows *r, int32_t dtype) {
+  if (!r || !r->k || !r->v || (dtype == RBT_DT_I8 && (!r->k_scale || !r->v_scale)))
+    return refuse(c, RBT_E_INVALID, "null %s rows or scales", what);
+  if (misaligned(r->k, 16) || misaligned(r->v, 16)) return refuse(c, RBT_E_INVALID, "%s rows must be 16-byte aligned", what);
+  if (dtype == RBT_DT_I8 && (misaligned(r->k_scale, 4) || misaligned(r->v_scale, 4)))
+    return refuse(c, RBT_E_INVALID, "%s scales must be aligned to their type", what);
+  return RBT_OK;
+}
+
+int rbt_gqa_prefix_d(rbt_ctx *c, const rbt_gqa_prefix_desc *d, size_t n_seq, size_t max_nodes, size_t n_prefix, const float *q,
+                     const rbt_kv_rows *prefix, const rbt_kv_rows *cache, const rbt_kv_rows *draft, const int32_t *prefix_len,
+                     const int32_t *prefix_first, const int32_t *len, const int32_t *n_nodes, const int32_t *parent,
+                     const float *gate, float *out) {
+  if (!d) return refuse(c, RBT_E_INVALID, "null descriptor");
+  RBT_TRY(tree_size(c, n_seq, max_nodes));
+  const size_t nh = d->n_heads, nkv = d->n_kv_heads, hd = d->head_dim;
+  if (nh == 0 || nkv == 0 || nh % nkv || nh > 4096)
+    return refuse(c, RBT_E_INVALID, "bad attention shape (heads %zu over %zu kv heads)", nh, nkv);
+  if (hd == 0 || hd > 1024) return refuse(c, RBT_E_UNSUPPORTED, "head_dim %zu (1..1024)", hd);
+  if (bad_dtype(d->kv_dtype) && d->kv_dtype != RBT_DT_I8) return refuse(c, RBT_E_INVALID, "cache type %d", d->kv_dtype);
+  if (!std::isfinite(1.5f * d->attn_scale)) return refuse(c, RBT_E_INVALID, "attn_scale %g", d->attn_scale);
+  if (d->cap == 0 || d->cap > (size_t)INT32_MAX || d->max_len > d->cap)
+    return refuse(c, RBT_E_INVALID, "cache of %zu rows, max_len %zu", d->cap, d->max_len);
+  if (n_prefix && (d->prefix_cap == 0 || d->prefix_cap > (size_t)INT32_MAX || d->max_prefix > d->prefix_cap))
+    return refuse(c, RBT_E_INVALID, "prefixes of %zu rows, max_prefix %zu", d->prefix_cap, d->max_prefix);
+  if (n_prefix > 1024) return refuse(c, RBT_E_UNSUPPORTED, "%zu prefixes (at most 1024)", n_prefix);
+  if (n_seq * max_nodes * (nh / nkv) > (size_t)1 << 20)
+    return refuse(c, RBT_E_UNSUPPORTED, "%zu sequences of %zu nodes are too many for one call", n_seq, max_nodes);
+  if (gate && (d->gate_token_stride > (size_t)1 << 40 || d->gate_head_stride > (size_t)1 << 40))
+    return refuse(c, RBT_E_INVALID, "a gate stride is past 2^40");
+  if (n_seq) {
+    if (!q || !len || !n_nodes || !out || (n_prefix && (!prefix_len || !prefix_first)))
+      return refuse(c, RBT_E_INVALID, "null attention buffer");
+    RBT_TRY(kv_rows_ok(c, "cache", cache, d->kv_dtype));
+    if (draft) RBT_TRY(kv_rows_ok(c, "draft", draft, d->kv_dtype));
+    if (n_prefix) RBT_TRY(kv_rows_ok(c, "prefix", prefix, d->kv_dtype));
+    if (misaligned(q, 16) || misaligned(out, 16) || misaligned(gate, 4))
+      return refuse(c, RBT_E_INVALID, "q and out must be 16-byte aligned");
+  }
+  if (!c) return refuse(c, RBT_E_INVALID, "null context");
+  if (n_seq == 0) return RBT_OK;
+  DeviceScope dev(c->device);
+  rbt::TreeArgs a{};
+  a.q = q;
+  a.kc = cache->k;
+  a.vc = cache->v;
+  a.kcs = cache->k_scale;
+  a.vcs = cache->v_scale;
+  a.in_cache = !draft;
+  if (draft) {
+    a.kd = draft->k;
+    a.vd = draft->v;
+    a.kds = draft->k_scale;
+    a.vds = draft->v_scale;
+  }
+  a.len = len;
+  a.n_nodes = n_nodes;
+  a.parent = parent;
+  a.gate = gate;
+  a.gts = (long)d->gate_token_stride;
+  a.ghs = (long)d->gate_head_stride;
+  a.out = out;
+  a.B = (int)n_seq;
+  a.T = (int)max_nodes;
+  a.H = (int)nh;
+  a.K = (int)nkv;
+  a.hd = (int)hd;
+  a.cap = (long)d->cap;
+  a.max_len = (long)(d->max_len ? d->max_len : d->cap);
+  a.scale = d->attn_scale;
+  a.kv16 = d->kv_dtype == RBT_DT_BF16;
+  a.kv8 = d->kv_dtype == RBT_DT_I8;
+  a.bad = c->d_flags + FLAG_BATCH;
+  if (n_prefix) {
+    a.G = (int)n_prefix;
+    a.kp = prefix->k;
+    a.vp = prefix->v;
+    a.kps = prefix->k_scale;
+    a.vps = prefix->v_scale;
+    a.prefix_len = prefix_len;
+    a.first = prefix_first;
+    a.pcap = (long)d->prefix_cap;
+    a.max_prefix = (long)(d->max_prefix ? d->max_prefix : d->prefix_cap);
+  }
+  a.tiled = 0;
+  HIP_OK(c, rbt::launch_tree(*c, a));
+  return RBT_OK;
+}
+
+int rbt_sample_d(rbt_ctx *c, const rbt_sample_desc *d, size_t n, const void *logits, const float *temperature,
+                 const int32_t *top_k, const float *top_p, const float *min_p, const float *u, int32_t *tokens, float *probs) {
+  if (!d) return refuse(c, RBT_E_INVALID, "null descriptor");
+  if (n > 65535) return refuse(c, RBT_E_INVALID, "%zu rows (at most 65535)", n);
+  if (bad_dtype(d->logits_dtype)) return refuse(c, RBT_E_INVALID, "logits type %d", d->logits_dtype);
+  if (d->vocab == 0) return refuse(c, RBT_E_INVALID, "vocabulary of %zu", d->vocab);
+  if (d->vocab > (size_t)1 << 24) return refuse(c, RBT_E_UNSUPPORTED, "vocabulary of %zu (at most 2^24)", d->vocab);
+  if (d->row_stride < d->vocab || d->row_stride > (size_t)1 << 40)
+    return refuse(c, RBT_E_INVALID, "rows of %zu entries %zu apart", d->vocab, d->row_stride);
+  if (n) {
+    if (!logits || !u || !tokens) return refuse(c, RBT_E_INVALID, "null logits, u or tokens");
+    if (misaligned(logits, dtype_size(d->logits_dtype)) || misaligned(probs, 4) || misaligned(tokens, 4) || misaligned(u, 4) ||
+        misaligned(temperature, 4) || misaligned(top_k, 4) || misaligned(top_p, 4) || misaligned(min_p, 4))
+      return refuse(c, RBT_E_INVALID, "a pointer is not aligned to its type");
+  }
+  if (!c) return refuse(c, RBT_E_INVALID, "null context");
+  if (n == 0) return RBT_OK;
+  DeviceScope dev(c->device);
+  rbt::SampleArgs a{};
+  a.x = logits;
+  a.x16 = d->logits_dtype == RBT_DT_BF16;
+  a.stride = (long)d->row_stride;
+  a.V = (int)d->vocab;
+  a.temp = temperature;
+  a.top_k = top_k;
+  a.top_p = top_p;
+  a.min_p = min_p;
+  a.u = u;
+  a.tokens = tokens;
+  a.probs = probs;
+  a.bad = c->d_flags + FLAG_BATCH;
+  void *work;
+  RBT_TRY(scratch(c, SC_MIXA, rbt::sample_scratch(*c, n, a.V), &work));
+  HIP_OK(c, rbt::launch_sample(*c, a, n, work));
   return RBT_OK;
 }
 

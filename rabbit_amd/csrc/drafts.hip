@@ -656,7 +656,7 @@ __global__ __launch_bounds__(256) void k_commit(CommitArgs a, const int *__restr
 hipError_t launch_commit(const Ctx &c, const CommitArgs &a, int unit, const int *path, const int *n_path, const int *len,
                          int B, int T, int cap, int row_units, int *len_out, int *bad) {
   const dim3 grid(B, std::max(1, a.sides));
-  auto k = unit == 16 ? k_commit<uint4> : unit == 4 ? k_commit<uint32_t> : k_commit<uint16_t>;
+  auto k = unit == 16 ? k_commit<uint4> : unit == 4 ? k_commit<uint32_t> : unit == 2 ? k_commit<uint16_t> : k_commit<uint8_t>;
   launch_k(c, k, grid, dim3(256), a, path, n_path, len, T, cap, row_units, len_out, bad);
   return hipGetLastError();
 }

@@ -464,7 +464,7 @@ struct CommitArgs {
   const void *src[COMMIT_SIDES];
   int sides;
 };
-// unit: bytes of one copy (16, 4 or 2), row_units of them per row.
+// unit: bytes of one copy (16, 4, 2 or 1), row_units of them per row.
 hipError_t launch_commit(const Ctx &c, const CommitArgs &a, int unit, const int *path, const int *n_path, const int *len,
                          int B, int T, int cap, int row_units, int *len_out, int *bad);
 
@@ -482,6 +482,14 @@ struct TreeArgs {
   float scale;
   int kv16;  // bf16 caches and draft rows
   int *bad;
+  // rbt_gqa_prefix_d: 8-bit rows' scales; nodes whose rows are in the cache; prefixes
+  int kv8, in_cache;
+  const float *kcs, *vcs, *kds, *vds;
+  int G;  // prefixes
+  const void *kp, *vp;
+  const float *kps, *vps;
+  const int *prefix_len, *first;
+  long pcap, max_prefix;
   // tree_plan: whether the matrix cores take it, row tiles, pieces of the cache (keys per piece), scratch
   int tiled, tiles, pieces;
   unsigned per, magic;
@@ -495,6 +503,36 @@ struct TreeArgs {
 bool tree_plan(const Ctx &c, TreeArgs &a);
 size_t tree_part_floats(const TreeArgs &a);
 hipError_t launch_tree(const Ctx &c, const TreeArgs &a);
+
+// kvquant.hip: rows to and from 8-bit caches.
+struct KvqArgs {
+  const void *k, *v;  // rows to write into the cache
+  void *ko, *vo;      // or to read out of it
+  int x16;            // bf16 rows
+  long seq, row, head;  // their strides in entries
+  int8_t *kc, *vc;
+  float *ks, *vs;
+  const int *len, *n_rows;
+  int T, K, hd;
+  long cap;
+  int *bad;
+};
+hipError_t launch_kvq(const Ctx &c, const KvqArgs &a, int B, bool read);
+
+// sample.hip: tokens and probabilities from logits.
+struct SampleArgs {
+  const void *x;
+  int x16;
+  long stride;
+  int V, S;  // entries; weights are summed in units of 2^-S
+  const float *temp, *top_p, *min_p, *u;
+  const int *top_k;
+  int *tokens;
+  float *probs;
+  int *bad;
+};
+size_t sample_scratch(const Ctx &c, size_t n, int V);
+hipError_t launch_sample(const Ctx &c, SampleArgs a, size_t n, void *scratch);
 
 // synth.hip
 hipError_t launch_synth_mxfp4(const Ctx &c, uint8_t *data, uint8_t *scale, size_t rows, size_t cols, uint64_t seed,

@@ -34,9 +34,34 @@ __device__ __forceinline__ float tree_ld(const void *p, long i, int b16) {
 __device__ __forceinline__ bool tree_fits(const TreeArgs &a, int b, int &n, int &L) {
   n = a.n_nodes[b];
   L = a.len[b];
-  if (n >= 0 && n <= a.T && L >= 0 && L <= a.cap) return true;
+  if (n >= 0 && n <= a.T && L >= 0 && L <= a.cap - (a.in_cache ? n : 0)) return true;
   if (threadIdx.x == 0) *a.bad = 1;
   return false;
+}
+
+// The prefix of sequence b, in every thread of the workgroup: its number (-1: none) and its rows. False where the
+// prefixes' first sequences do not follow each other within the batch, or the prefix is longer than its cache.
+__device__ bool tree_prefix(const TreeArgs &a, int b, int &g, int &P) {
+  __shared__ int found;
+  g = -1;
+  P = 0;
+  if (a.G == 0) return true;
+  if (threadIdx.x == 0) found = -1;
+  __syncthreads();
+  bool ok = true;
+  for (int i = threadIdx.x; i < a.G; i += blockDim.x) {
+    const int f0 = a.first[i], f1 = a.first[i + 1];
+    ok = ok && f0 >= 0 && f0 <= f1 && f1 <= a.B;
+    if (f0 <= b && b < f1) found = i;
+  }
+  ok = !__syncthreads_or(!ok);
+  if (ok && found >= 0) {
+    g = found;
+    P = a.prefix_len[g];
+    ok = P >= 0 && P <= a.pcap;
+  }
+  if (!ok && threadIdx.x == 0) *a.bad = 1;
+  return ok;
 }
 
 // Entries e .. e + 3 of a row: v / l, times sigmoid of the gate.
@@ -51,20 +76,53 @@ __device__ __forceinline__ void tree_store(const TreeArgs &a, int b, int i, int 
 }
 
 // Any shape: one workgroup per (query head, node, sequence), 256 keys at a time with the running maximum and
-// sum. Thread t takes key t's score, then entries t, t + 256, ... of the output; rows that the node does not
-// see are passed over.
+// sum, the prefix's first. Thread t takes key t's score, then entries t, t + 256, ... of the output; rows that the
+// node does not see are passed over.
+struct TreeRow {
+  const void *p;       // the row's first entry
+  const float *scale;  // of 8-bit rows
+};
+template <bool NEW>
+__device__ __forceinline__ TreeRow tree_row(const TreeArgs &a, bool v, int b, int g, int P, int L, int kv, long j) {
+  const void *base;
+  const float *sc;
+  long at;
+  if (NEW && j < P) {
+    base = v ? a.vp : a.kp;
+    sc = v ? a.vps : a.kps;
+    at = (long)g * a.pcap + j;
+  } else if (j < (long)P + L || (NEW && a.in_cache)) {
+    base = v ? a.vc : a.kc;
+    sc = v ? a.vcs : a.kcs;
+    at = (long)b * a.cap + (j - P);
+  } else {
+    base = v ? a.vd : a.kd;
+    sc = v ? a.vds : a.kds;
+    at = (long)b * a.T + (j - P - L);
+  }
+  at = at * a.K + kv;
+  return {(const char *)base + at * a.hd * (NEW && a.kv8 ? 1 : a.kv16 ? 2 : 4), NEW && a.kv8 ? sc + at : nullptr};
+}
+template <bool NEW>
+__device__ __forceinline__ float tree_at(const TreeArgs &a, const TreeRow &r, int e) {
+  return NEW && a.kv8 ? (float)((const int8_t *)r.p)[e] * *r.scale : tree_ld(r.p, e, a.kv16);
+}
+
+// NEW: with prefixes, 8-bit rows or nodes in the cache.
+template <bool NEW>
 __global__ __launch_bounds__(256) void k_tree_any(TreeArgs a) {
   __shared__ float q[1024], pr[256], red[4];
   __shared__ int par[TREE_MAX];
   __shared__ uint8_t sees[TREE_MAX];
   const int h = blockIdx.x, i = blockIdx.y, b = blockIdx.z, t = threadIdx.x;
-  int n, L;
+  int n, L, g = -1, P = 0;
   if (!tree_fits(a, b, n, L) || i >= n) return;
+  if (NEW && !tree_prefix(a, b, g, P)) return;
   const int kv = h / (a.H / a.K), hd = a.hd;
-  const long row = (long)a.K * hd, qi = (((long)b * a.T + i) * a.H + h) * hd;
+  const long qi = (((long)b * a.T + i) * a.H + h) * hd;
   for (int e = t; e < hd; e += 256) q[e] = a.q[qi + e];
   if (t < n) {
-    int p = a.parent[(long)b * a.T + t];
+    int p = a.parent ? a.parent[(long)b * a.T + t] : t - 1;
     if (p < -1 || p >= t) {
       *a.bad = 1;
       p = -1;
@@ -77,15 +135,14 @@ __global__ __launch_bounds__(256) void k_tree_any(TreeArgs a) {
     for (int j = i; j >= 0; j = par[j]) sees[j] = 1;
   __syncthreads();
   float m = -INFINITY, l = 0.0f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-  const int total = L + i + 1;  // no later node is an ancestor
-  for (int k0 = 0; k0 < total; k0 += 256) {
-    const int j = k0 + t;
+  const long old = (long)P + L, total = old + i + 1;  // no later node is an ancestor
+  for (long k0 = 0; k0 < total; k0 += 256) {
+    const long j = k0 + t;
     float s = -INFINITY;
-    if (j < total && (j < L || sees[j - L])) {
-      const void *src = j < L ? a.kc : a.kd;
-      const long at = (j < L ? (long)b * a.cap + j : (long)b * a.T + (j - L)) * row + (long)kv * hd;
+    if (j < total && (j < old || sees[j - old])) {
+      const TreeRow r = tree_row<NEW>(a, false, b, g, P, L, kv, j);
       float d = 0.0f;
-      for (int e = 0; e < hd; e++) d = fmaf(q[e], tree_ld(src, at + e, a.kv16), d);
+      for (int e = 0; e < hd; e++) d = fmaf(q[e], tree_at<NEW>(a, r, e), d);
       s = d * a.scale;
     }
     const float wm = rbt_wave_max_f(s);
@@ -101,18 +158,16 @@ __global__ __launch_bounds__(256) void k_tree_any(TreeArgs a) {
     __syncthreads();
     l = l * f + ((red[0] + red[1]) + (red[2] + red[3]));
     m = mn;
-    const int nk = min(256, total - k0);
+    const int nk = (int)min(256L, total - k0);
 #pragma unroll
     for (int c = 0; c < 4; c++) {
       const int e = t + 256 * c;
       if (e >= hd) break;
       float o = acc[c] * f;
       for (int jj = 0; jj < nk; jj++) {
-        const int j2 = k0 + jj;
-        if (j2 >= L && !sees[j2 - L]) continue;
-        const void *src = j2 < L ? a.vc : a.vd;
-        const long at = (j2 < L ? (long)b * a.cap + j2 : (long)b * a.T + (j2 - L)) * row + (long)kv * hd;
-        o = fmaf(pr[jj], tree_ld(src, at + e, a.kv16), o);
+        const long j2 = k0 + jj;
+        if (j2 >= old && !sees[j2 - old]) continue;
+        o = fmaf(pr[jj], tree_at<NEW>(a, tree_row<NEW>(a, true, b, g, P, L, kv, j2), e), o);
       }
       acc[c] = o;
     }
@@ -840,7 +895,7 @@ bool tree_plan(const Ctx &c, TreeArgs &a) {
   a.rw = a.kw = a.tiles = a.pieces = 1;
   a.four = 0;
   int rw = 1, kw = 1;
-  a.tiled = a.hd == 64 || a.hd == 128 || a.hd == 192 || a.hd == 256;
+  a.tiled = (a.hd == 64 || a.hd == 128 || a.hd == 192 || a.hd == 256) && !a.kv8 && a.G == 0 && !a.in_cache && a.parent;
   if (!a.tiled) return true;
   const int R = a.H / a.K, t16 = (a.T * R + 15) / 16;
   const int TK = a.kv16 ? 64 : 32;
@@ -950,7 +1005,8 @@ static hipError_t run_tree_hd(const Ctx &c, const TreeArgs &a) {
 
 hipError_t launch_tree(const Ctx &c, const TreeArgs &a) {
   if (!a.tiled) {
-    launch_k(c, k_tree_any, dim3(a.H, a.T, a.B), dim3(256), a);
+    const bool plain = a.parent && !a.kv8 && !a.in_cache && a.G == 0;
+    launch_k(c, plain ? k_tree_any<false> : k_tree_any<true>, dim3(a.H, a.T, a.B), dim3(256), a);
     return hipGetLastError();
   }
   hipError_t e = a.hd == 64 ? run_tree_hd<64>(c, a) : a.hd == 128 ? run_tree_hd<128>(c, a)
