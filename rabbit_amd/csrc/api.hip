@@ -2561,12 +2561,11 @@ int rbt_gqa_prefix_d(rbt_ctx *c, const rbt_gqa_prefix_desc *d, size_t n_seq, siz
   a.kcs = cache->k_scale;
   a.vcs = cache->v_scale;
   a.in_cache = !draft;
-  if (draft) {
-    a.kd = draft->k;
-    a.vd = draft->v;
-    a.kds = draft->k_scale;
-    a.vds = draft->v_scale;
-  }
+  const rbt_kv_rows *own = draft ? draft : cache;
+  a.kd = own->k;
+  a.vd = own->v;
+  a.kds = own->k_scale;
+  a.vds = own->v_scale;
   a.len = len;
   a.n_nodes = n_nodes;
   a.parent = parent;
@@ -2596,8 +2595,26 @@ int rbt_gqa_prefix_d(rbt_ctx *c, const rbt_gqa_prefix_desc *d, size_t n_seq, siz
     a.pcap = (long)d->prefix_cap;
     a.max_prefix = (long)(d->max_prefix ? d->max_prefix : d->prefix_cap);
   }
-  a.tiled = 0;
-  HIP_OK(c, rbt::launch_tree(*c, a));
+  rbt::TreeArgs p{};
+  a.joined = a.G > 0;
+  bool fits = rbt::tree_plan(*c, a);
+  if (a.joined && a.tiled) {
+    rbt::tree_prefix_args(a, p);
+    fits = rbt::tree_plan(*c, p) && fits;
+  }
+  if (!fits)
+    return refuse(c, RBT_E_UNSUPPORTED, "%zu sequences of %zu nodes are too many for one call", n_seq, max_nodes);
+  const size_t na = a.tiled ? rbt::tree_part_floats(a) : 0, np = p.tiled ? rbt::tree_part_floats(p) : 0;
+  if (na + np) {
+    RBT_TRY(scratch_t(c, SC_MIXB, na + np, &a.part));
+    p.part = a.part + na / (hd + 2) * hd;
+    a.part_ml = (float2 *)(p.part + np / (hd + 2) * hd);
+    p.part_ml = a.part_ml + na / (hd + 2);
+  }
+  if (p.tiled)
+    HIP_OK(c, rbt::launch_prefix(*c, a, p));
+  else
+    HIP_OK(c, rbt::launch_tree(*c, a));
   return RBT_OK;
 }
 

@@ -490,6 +490,8 @@ struct TreeArgs {
   const float *kps, *vps;
   const int *prefix_len, *first;
   long pcap, max_prefix;
+  int pre, joined;  // the pass over the prefixes (len and the caches are theirs); partial sums whatever the pieces
+  int seqs, tk;     // tree_plan: sequences of the grid, keys per stage
   // tree_plan: whether the matrix cores take it, row tiles, pieces of the cache (keys per piece), scratch
   int tiled, tiles, pieces;
   unsigned per, magic;
@@ -503,6 +505,10 @@ struct TreeArgs {
 bool tree_plan(const Ctx &c, TreeArgs &a);
 size_t tree_part_floats(const TreeArgs &a);
 hipError_t launch_tree(const Ctx &c, const TreeArgs &a);
+// Attention with prefixes on the matrix cores: a's pass over the prefixes as a call of its own (planned by tree_plan
+// too), and both, a with joined = 1.
+void tree_prefix_args(const TreeArgs &a, TreeArgs &p);
+hipError_t launch_prefix(const Ctx &c, const TreeArgs &a, const TreeArgs &p);
 
 // kvquant.hip: rows to and from 8-bit caches.
 struct KvqArgs {

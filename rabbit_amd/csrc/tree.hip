@@ -213,6 +213,10 @@ typedef __attribute__((address_space(3))) ts4 tree_lds_s4;
 __device__ __forceinline__ void tree_dma(const void *p, uint32_t base) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(base), "v"(p) : "memory");
 }
+// 64 lanes' 4 bytes, to `base` + 4 lane.
+__device__ __forceinline__ void tree_dma4(const void *p, uint32_t base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(base), "v"(p) : "memory");
+}
 
 // x = hi + mid + lo, each with its low 16 bits zero (fp32 has 24 significant bits, each part 8): for products with bf16
 // rows, of which all three are kept.
@@ -261,25 +265,35 @@ __device__ __forceinline__ float tree_xor_sum(float v) {
 // KV_PARTS4: by workgroups of four waves, several of them on a CU, for batches of up to four row tiles at head dims 64
 // and 128. 12 nodes of 32 query heads over 8 KV heads of 128: 32 sequences of up to 4096 rows 246 us with eight waves,
 // 207 with four, but one of 8192 rows (16 nodes) 27.6 and 30.9, where loading a stage is what it waits for.
-enum { KV_BF16 = 0, KV_F32 = 1, KV_PARTS = 2, KV_PARTS4 = 3 };
-constexpr bool tree_parts(int kv) { return kv >= KV_PARTS; }
+// KV_I8: 8-bit rows with a scale each, see tree_digits below.
+enum { KV_BF16 = 0, KV_F32 = 1, KV_PARTS = 2, KV_PARTS4 = 3, KV_I8 = 4 };
+constexpr bool tree_parts(int kv) { return kv == KV_PARTS || kv == KV_PARTS4; }
 
-template <int HD, int KV>
+// Keys per stage.
+constexpr int tree_tk(int kv, int kw) { return kv == KV_BF16 || (kv == KV_I8 && kw == 1) ? 64 : kv == KV_I8 ? 128 : 32; }
+
+template <int HD, int KV, int KW = 1>
 struct TreeTile {
-  static constexpr int ROWB = HD * (KV == KV_F32 ? 4 : 2), CH = ROWB / 16;  // bytes and chunks of a row in LDS
-  static constexpr int GROW = HD * (KV == KV_BF16 ? 2 : 4);                 // bytes of a row of the cache
-  static constexpr int TK = KV == KV_BF16 ? 64 : 32;                        // keys per stage
-  static constexpr int PART = TK * ROWB, SIDE = PART * (tree_parts(KV) ? 3 : 1), STAGE = 2 * SIDE;  // K, then V
+  static constexpr int ROWB = HD * (KV == KV_F32 ? 4 : KV == KV_I8 ? 1 : 2), CH = ROWB / 16;  // bytes and chunks of a row in LDS
+  static constexpr int GROW = HD * (KV == KV_BF16 ? 2 : KV == KV_I8 ? 1 : 4);  // bytes of a row of the cache
+  static constexpr int TK = tree_tk(KV, KW);
+  static constexpr int PART = TK * ROWB, SIDE = PART * (tree_parts(KV) ? 3 : 1);
+  static constexpr int STAGE = 2 * SIDE + (KV == KV_I8 ? 8 * TK : 0);       // K, then V, then 8-bit rows' scales of K and V
   static constexpr int LDS = tree_parts(KV) ? STAGE : 2 * STAGE;
   static constexpr int INSTR = TK * CH / 64;                                // 1 KB loads per side
-  static_assert(TK * CH % 64 == 0 && CH % 8 == 0, "whole loads");
+  static_assert(TK * CH % 64 == 0 && CH % (KV == KV_I8 ? 4 : 8) == 0, "whole loads");
   // Where chunk c of row r lies in its row: c ^ k_turn(r), c ^ v_turn(r). The LDS serves 256 bytes a cycle from 64
   // banks, to lanes 0-3, 12-15, 20-23 and 24-27 of a 16-byte read (four such sets) or to half a wave of an 8-byte
   // one; the turns spread the rows of each set over all banks. (Turns within 128 bytes made every read take
   // two cycles: half of the LDS's cycles at 64 nodes over 32749 rows.)
   static constexpr bool WIDE = CH % 16 == 0;  // rows of whole 256 bytes; others begin half a cycle apart
-  static __device__ __forceinline__ int k_turn(int r) { return WIDE ? r & 15 : r & 7; }
+  static __device__ __forceinline__ int k_turn(int r) {
+    return WIDE ? r & 15 : CH % 8 == 0 ? r & 7 : -(r >> 2) & 3;  // (rows of 64 and 192 bytes: four, or a multiple, to a cycle)
+  }
   static __device__ __forceinline__ int v_turn(int r) {
+    // (a 16-lane read of 8-bit values takes rows 0-3 and 16-19 of its column's four)
+    if constexpr (KV == KV_I8)
+      return WIDE ? (r & 7) | (r >> 4 & 1) << 3 : CH % 8 == 0 ? (r >> 1 & 3) | (r >> 4 & 1) << 2 : (r >> 2 & 1) | (r >> 4 & 1) << 1;
     return KV == KV_F32 ? 0 : WIDE ? (r & 7) << 1 : (r >> 1 & 3) << 1;
   }
 };
@@ -303,12 +317,61 @@ __device__ __forceinline__ void tree_pieces(const TreeArgs &a, int L, int TK, un
   }
 }
 
+// 8-bit rows. Their entries go to the matrix cores as they are (v_mfma_i32_16x16x64_i8, at twice the rate of bf16), and
+// so do three digits of each query and probability: a number x is taken as the whole number X nearest to x f, where f
+// brings the row's largest |x| to just below 2^23, and X = 65536 d2 + 256 d1 + d0 with digits in -128..127. A digit's
+// products and sums are exact in 32 bits (256 * 128 * 127 and 64 * 128 * 127 at most), and two digits' sums
+// fit 32 bits together. So a score is exact up to the query's rounding (half of 2^-22 of its largest entry), and the sum over a
+// stage's values up to the probabilities' (half of 2^-22 of the stage's largest probability times scale); f32 sums
+// over stages. A key's scale multiplies its score, a value's its probability. Three products at twice the
+// rate are half of what bf16 rows take.
+constexpr float TREE_TOP = 8355711.0f;           // 127 * 65536 + 127 * 256 + 127
+constexpr float TREE_BIAS = 8421504.0f;          // 128 in every digit: those of X + TREE_BIAS are not negative
+constexpr float TREE_FIT = TREE_TOP / 0x1p23f;   // [2^22, 2^23) times this is at most TREE_TOP
+
+// Byte k of four words as digit words; the words hold X + TREE_BIAS in [2^23, 2^24) as floats (X not negative), so
+// that bits 0-22 are that less 2^23: byte 2 is the digit itself, bytes 1 and 0 are 128 more than theirs.
+__device__ __forceinline__ void tree_digits(const uint32_t (&w)[4], uint32_t &d2, uint32_t &d1, uint32_t &d0) {
+  const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), b = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
+  const uint32_t c = __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0602u), d = __builtin_amdgcn_perm(w[3], w[2], 0x0c0c0602u);
+  d0 = __builtin_amdgcn_perm(b, a, 0x05040100u) ^ 0x80808080u;
+  d1 = __builtin_amdgcn_perm(b, a, 0x07060302u) ^ 0x80808080u;
+  d2 = __builtin_amdgcn_perm(d, c, 0x05040100u);
+}
+typedef int ti4 __attribute__((ext_vector_type(4)));
+typedef int ti2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) ti2 tree_lds_i2;
+
+// The prefix and its tile of 16 rw rows that flat tile `rt` of a pass over the prefixes is. A prefix's tiles begin at
+// (f TR + g (U - 1)) / U, with f its first sequence and U = 16 rw: at least its own number from the one before.
+__device__ __forceinline__ int tree_tile0(const TreeArgs &a, int f, int g, int U) {
+  return (f * a.T * a.R + g * (U - 1)) / U;
+}
+__device__ __forceinline__ bool tree_group(const TreeArgs &a, int rt, int &g, int &f0, int &f1) {
+  const int lane = threadIdx.x & 63, U = 16 * a.rw;
+  for (int i0 = 0; i0 < a.G; i0 += 64) {
+    const int i = min(i0 + lane, a.G - 1), x0 = a.first[i], x1 = a.first[i + 1];
+    const bool in = x0 >= 0 && x0 < x1 && x1 <= a.B && tree_tile0(a, x0, i, U) <= rt && rt < tree_tile0(a, x1, i + 1, U);
+    const unsigned long long m = __ballot(in);
+    if (m) {
+      const int l = __ffsll((long long)m) - 1;
+      g = __builtin_amdgcn_readlane(i, l);
+      f0 = __builtin_amdgcn_readlane(x0, l);
+      f1 = __builtin_amdgcn_readlane(x1, l);
+      return true;
+    }
+  }
+  return false;
+}
+
 template <int HD, int KV, int KW>
 __global__ __launch_bounds__(KW == 1 && KV != KV_PARTS4 ? 512 : 256, KW == 1 && KV != KV_PARTS4 ? 1 : 2)
 void k_tree(TreeArgs a) {
-  using TT = TreeTile<HD, KV>;
-  constexpr bool B16 = KV != KV_F32, PARTS = tree_parts(KV);  // bf16 products; of split rows
+  using TT = TreeTile<HD, KV, KW>;
+  constexpr bool I8 = KV == KV_I8;
+  constexpr bool B16 = KV != KV_F32, PARTS = tree_parts(KV);  // values' tiles of 16 entries; split rows
   constexpr int ROWB = TT::ROWB, CH = TT::CH, TK = TT::TK, SK = TK / KW, NT = SK / 16;
+  static_assert(!I8 || SK == 64 || SK == 32, "whole products");
   static_assert(!PARTS || KW == 1, "one group of waves");
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   __shared__ int par[TREE_MAX];
@@ -320,7 +383,7 @@ void k_tree(TreeArgs a) {
   // consecutive ones of an XCD (id % 8)
   int piece = blockIdx.x, rt = 0, kv = blockIdx.y, b = blockIdx.z;
   if (a.tiles > 1) {
-    const unsigned id = blockIdx.x, g = id / 8 / a.tiles * 8 + id % 8, KB = a.K * a.B;
+    const unsigned id = blockIdx.x, g = id / 8 / a.tiles * 8 + id % 8, KB = a.K * a.seqs;
     if (g >= a.pieces * KB) return;
     rt = id / 8 % a.tiles;
     piece = g / KB;
@@ -328,10 +391,23 @@ void k_tree(TreeArgs a) {
     b = r / a.K;
     kv = r - b * a.K;
   }
-  int n, L;
-  if (!tree_fits(a, b, n, L)) return;
-  const int R = a.R, rows = n * R;
-  const int NW = blockDim.x >> 6, RW = a.rw;
+  int n, L, node0 = b * a.T;  // nodes, rows of the cache, first node's place among all
+  const int R = a.R, RW = a.rw;
+  long unit = (((long)piece * a.seqs + b) * a.K + kv) * a.t16;  // of the partial sums' 16-row tiles
+  if (a.pre) {  // the cache is a prefix, the nodes are those of all its sequences
+    int f0, f1;
+    if (!tree_group(a, rt, b, f0, f1)) return;
+    L = a.len[b];
+    if (L <= 0 || L > a.cap) return;  // (reported where the parts are joined)
+    rt -= tree_tile0(a, f0, b, 16 * RW);
+    unit += tree_tile0(a, f0, b, 16);
+    node0 = f0 * a.T;
+    n = (f1 - f0) * a.T;
+  } else if (!tree_fits(a, b, n, L)) {
+    return;
+  }
+  const int rows = n * R;
+  const int NW = blockDim.x >> 6;
   const int row0 = rt * RW * 16;
   if (row0 >= rows) return;
   unsigned per, np;
@@ -341,11 +417,12 @@ void k_tree(TreeArgs a) {
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int rg = KW == 1 ? w : w % RW, kgp = KW == 1 ? 0 : w / RW, col = lane & 15, kg = lane >> 4;
   const int node_lo = tree_div(row0, a), node_hi = tree_div(min(rows, row0 + RW * 16) - 1, a);
-  const int nd = piece == (int)np - 1 ? node_hi + 1 : 0;  // drafted rows: those up to the last node of the tile
+  const int nd = !a.pre && piece == (int)np - 1 ? node_hi + 1 : 0;  // drafted rows: those up to the tile's last node
   const int keys = nc + nd, st_n = (keys + TK - 1) / TK;
 
   const long seq_row = (long)a.K * TT::GROW;  // bytes from a row to the next
-  const long off_c = (((long)b * a.cap + k0) * a.K + kv) * TT::GROW, off_d = ((long)b * a.T * a.K + kv) * TT::GROW;
+  const long at_c = ((long)b * a.cap + k0) * a.K + kv, at_d = (a.in_cache ? (long)b * a.cap + L : (long)b * a.T) * a.K + kv;
+  const long off_c = at_c * TT::GROW, off_d = at_d * TT::GROW;
   const char *kc = (const char *)a.kc + off_c, *vc = (const char *)a.vc + off_c;
   const char *kd = (const char *)a.kd + off_d, *vd = (const char *)a.vd + off_d;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)smem;
@@ -369,6 +446,14 @@ void k_tree(TreeArgs a) {
         tree_dma((j < nc ? vc : vd) + at + (c ^ TT::v_turn(r)) * 16, to + TT::SIDE + i * 1024);
       }
     }
+    if constexpr (I8)
+      for (int i = w; i < 2 * TK / 64; i += NW) {
+        constexpr int per = TK / 64;
+        const bool v = i >= per;
+        const int j = min(base + (v ? i - per : i) * 64 + lane, keys - 1);
+        const float *from = j < nc ? (v ? a.vcs : a.kcs) + at_c : (v ? a.vds : a.kds) + at_d;
+        tree_dma4(from + (long)(j < nc ? j : j - nc) * a.K, to + 2 * TT::SIDE + i * 256);
+      }
   };
   // key i of the piece holds a non-finite value (one past the last repeats it)
   auto mark = [&](int i) { atomicOr(&dirty[(min(i, keys - 1) - nc) >> 5], 1u << ((min(i, keys - 1) - nc) & 31)); };
@@ -442,11 +527,47 @@ void k_tree(TreeArgs a) {
   const bool active = rg < RW && kgp < KW && row0 + rg * 16 < rows;  // a wave without rows or keys only loads
   const int row = row0 + rg * 16 + col, rc = min(row, rows - 1);
   const int node = tree_div(rc, a), head = kv * R + (rc - node * R);
-  const long qrow = ((long)b * a.T + node) * a.H + head;
+  const long qrow = (long)(node0 + node) * a.H + head;
   const float *qp = a.q + qrow * HD;
-  tb8 qb[B16 ? HD / 32 : 1][3];
+  tb8 qb[B16 && !I8 ? HD / 32 : 1][3];
   float4 qf[B16 ? 1 : HD / 16];
-  if constexpr (B16) {
+  ti4 qd[I8 ? HD / 64 : 1][3];
+  float qs = 1.0f;  // what a score's whole number stands for, in powers of two
+  if constexpr (I8) {
+    float4 x[HD / 64][4];
+    uint32_t top = 0;
+#pragma unroll
+    for (int s = 0; s < HD / 64; s++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        x[s][i] = *(const float4 *)(qp + 64 * s + 16 * kg + 4 * i);
+        const float4 v = x[s][i];
+        top = max(max(max(top, __float_as_uint(v.x) & 0x7fffffffu), __float_as_uint(v.y) & 0x7fffffffu),
+                  max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu));
+      }
+    top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+    const float most = __uint_as_float(top);
+    int e = __builtin_amdgcn_frexp_expf(most);  // most in [2^(e - 1), 2^e)
+    if (__builtin_amdgcn_ldexpf(most, 23 - e) > TREE_TOP) e++;
+    e = max(e, -100);
+    const bool whole = top < 0x7f800000u;
+    qs = whole ? a.scale * 1.44269504088896341f * __builtin_amdgcn_ldexpf(1.0f, e - 23) : __uint_as_float(0x7fc00000u);
+#pragma unroll
+    for (int s = 0; s < HD / 64; s++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float v[4] = {x[s][i].x, x[s][i].y, x[s][i].z, x[s][i].w};
+        uint32_t u[4], d2, d1, d0;
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+          u[k] = whole ? (uint32_t)((int)rintf(__builtin_amdgcn_ldexpf(v[k], 23 - e)) + (int)TREE_BIAS) : (uint32_t)TREE_BIAS;
+        tree_digits(u, d2, d1, d0);
+        qd[s][0][i] = (int)d0;
+        qd[s][1][i] = (int)d1;
+        qd[s][2][i] = (int)(d2 ^ 0x80808080u);
+      }
+  } else if constexpr (B16) {
 #pragma unroll
     for (int s = 0; s < HD / 32; s++) {
       const float4 x = *(const float4 *)(qp + 32 * s + 8 * kg), y = *(const float4 *)(qp + 32 * s + 8 * kg + 4);
@@ -474,7 +595,7 @@ void k_tree(TreeArgs a) {
   if (nd > 0) {
     if (t < TREE_MAX / 32) dirty[t] = 0;
     for (int j = t; j < n; j += blockDim.x) {
-      int p = a.parent[(long)b * a.T + j];
+      int p = a.parent ? a.parent[(long)b * a.T + j] : j - 1;
       if (p < -1 || p >= j) {
         *a.bad = 1;
         p = -1;
@@ -491,6 +612,7 @@ void k_tree(TreeArgs a) {
 
   const float c1 = a.scale * 1.44269504088896341f;  // scores in powers of two
   float m = -INFINITY, l = 0.0f;
+  float gone = 0.0f;  // NaN where a value's scale was not finite
   tf4 o[HD / 16];
 #pragma unroll
   for (int x = 0; x < HD / 16; x++) o[x] = tf4{0.f, 0.f, 0.f, 0.f};
@@ -508,7 +630,7 @@ void k_tree(TreeArgs a) {
       lds_barrier();  // the stage has landed, and the other buffer's readers are done
       if (s + 1 < st_n) issue(s + 1);
     }
-    if (!PARTS && nd > 1 && base + TK > nc) {
+    if (!PARTS && !I8 && nd > 1 && base + TK > nc) {
       // a value that some rows do not see must not meet their zero probabilities: non-finite ones are taken
       // out of the tile (its repeated last row too) and make NaNs at the end of the rows that do see them
       for (int u = t + max(nc - base, 0) * CH; u < TK * CH; u += blockDim.x) {
@@ -539,10 +661,33 @@ void k_tree(TreeArgs a) {
     for (int x = 0; x < NT; x++) sc[x] = tf4{0.f, 0.f, 0.f, 0.f};
     const char *kb = kt + (kgp * SK + col) * ROWB;
     // byte of chunk 4 st + kg in the lane's rows (rows 16 apart turn alike): a few offsets per lane and a constant
-    constexpr int KP = TT::WIDE ? 4 : 2;
+    constexpr int KP = TT::WIDE ? 4 : CH % 8 == 0 ? 2 : 1;
     auto kc_at = [&](int st) { return ((4 * (st % KP) + kg) ^ TT::k_turn(col)) * 16 + st / KP * KP * 64; };
     constexpr int NP = PARTS ? 3 : 1;  // parts of a key or value
-    if constexpr (B16) {
+    const float *ks = (const float *)(kt + 2 * TT::SIDE) + kgp * SK + 4 * kg, *vs = ks + TK;  // 8-bit rows' scales
+    if constexpr (I8) {
+      ti4 d[NT][3];
+#pragma unroll
+      for (int x = 0; x < NT; x++)
+#pragma unroll
+        for (int p = 0; p < 3; p++) d[x][p] = ti4{0, 0, 0, 0};
+#pragma unroll
+      for (int st = 0; st < HD / 64; st++)
+#pragma unroll
+        for (int x = 0; x < NT; x++) {
+          const ti4 kf = *(const ti4 *)(kb + x * 16 * ROWB + kc_at(st));
+#pragma unroll
+          for (int p = 2; p >= 0; p--) d[x][p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf, qd[st][p], d[x][p], 0, 0, 0);
+        }
+#pragma unroll
+      for (int x = 0; x < NT; x++) {
+        const float4 k4 = *(const float4 *)(ks + 16 * x);
+        const float kk[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          sc[x][i] = fmaf((float)(d[x][2][i] * 256 + d[x][1][i]), 256.0f, (float)d[x][0][i]) * (kk[i] * qs);
+      }
+    } else if constexpr (B16) {
       // a step: 32 entries of one part for up to two tiles of keys, the next step's read while this one's multiply.
       // Small parts first; of two split operands the three products that come to 2^-24 at most are left out.
       constexpr int XS = NT > 1 ? 2 : 1, QS = HD / 32 * NP * (NT / XS);
@@ -581,6 +726,7 @@ void k_tree(TreeArgs a) {
       }
     }
     float mt = -INFINITY;
+    uint32_t hid = 0;  // the lane's keys that its row does not see
     if (base + TK > nc) {
       const int kfirst = base + kgp * SK + 4 * kg - nc;  // drafted row of the lane's first key, below 0 in the cache
 #pragma unroll
@@ -589,9 +735,10 @@ void k_tree(TreeArgs a) {
         for (int i = 0; i < 4; i++) {
           const int j = kfirst + 16 * x + i;
           const bool see = j < 0 || (j < nd && (vis[node - node_lo][min(j, TREE_MAX - 1) >> 5] >> (j & 31) & 1));
-          sc[x][i] = see ? sc[x][i] * c1 : -INFINITY;
+          sc[x][i] = see ? (I8 ? sc[x][i] : sc[x][i] * c1) : -INFINITY;
+          if (I8 && !see) hid |= 1u << (4 * x + i);
         }
-    } else {
+    } else if constexpr (!I8) {
 #pragma unroll
       for (int x = 0; x < NT; x++)
 #pragma unroll
@@ -617,7 +764,68 @@ void k_tree(TreeArgs a) {
       }
 
     // values
-    if constexpr (B16) {
+    if constexpr (I8) {
+      float pv[NT][4], mx = 0.0f, sum = 0.0f;
+#pragma unroll
+      for (int x = 0; x < NT; x++) {
+        const float4 v4 = *(const float4 *)(vs + 16 * x);
+        float vv[4] = {v4.x, v4.y, v4.z, v4.w};
+        if (base + TK > nc)
+#pragma unroll
+          for (int i = 0; i < 4; i++) vv[i] = hid >> (4 * x + i) & 1 ? 0.0f : vv[i];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          sum += vv[i];
+          pv[x][i] = sc[x][i] * vv[i];
+          mx = fmaxf(mx, pv[x][i]);
+        }
+      }
+      if (__any(!(sum < INFINITY))) {  // (a sum that overflowed, or a scale that is not finite)
+#pragma unroll
+        for (int x = 0; x < NT; x++)
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if (!(hid >> (4 * x + i) & 1) && !(fabsf(vs[16 * x + i]) < INFINITY)) gone = __uint_as_float(0x7fc00000u);
+      }
+      mx = tree_xor_max(mx);
+      const int e = max(__builtin_amdgcn_frexp_expf(mx), -100);
+      const float f = __builtin_amdgcn_ldexpf(TREE_FIT, 23 - e), inv = __builtin_amdgcn_ldexpf(1.0f / TREE_FIT, e - 23);
+      uint32_t pd[3][NT];
+#pragma unroll
+      for (int x = 0; x < NT; x++) {
+        uint32_t u[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) u[i] = __float_as_uint(fmaf(pv[x][i], f, TREE_BIAS));  // rounded to a whole number
+        tree_digits(u, pd[2][x], pd[1][x], pd[0][x]);
+      }
+      const int j = (lane & 15) >> 1, vr = 16 * (j >> 2) + 4 * kg + (j & 3), turn = TT::v_turn(vr);
+      const char *vb = vt + (kgp * SK + vr) * ROWB + (lane & 1) * 8;
+      constexpr int VP = TT::WIDE ? 16 : CH % 8 == 0 ? 8 : 4;
+      const float inv256 = inv * 256.0f;
+#pragma unroll
+      for (int dt = 0; dt < HD / 16; dt++) {
+        const char *at = vb + (dt / VP * VP + ((dt % VP) ^ turn)) * 16;
+        const ti2 lo = __builtin_amdgcn_ds_read_tr8_b64_v2i32((tree_lds_i2 *)at);
+        ti4 d[3];
+        if constexpr (NT == 4) {
+          const ti2 hi = __builtin_amdgcn_ds_read_tr8_b64_v2i32((tree_lds_i2 *)(at + 32 * ROWB));
+          const ti4 v = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+          for (int p = 0; p < 3; p++)
+            d[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(v, ti4{(int)pd[p][0], (int)pd[p][1], (int)pd[p][2], (int)pd[p][3]},
+                                                         ti4{0, 0, 0, 0}, 0, 0, 0);
+        } else {
+          const long v = __builtin_bit_cast(long, lo);
+#pragma unroll
+          for (int p = 0; p < 3; p++)
+            d[p] = __builtin_amdgcn_mfma_i32_16x16x32_i8(v, __builtin_bit_cast(long, ti2{(int)pd[p][0], (int)pd[p][1]}),
+                                                         ti4{0, 0, 0, 0}, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          o[dt][i] = fmaf((float)(d[2][i] * 256 + d[1][i]), inv256, fmaf((float)d[0][i], inv, o[dt][i]));
+      }
+    } else if constexpr (B16) {
       const int cv = again(lane) & 15, xr = cv >> 2;
       const char *vb = vt + (kgp * SK + 4 * kg + xr) * ROWB + (cv & 1) * 8 + ((cv >> 1) & 1) * 16;
       constexpr int VP = TT::WIDE ? 8 : 4;
@@ -694,7 +902,11 @@ void k_tree(TreeArgs a) {
     }
   }
 
-  if (nd > 1) {  // the non-finite values that were taken out, for the rows that see them; none in a healthy step
+  if constexpr (I8) {
+    gone = tree_xor_sum(gone);
+#pragma unroll
+    for (int d = 0; d < HD / 16; d++) o[d] += gone;
+  } else if (nd > 1) {  // the non-finite values that were taken out, for the rows that see them; none in a healthy step
     for (int x = 0; x < TREE_MAX / 32; x++)
       for (uint32_t bits = dirty[x]; bits; bits &= bits - 1) {
         const int j = 32 * x + __ffs(bits) - 1;
@@ -712,10 +924,10 @@ void k_tree(TreeArgs a) {
 
   // the column's four lanes hold parts of the row's sum
   l = tree_xor_sum(l);
-  const bool direct = np == 1;
+  const bool direct = np == 1 && !a.joined;
   // partial sums lie by 16-row tiles in the order of the lanes: quad 64 d + lane holds row col's entries
   // 16 d + 4 kg .. + 3, so that they are written and read in whole lines
-  const long unit = (((long)piece * a.B + b) * a.K + kv) * a.t16 + rt * RW + rg;
+  unit += rt * RW + rg;
   float *po = a.part + unit * 16 * HD;
   float2 *pm = a.part_ml + unit * 16;
   // entry e of value tile d is entry at(d, e) of the head
@@ -860,6 +1072,67 @@ __global__ __launch_bounds__(256) void k_tree_join(TreeArgs a, int TK) {
   if (i < n) tree_store(a, b, i, kv * a.R + (row - i * a.R), 16 * d + 4 * (lane >> 4), v, l);
 }
 
+// What the pieces of a sequence and those of its prefix left, joined: a workgroup takes 16 rows of a sequence and 64
+// entries, 16 per wave. `a` is the sequences' pass, `p` the prefixes'. A row's place in the prefix's tiles is its own.
+__global__ __launch_bounds__(256) void k_prefix_join(TreeArgs a, TreeArgs p, int TK) {
+  __shared__ float wt[512][16], red[16][16];
+  const int t = threadIdx.x, w = t >> 6, lane = t & 63, col = lane & 15, kg = lane >> 4, kv = blockIdx.y, b = blockIdx.z;
+  const int nd = a.hd / 16, tile = blockIdx.x * 4 / nd, d = blockIdx.x * 4 - tile * nd + w;
+  const int n = a.n_nodes[b], L = a.len[b];
+  int g, P;
+  if (!tree_prefix(p, b, g, P)) return;
+  if (n < 0 || n > a.T || L < 0 || L > a.cap - (a.in_cache ? n : 0) || tile * 16 >= n * a.R) return;
+  unsigned per, n1, n2 = 0;
+  tree_pieces(a, L, TK, per, n1);
+  if (P > 0) tree_pieces(p, P, p.tk, per, n2);
+  const int np = (int)(n1 + n2), TR = a.T * a.R, rows = n * a.R;
+  // row r of the tile among the prefix's partial sums
+  auto place = [&](int r, long &unit, int &c) {
+    const int f = g >= 0 ? p.first[g] : 0, x = (b - f) * TR + min(tile * 16 + r, rows - 1);
+    unit = (long)kv * p.t16 + tree_tile0(p, f, max(g, 0), 16) + x / 16;
+    c = x % 16;
+  };
+  const long ps = (long)a.B * a.K * a.t16, pp = (long)p.K * p.t16, own = ((long)b * a.K + kv) * a.t16 + tile;
+  const int r = t & 15, j0 = t >> 4;
+  long pu;
+  int pc;
+  place(r, pu, pc);
+  float M = -INFINITY;
+  auto ml = [&](int j) {
+    return j < (int)n1 ? a.part_ml[(j * ps + own) * 16 + r] : p.part_ml[((j - (int)n1) * pp + pu) * 16 + pc];
+  };
+  for (int j = j0; j < np; j += 16) M = fmaxf(M, ml(j).x);
+  red[j0][r] = M;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 16; k++) M = fmaxf(M, red[k][r]);
+  const float Ms = M == -INFINITY ? 0.0f : M;
+  float l = 0.0f;
+  for (int j = j0; j < np; j += 16) {
+    const float2 x = ml(j);
+    const float f = __builtin_amdgcn_exp2f(x.x - Ms);
+    wt[j][r] = f;
+    l += x.y * f;
+  }
+  __syncthreads();
+  red[j0][r] = l;
+  __syncthreads();
+  l = 0.0f;
+#pragma unroll
+  for (int k = 0; k < 16; k++) l += red[k][col];
+  place(col, pu, pc);
+  const float *po = a.part + own * 16 * a.hd + (d * 64 + lane) * 4, *pq = p.part + pu * 16 * a.hd + (d * 64 + kg * 16 + pc) * 4;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int j = 0; j < np; j++) {
+    const float4 y = j < (int)n1 ? *(const float4 *)(po + j * ps * 16 * a.hd) : *(const float4 *)(pq + (j - (int)n1) * pp * 16 * a.hd);
+    const float f = wt[j][col];
+    v = make_float4(v.x + y.x * f, v.y + y.y * f, v.z + y.z * f, v.w + y.w * f);
+  }
+  const int row = tile * 16 + col, i = tree_div(row, a);
+  if (i < n) tree_store(a, b, i, kv * a.R + (row - i * a.R), 16 * d + 4 * kg, v, l);
+}
+
 // Workgroups of `threads` that a CU holds at once (their LDS and registers), asked once per kernel and size.
 template <int HD, int KV, int KW>
 static int tree_per_cu(int threads) {
@@ -867,7 +1140,8 @@ static int tree_per_cu(int threads) {
   std::atomic<int> &k = known[threads / 64];
   int n = k.load(std::memory_order_relaxed);
   if (n == 0) {
-    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, k_tree<HD, KV, KW>, threads, TreeTile<HD, KV>::LDS) !=
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, k_tree<HD, KV, KW>, threads,
+                                                     TreeTile<HD, KV, KW>::LDS) !=
         hipSuccess) {
       (void)hipGetLastError();
       n = 1;
@@ -887,7 +1161,7 @@ static int tree_per_cu(int hd, int threads) {
 
 // Threads of a workgroup.
 static int tree_threads(const TreeArgs &a) {
-  return a.kw > 1 || a.four ? 256 : a.kv16 ? 64 * a.rw : 512;
+  return a.kw > 1 || a.four ? 256 : a.kv16 || a.kv8 ? 64 * a.rw : 512;
 }
 
 // Pieces and row tiles for a call on the matrix cores.
@@ -895,16 +1169,17 @@ bool tree_plan(const Ctx &c, TreeArgs &a) {
   a.rw = a.kw = a.tiles = a.pieces = 1;
   a.four = 0;
   int rw = 1, kw = 1;
-  a.tiled = (a.hd == 64 || a.hd == 128 || a.hd == 192 || a.hd == 256) && !a.kv8 && a.G == 0 && !a.in_cache && a.parent;
+  a.tiled = a.hd == 64 || a.hd == 128 || a.hd == 192 || a.hd == 256;
   if (!a.tiled) return true;
-  const int R = a.H / a.K, t16 = (a.T * R + 15) / 16;
-  const int TK = a.kv16 ? 64 : 32;
+  // (a pass over prefixes: row tiles of a prefix of average size)
+  const int R = a.H / a.K, t16 = a.pre ? (int)(((long)a.B * a.T * R + 16L * a.G - 1) / (16L * a.G)) : (a.T * R + 15) / 16;
+  a.seqs = a.pre ? 1 : a.B;
   a.t16 = t16;
   a.R = R;
   a.magic = R == 1 ? 0 : (unsigned)((0x100000000ull + R - 1) / R);
   if (t16 <= 2) {
     rw = t16;
-    kw = a.kv16 ? 4 / rw : 2;
+    kw = a.kv16 || a.kv8 ? 4 / rw : 2;
   } else {
     kw = 1;
     a.tiles = (t16 + 7) / 8;
@@ -913,6 +1188,12 @@ bool tree_plan(const Ctx &c, TreeArgs &a) {
   a.tiles = (t16 + rw - 1) / rw;
   a.rw = rw;
   a.kw = kw;
+  if (a.pre) {
+    a.tiles = (int)(((long)a.B * a.T * R + a.G * (16L * rw - 1)) / (16 * rw));
+    a.t16 = (int)(((long)a.B * a.T * R + 15L * a.G) / 16);
+  }
+  a.tk = tree_tk(a.kv8 ? KV_I8 : a.kv16 ? KV_BF16 : KV_F32, kw);
+  const int TK = a.tk, seqs = a.pre ? a.G : a.B;
   // Pieces by the time they should take, in microseconds. A workgroup starts and ends in 7 and takes `stage` per stage
   // (measured at head_dim 256, where a CU holds one; it goes with the head dim), and several pieces cost a second
   // launch and a write and read of their rows' partial sums. Equal sequences end together, so their workgroups count
@@ -928,19 +1209,25 @@ bool tree_plan(const Ctx &c, TreeArgs &a) {
   // f32 rows of 128 254 in 1, 189 in 2, 212 in 8, of 64 183 in 1, 88 in 3, 102 in 8; 12 nodes over bf16 rows of 128
   // 133 in 1, 113 in 2, 124 in 8, of 64 90 in 1, 60 in 3, 66 in 8.
   const bool wide = rw > 4;  // two waves on a SIMD
-  const double ncu = c.num_cu, base = (double)a.tiles * a.K * a.B, most = std::ceil((double)(a.max_len + a.T) / TK);
+  const double ncu = c.num_cu, base = (double)a.tiles * a.K * a.seqs;
+  const double most = std::ceil((double)(a.max_len + (a.pre ? 0 : a.T)) / TK);
   const double part = a.hd / 256.0;
   // (from eight stages a CU on, a point between two measured ones: three sequences of 1001 rows, one and a half a CU,
   // 15.2 us with eight waves, 15.6 with four; eight of 4096, 32 a CU, 72 and 63)
-  a.four = !a.kv16 && kw == 1 && a.hd <= 128 && rw <= 4 && a.B > 1 && base * most >= 8 * ncu;
+  a.four = !a.kv16 && !a.kv8 && kw == 1 && a.hd <= 128 && rw <= 4 && seqs > 1 && base * most >= 8 * ncu;
   double stage, busy = 1.0, hold = 1.0;
-  if (a.B == 1) {
-    stage = (kw > 1 ? (a.kv16 ? 1.6 : 2.6) : a.kv16 ? (wide ? 4.4 : 2.6) : (wide ? 6.5 : 4.0)) * part;
+  if (seqs == 1) {
+    stage = (kw > 1 ? (a.kv16 || a.kv8 ? 1.6 : 2.6) : a.kv8 ? (wide ? 3.0 : 1.8) : a.kv16 ? (wide ? 4.4 : 2.6) : (wide ? 6.5 : 4.0)) * part;
   } else if (kw > 1) {
-    stage = (a.kv16 ? 1.6 : 2.6) * (0.3 + 0.7 * part);
+    stage = (a.kv16 || a.kv8 ? 1.6 : 2.6) * (0.3 + 0.7 * part);
     busy = 0.25;
-    hold = a.kv16 ? (kw == 4 ? tree_per_cu<KV_BF16, 4>(a.hd, 256) : tree_per_cu<KV_BF16, 2>(a.hd, 256))
+    hold = a.kv8 ? (kw == 4 ? tree_per_cu<KV_I8, 4>(a.hd, 256) : tree_per_cu<KV_I8, 2>(a.hd, 256))
+           : a.kv16 ? (kw == 4 ? tree_per_cu<KV_BF16, 4>(a.hd, 256) : tree_per_cu<KV_BF16, 2>(a.hd, 256))
                   : tree_per_cu<KV_F32, 2>(a.hd, 256);
+  } else if (a.kv8) {
+    stage = (wide ? 3.0 : 1.8) * (0.3 + 0.7 * part);
+    busy = wide ? 0.9 : 0.4;
+    hold = tree_per_cu<KV_I8, 1>(a.hd, tree_threads(a));
   } else if (a.kv16) {
     stage = (wide ? 4.4 : 2.6) * (0.3 + 0.7 * part);
     busy = wide ? 0.9 : 0.4;
@@ -952,8 +1239,8 @@ bool tree_plan(const Ctx &c, TreeArgs &a) {
            : a.hd == 64 ? tree_per_cu<64, KV_PARTS4, 1>(256)
                         : tree_per_cu<128, KV_PARTS4, 1>(256);
   }
-  const double bytes = (double)a.B * a.K * a.t16 * 16 * a.hd * 8.0;
-  const double pass = a.B > 1 ? 0.75 * a.B * a.K * a.max_len * a.hd * (a.kv16 ? 4.0 : 8.0) / 5.0e6 : 0.0;
+  const double bytes = (double)a.seqs * a.K * a.t16 * 16 * a.hd * 8.0;
+  const double pass = seqs > 1 ? 0.75 * seqs * a.K * a.max_len * a.hd * (a.kv8 ? 2.0 : a.kv16 ? 4.0 : 8.0) / 5.0e6 : 0.0;
   double best = 0.0;
   long pieces = 1;
   auto consider = [&](long p) {
@@ -961,7 +1248,7 @@ bool tree_plan(const Ctx &c, TreeArgs &a) {
     if (p < 1 || p > 256 || (p > 1 && (p > most || bytes * p > 2.0 * (256u << 20)))) return;
     const double groups = base * p, rounds = groups / (ncu * hold), beside = std::min(hold, std::ceil(groups / ncu));
     const double one = 7.0 + stage * std::max(1.0, beside * busy) * std::ceil(most / p);
-    double t = rounds <= 1.0 ? one : a.B == 1 ? std::ceil(rounds) * one : (0.8 * rounds + 0.4) * one;
+    double t = rounds <= 1.0 ? one : seqs == 1 ? std::ceil(rounds) * one : (0.8 * rounds + 0.4) * one;
     const double uneven = rounds > 1.0 ? 1.0 : beside * ncu / groups;
     t = std::max(t, pass * uneven * (hold > 1.0 && groups <= ncu ? 1.2 : 1.0));
     if (p > 1) t += 4.0 + bytes * p / 1.2e7;
@@ -973,27 +1260,31 @@ bool tree_plan(const Ctx &c, TreeArgs &a) {
   a.per = (unsigned)((long)((most + pieces - 1) / pieces) * TK);
   a.pieces = (int)std::max(1L, (a.max_len + a.per - 1) / (long)a.per);
   // a launch holds fewer than 2^32 threads in x
-  if (a.tiles > 1 && ((long)a.pieces * a.K * a.B + 7) / 8 * 8 * a.tiles > (1L << 23) - 1) return false;
+  if (a.tiles > 1 && ((long)a.pieces * a.K * a.seqs + 7) / 8 * 8 * a.tiles > (1L << 23) - 1) return false;
   return true;
 }
 
 size_t tree_part_floats(const TreeArgs &a) {
-  return a.pieces > 1 ? (size_t)a.pieces * a.B * a.K * a.t16 * 16 * (a.hd + 2) : 0;
+  return a.pieces > 1 || a.joined ? (size_t)a.pieces * a.seqs * a.K * a.t16 * 16 * (a.hd + 2) : 0;
 }
 
 template <int HD, int KV, int KW>
 static hipError_t run_tree(const Ctx &c, const TreeArgs &a) {
-  constexpr int lds = TreeTile<HD, KV>::LDS;
+  constexpr int lds = TreeTile<HD, KV, KW>::LDS;
   static_assert(4 * 16 * (HD + 4) * 4 <= lds || KW == 1, "the key groups' join fits the stages' LDS");
-  const long groups = (long)a.pieces * a.K * a.B;
+  const long groups = (long)a.pieces * a.K * a.seqs;
   const long blocks = (groups + 7) / 8 * 8 * a.tiles;
-  const dim3 grid = a.tiles > 1 ? dim3((unsigned)blocks) : dim3(a.pieces, a.K, a.B);
+  const dim3 grid = a.tiles > 1 ? dim3((unsigned)blocks) : dim3(a.pieces, a.K, a.seqs);
   launch_ks(c, k_tree<HD, KV, KW>, grid, dim3(tree_threads(a)), (unsigned)lds, a);
   return hipGetLastError();
 }
 
 template <int HD>
 static hipError_t run_tree_hd(const Ctx &c, const TreeArgs &a) {
+  if (a.kv8)
+    return a.kw == 4   ? run_tree<HD, KV_I8, 4>(c, a)
+           : a.kw == 2 ? run_tree<HD, KV_I8, 2>(c, a)
+                       : run_tree<HD, KV_I8, 1>(c, a);
   if (a.kv16)
     return a.kw == 4   ? run_tree<HD, KV_BF16, 4>(c, a)
            : a.kw == 2 ? run_tree<HD, KV_BF16, 2>(c, a)
@@ -1003,21 +1294,47 @@ static hipError_t run_tree_hd(const Ctx &c, const TreeArgs &a) {
   return a.kw == 2 ? run_tree<HD, KV_F32, 2>(c, a) : run_tree<HD, KV_PARTS, 1>(c, a);
 }
 
+static hipError_t run_tree_pass(const Ctx &c, const TreeArgs &a) {
+  return a.hd == 64 ? run_tree_hd<64>(c, a) : a.hd == 128 ? run_tree_hd<128>(c, a)
+         : a.hd == 192 ? run_tree_hd<192>(c, a) : run_tree_hd<256>(c, a);
+}
+
 hipError_t launch_tree(const Ctx &c, const TreeArgs &a) {
   if (!a.tiled) {
     const bool plain = a.parent && !a.kv8 && !a.in_cache && a.G == 0;
     launch_k(c, plain ? k_tree_any<false> : k_tree_any<true>, dim3(a.H, a.T, a.B), dim3(256), a);
     return hipGetLastError();
   }
-  hipError_t e = a.hd == 64 ? run_tree_hd<64>(c, a) : a.hd == 128 ? run_tree_hd<128>(c, a)
-                 : a.hd == 192 ? run_tree_hd<192>(c, a) : run_tree_hd<256>(c, a);
+  const hipError_t e = run_tree_pass(c, a);
   if (e != hipSuccess || a.pieces == 1) return e;
-  const int TK = a.kv16 ? 64 : 32;
   // few rows, many pieces: the pieces too over the waves
   if (a.pieces > 4 && (long)a.t16 * a.K * a.B <= 256)
-    launch_k(c, k_tree_join<4>, dim3(a.t16 * (a.hd / 16), a.K, a.B), dim3(256), a, TK);
+    launch_k(c, k_tree_join<4>, dim3(a.t16 * (a.hd / 16), a.K, a.B), dim3(256), a, a.tk);
   else
-    launch_k(c, k_tree_join<1>, dim3(a.t16 * (a.hd / 64), a.K, a.B), dim3(256), a, TK);
+    launch_k(c, k_tree_join<1>, dim3(a.t16 * (a.hd / 64), a.K, a.B), dim3(256), a, a.tk);
+  return hipGetLastError();
+}
+
+void tree_prefix_args(const TreeArgs &a, TreeArgs &p) {
+  p = a;
+  p.pre = 1;
+  p.kc = a.kp;
+  p.vc = a.vp;
+  p.kcs = a.kps;
+  p.vcs = a.vps;
+  p.len = a.prefix_len;
+  p.cap = a.pcap;
+  p.max_len = a.max_prefix;
+  p.in_cache = 0;
+  p.joined = 1;
+}
+
+hipError_t launch_prefix(const Ctx &c, const TreeArgs &a, const TreeArgs &p) {
+  hipError_t e = run_tree_pass(c, p);
+  if (e == hipSuccess) e = run_tree_pass(c, a);
+  if (e != hipSuccess) return e;
+  const int tiles = (a.T * a.R + 15) / 16;
+  launch_k(c, k_prefix_join, dim3(tiles * (a.hd / 64), a.K, a.B), dim3(256), a, p, a.tk);
   return hipGetLastError();
 }
 
