@@ -252,13 +252,28 @@ __device__ __forceinline__ void tree_round(float a, float b, uint32_t &hi, uint3
                  __float_as_uint(b - __uint_as_float(mid & 0xffff0000u)));
 }
 
+// Over a column's four lanes (lane % 16): a swap of rows, then of halves, leaves both sides' values in every lane,
+// without the LDS trip of a shuffle.
+struct TreePair { float a, b; };
+__device__ __forceinline__ TreePair tree_rows(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return {__uint_as_float(p[0]), __uint_as_float(p[1])};
+}
+__device__ __forceinline__ TreePair tree_halves(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto p = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return {__uint_as_float(p[0]), __uint_as_float(p[1])};
+}
 __device__ __forceinline__ float tree_xor_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16, 64));
-  return fmaxf(v, __shfl_xor(v, 32, 64));
+  TreePair p = tree_rows(v);
+  p = tree_halves(fmaxf(p.a, p.b));
+  return fmaxf(p.a, p.b);
 }
 __device__ __forceinline__ float tree_xor_sum(float v) {
-  v = v + __shfl_xor(v, 16, 64);
-  return v + __shfl_xor(v, 32, 64);
+  TreePair p = tree_rows(v);
+  p = tree_halves(p.a + p.b);
+  return p.a + p.b;
 }
 
 // How keys and values reach the matrix cores: bf16 as they are, f32 as they are, f32 in three bf16 parts.
@@ -269,8 +284,11 @@ __device__ __forceinline__ float tree_xor_sum(float v) {
 enum { KV_BF16 = 0, KV_F32 = 1, KV_PARTS = 2, KV_PARTS4 = 3, KV_I8 = 4 };
 constexpr bool tree_parts(int kv) { return kv == KV_PARTS || kv == KV_PARTS4; }
 
+// Workgroups of eight waves, one on a CU; else of four, two or more.
+constexpr bool tree_wide(int kv, int kw) { return kw == 1 && kv != KV_PARTS4; }
+
 // Keys per stage.
-constexpr int tree_tk(int kv, int kw) { return kv == KV_BF16 || (kv == KV_I8 && kw == 1) ? 64 : kv == KV_I8 ? 128 : 32; }
+constexpr int tree_tk(int kv, int kw) { return kv == KV_I8 && kw == 1 ? 128 : kv == KV_BF16 || kv == KV_I8 ? 64 : 32; }
 
 template <int HD, int KV, int KW = 1>
 struct TreeTile {
@@ -320,8 +338,7 @@ __device__ __forceinline__ void tree_pieces(const TreeArgs &a, int L, int TK, un
 // 8-bit rows. Their entries go to the matrix cores as they are (v_mfma_i32_16x16x64_i8, at twice the rate of bf16), and
 // so do three digits of each query and probability: a number x is taken as the whole number X nearest to x f, where f
 // brings the row's largest |x| to just below 2^23, and X = 65536 d2 + 256 d1 + d0 with digits in -128..127. A digit's
-// products and sums are exact in 32 bits (256 * 128 * 127 and 64 * 128 * 127 at most), and two digits' sums
-// fit 32 bits together. So a score is exact up to the query's rounding (half of 2^-22 of its largest entry), and the sum over a
+// products and sums are exact (256 * 128 * 127 at most, below 2^22). So a score is exact up to the query's rounding (half of 2^-22 of its largest entry), and the sum over a
 // stage's values up to the probabilities' (half of 2^-22 of the stage's largest probability times scale); f32 sums
 // over stages. A key's scale multiplies its score, a value's its probability. Three products at twice the
 // rate are half of what bf16 rows take.
@@ -341,6 +358,13 @@ __device__ __forceinline__ void tree_digits(const uint32_t (&w)[4], uint32_t &d2
 typedef int ti4 __attribute__((ext_vector_type(4)));
 typedef int ti2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) ti2 tree_lds_i2;
+// Sums start from the bits of C = 1.5 * 2^23, so that one of n (within 2^22) holds the bits of C + n and needs no
+// conversion (which takes the time of four instructions). With s2, s1, s0 read so, 256 s2 - K + s1 is
+// 256 n2 + n1 - C / 256 for K = 257 C + C / 256 (all but the last sum exact), and 256 times that plus s0 is the whole.
+__device__ __forceinline__ ti4 tree_zero() { return ti4{0x4b400000, 0x4b400000, 0x4b400000, 0x4b400000}; }
+__device__ __forceinline__ float tree_high(int s2, int s1) {
+  return fmaf(__int_as_float(s2), 256.0f, -0xc0c0c000p0f) + __int_as_float(s1);
+}
 
 // The prefix and its tile of 16 rw rows that flat tile `rt` of a pass over the prefixes is. A prefix's tiles begin at
 // (f TR + g (U - 1)) / U, with f its first sequence and U = 16 rw: at least its own number from the one before.
@@ -365,13 +389,13 @@ __device__ __forceinline__ bool tree_group(const TreeArgs &a, int rt, int &g, in
 }
 
 template <int HD, int KV, int KW>
-__global__ __launch_bounds__(KW == 1 && KV != KV_PARTS4 ? 512 : 256, KW == 1 && KV != KV_PARTS4 ? 1 : 2)
+__global__ __launch_bounds__(tree_wide(KV, KW) ? 512 : 256, tree_wide(KV, KW) ? 1 : 2)
 void k_tree(TreeArgs a) {
   using TT = TreeTile<HD, KV, KW>;
   constexpr bool I8 = KV == KV_I8;
   constexpr bool B16 = KV != KV_F32, PARTS = tree_parts(KV);  // values' tiles of 16 entries; split rows
   constexpr int ROWB = TT::ROWB, CH = TT::CH, TK = TT::TK, SK = TK / KW, NT = SK / 16;
-  static_assert(!I8 || SK == 64 || SK == 32, "whole products");
+  static_assert(!I8 || SK == 128 || SK == 32, "whole products");
   static_assert(!PARTS || KW == 1, "one group of waves");
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   __shared__ int par[TREE_MAX];
@@ -552,7 +576,9 @@ void k_tree(TreeArgs a) {
     if (__builtin_amdgcn_ldexpf(most, 23 - e) > TREE_TOP) e++;
     e = max(e, -100);
     const bool whole = top < 0x7f800000u;
-    qs = whole ? a.scale * 1.44269504088896341f * __builtin_amdgcn_ldexpf(1.0f, e - 23) : __uint_as_float(0x7fc00000u);
+    // (the scale's sign goes to the query; a scale of 0 is one that makes nothing of any score)
+    qs = whole ? fmaxf(fabsf(a.scale), 1e-30f) * 1.44269504088896341f * __builtin_amdgcn_ldexpf(1.0f, e - 23) : __uint_as_float(0x7fc00000u);
+    const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
     for (int s = 0; s < HD / 64; s++)
 #pragma unroll
@@ -561,7 +587,7 @@ void k_tree(TreeArgs a) {
         uint32_t u[4], d2, d1, d0;
 #pragma unroll
         for (int k = 0; k < 4; k++)
-          u[k] = whole ? (uint32_t)((int)rintf(__builtin_amdgcn_ldexpf(v[k], 23 - e)) + (int)TREE_BIAS) : (uint32_t)TREE_BIAS;
+          u[k] = whole ? (uint32_t)((int)rintf(__builtin_amdgcn_ldexpf(v[k] * sign, 23 - e)) + (int)TREE_BIAS) : (uint32_t)TREE_BIAS;
         tree_digits(u, d2, d1, d0);
         qd[s][0][i] = (int)d0;
         qd[s][1][i] = (int)d1;
@@ -666,26 +692,41 @@ void k_tree(TreeArgs a) {
     constexpr int NP = PARTS ? 3 : 1;  // parts of a key or value
     const float *ks = (const float *)(kt + 2 * TT::SIDE) + kgp * SK + 4 * kg, *vs = ks + TK;  // 8-bit rows' scales
     if constexpr (I8) {
-      ti4 d[NT][3];
+      // a tile of 16 keys at a time: its reads go out a tile ahead, and a tile's sums are put together while the
+      // next one's multiply
+      constexpr int NS = HD / 64;
+      ti4 kf[2][NS], d[2][3];
+      float4 k4[2];
+      float kq[4] = {0.f, 0.f, 0.f, 0.f};
+      auto read = [&](int x) {
+        k4[x & 1] = *(const float4 *)(ks + 16 * x);
 #pragma unroll
-      for (int x = 0; x < NT; x++)
+        for (int st = 0; st < NS; st++) kf[x & 1][st] = *(const ti4 *)(kb + x * 16 * ROWB + kc_at(st));
+      };
+      read(0);
 #pragma unroll
-        for (int p = 0; p < 3; p++) d[x][p] = ti4{0, 0, 0, 0};
+      for (int x = 0; x <= NT; x++) {
+        if (x + 1 < NT) read(x + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        if (x < NT) {
 #pragma unroll
-      for (int st = 0; st < HD / 64; st++)
+          for (int p = 0; p < 3; p++) d[x & 1][p] = tree_zero();
 #pragma unroll
-        for (int x = 0; x < NT; x++) {
-          const ti4 kf = *(const ti4 *)(kb + x * 16 * ROWB + kc_at(st));
+          for (int st = 0; st < NS; st++)
 #pragma unroll
-          for (int p = 2; p >= 0; p--) d[x][p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf, qd[st][p], d[x][p], 0, 0, 0);
+            for (int p = 2; p >= 0; p--)
+              d[x & 1][p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[x & 1][st], qd[st][p], d[x & 1][p], 0, 0, 0);
         }
+        if (x > 0) {
+          const int y = x - 1;
+          const float kk[4] = {kq[0], kq[1], kq[2], kq[3]};
 #pragma unroll
-      for (int x = 0; x < NT; x++) {
-        const float4 k4 = *(const float4 *)(ks + 16 * x);
-        const float kk[4] = {k4.x, k4.y, k4.z, k4.w};
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-          sc[x][i] = fmaf((float)(d[x][2][i] * 256 + d[x][1][i]), 256.0f, (float)d[x][0][i]) * (kk[i] * qs);
+          for (int i = 0; i < 4; i++)
+            sc[y][i] = fmaf(tree_high(d[y & 1][2][i], d[y & 1][1][i]), 256.0f, __int_as_float(d[y & 1][0][i])) * kk[i];
+        }
+        if (x < NT) {
+          kq[0] = k4[x & 1].x, kq[1] = k4[x & 1].y, kq[2] = k4[x & 1].z, kq[3] = k4[x & 1].w;
+        }
       }
     } else if constexpr (B16) {
       // a step: 32 entries of one part for up to two tiles of keys, the next step's read while this one's multiply.
@@ -746,8 +787,11 @@ void k_tree(TreeArgs a) {
     }
 #pragma unroll
     for (int x = 0; x < NT; x++) mt = fmaxf(mt, fmaxf(fmaxf(sc[x][0], sc[x][1]), fmaxf(sc[x][2], sc[x][3])));
-    mt = fmaxf(m, tree_xor_max(mt));
-    if (__any(mt > m)) {
+    mt = tree_xor_max(mt);
+    mt = fmaxf(m, I8 ? mt * qs : mt);
+    // (8-bit rows: only past 2^8, their probabilities' digits being made for each stage's largest)
+    if (__any(I8 ? mt > m + 8.0f : mt > m)) {
+      if (I8 && !(mt > m + 8.0f)) mt = m;
       const float f = mt == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mt);
       l *= f;
 #pragma unroll
@@ -759,28 +803,34 @@ void k_tree(TreeArgs a) {
     for (int x = 0; x < NT; x++)
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        sc[x][i] = __builtin_amdgcn_exp2f(sc[x][i] - ms);
+        sc[x][i] = __builtin_amdgcn_exp2f(I8 ? fmaf(sc[x][i], qs, -ms) : sc[x][i] - ms);
         l += sc[x][i];
       }
 
     // values
     if constexpr (I8) {
-      float pv[NT][4], mx = 0.0f, sum = 0.0f;
+      float pv[NT][4], mx = 0.0f;
 #pragma unroll
       for (int x = 0; x < NT; x++) {
         const float4 v4 = *(const float4 *)(vs + 16 * x);
-        float vv[4] = {v4.x, v4.y, v4.z, v4.w};
-        if (base + TK > nc)
+        pv[x][0] = v4.x, pv[x][1] = v4.y, pv[x][2] = v4.z, pv[x][3] = v4.w;
+      }
+      if (base + TK > nc) {
 #pragma unroll
-          for (int i = 0; i < 4; i++) vv[i] = hid >> (4 * x + i) & 1 ? 0.0f : vv[i];
+        for (int x = 0; x < NT; x++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) pv[x][i] = hid >> (4 * x + i) & 1 ? 0.0f : pv[x][i];
+      }
+#pragma unroll
+      for (int x = 0; x < NT; x++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          sum += vv[i];
-          pv[x][i] = sc[x][i] * vv[i];
+          pv[x][i] *= sc[x][i];
           mx = fmaxf(mx, pv[x][i]);
         }
-      }
-      if (__any(!(sum < INFINITY))) {  // (a sum that overflowed, or a scale that is not finite)
+      // scales that are not finite, two a lane
+      const float2 two = *(const float2 *)((const float *)(kt + 2 * TT::SIDE) + TK + kgp * SK + 2 * (lane % (SK / 2)));
+      if (__any(!(fabsf(two.x) + fabsf(two.y) < INFINITY))) {
 #pragma unroll
         for (int x = 0; x < NT; x++)
 #pragma unroll
@@ -802,28 +852,48 @@ void k_tree(TreeArgs a) {
       const char *vb = vt + (kgp * SK + vr) * ROWB + (lane & 1) * 8;
       constexpr int VP = TT::WIDE ? 16 : CH % 8 == 0 ? 8 : 4;
       const float inv256 = inv * 256.0f;
-#pragma unroll
-      for (int dt = 0; dt < HD / 16; dt++) {
+      // a tile's reads go out ahead, and its sums are added while the next one's multiply
+      constexpr int ND = HD / 16, AHEAD = NT == 2 ? 2 : 1, NR = NT / 2;
+      ti2 vf[AHEAD + 1][NR];
+      ti4 d[2][3];
+      auto read = [&](int dt) {
         const char *at = vb + (dt / VP * VP + ((dt % VP) ^ turn)) * 16;
-        const ti2 lo = __builtin_amdgcn_ds_read_tr8_b64_v2i32((tree_lds_i2 *)at);
-        ti4 d[3];
-        if constexpr (NT == 4) {
-          const ti2 hi = __builtin_amdgcn_ds_read_tr8_b64_v2i32((tree_lds_i2 *)(at + 32 * ROWB));
-          const ti4 v = {lo.x, lo.y, hi.x, hi.y};
 #pragma unroll
-          for (int p = 0; p < 3; p++)
-            d[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(v, ti4{(int)pd[p][0], (int)pd[p][1], (int)pd[p][2], (int)pd[p][3]},
-                                                         ti4{0, 0, 0, 0}, 0, 0, 0);
-        } else {
-          const long v = __builtin_bit_cast(long, lo);
+        for (int h = 0; h < NR; h++)
+          vf[dt % (AHEAD + 1)][h] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((tree_lds_i2 *)(at + h * 32 * ROWB));
+      };
 #pragma unroll
-          for (int p = 0; p < 3; p++)
-            d[p] = __builtin_amdgcn_mfma_i32_16x16x32_i8(v, __builtin_bit_cast(long, ti2{(int)pd[p][0], (int)pd[p][1]}),
-                                                         ti4{0, 0, 0, 0}, 0, 0, 0);
+      for (int dt = 0; dt < AHEAD; dt++) read(dt);
+#pragma unroll
+      for (int dt = 0; dt <= ND; dt++) {
+        if (dt + AHEAD < ND) read(dt + AHEAD);
+        __builtin_amdgcn_sched_barrier(0);
+        if (dt < ND) {
+          const ti2 *v = vf[dt % (AHEAD + 1)];
+#pragma unroll
+          for (int p = 2; p >= 0; p--) {
+            if constexpr (NT == 2) {
+              d[dt & 1][p] = __builtin_amdgcn_mfma_i32_16x16x32_i8(
+                  __builtin_bit_cast(long, v[0]), __builtin_bit_cast(long, ti2{(int)pd[p][0], (int)pd[p][1]}),
+                  tree_zero(), 0, 0, 0);
+            } else {
+              d[dt & 1][p] = tree_zero();
+#pragma unroll
+              for (int h = 0; h < NT / 4; h++)
+                d[dt & 1][p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
+                    ti4{v[2 * h].x, v[2 * h].y, v[2 * h + 1].x, v[2 * h + 1].y},
+                    ti4{(int)pd[p][4 * h], (int)pd[p][4 * h + 1], (int)pd[p][4 * h + 2], (int)pd[p][4 * h + 3]},
+                    d[dt & 1][p], 0, 0, 0);
+            }
+          }
         }
+        __builtin_amdgcn_sched_barrier(0);
+        if (dt > 0) {
+          const ti4 *e = d[(dt - 1) & 1];
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-          o[dt][i] = fmaf((float)(d[2][i] * 256 + d[1][i]), inv256, fmaf((float)d[0][i], inv, o[dt][i]));
+          for (int i = 0; i < 4; i++)
+            o[dt - 1][i] = fmaf(tree_high(e[2][i], e[1][i]), inv256, fmaf(__int_as_float(e[0][i]), inv, o[dt - 1][i]));
+        }
       }
     } else if constexpr (B16) {
       const int cv = again(lane) & 15, xr = cv >> 2;
@@ -1179,7 +1249,7 @@ bool tree_plan(const Ctx &c, TreeArgs &a) {
   a.magic = R == 1 ? 0 : (unsigned)((0x100000000ull + R - 1) / R);
   if (t16 <= 2) {
     rw = t16;
-    kw = a.kv16 || a.kv8 ? 4 / rw : 2;
+    kw = a.kv16 ? 4 / rw : 2;
   } else {
     kw = 1;
     a.tiles = (t16 + 7) / 8;
@@ -1217,16 +1287,16 @@ bool tree_plan(const Ctx &c, TreeArgs &a) {
   a.four = !a.kv16 && !a.kv8 && kw == 1 && a.hd <= 128 && rw <= 4 && seqs > 1 && base * most >= 8 * ncu;
   double stage, busy = 1.0, hold = 1.0;
   if (seqs == 1) {
-    stage = (kw > 1 ? (a.kv16 || a.kv8 ? 1.6 : 2.6) : a.kv8 ? (wide ? 3.0 : 1.8) : a.kv16 ? (wide ? 4.4 : 2.6) : (wide ? 6.5 : 4.0)) * part;
+    stage = (kw > 1 ? (a.kv8 ? 1.0 : a.kv16 ? 1.6 : 2.6) : a.kv8 ? (wide ? 5.0 : 3.0) : a.kv16 ? (wide ? 4.4 : 2.6) : (wide ? 6.5 : 4.0)) * part;
   } else if (kw > 1) {
-    stage = (a.kv16 || a.kv8 ? 1.6 : 2.6) * (0.3 + 0.7 * part);
+    stage = (a.kv8 ? 1.0 : a.kv16 ? 1.6 : 2.6) * (0.3 + 0.7 * part);
     busy = 0.25;
-    hold = a.kv8 ? (kw == 4 ? tree_per_cu<KV_I8, 4>(a.hd, 256) : tree_per_cu<KV_I8, 2>(a.hd, 256))
+    hold = a.kv8 ? tree_per_cu<KV_I8, 2>(a.hd, 256)
            : a.kv16 ? (kw == 4 ? tree_per_cu<KV_BF16, 4>(a.hd, 256) : tree_per_cu<KV_BF16, 2>(a.hd, 256))
                   : tree_per_cu<KV_F32, 2>(a.hd, 256);
   } else if (a.kv8) {
-    stage = (wide ? 3.0 : 1.8) * (0.3 + 0.7 * part);
-    busy = wide ? 0.9 : 0.4;
+    stage = (wide ? 5.0 : 3.0) * (0.3 + 0.7 * part);
+    busy = wide ? 0.9 : 0.6;
     hold = tree_per_cu<KV_I8, 1>(a.hd, tree_threads(a));
   } else if (a.kv16) {
     stage = (wide ? 4.4 : 2.6) * (0.3 + 0.7 * part);
@@ -1282,9 +1352,7 @@ static hipError_t run_tree(const Ctx &c, const TreeArgs &a) {
 template <int HD>
 static hipError_t run_tree_hd(const Ctx &c, const TreeArgs &a) {
   if (a.kv8)
-    return a.kw == 4   ? run_tree<HD, KV_I8, 4>(c, a)
-           : a.kw == 2 ? run_tree<HD, KV_I8, 2>(c, a)
-                       : run_tree<HD, KV_I8, 1>(c, a);
+    return a.kw == 2 ? run_tree<HD, KV_I8, 2>(c, a) : run_tree<HD, KV_I8, 1>(c, a);
   if (a.kv16)
     return a.kw == 4   ? run_tree<HD, KV_BF16, 4>(c, a)
            : a.kw == 2 ? run_tree<HD, KV_BF16, 2>(c, a)
