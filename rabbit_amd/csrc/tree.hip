@@ -39,25 +39,31 @@ __device__ __forceinline__ bool tree_fits(const TreeArgs &a, int b, int &n, int 
   return false;
 }
 
-// The prefix of sequence b, in every thread of the workgroup: its number (-1: none) and its rows. False where the
-// prefixes' first sequences do not follow each other within the batch, or the prefix is longer than its cache.
-__device__ bool tree_prefix(const TreeArgs &a, int b, int &g, int &P) {
-  __shared__ int found;
+// The prefix of sequence b, in every thread of the workgroup: its number (-1: none), its first sequence and its rows.
+// False where the prefixes' first sequences do not follow each other within the batch, or the prefix is longer than its
+// cache.
+__device__ __forceinline__ bool tree_prefix(const TreeArgs &a, int b, int &g, int &f, int &P) {
+  __shared__ int found[3];
   g = -1;
-  P = 0;
+  f = P = 0;
   if (a.G == 0) return true;
-  if (threadIdx.x == 0) found = -1;
+  if (threadIdx.x == 0) found[0] = -1;
   __syncthreads();
   bool ok = true;
   for (int i = threadIdx.x; i < a.G; i += blockDim.x) {
-    const int f0 = a.first[i], f1 = a.first[i + 1];
+    const int f0 = a.first[i], f1 = a.first[i + 1], n = a.prefix_len[i];
     ok = ok && f0 >= 0 && f0 <= f1 && f1 <= a.B;
-    if (f0 <= b && b < f1) found = i;
+    if (f0 <= b && b < f1) {
+      found[0] = i;
+      found[1] = f0;
+      found[2] = n;
+    }
   }
   ok = !__syncthreads_or(!ok);
-  if (ok && found >= 0) {
-    g = found;
-    P = a.prefix_len[g];
+  if (ok && found[0] >= 0) {
+    g = found[0];
+    f = found[1];
+    P = found[2];
     ok = P >= 0 && P <= a.pcap;
   }
   if (!ok && threadIdx.x == 0) *a.bad = 1;
@@ -115,9 +121,9 @@ __global__ __launch_bounds__(256) void k_tree_any(TreeArgs a) {
   __shared__ int par[TREE_MAX];
   __shared__ uint8_t sees[TREE_MAX];
   const int h = blockIdx.x, i = blockIdx.y, b = blockIdx.z, t = threadIdx.x;
-  int n, L, g = -1, P = 0;
+  int n, L, g = -1, f0 = 0, P = 0;
   if (!tree_fits(a, b, n, L) || i >= n) return;
-  if (NEW && !tree_prefix(a, b, g, P)) return;
+  if (NEW && !tree_prefix(a, b, g, f0, P)) return;
   const int kv = h / (a.H / a.K), hd = a.hd;
   const long qi = (((long)b * a.T + i) * a.H + h) * hd;
   for (int e = t; e < hd; e += 256) q[e] = a.q[qi + e];
@@ -371,10 +377,10 @@ __device__ __forceinline__ float tree_high(int s2, int s1) {
 __device__ __forceinline__ int tree_tile0(const TreeArgs &a, int f, int g, int U) {
   return (f * a.T * a.R + g * (U - 1)) / U;
 }
-__device__ __forceinline__ bool tree_group(const TreeArgs &a, int rt, int &g, int &f0, int &f1) {
+__device__ __forceinline__ bool tree_group(const TreeArgs &a, int rt, int &g, int &f0, int &f1, int &L) {
   const int lane = threadIdx.x & 63, U = 16 * a.rw;
   for (int i0 = 0; i0 < a.G; i0 += 64) {
-    const int i = min(i0 + lane, a.G - 1), x0 = a.first[i], x1 = a.first[i + 1];
+    const int i = min(i0 + lane, a.G - 1), x0 = a.first[i], x1 = a.first[i + 1], n = a.len[i];
     const bool in = x0 >= 0 && x0 < x1 && x1 <= a.B && tree_tile0(a, x0, i, U) <= rt && rt < tree_tile0(a, x1, i + 1, U);
     const unsigned long long m = __ballot(in);
     if (m) {
@@ -382,6 +388,7 @@ __device__ __forceinline__ bool tree_group(const TreeArgs &a, int rt, int &g, in
       g = __builtin_amdgcn_readlane(i, l);
       f0 = __builtin_amdgcn_readlane(x0, l);
       f1 = __builtin_amdgcn_readlane(x1, l);
+      L = __builtin_amdgcn_readlane(n, l);
       return true;
     }
   }
@@ -420,8 +427,7 @@ void k_tree(TreeArgs a) {
   long unit = (((long)piece * a.seqs + b) * a.K + kv) * a.t16;  // of the partial sums' 16-row tiles
   if (a.pre) {  // the cache is a prefix, the nodes are those of all its sequences
     int f0, f1;
-    if (!tree_group(a, rt, b, f0, f1)) return;
-    L = a.len[b];
+    if (!tree_group(a, rt, b, f0, f1, L)) return;
     if (L <= 0 || L > a.cap) return;  // (reported where the parts are joined)
     rt -= tree_tile0(a, f0, b, 16 * RW);
     unit += tree_tile0(a, f0, b, 16);
@@ -878,13 +884,17 @@ void k_tree(TreeArgs a) {
                   tree_zero(), 0, 0, 0);
             } else {
               d[dt & 1][p] = tree_zero();
+            }
+          }
+          if constexpr (NT > 2) {
 #pragma unroll
-              for (int h = 0; h < NT / 4; h++)
+            for (int h = 0; h < NT / 4; h++)
+#pragma unroll
+              for (int p = 2; p >= 0; p--)
                 d[dt & 1][p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
                     ti4{v[2 * h].x, v[2 * h].y, v[2 * h + 1].x, v[2 * h + 1].y},
                     ti4{(int)pd[p][4 * h], (int)pd[p][4 * h + 1], (int)pd[p][4 * h + 2], (int)pd[p][4 * h + 3]},
                     d[dt & 1][p], 0, 0, 0);
-            }
           }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -1143,64 +1153,95 @@ __global__ __launch_bounds__(256) void k_tree_join(TreeArgs a, int TK) {
 }
 
 // What the pieces of a sequence and those of its prefix left, joined: a workgroup takes 16 rows of a sequence and 64
-// entries, 16 per wave. `a` is the sequences' pass, `p` the prefixes'. A row's place in the prefix's tiles is its own.
-__global__ __launch_bounds__(256) void k_prefix_join(TreeArgs a, TreeArgs p, int TK) {
+// entries, 16 per wave. `a` is the sequences' pass, `p` the prefixes'. Bound by trips to memory: the sequence's own sums, its
+// gate and its numbers are asked for at once, then the prefix's sums, whose place the numbers tell.
+__global__ __launch_bounds__(256) void k_prefix_join(TreeArgs a, TreeArgs p) {
   __shared__ float wt[512][16], red[16][16];
   const int t = threadIdx.x, w = t >> 6, lane = t & 63, col = lane & 15, kg = lane >> 4, kv = blockIdx.y, b = blockIdx.z;
-  const int nd = a.hd / 16, tile = blockIdx.x * 4 / nd, d = blockIdx.x * 4 - tile * nd + w;
-  const int n = a.n_nodes[b], L = a.len[b];
-  int g, P;
-  if (!tree_prefix(p, b, g, P)) return;
-  if (n < 0 || n > a.T || L < 0 || L > a.cap - (a.in_cache ? n : 0) || tile * 16 >= n * a.R) return;
-  unsigned per, n1, n2 = 0;
-  tree_pieces(a, L, TK, per, n1);
-  if (P > 0) tree_pieces(p, P, p.tk, per, n2);
-  const int np = (int)(n1 + n2), TR = a.T * a.R, rows = n * a.R;
-  // row r of the tile among the prefix's partial sums
-  auto place = [&](int r, long &unit, int &c) {
-    const int f = g >= 0 ? p.first[g] : 0, x = (b - f) * TR + min(tile * 16 + r, rows - 1);
-    unit = (long)kv * p.t16 + tree_tile0(p, f, max(g, 0), 16) + x / 16;
-    c = x % 16;
-  };
+  const int nd = a.hd / 16, tile = blockIdx.x * 4 / nd, d = blockIdx.x * 4 - tile * nd + w, TR = a.T * a.R;
   const long ps = (long)a.B * a.K * a.t16, pp = (long)p.K * p.t16, own = ((long)b * a.K + kv) * a.t16 + tile;
-  const int r = t & 15, j0 = t >> 4;
-  long pu;
-  int pc;
-  place(r, pu, pc);
-  float M = -INFINITY;
-  auto ml = [&](int j) {
-    return j < (int)n1 ? a.part_ml[(j * ps + own) * 16 + r] : p.part_ml[((j - (int)n1) * pp + pu) * 16 + pc];
-  };
-  for (int j = j0; j < np; j += 16) M = fmaxf(M, ml(j).x);
+  const int r = t & 15, j0 = t >> 4, most = a.pieces - 1;
+  // the first pieces' maxima, sums and outputs (of pieces that the sequence does not have too: read, not used)
+  constexpr int PO = 4, PP = 16;
+  const float *po = a.part + own * 16 * a.hd + (d * 64 + lane) * 4;
+  const float2 ml0 = a.part_ml[(min(j0, most) * ps + own) * 16 + r];
+  float4 yo[PO], yp[PP];
+#pragma unroll
+  for (int k = 0; k < PO; k++) yo[k] = *(const float4 *)(po + min(k, most) * ps * 16 * a.hd);
+  const int row = tile * 16 + col, i = tree_div(row, a), h = kv * a.R + (row - i * a.R), e = 16 * d + 4 * kg;
+  float gate[4] = {0.f, 0.f, 0.f, 0.f};
+  if (a.gate && i < a.T) {
+    const float *g = a.gate + ((long)b * a.T + i) * a.gts + (long)h * a.ghs + e;
+#pragma unroll
+    for (int k = 0; k < 4; k++) gate[k] = g[k];
+  }
+  const int n = a.n_nodes[b], L = a.len[b];
+  int g, f0, P;
+  if (!tree_prefix(p, b, g, f0, P)) return;
+  if (n < 0 || n > a.T || L < 0 || L > a.cap - (a.in_cache ? n : 0) || tile * 16 >= n * a.R) return;
+  unsigned per, u1, u2 = 0;
+  tree_pieces(a, L, a.tk, per, u1);
+  if (P > 0) tree_pieces(p, P, p.tk, per, u2);
+  const int n1 = (int)u1, n2 = (int)u2, np = n1 + n2;
+  // row r of the tile among the prefix's partial sums
+  const long pu = (long)kv * p.t16 + tree_tile0(p, f0, max(g, 0), 16);
+  const int x0 = (b - f0) * TR + tile * 16, last = (b - f0) * TR + n * a.R - 1;
+  const int xr = min(x0 + r, last), xc = min(x0 + col, last);
+  const float *pq = p.part + (pu + xc / 16) * 16 * a.hd + (d * 64 + kg * 16 + xc % 16) * 4;
+  const float2 *pm = p.part_ml + (pu + xr / 16) * 16 + xr % 16;
+  float2 ml1 = make_float2(-INFINITY, 0.0f);
+  if (n2 > 0) {
+    ml1 = pm[min(j0, n2 - 1) * pp * 16];
+#pragma unroll
+    for (int k = 0; k < PP; k++) yp[k] = *(const float4 *)(pq + min(k, n2 - 1) * pp * 16 * a.hd);
+  }
+  float M = j0 < n1 ? ml0.x : -INFINITY;
+  if (j0 < n2) M = fmaxf(M, ml1.x);
+  for (int j = j0 + 16; j < n1; j += 16) M = fmaxf(M, a.part_ml[(j * ps + own) * 16 + r].x);
+  for (int j = j0 + 16; j < n2; j += 16) M = fmaxf(M, pm[j * pp * 16].x);
   red[j0][r] = M;
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < 16; k++) M = fmaxf(M, red[k][r]);
   const float Ms = M == -INFINITY ? 0.0f : M;
   float l = 0.0f;
-  for (int j = j0; j < np; j += 16) {
-    const float2 x = ml(j);
+  auto weigh = [&](int at, float2 x) {
     const float f = __builtin_amdgcn_exp2f(x.x - Ms);
-    wt[j][r] = f;
+    wt[at][r] = f;
     l += x.y * f;
-  }
+  };
+  if (j0 < n1) weigh(j0, ml0);
+  for (int j = j0 + 16; j < n1; j += 16) weigh(j, a.part_ml[(j * ps + own) * 16 + r]);
+  if (j0 < n2) weigh(n1 + j0, ml1);
+  for (int j = j0 + 16; j < n2; j += 16) weigh(n1 + j, pm[j * pp * 16]);
   __syncthreads();
   red[j0][r] = l;
   __syncthreads();
   l = 0.0f;
 #pragma unroll
   for (int k = 0; k < 16; k++) l += red[k][col];
-  place(col, pu, pc);
-  const float *po = a.part + own * 16 * a.hd + (d * 64 + lane) * 4, *pq = p.part + pu * 16 * a.hd + (d * 64 + kg * 16 + pc) * 4;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-  for (int j = 0; j < np; j++) {
-    const float4 y = j < (int)n1 ? *(const float4 *)(po + j * ps * 16 * a.hd) : *(const float4 *)(pq + (j - (int)n1) * pp * 16 * a.hd);
+  auto add = [&](float4 y, int j) {
     const float f = wt[j][col];
     v = make_float4(v.x + y.x * f, v.y + y.y * f, v.z + y.z * f, v.w + y.w * f);
+  };
+#pragma unroll
+  for (int k = 0; k < PO; k++)
+    if (k < n1) add(yo[k], k);
+#pragma unroll 8
+  for (int j = PO; j < n1; j++) add(*(const float4 *)(po + j * ps * 16 * a.hd), j);
+#pragma unroll
+  for (int k = 0; k < PP; k++)
+    if (k < n2) add(yp[k], n1 + k);
+#pragma unroll 8
+  for (int j = PP; j < n2; j++) add(*(const float4 *)(pq + j * pp * 16 * a.hd), n1 + j);
+  if (i >= n) return;
+  float o[4] = {v.x / l, v.y / l, v.z / l, v.w / l};
+  if (a.gate) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) o[k] = __fmul_rn(o[k], rbt_sigmoid(gate[k]));
   }
-  const int row = tile * 16 + col, i = tree_div(row, a);
-  if (i < n) tree_store(a, b, i, kv * a.R + (row - i * a.R), 16 * d + 4 * kg, v, l);
+  *(float4 *)(a.out + (((long)b * a.T + i) * a.H + h) * a.hd + e) = make_float4(o[0], o[1], o[2], o[3]);
 }
 
 // Workgroups of `threads` that a CU holds at once (their LDS and registers), asked once per kernel and size.
@@ -1402,7 +1443,7 @@ hipError_t launch_prefix(const Ctx &c, const TreeArgs &a, const TreeArgs &p) {
   if (e == hipSuccess) e = run_tree_pass(c, a);
   if (e != hipSuccess) return e;
   const int tiles = (a.T * a.R + 15) / 16;
-  launch_k(c, k_prefix_join, dim3(tiles * (a.hd / 64), a.K, a.B), dim3(256), a, p, a.tk);
+  launch_k(c, k_prefix_join, dim3(tiles * (a.hd / 64), a.K, a.B), dim3(256), a, p);
   return hipGetLastError();
 }
 
