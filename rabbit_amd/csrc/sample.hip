@@ -33,33 +33,37 @@ struct SmpRow {
   }
 };
 
-// exp(y), y <= 0: 2^(k/32) from a table times a Taylor polynomial of what is left (at most ln 2 / 64: the seventh
-// term is below 2^-52).
+// exp(y), y <= 0, times 2^sh: 2^(k/32) from a table times a Taylor polynomial of what is left (at most ln 2 / 64: the
+// sixth term is below 2^-48).
 __device__ __forceinline__ void smp_table(double *tab) {
   if (threadIdx.x < 32) tab[threadIdx.x] = exp2((double)threadIdx.x * 0.03125);
 }
-__device__ __forceinline__ double smp_exp(double y, const double *tab) {
-  if (!(y > -690.0)) return 0.0;
+__device__ __forceinline__ double smp_exp(double y, int sh, const double *tab) {
   const double k = rint(y * 46.16624130844683);
   const double r = fma(k, -7.247021293269686e-19, fma(k, -0.02166084939249829, y));
   const int n = (int)k;
-  double p = fma(r, 1.0 / 720.0, 1.0 / 120.0);
-  p = fma(r, p, 1.0 / 24.0);
+  double p = fma(r, 1.0 / 120.0, 1.0 / 24.0);
   p = fma(r, p, 1.0 / 6.0);
   p = fma(r, p, 0.5);
   p = fma(r, p, 1.0);
   p = fma(r, p, 1.0);
-  return ldexp(tab[n & 31] * p, n >> 5);
+  return ldexp(tab[n & 31] * p, (n >> 5) + sh);
 }
 __device__ __forceinline__ double smp_weight(const SmpRow &r, float x, const double *tab) {
-  return smp_exp(((double)x - r.m) * r.inv_t, tab);
+  const double y = ((double)x - r.m) * r.inv_t;
+  return y > -690.0 ? smp_exp(y, 0, tab) : 0.0;
 }
-// in units of 2^-S, to the nearest (w <= 1, S <= 45)
-__device__ __forceinline__ u64 smp_mass(const SmpRow &r, double w) {
-  return (u64)__double_as_longlong(ldexp(w, r.S) + 0x1p52) & 0xfffffffffffffull;
+// The weight in units of 2^-S, to the nearest (w <= 1, S <= 45).
+__device__ __forceinline__ u64 smp_round(double w) {
+  return (u64)__double_as_longlong(w + 0x1p52) & 0xfffffffffffffull;
+}
+__device__ __forceinline__ u64 smp_mass(const SmpRow &r, float x, const double *tab) {
+  const double y = ((double)x - r.m) * r.inv_t;
+  return y > -34.0 ? smp_round(smp_exp(y, r.S, tab)) : 0;  // (e^-34 is below 2^-46)
 }
 
-// The bucket of a logit: sixteenths of (m - x) / t, never falling along the order.
+// The bucket of a logit: 24ths of (m - x) / t, never falling along the order; the last holds all from 21.3 on.
+__device__ __forceinline__ float smp_scale(double t) { return fminf(24.0f / (float)t, 1e30f); }
 __device__ __forceinline__ int smp_bucket(float m, float x, float cf) {
   return x > -INFINITY ? (int)fminf((m - x) * cf, 511.0f) : 511;
 }
@@ -100,31 +104,32 @@ __device__ __forceinline__ u64 smp_wave_scan(u64 v) {  // inclusive
 
 // A row is cut in G chunks, a workgroup each, over three launches (no workgroup waits for another; the last one of a row
 // to arrive goes on):
-//   k_sample_top   the chunk's first entry of the order
-//   k_sample_hist  with the row's m, the counts and masses of 512 buckets of (m - x) / t, a sixteenth wide (the last is
-//                  all from 32 on). The last workgroup sums the chunks' and finds the buckets where the
-//                  thresholds lie; without thresholds it draws.
-//   k_sample_list  the entries of those buckets into a list (at most SMP_LIST). The last workgroup sorts it, finds
-//                  the thresholds in it, and draws: the chunk by the chunks' masses, then the entry. A row whose list
-//                  would be longer (thousands of equal logits; a temperature that leaves all mass in one bucket) is taken by one
-//                  workgroup digit by digit.
+//   k_sample_top   the chunk's first entry of the order, and the largest logits of 64 parts of it
+//   k_sample_cut   with the row's m. top-k of up to 512: at least k entries are as large as the k-th of all chunks' part
+//                  maxima, and few more, so those go to a list, and the last workgroup sorts it, finds every threshold in it
+//                  and draws. Else the counts and rounded masses of 512 buckets of (m - x) / t, of which the last workgroup
+//                  takes those where the thresholds may lie; without thresholds it draws.
+//   k_sample_list  the entries of those buckets as a list, the masses of those before; the last workgroup goes on as above,
+//                  and draws the chunk by the chunks' masses, then the entry.
 //   k_sample_probs the probabilities, where they are wanted.
-constexpr int SMP_NT = 256, SMP_NB = 512, SMP_LIST = 2048, SMP_GMAX = 64;
+// A row whose list would be longer than SMP_LIST (thousands of equal logits; a temperature that leaves all mass in one
+// bucket) is taken by one workgroup digit by digit. Rows of up to SMP_LIST entries are lists as they are.
+constexpr int SMP_NT = 256, SMP_NB = 512, SMP_LIST = 2048, SMP_GMAX = 32, SMP_PARTS = 64, SMP_KMAX = 512;
 enum { SMP_DONE = 0, SMP_FIND = 1, SMP_SLOW = 2 };
 
 struct SmpState {  // a row between launches
   u64 thr, total;  // kept: entries up to thr, their mass (0: none, token -1)
-  u64 mass0, massk;  // mass before bucket b0, before bucket kb
   int mode, b0, b1, kb;  // listed: buckets b0 .. b1, and kb
   int cnt0, cntk, n1;  // entries before b0, before kb, in b0 .. b1
   unsigned n;          // list entries so far
 };
 struct SmpWork {  // scratch of up to CNT_N rows
-  u64 *top, *mass, *cert, *list;  // [rows, G], [rows, G, SMP_NB], [rows, G], [rows, SMP_LIST]
-  unsigned *cnt;                  // [rows, G, SMP_NB]
+  u64 *top, *hist, *cert, *list;  // [rows, G], [rows, G, SMP_NB], [rows, 2, G], [rows, SMP_LIST]
+  unsigned *part;                 // [rows, G, SMP_PARTS]
   SmpState *state;
   unsigned *arrive;               // arrival counters, left at 0
   int G, len, row0;               // chunks of a row, entries of a chunk (a multiple of 4), first row
+  int cb, sh;                     // buckets: count in the low cb bits, above them mass / 2^sh
 };
 
 template <typename T>
@@ -151,16 +156,17 @@ __device__ __forceinline__ bool smp_last(const SmpWork &k, int row) {
   return last;
 }
 
-// Entries lo .. hi - 1 of the row, four in a row at a time per thread: f(first index, four values); past hi the values
-// are -inf. UN loads of a thread are on their way at once.
-template <bool QUADS, int UN, typename F>
+// Entries lo .. hi - 1 of the row, four in a row at a time per thread: f(first index, four values), with -inf for those
+// outside [lo, hi). The fours begin at aligned places; UN loads of a thread are on their way at once.
+template <int UN, typename F>
 __device__ __forceinline__ void smp_each(const SmpRow &r, int lo, int hi, F f) {
-  for (int i0 = lo + 4 * threadIdx.x; i0 < hi; i0 += UN * 4 * SMP_NT) {
+  const int pad = (int)(((uintptr_t)r.x >> (r.x16 ? 1 : 2)) + lo) & 3;
+  for (int i0 = lo - pad + 4 * threadIdx.x; i0 < hi; i0 += UN * 4 * SMP_NT) {
     float x[UN][4];
 #pragma unroll
     for (int k = 0; k < UN; k++) {
       const int i = i0 + k * 4 * SMP_NT;
-      if (QUADS && i + 4 <= hi) {
+      if (i >= lo && i + 4 <= hi) {
         if (r.x16) {
           const uint2 v = *(const uint2 *)((const uint16_t *)r.x + i);
           x[k][0] = __uint_as_float(v.x << 16), x[k][1] = __uint_as_float(v.x & 0xffff0000u);
@@ -171,7 +177,7 @@ __device__ __forceinline__ void smp_each(const SmpRow &r, int lo, int hi, F f) {
         }
       } else {
 #pragma unroll
-        for (int e = 0; e < 4; e++) x[k][e] = i + e < hi ? r.at(i + e) : -INFINITY;
+        for (int e = 0; e < 4; e++) x[k][e] = i + e >= lo && i + e < hi ? r.at(i + e) : -INFINITY;
       }
     }
 #pragma unroll
@@ -225,30 +231,39 @@ __device__ __forceinline__ u64 smp_least(u64 v, SmpRed &red) {
   return v;
 }
 
-template <bool QUADS>
 __global__ __launch_bounds__(SMP_NT) void k_sample_top(SampleArgs a, SmpWork k) {
   __shared__ SmpRed red;
-  const int g = blockIdx.x, row = blockIdx.y, lo = min(a.V, g * k.len), hi = min(a.V, lo + k.len);
+  const int g = blockIdx.x, row = blockIdx.y, t = threadIdx.x, lo = min(a.V, g * k.len), hi = min(a.V, lo + k.len);
   const SmpRow r = smp_row(a, k.row0 + row);
-  u64 top = ~0ull;
-  smp_each<QUADS, 8>(r, lo, hi, [&](int i, const float (&x)[4]) {
+  float best = -INFINITY;  // (the first of equal ones: indexes rise)
+  int at = 0;
+  smp_each<8>(r, lo, hi, [&](int i, const float (&x)[4]) {
 #pragma unroll
-    for (int e = 0; e < 4; e++) top = min(top, smp_ord(x[e], i + e));
+    for (int e = 0; e < 4; e++)
+      if (x[e] > best) best = x[e], at = i + e;
   });
-  top = smp_least(top, red);
-  if (threadIdx.x == 0) k.top[(long)row * k.G + g] = top;
+  const u64 mine = best > -INFINITY ? smp_ord(best, at) : ~0ull;
+  unsigned key = (unsigned)(mine >> 32);
+  key = min(key, (unsigned)__shfl_xor((int)key, 1, 64));
+  key = min(key, (unsigned)__shfl_xor((int)key, 2, 64));
+  const long chunk = (long)row * k.G + g;
+  if (t % 4 == 0) k.part[chunk * SMP_PARTS + t / 4] = key;
+  const u64 top = smp_least(mine, red);
+  if (t == 0) {
+    k.top[chunk] = top;
+    if (g == 0) k.state[row].n = 0;
+  }
 }
 
 // The least index in [lo, hi) at which the running mass of entries up to thr passes `left`; every wave first sums its
 // quarter, then the workgroup scans the one where it passes.
-template <bool QUADS>
-__device__ int smp_draw(const SmpRow &r, const double *tab, int lo, int hi, u64 thr, double left, SmpRed &red) {
+__device__ __forceinline__ int smp_draw(const SmpRow &r, const double *tab, int lo, int hi, u64 thr, double left, SmpRed &red) {
   __shared__ int found;
   const int t = threadIdx.x, w = t >> 6, lane = t & 63, part = ((hi - lo + 3) / 4 + 3) & ~3;
   u64 v = 0;
   for (int i = lo + w * part + lane; i < min(hi, lo + (w + 1) * part); i += 64) {
     const float x = r.at(i);
-    if (smp_ord(x, i) <= thr) v += smp_mass(r, smp_weight(r, x, tab));
+    if (smp_ord(x, i) <= thr) v += smp_mass(r, x, tab);
   }
   v = smp_wave_sum(v);
   __syncthreads();
@@ -269,7 +284,7 @@ __device__ int smp_draw(const SmpRow &r, const double *tab, int lo, int hi, u64 
     for (int e = 0; e < 4; e++) {
       const int i = i0 + 4 * t + e;
       const float x = i < end ? r.at(i) : -INFINITY;
-      mine[e] = i < end && smp_ord(x, i) <= thr ? smp_mass(r, smp_weight(r, x, tab)) : 0;
+      mine[e] = i < end && smp_ord(x, i) <= thr ? smp_mass(r, x, tab) : 0;
       sum += mine[e];
     }
     u64 at = run + smp_scan(sum, all, red) - sum;
@@ -298,166 +313,6 @@ __device__ __forceinline__ int smp_chunk(const u64 *mass, int G, double left, u6
   return -1;
 }
 
-template <bool QUADS>
-__global__ __launch_bounds__(SMP_NT) void k_sample_hist(SampleArgs a, SmpWork k) {
-  __shared__ double tab[32];
-  __shared__ u64 mass[SMP_NB + 1], cert[SMP_GMAX];
-  __shared__ unsigned cnt[SMP_NB + 1];
-  __shared__ SmpRed red;
-  __shared__ int kb_s, p0_s, p1_s, held_s;
-  const int g = blockIdx.x, row = blockIdx.y, gr = k.row0 + row, t = threadIdx.x, G = k.G;
-  SmpRow r = smp_row(a, gr);
-  SmpSet s;
-  const bool ok = smp_set(a, gr, s);
-  smp_table(tab);
-  for (int i = t; i <= SMP_NB; i += SMP_NT) mass[i] = 0, cnt[i] = 0;
-  const u64 top = smp_least(t < G ? k.top[(long)row * G + t] : ~0ull, red);
-  const float m = smp_value((uint32_t)(top >> 32));
-  SmpState &st = k.state[row];
-  if (!ok || !(fabsf(m) < INFINITY) || s.k == 1) {  // nothing to draw from, or one entry
-    if (g == 0 && t == 0) {
-      const bool none = !ok || !(fabsf(m) < INFINITY);
-      if (!ok) *a.bad = 1;
-      a.tokens[gr] = none ? -1 : (int)(unsigned)top;
-      st.mode = SMP_DONE;
-      st.thr = top;
-      st.total = none ? 0 : 1ull << a.S;
-    }
-    return;
-  }
-  r.m = m;
-  r.inv_t = 1.0 / s.t;
-  const float cf = fminf(16.0f / (float)s.t, 1e30f);
-  const int lo = min(a.V, g * k.len), hi = min(a.V, lo + k.len);
-  smp_each<QUADS, 4>(r, lo, hi, [&](int i, const float (&x)[4]) {
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const int b = smp_bucket(m, x[e], cf);
-      const u64 v = smp_mass(r, smp_weight(r, x[e], tab));
-      if (v) atomicAdd(&mass[b], v);
-      if (b < SMP_NB - 1) atomicAdd(&cnt[b], 1u);  // (the last bucket's is what is left of the row)
-    }
-  });
-  __syncthreads();
-  if (G > 1) {
-    const long at = ((long)row * G + g) * SMP_NB;
-    for (int b = t; b < SMP_NB; b += SMP_NT) {
-      smp_put(k.mass + at + b, mass[b]);
-      smp_put(k.cnt + at + b, cnt[b]);
-    }
-  }
-  if (!smp_last(k, row)) return;
-  // the row's buckets, two a thread, and what lies before each
-  u64 v[2] = {mass[2 * t], mass[2 * t + 1]};
-  unsigned c[2] = {cnt[2 * t], cnt[2 * t + 1]};
-  if (G > 1) {
-    v[0] = v[1] = 0;
-    c[0] = c[1] = 0;
-    const long at = (long)row * G * SMP_NB + 2 * t;
-    constexpr int UN = 8;  // chunks whose loads are on their way at once
-    for (int j0 = 0; j0 < G; j0 += UN) {
-      u64 x[UN][2];
-      unsigned y[UN][2];
-#pragma unroll
-      for (int j = 0; j < UN; j++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-          const long from = at + (long)min(j0 + j, G - 1) * SMP_NB + e;
-          x[j][e] = smp_get(k.mass + from);
-          y[j][e] = smp_get(k.cnt + from);
-        }
-#pragma unroll
-      for (int j = 0; j < UN; j++)
-#pragma unroll
-        for (int e = 0; e < 2; e++)
-          if (j0 + j < G) v[e] += x[j][e], c[e] += y[j][e];
-    }
-  }
-  u64 all, any;
-  const u64 upto = smp_scan(v[0] + v[1], all, red), cupto = smp_scan((u64)c[0] + c[1], any, red);
-  __syncthreads();
-  mass[2 * t + 1] = upto - v[1];
-  mass[2 * t] = upto - v[1] - v[0];
-  cnt[2 * t + 1] = (unsigned)(cupto - c[1]);
-  cnt[2 * t] = (unsigned)(cupto - c[1] - c[0]);
-  if (t == 0) {
-    mass[SMP_NB] = all;
-    cnt[SMP_NB] = a.V;
-    kb_s = p0_s = p1_s = SMP_NB;
-    held_s = 0;
-  }
-  __syncthreads();
-  const bool by_k = s.k > 0 && s.k < a.V, by_p = s.top_p < 1.0, by_m = s.min_p > 0.0;
-  if (by_k)
-    for (int e = 0; e < 2; e++)
-      if (cnt[2 * t + e] < (unsigned)s.k && cnt[2 * t + e + 1] >= (unsigned)s.k) kb_s = 2 * t + e;
-  __syncthreads();
-  const int kb = kb_s;
-  if (by_p) {  // of the mass that top-k leaves, known up to its last bucket
-    const double f0 = s.top_p * (double)mass[by_k ? kb : SMP_NB], f1 = s.top_p * (double)mass[by_k ? kb + 1 : SMP_NB];
-    for (int e = 0; e < 2; e++) {
-      if ((double)mass[2 * t + e + 1] >= f0) atomicMin(&p0_s, 2 * t + e);
-      if ((double)mass[2 * t + e + 1] >= f1) atomicMin(&p1_s, 2 * t + e);
-    }
-  } else if (t == 0) {
-    p0_s = p1_s = kb;
-  }
-  __syncthreads();
-  int b0 = p0_s, b1 = p1_s;
-  if (by_m) {  // the bucket of the least weight, and its neighbours for their rounding
-    const int b = (int)fmin(-log(s.min_p) * 16.0, 600.0);
-    b0 = min(b0, max(b - 1, 0));
-    b1 = min(b1, min(b + 1, SMP_NB - 1));
-  }
-  const bool list = b0 < SMP_NB;
-  if (list && cnt[b1 + 1] == cnt[b0]) {  // no entry near min_p: the threshold is the last of the bucket before
-    for (int e = 0; e < 2; e++)
-      if (2 * t + e < b0 && cnt[2 * t + e + 1] > cnt[2 * t + e]) atomicMax(&held_s, 2 * t + e);
-    __syncthreads();
-    b0 = held_s;  // (the largest logit is in bucket 0)
-  }
-  const int n1 = list ? cnt[b1 + 1] - cnt[b0] : 0, nk = list && by_k && kb > b1 ? cnt[kb + 1] - cnt[kb] : 0;
-  if (t == 0) {
-    st.mode = !list ? SMP_DONE : n1 + nk > SMP_LIST ? SMP_SLOW : SMP_FIND;
-    st.thr = ~0ull;
-    st.total = all;
-    st.b0 = b0;
-    st.b1 = b1;
-    st.kb = by_k ? kb : -1;
-    st.n1 = n1;
-    st.n = 0;
-    if (list) {
-      st.mass0 = mass[b0];
-      st.cnt0 = cnt[b0];
-      if (by_k) st.massk = mass[kb], st.cntk = cnt[kb];
-    }
-  }
-  if (list && n1 + nk > SMP_LIST) return;
-  // the chunks' masses below the listed buckets
-  if (G > 1) {
-    const int w = t >> 6, lane = t & 63;
-    for (int j = w; j < G; j += SMP_NT / 64) {
-      u64 x = 0;
-      const long at = ((long)row * G + j) * SMP_NB;
-      for (int b = lane; b < min(b0, SMP_NB); b += 64) x += smp_get(k.mass + at + b);
-      x = smp_wave_sum(x);
-      if (lane == 0) {
-        cert[j] = x;
-        k.cert[(long)row * G + j] = x;
-      }
-    }
-  } else if (t == 0) {
-    cert[0] = k.cert[row] = mass[min(b0, SMP_NB)];
-  }
-  __syncthreads();
-  if (list) return;
-  u64 before;
-  const double left = s.u * (double)all;
-  const int ch = smp_chunk(cert, G, left, before);
-  const int tok = ch < 0 ? -1 : smp_draw<QUADS>(r, tab, ch * k.len, min(a.V, (ch + 1) * k.len), ~0ull, left - (double)before, red);
-  if (t == 0) a.tokens[gr] = tok;
-}
-
 // ---- one workgroup for a whole row ---------------------------------------------------------------
 struct SmpSlow {
   u64 mass[256];
@@ -481,7 +336,7 @@ __device__ u64 smp_select(const SmpRow &r, const double *tab, SmpSlow &sh, unsig
       if ((shift == 56 || o >> (shift + 8) == pre >> (shift + 8)) && o <= most) {
         const int d = (int)(o >> shift & 255);
         atomicAdd(&sh.cnt[d], 1u);
-        const u64 w = smp_mass(r, smp_weight(r, x, tab));
+        const u64 w = smp_mass(r, x, tab);
         if (w) atomicAdd(&sh.mass[d], w);
       }
     }
@@ -516,19 +371,326 @@ __device__ u64 smp_select(const SmpRow &r, const double *tab, SmpSlow &sh, unsig
 struct SmpFind {
   u64 ord[SMP_LIST], run[SMP_LIST];  // the list in order, its masses summed up to each
 };
-union SmpListLds {
+union SmpLds {
   SmpFind f;
   SmpSlow slow;
+  struct {
+    u64 hist[SMP_NB + 1];
+    unsigned key[SMP_GMAX * SMP_PARTS];
+  } cut;
 };
 
-template <bool QUADS>
+// The list's n entries (in lds.f.ord, any order) put in order, the thresholds found among the first n1 of them, which
+// begin after cnt0 entries and a mass of mass0; and top-k's entry, where it lies beyond (n1 and cntk, massk) or
+// among them. Returns the last kept entry (-1: none of the list), with kept mass `total`.
+__device__ int smp_find(const SmpRow &r, const SmpSet &s, const double *tab, SmpFind &f, int n, int n1, bool by_k, bool beyond, int cnt0,
+                        int cntk, u64 mass0, u64 massk, u64 whole, u64 &total, SmpRed &red) {
+  __shared__ int ip, im;
+  const int t = threadIdx.x;
+  int n2 = 2;
+  while (n2 < n) n2 *= 2;
+  for (int i = n + t; i < n2; i += SMP_NT) f.ord[i] = ~0ull;
+  if (t == 0) ip = n1, im = -1;
+  __syncthreads();
+  for (int len = 2; len <= n2; len *= 2)  // bitonic, padded to a power of two
+    for (int d = len / 2; d; d /= 2) {
+      for (int i = t; i < n2 / 2; i += SMP_NT) {
+        const int x = (i / d) * 2 * d + i % d, y = x + d;
+        const u64 p = f.ord[x], q = f.ord[y];
+        if ((p > q) == !(x & len)) f.ord[x] = q, f.ord[y] = p;
+      }
+      __syncthreads();
+    }
+  u64 run = 0;
+  for (int i0 = 0; i0 < n; i0 += SMP_NT) {
+    const int i = i0 + t;
+    const float x = i < n ? smp_value((uint32_t)(f.ord[i] >> 32)) : -INFINITY;
+    u64 all;
+    const u64 up = run + smp_scan(smp_mass(r, x, tab), all, red);
+    if (i < n) f.run[i] = up;
+    if (i < n1 && (s.min_p == 0.0 || smp_weight(r, x, tab) >= s.min_p)) atomicMax(&im, i);
+    run += all;
+  }
+  __syncthreads();
+  int last = n1 - 1;
+  u64 left = whole == ~0ull ? run : whole;  // the mass that top-k leaves (~0: the list is all there is)
+  if (by_k && !beyond) {
+    last = s.k - 1 - cnt0;
+    left = mass0 + f.run[last];
+  } else if (by_k) {
+    left = massk + f.run[n1 + s.k - 1 - cntk] - (n1 ? f.run[n1 - 1] : 0);
+  }
+  if (s.top_p < 1.0) {
+    const double target = s.top_p * (double)left;
+    for (int i = t; i < n1; i += SMP_NT)
+      if ((double)(mass0 + f.run[i]) >= target) atomicMin(&ip, i);
+    __syncthreads();
+    last = min(last, ip);
+  }
+  last = min(last, min(im, n1 - 1));
+  total = mass0 + (last >= 0 ? f.run[last] : 0);
+  return last;
+}
+
+// Where nothing is kept before the list: the draw among its entries up to `last`, in the order of their indexes.
+__device__ int smp_draw_list(const SmpFind &f, int last, double left) {
+  __shared__ u64 first;
+  const int t = threadIdx.x;
+  if (t == 0) first = ~0ull;
+  __syncthreads();
+  for (int i = t; i <= last; i += SMP_NT) {
+    const unsigned at = (unsigned)f.ord[i];
+    u64 run = 0, before = 0;
+    for (int j = 0; j <= last; j++) {
+      const u64 up = f.run[j];
+      if ((unsigned)f.ord[j] <= at) run += up - before;
+      before = up;
+    }
+    if ((double)run > left) atomicMin(&first, (u64)at);
+  }
+  __syncthreads();
+  return first == ~0ull ? -1 : (int)first;
+}
+
+// The token: of the list up to `last`, and of what lies before it (mass0, by chunks in `chunk`).
+__device__ int smp_token(const SmpRow &r, const SmpWork &k, const SmpSet &s, const double *tab, const SmpFind &f, int last, u64 thr,
+                         u64 total, u64 mass0, u64 *chunk, SmpRed &red) {
+  const double left = s.u * (double)total;
+  if (mass0 == 0 && last < 256) return smp_draw_list(f, last, left);
+  for (int i = threadIdx.x; i <= last; i += SMP_NT) {
+    const u64 v = f.run[i] - (i ? f.run[i - 1] : 0);
+    if (v) atomicAdd(&chunk[(int)((unsigned)f.ord[i] / (unsigned)k.len)], v);
+  }
+  __syncthreads();
+  u64 before;
+  const int ch = smp_chunk(chunk, k.G, left, before);
+  return ch < 0 ? -1 : smp_draw(r, tab, ch * k.len, min(r.V, (ch + 1) * k.len), thr, left - (double)before, red);
+}
+
+// The k-th smallest of n keys in LDS, bit by bit.
+__device__ unsigned smp_kth(const unsigned *key, int n, int k, SmpRed &red) {
+  const int t = threadIdx.x;
+  unsigned mine[SMP_GMAX * SMP_PARTS / SMP_NT], lo = 0;
+#pragma unroll
+  for (int i = 0; i < SMP_GMAX * SMP_PARTS / SMP_NT; i++) mine[i] = t + i * SMP_NT < n ? key[t + i * SMP_NT] : 0xffffffffu;
+  // the largest value that fewer than k keys are below
+  for (int b = 31; b >= 0; b--) {
+    const unsigned x = lo | 1u << b;
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < SMP_GMAX * SMP_PARTS / SMP_NT; i++) c += __popcll(__ballot(mine[i] < x));
+    unsigned *cnt = (unsigned *)red.w + (b & 1) * (SMP_NT / 64);  // (two sets in turn: one barrier a bit)
+    if ((t & 63) == 0) cnt[t >> 6] = c;
+    __syncthreads();
+    c = 0;
+#pragma unroll
+    for (int i = 0; i < SMP_NT / 64; i++) c += cnt[i];
+    if (c < k) lo = x;
+  }
+  __syncthreads();
+  return lo;
+}
+
+__device__ __forceinline__ void smp_finish(const SampleArgs &a, SmpState &st, int row, int tok, u64 thr, u64 total) {
+  if (threadIdx.x == 0) {
+    a.tokens[row] = tok;
+    st.mode = SMP_DONE;
+    st.thr = thr;
+    st.total = total;
+  }
+}
+
+// The entries of [lo, hi) that `take` wants, appended to the row's list: by the last workgroup the whole list is in lds.
+// Its length goes past SMP_LIST where it does not fit. `then` runs before the workgroup's arrival. False for the
+// workgroups that are not the last.
+template <int UN, typename F, typename H>
+__device__ bool smp_gather(const SmpRow &r, const SmpWork &k, SmpState &st, int row, int lo, int hi, SmpFind &f, unsigned &n, F take, H then) {
+  __shared__ unsigned here, base;
+  const int t = threadIdx.x;
+  if (t == 0) here = 0;
+  __syncthreads();
+  smp_each<UN>(r, lo, hi, [&](int i, const float (&x)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+      if (take(x[e]) && i + e >= lo && i + e < hi) {
+        const unsigned at = atomicAdd(&here, 1u);
+        if (at < SMP_LIST) f.ord[at] = smp_ord(x[e], i + e);
+      }
+  });
+  __syncthreads();
+  n = here;
+  then();
+  if (k.G == 1) return true;
+  u64 *list = k.list + (long)row * SMP_LIST;
+  if (t == 0 && n) base = __hip_atomic_fetch_add(&st.n, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  for (unsigned i = t; i < min(n, (unsigned)SMP_LIST); i += SMP_NT)
+    if (base + i < SMP_LIST) smp_put(list + base + i, f.ord[i]);
+  if (!smp_last(k, row)) return false;
+  n = smp_get(&st.n);
+  for (unsigned i = t; i < min(n, (unsigned)SMP_LIST); i += SMP_NT) f.ord[i] = smp_get(list + i);
+  __syncthreads();
+  return true;
+}
+
+__global__ __launch_bounds__(SMP_NT) void k_sample_cut(SampleArgs a, SmpWork k) {
+  __shared__ SmpLds lds;
+  __shared__ double tab[32];
+  __shared__ u64 cert[SMP_GMAX];
+  __shared__ SmpRed red;
+  __shared__ int kb_s, p0_s, p1_s, held_s;
+  const int g = blockIdx.x, row = blockIdx.y, gr = k.row0 + row, t = threadIdx.x, G = k.G;
+  SmpRow r = smp_row(a, gr);
+  SmpSet s;
+  const u64 top1 = t < G ? k.top[(long)row * G + t] : ~0ull;
+  const bool ok = smp_set(a, gr, s);
+  smp_table(tab);
+  const u64 top = smp_least(top1, red);
+  const float m = smp_value((uint32_t)(top >> 32));
+  SmpState &st = k.state[row];
+  const bool none = !ok || top == ~0ull || !(fabsf(m) < INFINITY);
+  if (none || s.k == 1) {  // nothing to draw from, or one entry
+    if (g == 0) {
+      if (!ok && t == 0) *a.bad = 1;
+      smp_finish(a, st, gr, none ? -1 : (int)(unsigned)top, top, none ? 0 : 1ull << a.S);
+    }
+    return;
+  }
+  r.m = m;
+  r.inv_t = 1.0 / s.t;
+  const bool by_k = s.k > 0 && s.k < a.V, by_p = s.top_p < 1.0, by_m = s.min_p > 0.0;
+  const int lo = min(a.V, g * k.len), hi = min(a.V, lo + k.len), np = G * SMP_PARTS;
+  const bool whole = a.V <= SMP_LIST;
+  if (whole || (by_k && s.k <= min(SMP_KMAX, np))) {
+    unsigned most = ~0u, n;
+    if (!whole) {
+      for (int i = t; i < np; i += SMP_NT) lds.cut.key[i] = k.part[(long)row * np + i];
+      __syncthreads();
+      most = smp_kth(lds.cut.key, np, s.k, red);
+    }
+    if (!smp_gather<8>(r, k, st, row, lo, hi, lds.f, n, [&](float x) { return smp_key(x) <= most; }, [] {})) return;
+    if (n <= SMP_LIST) {
+      u64 total;
+      const int last = smp_find(r, s, tab, lds.f, n, n, by_k, false, 0, 0, 0, 0, ~0ull, total, red);
+      if (t < G) cert[t] = 0;
+      __syncthreads();
+      const u64 thr = lds.f.ord[last];
+      smp_finish(a, st, gr, smp_token(r, k, s, tab, lds.f, last, thr, total, 0, cert, red), thr, total);
+    } else if (t == 0) {
+      st.mode = SMP_SLOW;
+    }
+    return;
+  }
+  for (int i = t; i <= SMP_NB; i += SMP_NT) lds.cut.hist[i] = 0;
+  __syncthreads();
+  const float cf = smp_scale(s.t);
+  u64 sum = 0;
+  const bool any = by_k || by_p || by_m;
+  smp_each<4>(r, lo, hi, [&](int, const float (&x)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const u64 v = smp_mass(r, x[e], tab);
+      sum += v;
+      const int b = smp_bucket(m, x[e], cf);
+      if (any && b < SMP_NB - 1) atomicAdd(&lds.cut.hist[b], (v >> k.sh) << k.cb | 1);  // (the last is what is left)
+    }
+  });
+  sum = smp_sum(sum, red);
+  u64 *mine = k.cert + (long)row * 2 * G;
+  if (t == 0) G > 1 ? smp_put(mine + g, sum) : (void)(cert[0] = sum);
+  const long at = (long)row * G * SMP_NB;
+  if (G > 1 && any)
+    for (int b = t; b < SMP_NB; b += SMP_NT) smp_put(k.hist + at + (long)g * SMP_NB + b, lds.cut.hist[b]);
+  if (!smp_last(k, row)) return;
+  if (G > 1 && t < G) cert[t] = smp_get(mine + t);
+  // the row's buckets, two a thread, and what lies before each
+  u64 v[2] = {lds.cut.hist[2 * t], lds.cut.hist[2 * t + 1]};
+  if (G > 1 && any) {
+    v[0] = v[1] = 0;
+    constexpr int UN = 8;  // chunks whose loads are on their way at once
+    for (int j0 = 0; j0 < G; j0 += UN) {
+      u64 x[UN][2];
+#pragma unroll
+      for (int j = 0; j < UN; j++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) x[j][e] = smp_get(k.hist + at + (long)min(j0 + j, G - 1) * SMP_NB + 2 * t + e);
+#pragma unroll
+      for (int j = 0; j < UN; j++)
+        if (j0 + j < G) v[0] += x[j][0], v[1] += x[j][1];
+    }
+  }
+  __syncthreads();
+  u64 all = 0, before;
+  for (int j = 0; j < G; j++) all += cert[j];
+  if (!any) {
+    const double left = s.u * (double)all;
+    const int ch = smp_chunk(cert, G, left, before);
+    const int tok = ch < 0 ? -1 : smp_draw(r, tab, ch * k.len, min(a.V, (ch + 1) * k.len), ~0ull, left - (double)before, red);
+    smp_finish(a, st, gr, tok, ~0ull, all);
+    return;
+  }
+  u64 rest;
+  const u64 upto = smp_scan(v[0] + v[1], rest, red);
+  __syncthreads();
+  u64 *hist = lds.cut.hist;
+  hist[2 * t + 1] = upto - v[1];
+  hist[2 * t] = upto - v[1] - v[0];
+  if (t == 0) {
+    hist[SMP_NB] = rest;
+    kb_s = p0_s = p1_s = SMP_NB;
+    held_s = 0;
+  }
+  __syncthreads();
+  const unsigned one = (1u << k.cb) - 1;
+  auto cnt = [&](int b) { return b == SMP_NB ? (unsigned)a.V : (unsigned)hist[b] & one; };
+  // the mass before bucket b, in units of 2^(sh - S): at least, and below
+  auto low = [&](int b) { return (double)(hist[b] >> k.cb); };
+  auto high = [&](int b) { return b == SMP_NB ? ldexp((double)all, -k.sh) + 1.0 : low(b) + (double)cnt(b); };
+  if (by_k)
+    for (int e = 0; e < 2; e++)
+      if (cnt(2 * t + e) < (unsigned)s.k && cnt(2 * t + e + 1) >= (unsigned)s.k) kb_s = 2 * t + e;
+  __syncthreads();
+  const int kb = kb_s;
+  if (by_p) {  // of the mass that top-k leaves
+    const double whole0 = by_k ? low(kb) : ldexp((double)all, -k.sh), whole1 = by_k ? high(kb + 1) : whole0;
+    for (int e = 0; e < 2; e++) {
+      if (high(2 * t + e + 1) >= s.top_p * whole0) atomicMin(&p0_s, 2 * t + e);
+      if (low(2 * t + e + 1) >= s.top_p * whole1) atomicMin(&p1_s, 2 * t + e);
+    }
+  }
+  __syncthreads();
+  int b0 = by_p ? min(p0_s, kb) : kb, b1 = by_p ? min(min(p1_s, kb), SMP_NB - 1) : kb;
+  if (by_m) {  // the bucket of the least weight, and its neighbours for their rounding
+    const int b = (int)fmin(-log(s.min_p) * 24.0, 600.0);
+    b0 = min(b0, max(b - 1, 0));
+    b1 = min(b1, min(b + 1, SMP_NB - 1));
+  }
+  b0 = min(b0, SMP_NB - 1);
+  if (cnt(b1 + 1) == cnt(b0)) {  // no entry near min_p: the threshold is the last of the bucket before
+    for (int e = 0; e < 2; e++)
+      if (2 * t + e < b0 && cnt(2 * t + e + 1) > cnt(2 * t + e)) atomicMax(&held_s, 2 * t + e);
+    __syncthreads();
+    b0 = held_s;  // (the largest logit is in bucket 0)
+  }
+  if (t == 0) {
+    const unsigned n1 = cnt(b1 + 1) - cnt(b0), nk = by_k && kb > b1 ? cnt(kb + 1) - cnt(kb) : 0;
+    st.mode = n1 + nk > SMP_LIST ? SMP_SLOW : SMP_FIND;
+    st.total = all;
+    st.b0 = b0;
+    st.b1 = b1;
+    st.kb = by_k ? kb : -1;
+    st.n1 = (int)n1;
+    st.cnt0 = (int)cnt(b0);
+    st.cntk = by_k ? (int)cnt(kb) : 0;
+    st.n = 0;
+  }
+}
+
 __global__ __launch_bounds__(SMP_NT) void k_sample_list(SampleArgs a, SmpWork k) {
-  __shared__ SmpListLds lds;
+  __shared__ SmpLds lds;
   __shared__ double tab[32];
   __shared__ u64 chunk[SMP_GMAX];
   __shared__ SmpRed red;
-  __shared__ unsigned n_s, base_s;
-  __shared__ int ip_s, im_s;
   const int g = blockIdx.x, row = blockIdx.y, gr = k.row0 + row, t = threadIdx.x, G = k.G;
   SmpState &st = k.state[row];
   const int mode = st.mode;
@@ -543,122 +705,64 @@ __global__ __launch_bounds__(SMP_NT) void k_sample_list(SampleArgs a, SmpWork k)
   r.inv_t = 1.0 / s.t;
   const bool by_k = s.k > 0 && s.k < a.V, by_p = s.top_p < 1.0, by_m = s.min_p > 0.0;
   if (mode == SMP_SLOW) {
-    u64 thr = ~0ull, mass = st.total;
-    if (by_k) thr = smp_select(r, tab, lds.slow, s.k, 0.0, thr, mass);
+    u64 thr = ~0ull, mass = 0, total = 0, last = 0;
+    if (by_k) {
+      thr = smp_select(r, tab, lds.slow, s.k, 0.0, thr, mass);
+    } else if (by_p) {
+      for (int i = t; i < a.V; i += SMP_NT) mass += smp_mass(r, r.at(i), tab);
+      mass = smp_sum(mass, red);
+    }
     if (by_p) thr = smp_select(r, tab, lds.slow, 0, s.top_p * (double)mass, thr, mass);
-    u64 total = 0, last = 0;
     for (int i = t; i < a.V; i += SMP_NT) {
       const float x = r.at(i);
-      const double wt = smp_weight(r, x, tab);
       const u64 o = smp_ord(x, i);
-      if (o <= thr && wt >= s.min_p) {
-        total += smp_mass(r, wt);
+      if (o <= thr && (!by_m || smp_weight(r, x, tab) >= s.min_p)) {
+        total += smp_mass(r, x, tab);
         last = max(last, o);
       }
     }
     total = smp_sum(total, red);
     if (by_m) thr = ~smp_least(~last, red);  // the last that is heavy enough
-    const int tok = smp_draw<QUADS>(r, tab, 0, a.V, thr, s.u * (double)total, red);
-    if (t == 0) {
-      a.tokens[gr] = tok;
-      st.thr = thr;
-      st.total = total;
-    }
+    smp_finish(a, st, gr, smp_draw(r, tab, 0, a.V, thr, s.u * (double)total, red), thr, total);
     return;
   }
-  if (t == 0) n_s = 0;
-  __syncthreads();
-  const int b0 = st.b0, b1 = st.b1, kb = st.kb, n1 = st.n1;
-  const float cf = fminf(16.0f / (float)s.t, 1e30f);
+  const int b0 = st.b0, b1 = st.b1, kb = st.kb, n1 = st.n1, cnt0 = st.cnt0, cntk = st.cntk;
+  const u64 all = st.total;
+  const bool beyond = by_k && kb > b1;
+  const float cf = smp_scale(s.t);
   const int lo = min(a.V, g * k.len), hi = min(a.V, lo + k.len);
-  smp_each<QUADS, 8>(r, lo, hi, [&](int i, const float (&x)[4]) {
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const int b = smp_bucket(m, x[e], cf);
-      if (((b >= b0 && b <= b1) || b == kb) && i + e < hi) {
-        const unsigned at = atomicAdd(&n_s, 1u);
-        if (at < SMP_LIST) lds.f.ord[at] = smp_ord(x[e], i + e);
-      }
+  // the masses before the listed buckets, and before top-k's where that is another
+  u64 sum0 = 0, sumk = 0, *mine = k.cert + (long)row * 2 * G;
+  unsigned n;
+  const bool last_one = smp_gather<8>(r, k, st, row, lo, hi, lds.f, n, [&](float x) {
+    const int b = smp_bucket(m, x, cf);
+    if (b < b0 || (beyond && b < kb)) {
+      const u64 v = smp_mass(r, x, tab);
+      if (b < b0) sum0 += v;
+      sumk += v;
     }
+    return (b >= b0 && b <= b1) || b == kb;
+  }, [&]() {
+    sum0 = smp_sum(sum0, red);
+    sumk = smp_sum(sumk, red);
+    if (t == 0) smp_put(mine + g, sum0), smp_put(mine + G + g, sumk);
   });
-  __syncthreads();
-  unsigned n = min(n_s, (unsigned)SMP_LIST);
-  u64 *list = k.list + (long)row * SMP_LIST;
-  if (G > 1) {
-    if (t == 0 && n) base_s = __hip_atomic_fetch_add(&st.n, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    for (unsigned i = t; i < n; i += SMP_NT)
-      if (base_s + i < SMP_LIST) smp_put(list + base_s + i, lds.f.ord[i]);
-    if (!smp_last(k, row)) return;
-    n = min(smp_get(&st.n), (unsigned)SMP_LIST);
-    for (unsigned i = t; i < n; i += SMP_NT) lds.f.ord[i] = smp_get(list + i);
+  if (!last_one) return;
+  u64 v0 = 0, vk = 0;
+  if (t < G) {  // (the chunks' masses are read by all after the sums' barriers)
+    v0 = smp_get(mine + t);
+    vk = smp_get(mine + G + t);
+    chunk[t] = v0;
   }
-  // in order (bitonic, padded to a power of two)
-  int n2 = 2;
-  while (n2 < (int)n) n2 *= 2;
-  for (int i = n + t; i < n2; i += SMP_NT) lds.f.ord[i] = ~0ull;
-  __syncthreads();
-  for (int len = 2; len <= n2; len *= 2)
-    for (int d = len / 2; d; d /= 2) {
-      for (int i = t; i < n2 / 2; i += SMP_NT) {
-        const int x = (i / d) * 2 * d + i % d, y = x + d;
-        const u64 p = lds.f.ord[x], q = lds.f.ord[y];
-        if ((p > q) == !(x & len)) lds.f.ord[x] = q, lds.f.ord[y] = p;
-      }
-      __syncthreads();
-    }
-  // masses up to each entry; the last of b0 .. b1 that is heavy enough
-  if (t == 0) ip_s = n1, im_s = -1;
-  u64 run = 0;
-  for (int i0 = 0; i0 < (int)n; i0 += SMP_NT) {
-    const int i = i0 + t;
-    const double wt = i < (int)n ? smp_weight(r, smp_value((uint32_t)(lds.f.ord[i] >> 32)), tab) : 0.0;
-    u64 all;
-    const u64 up = run + smp_scan(i < (int)n ? smp_mass(r, wt) : 0, all, red);
-    if (i < (int)n) lds.f.run[i] = up;
-    if (i < n1 && wt >= s.min_p) atomicMax(&im_s, i);
-    run += all;
-  }
-  __syncthreads();
-  int last = n1 - 1;
-  u64 kept = st.total;  // mass that top-k leaves
-  if (by_k) {
-    if (kb <= b1) {
-      last = s.k - 1 - st.cnt0;
-      kept = st.mass0 + lds.f.run[last];
-    } else {
-      kept = st.massk + lds.f.run[n1 + s.k - 1 - st.cntk] - (n1 ? lds.f.run[n1 - 1] : 0);
-    }
-  }
-  if (by_p) {
-    const double target = s.top_p * (double)kept;
-    for (int i = t; i < n1; i += SMP_NT)
-      if ((double)(st.mass0 + lds.f.run[i]) >= target) atomicMin(&ip_s, i);
-    __syncthreads();
-    last = min(last, ip_s);
-  }
-  if (by_m) last = min(last, im_s);
-  last = min(last, n1 - 1);
-  const u64 total = st.mass0 + (last >= 0 ? lds.f.run[last] : 0), thr = last >= 0 ? lds.f.ord[last] : lds.f.ord[0] - 1;
-  for (int j = t; j < G; j += SMP_NT) chunk[j] = k.cert[(long)row * G + j];
-  __syncthreads();
-  for (int i = t; i <= last; i += SMP_NT) {
-    const u64 v = lds.f.run[i] - (i ? lds.f.run[i - 1] : 0);
-    if (v) atomicAdd(&chunk[(int)((unsigned)lds.f.ord[i] / (unsigned)k.len)], v);
-  }
-  __syncthreads();
-  u64 before;
-  const double left = s.u * (double)total;
-  const int ch = smp_chunk(chunk, G, left, before);
-  const int tok = ch < 0 ? -1 : smp_draw<QUADS>(r, tab, ch * k.len, min(a.V, (ch + 1) * k.len), thr, left - (double)before, red);
-  if (t == 0) {
-    a.tokens[gr] = tok;
-    st.thr = thr;
-    st.total = total;
-  }
+  const u64 mass0 = smp_sum(v0, red), massk = smp_sum(vk, red);
+  u64 total;
+  const int last = smp_find(r, s, tab, lds.f, (int)min(n, (unsigned)SMP_LIST), n1, by_k, beyond, cnt0, cntk, mass0, massk, all, total, red);
+  const u64 thr = last >= 0 ? lds.f.ord[last] : lds.f.ord[0] - 1;
+  const int tok = smp_token(r, k, s, tab, lds.f, last, thr, total, mass0, chunk, red);
+  smp_finish(a, st, gr, tok, thr, total);
 }
 
-template <bool QUADS>
+typedef float smp_f4 __attribute__((ext_vector_type(4), aligned(4)));  // (stores of four words want four bytes' alignment)
 __global__ __launch_bounds__(SMP_NT) void k_sample_probs(SampleArgs a, SmpWork k) {
   __shared__ double tab[32];
   __shared__ SmpRed red;
@@ -673,18 +777,17 @@ __global__ __launch_bounds__(SMP_NT) void k_sample_probs(SampleArgs a, SmpWork k
   const double scale = total ? ldexp(1.0, a.S) / (double)total : 0.0;
   const int lo = min(a.V, g * k.len), hi = min(a.V, lo + k.len);
   float *to = a.probs + (long)gr * a.V;
-  const bool quads = a.V % 4 == 0 && (uintptr_t)a.probs % 16 == 0;
-  smp_each<QUADS, 4>(r, lo, hi, [&](int i, const float (&x)[4]) {
+  smp_each<4>(r, lo, hi, [&](int i, const float (&x)[4]) {
     float p[4];
 #pragma unroll
     for (int e = 0; e < 4; e++)
       p[e] = total && smp_ord(x[e], i + e) <= thr ? (float)(smp_weight(r, x[e], tab) * scale) : 0.0f;
-    if (quads && i + 4 <= hi) {
-      *(float4 *)(to + i) = make_float4(p[0], p[1], p[2], p[3]);
+    if (i >= lo && i + 4 <= hi) {
+      *(smp_f4 *)(to + i) = smp_f4{p[0], p[1], p[2], p[3]};
     } else {
 #pragma unroll
       for (int e = 0; e < 4; e++)
-        if (i + e < hi) to[i + e] = p[e];
+        if (i + e >= lo && i + e < hi) to[i + e] = p[e];
     }
   });
 }
@@ -705,25 +808,16 @@ static size_t smp_carve(const Ctx &c, size_t n, int V, char *base, SmpWork *k) {
   w.G = (int)G;
   w.len = (int)(((V + G - 1) / G + 3) & ~3L);
   w.top = (u64 *)take(rows * G * 8);
-  w.cert = (u64 *)take(rows * G * 8);
+  w.cert = (u64 *)take(rows * 2 * G * 8);
+  w.part = (unsigned *)take(rows * G * SMP_PARTS * 4);
   w.state = (SmpState *)take(rows * sizeof(SmpState));
-  w.list = (u64 *)take(rows * SMP_LIST * 8);
-  w.mass = (u64 *)take(G > 1 ? rows * G * SMP_NB * 8 : 0);
-  w.cnt = (unsigned *)take(G > 1 ? rows * G * SMP_NB * 4 : 0);
+  w.list = (u64 *)take(G > 1 ? rows * SMP_LIST * 8 : 0);
+  w.hist = (u64 *)take(G > 1 ? rows * G * SMP_NB * 8 : 0);
   w.arrive = c.d_cnt;
   if (k) *k = w;
   return at;
 }
 size_t sample_scratch(const Ctx &c, size_t n, int V) { return smp_carve(c, n, V, nullptr, nullptr); }
-
-template <bool QUADS>
-static void run_sample(const Ctx &c, const SampleArgs &a, const SmpWork &k, int rows) {
-  const dim3 grid(k.G, rows), block(SMP_NT);
-  launch_k(c, k_sample_top<QUADS>, grid, block, a, k);
-  launch_k(c, k_sample_hist<QUADS>, grid, block, a, k);
-  if (a.top_k || a.top_p || a.min_p) launch_k(c, k_sample_list<QUADS>, grid, block, a, k);
-  if (a.probs) launch_k(c, k_sample_probs<QUADS>, grid, block, a, k);
-}
 
 hipError_t launch_sample(const Ctx &c, SampleArgs a, size_t n, void *scratch) {
   int bits = 0;
@@ -731,11 +825,17 @@ hipError_t launch_sample(const Ctx &c, SampleArgs a, size_t n, void *scratch) {
   a.S = std::min(45, 62 - bits);
   SmpWork k;
   smp_carve(c, n, a.V, (char *)scratch, &k);
-  const bool quads = a.stride % 4 == 0 && (uintptr_t)a.x % (a.x16 ? 8 : 16) == 0;
+  // a bucket's count is at most 2^bits, its mass V of 2^(S - sh)
+  k.cb = bits + 1;
+  k.sh = a.S - std::min(30, 63 - k.cb - bits);
   for (size_t r0 = 0; r0 < n; r0 += CNT_N) {
     k.row0 = (int)r0;
     const int rows = (int)std::min<size_t>(CNT_N, n - r0);
-    quads ? run_sample<true>(c, a, k, rows) : run_sample<false>(c, a, k, rows);
+    const dim3 grid(k.G, rows), block(SMP_NT);
+    launch_k(c, k_sample_top, grid, block, a, k);
+    launch_k(c, k_sample_cut, grid, block, a, k);
+    if (a.V > SMP_LIST && (a.top_k || a.top_p || a.min_p)) launch_k(c, k_sample_list, grid, block, a, k);
+    if (a.probs) launch_k(c, k_sample_probs, grid, block, a, k);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
