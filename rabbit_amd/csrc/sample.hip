@@ -9,7 +9,7 @@
 // only where u is within 2^-S times the number of entries of a border. (Sums in fp32 would move every border by 1e-7.)
 //
 // How the thresholds are found:
-//   top-k of up to 512: the row's parts (a thread's or four threads' entries) have a largest entry each; at least k
+//   top-k of up to three quarters of the row's parts (some threads' entries), which have a largest entry each; at least k
 //     entries are as large as the k-th of those, and few more, so those go to a list.
 //   else 512 buckets of (m - x) / t, with counts and rounded masses, tell the buckets where the thresholds may lie, and
 //     those buckets' entries go to a list.
@@ -30,7 +30,7 @@ namespace rbt {
 typedef unsigned long long u64;
 
 constexpr int SMP_NT = 256, SMP_ONE = 1024;  // threads of a chunk's workgroup, of a row's
-constexpr int SMP_NB = 512, SMP_LIST = 2048, SMP_GMAX = 32, SMP_PARTS = 64, SMP_KMAX = 512;
+constexpr int SMP_NB = 512, SMP_LIST = 2048, SMP_GMAX = 32, SMP_PARTS = 32;
 
 // A logit's bits, larger logits first; NaN counts as -inf, and -0 as 0.
 __device__ __forceinline__ uint32_t smp_key(float x) {
@@ -80,32 +80,57 @@ __device__ __forceinline__ SmpSet smp_set(const SampleArgs &a, int r) {
 }
 
 // ---- weights ---------------------------------------------------------------------------------------
-// 2^(k / 32)
-__device__ const double SMP_POW[32] = {
-    0x1.0000000000000p+0, 0x1.059b0d3158574p+0, 0x1.0b5586cf9890fp+0, 0x1.11301d0125b51p+0,
-    0x1.172b83c7d517bp+0, 0x1.1d4873168b9aap+0, 0x1.2387a6e756238p+0, 0x1.29e9df51fdee1p+0,
-    0x1.306fe0a31b715p+0, 0x1.371a7373aa9cbp+0, 0x1.3dea64c123422p+0, 0x1.44e086061892dp+0,
-    0x1.4bfdad5362a27p+0, 0x1.5342b569d4f82p+0, 0x1.5ab07dd485429p+0, 0x1.6247eb03a5585p+0,
-    0x1.6a09e667f3bcdp+0, 0x1.71f75e8ec5f74p+0, 0x1.7a11473eb0187p+0, 0x1.82589994cce13p+0,
-    0x1.8ace5422aa0dbp+0, 0x1.93737b0cdc5e5p+0, 0x1.9c49182a3f090p+0, 0x1.a5503b23e255dp+0,
-    0x1.ae89f995ad3adp+0, 0x1.b7f76f2fb5e47p+0, 0x1.c199bdd85529cp+0, 0x1.cb720dcef9069p+0,
-    0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0, 0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0,
+// 2^(k / 128)
+__device__ const double SMP_POW[128] = {
+    0x1.0000000000000p+0, 0x1.0163da9fb3335p+0, 0x1.02c9a3e778061p+0, 0x1.04315e86e7f85p+0,
+    0x1.059b0d3158574p+0, 0x1.0706b29ddf6dep+0, 0x1.0874518759bc8p+0, 0x1.09e3ecac6f383p+0,
+    0x1.0b5586cf9890fp+0, 0x1.0cc922b7247f7p+0, 0x1.0e3ec32d3d1a2p+0, 0x1.0fb66affed31bp+0,
+    0x1.11301d0125b51p+0, 0x1.12abdc06c31ccp+0, 0x1.1429aaea92de0p+0, 0x1.15a98c8a58e51p+0,
+    0x1.172b83c7d517bp+0, 0x1.18af9388c8deap+0, 0x1.1a35beb6fcb75p+0, 0x1.1bbe084045cd4p+0,
+    0x1.1d4873168b9aap+0, 0x1.1ed5022fcd91dp+0, 0x1.2063b88628cd6p+0, 0x1.21f49917ddc96p+0,
+    0x1.2387a6e756238p+0, 0x1.251ce4fb2a63fp+0, 0x1.26b4565e27cddp+0, 0x1.284dfe1f56381p+0,
+    0x1.29e9df51fdee1p+0, 0x1.2b87fd0dad990p+0, 0x1.2d285a6e4030bp+0, 0x1.2ecafa93e2f56p+0,
+    0x1.306fe0a31b715p+0, 0x1.32170fc4cd831p+0, 0x1.33c08b26416ffp+0, 0x1.356c55f929ff1p+0,
+    0x1.371a7373aa9cbp+0, 0x1.38cae6d05d866p+0, 0x1.3a7db34e59ff7p+0, 0x1.3c32dc313a8e5p+0,
+    0x1.3dea64c123422p+0, 0x1.3fa4504ac801cp+0, 0x1.4160a21f72e2ap+0, 0x1.431f5d950a897p+0,
+    0x1.44e086061892dp+0, 0x1.46a41ed1d0057p+0, 0x1.486a2b5c13cd0p+0, 0x1.4a32af0d7d3dep+0,
+    0x1.4bfdad5362a27p+0, 0x1.4dcb299fddd0dp+0, 0x1.4f9b2769d2ca7p+0, 0x1.516daa2cf6642p+0,
+    0x1.5342b569d4f82p+0, 0x1.551a4ca5d920fp+0, 0x1.56f4736b527dap+0, 0x1.58d12d497c7fdp+0,
+    0x1.5ab07dd485429p+0, 0x1.5c9268a5946b7p+0, 0x1.5e76f15ad2148p+0, 0x1.605e1b976dc09p+0,
+    0x1.6247eb03a5585p+0, 0x1.6434634ccc320p+0, 0x1.6623882552225p+0, 0x1.68155d44ca973p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.6c012750bdabfp+0, 0x1.6dfb23c651a2fp+0, 0x1.6ff7df9519484p+0,
+    0x1.71f75e8ec5f74p+0, 0x1.73f9a48a58174p+0, 0x1.75feb564267c9p+0, 0x1.780694fde5d3fp+0,
+    0x1.7a11473eb0187p+0, 0x1.7c1ed0130c132p+0, 0x1.7e2f336cf4e62p+0, 0x1.80427543e1a12p+0,
+    0x1.82589994cce13p+0, 0x1.8471a4623c7adp+0, 0x1.868d99b4492edp+0, 0x1.88ac7d98a6699p+0,
+    0x1.8ace5422aa0dbp+0, 0x1.8cf3216b5448cp+0, 0x1.8f1ae99157736p+0, 0x1.9145b0b91ffc6p+0,
+    0x1.93737b0cdc5e5p+0, 0x1.95a44cbc8520fp+0, 0x1.97d829fde4e50p+0, 0x1.9a0f170ca07bap+0,
+    0x1.9c49182a3f090p+0, 0x1.9e86319e32323p+0, 0x1.a0c667b5de565p+0, 0x1.a309bec4a2d33p+0,
+    0x1.a5503b23e255dp+0, 0x1.a799e1330b358p+0, 0x1.a9e6b5579fdbfp+0, 0x1.ac36bbfd3f37ap+0,
+    0x1.ae89f995ad3adp+0, 0x1.b0e07298db666p+0, 0x1.b33a2b84f15fbp+0, 0x1.b59728de5593ap+0,
+    0x1.b7f76f2fb5e47p+0, 0x1.ba5b030a1064ap+0, 0x1.bcc1e904bc1d2p+0, 0x1.bf2c25bd71e09p+0,
+    0x1.c199bdd85529cp+0, 0x1.c40ab5fffd07ap+0, 0x1.c67f12e57d14bp+0, 0x1.c8f6d9406e7b5p+0,
+    0x1.cb720dcef9069p+0, 0x1.cdf0b555dc3fap+0, 0x1.d072d4a07897cp+0, 0x1.d2f87080d89f2p+0,
+    0x1.d5818dcfba487p+0, 0x1.d80e316c98398p+0, 0x1.da9e603db3285p+0, 0x1.dd321f301b460p+0,
+    0x1.dfc97337b9b5fp+0, 0x1.e264614f5a129p+0, 0x1.e502ee78b3ff6p+0, 0x1.e7a51fbc74c83p+0,
+    0x1.ea4afa2a490dap+0, 0x1.ecf482d8e67f1p+0, 0x1.efa1bee615a27p+0, 0x1.f252b376bba97p+0,
+    0x1.f50765b6e4540p+0, 0x1.f7bfdad9cbe14p+0, 0x1.fa7c1819e90d8p+0, 0x1.fd3c22b8f71f1p+0,
 };
 __device__ __forceinline__ void smp_table(double *tab) {
-  if (threadIdx.x < 32) tab[threadIdx.x] = SMP_POW[threadIdx.x];
+  if (threadIdx.x < 128) tab[threadIdx.x] = SMP_POW[threadIdx.x];
 }
-// exp(y), y <= 0, times 2^sh: 2^(k/32) from the table times a Taylor polynomial of what is left (at most ln 2 / 64: the
-// sixth term is below 2^-48).
+// exp(y) times 2^sh for y in [-690, 0]: 2^(k/128) from the table times a Taylor polynomial of what is left (at most
+// ln 2 / 256: the fifth term is below 2^-49), and a whole power of two in the exponent's bits (which stay in range for sh
+// of 0 and y >= -690, and for sh up to 45). k is read off a sum with 1.5 * 2^52 instead of converted.
 __device__ __forceinline__ double smp_exp(double y, int sh, const double *tab) {
-  const double k = rint(y * 46.16624130844683);
-  const double r = fma(k, -7.247021293269686e-19, fma(k, -0.02166084939249829, y));
-  const int n = (int)k;
-  double p = fma(r, 1.0 / 120.0, 1.0 / 24.0);
-  p = fma(r, p, 1.0 / 6.0);
+  const double big = 0x1.8p52, kb = fma(y, 184.6649652337873, big);
+  const int n = (int)(unsigned)__double_as_longlong(kb);
+  const double r = fma(kb - big, -0.0054152123481245725, y);
+  double p = fma(r, 1.0 / 24.0, 1.0 / 6.0);
   p = fma(r, p, 0.5);
   p = fma(r, p, 1.0);
   p = fma(r, p, 1.0);
-  return ldexp(tab[n & 31] * p, (n >> 5) + sh);
+  const long long v = __double_as_longlong(tab[n & 127] * p);
+  return __longlong_as_double(v + ((long long)((n >> 7) + sh) << 52));
 }
 __device__ __forceinline__ double smp_weight(const SmpRow &r, float x, const double *tab) {
   const double y = ((double)x - r.m) * r.inv_t;
@@ -231,32 +256,33 @@ __device__ __forceinline__ u64 smp_best(const SmpRow &r, int lo, int hi) {
   return best > -INFINITY ? smp_ord(best, at) : ~0ull;
 }
 
-// A key that at least k of the workgroup's keys (of parts of the row) are not above, and few more: bit by bit to the
-// largest value that fewer than k keys are below, or to one that a few more than k are.
-template <int NT, int N>
-__device__ __forceinline__ unsigned smp_kth(const unsigned (&mine)[N], int k, SmpRed &red) {
+// A key that at least k of n <= 64 N keys (of parts of the row; in LDS) are not above, and few more: bit by bit to the
+// largest value that fewer than k keys are below, or to one that a few more than k are. By one wave: a barrier for
+// every bit cost 5 us.
+template <int N>
+__device__ __forceinline__ unsigned smp_kth(const unsigned *key, int n, int k) {
+  __shared__ unsigned got;
   const int t = threadIdx.x;
-  unsigned lo = 0;
-  __syncthreads();  // (red's last readers)
-  for (int b = 31; b >= 0; b--) {
-    const unsigned x = lo | 1u << b;
-    int c = 0;
+  if (t < 64) {
+    unsigned mine[N], lo = 0;
 #pragma unroll
-    for (int i = 0; i < N; i++) c += __popcll(__ballot(mine[i] < x));
-    unsigned *cnt = (unsigned *)red.w + (b & 1) * (NT / 64);  // (two sets in turn: one barrier a bit)
-    if ((t & 63) == 0) cnt[t >> 6] = c;
-    __syncthreads();
-    c = 0;
+    for (int i = 0; i < N; i++) mine[i] = t + 64 * i < n ? key[t + 64 * i] : 0xffffffffu;
+#pragma unroll 1
+    for (int b = 31; b >= 0; b--) {
+      const unsigned x = lo | 1u << b;
+      int c = 0;
 #pragma unroll
-    for (int i = 0; i < NT / 64; i++) c += cnt[i];
-    if (c >= k && c <= k + k / 4 + 8) {
-      lo = x - 1;
-      break;
+      for (int i = 0; i < N; i++) c += __popcll(__ballot(mine[i] < x));
+      if (c >= k && c <= k + k / 4 + 8) {
+        lo = x - 1;
+        break;
+      }
+      if (c < k) lo = x;
     }
-    if (c < k) lo = x;
+    if (t == 0) got = lo;
   }
   __syncthreads();
-  return lo;
+  return got;
 }
 
 // ---- the list --------------------------------------------------------------------------------------
@@ -289,39 +315,67 @@ __device__ __forceinline__ int smp_find(const SmpRow &r, const SmpSet &s, const 
                                         u64 massk, u64 whole, u64 &total, SmpRed &red) {
   __shared__ int ip, im;
   const int t = threadIdx.x, n1 = c.n1;
-  int n2 = 2;
-  while (n2 < n) n2 *= 2;
-  for (int i = n + t; i < n2; i += NT) f.ord[i] = ~0ull;
+  u64 run = 0;
   if (t == 0) ip = n1, im = -1;
-  __syncthreads();
-  // bitonic, padded to a power of two; up to 128 entries by one wave, without barriers
-  if (n2 <= 128 ? t < 64 : true) {
-    const int step = n2 <= 128 ? 64 : NT;
-    for (int len = 2; len <= n2; len *= 2)
+  if (n <= 256) {
+    // every entry counts those before it and their masses; NT / n2 threads share an entry's
+    int n2 = 64;
+    while (n2 < n) n2 *= 2;
+    const int i = t % n2, part = t / n2, parts = NT / n2;
+    u64 *mass = f.ord + SMP_LIST / 2, *sum = f.run + SMP_LIST / 2, *at = sum + 256;
+    __syncthreads();
+    const u64 o = i < n ? f.ord[i] : ~0ull;
+    if (part == 0) {
+      mass[i] = i < n ? smp_mass(r, smp_value((uint32_t)(o >> 32)), tab) : 0;
+      sum[i] = at[i] = 0;
+      if (i >= n) f.ord[i] = ~0ull;
+    }
+    __syncthreads();
+    u64 v = 0;
+    int c = 0;
+    for (int j = part; j < n; j += parts) {
+      const bool in = f.ord[j] <= o;
+      v += in ? mass[j] : 0;
+      c += in;
+    }
+    if (i < n) {
+      atomicAdd(&sum[i], v);
+      atomicAdd(&at[i], (u64)c);
+    }
+    __syncthreads();
+    if (part == 0 && i < n) {
+      const int to = (int)at[i] - 1;
+      f.ord[to] = o;
+      f.run[to] = sum[i];
+      if (to < n1 && (!s.by_m || smp_weight(r, smp_value((uint32_t)(o >> 32)), tab) >= s.min_p)) atomicMax(&im, to);
+    }
+    __syncthreads();
+    run = f.run[n - 1];
+  } else {
+    int n2 = 512;
+    while (n2 < n) n2 *= 2;
+    for (int i = n + t; i < n2; i += NT) f.ord[i] = ~0ull;
+    __syncthreads();
+    for (int len = 2; len <= n2; len *= 2)  // bitonic, padded to a power of two
       for (int d = len / 2; d; d /= 2) {
-        for (int i = t; i < n2 / 2; i += step) {
+        for (int i = t; i < n2 / 2; i += NT) {
           const int x = 2 * i - (i & (d - 1)), y = x + d;
           const u64 p = f.ord[x], q = f.ord[y];
           if ((p > q) == !(x & len)) f.ord[x] = q, f.ord[y] = p;
         }
-        if (n2 <= 128)
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
-        else
-          __syncthreads();
+        __syncthreads();
       }
+    for (int i0 = 0; i0 < n; i0 += NT) {
+      const int i = i0 + t;
+      const float x = i < n ? smp_value((uint32_t)(f.ord[i] >> 32)) : -INFINITY;
+      u64 all;
+      const u64 up = run + smp_scan<NT>(smp_mass(r, x, tab), all, red);
+      if (i < n) f.run[i] = up;
+      if (i < n1 && (!s.by_m || smp_weight(r, x, tab) >= s.min_p)) atomicMax(&im, i);
+      run += all;
+    }
+    __syncthreads();
   }
-  __syncthreads();
-  u64 run = 0;
-  for (int i0 = 0; i0 < n; i0 += NT) {
-    const int i = i0 + t;
-    const float x = i < n ? smp_value((uint32_t)(f.ord[i] >> 32)) : -INFINITY;
-    u64 all;
-    const u64 up = run + smp_scan<NT>(smp_mass(r, x, tab), all, red);
-    if (i < n) f.run[i] = up;
-    if (i < n1 && (!s.by_m || smp_weight(r, x, tab) >= s.min_p)) atomicMax(&im, i);
-    run += all;
-  }
-  __syncthreads();
   int last = n1 - 1;
   u64 left = whole == ~0ull ? run : whole;  // the mass that top-k leaves
   if (s.by_k && !c.beyond) {
@@ -387,12 +441,17 @@ __device__ __forceinline__ int smp_draw(const SmpRow &r, const double *tab, int 
     u64 up = run + smp_scan<NT>(sum, all, red);
     if ((double)up > left && !((double)(up - sum) > left)) {  // this thread's (one's alone)
       up -= sum;
-      int at = i;
+      int at = INT32_MAX;
 #pragma unroll 1
-      for (; at < hi; at++) {
-        const float x = r.at(at);
-        if (smp_ord(x, at) <= thr) up += smp_mass(r, x, tab);
-        if ((double)up > left) break;
+      for (int k = 0; k < RUN && at == INT32_MAX; k += 8) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = r.at(min(i + k + e, hi - 1));
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          if (i + k + e < hi && smp_ord(x[e], i + k + e) <= thr) up += smp_mass(r, x[e], tab);
+          if (at == INT32_MAX && (double)up > left) at = i + k + e;
+        }
       }
       found = at;
     }
@@ -563,7 +622,7 @@ __device__ __forceinline__ void smp_probs(const SampleArgs &a, const SmpRow &r, 
 __global__ __launch_bounds__(SMP_ONE) void k_sample_one(SampleArgs a, SmpUnits un) {
   constexpr int NT = SMP_ONE;
   __shared__ SmpLds lds;
-  __shared__ double tab[32];
+  __shared__ double tab[128];
   __shared__ SmpRed red;
   __shared__ unsigned here;
   const int row = blockIdx.x, t = threadIdx.x, V = a.V;
@@ -592,9 +651,12 @@ __global__ __launch_bounds__(SMP_ONE) void k_sample_one(SampleArgs a, SmpUnits u
       n = here;
     };
     bool slow = false, drawn = false;
-    if (s.by_k && s.k <= SMP_KMAX) {
-      const unsigned keys[1] = {(unsigned)(mine >> 32)};
-      const unsigned most = smp_kth<NT>(keys, s.k, red);
+    if (s.by_k && s.k <= NT / 2 * 3 / 4) {  // (more parts than that make longer lists)
+      unsigned key = (unsigned)(mine >> 32), *keys = (unsigned *)lds.f.run;
+      key = min(key, (unsigned)__shfl_xor((int)key, 1, 64));
+      if (t % 2 == 0) keys[t / 2] = key;
+      __syncthreads();
+      const unsigned most = smp_kth<NT / 128>(keys, NT / 2, s.k);
       gather([&](float x) { return smp_key(x) <= most; });
       slow = n > SMP_LIST;
       if (!slow) {
@@ -703,8 +765,9 @@ __global__ __launch_bounds__(SMP_NT) void k_sample_top(SampleArgs a, SmpWork k) 
   unsigned key = (unsigned)(mine >> 32);
   key = min(key, (unsigned)__shfl_xor((int)key, 1, 64));
   key = min(key, (unsigned)__shfl_xor((int)key, 2, 64));
+  key = min(key, (unsigned)__shfl_xor((int)key, 4, 64));
   const long chunk = (long)row * k.G + g;
-  if (t % 4 == 0) k.part[chunk * SMP_PARTS + t / 4] = key;
+  if (t % 8 == 0) k.part[chunk * SMP_PARTS + t / 8] = key;
   const u64 top = smp_least<SMP_NT>(mine, red);
   if (t == 0) {
     k.top[chunk] = top;
@@ -782,18 +845,17 @@ __device__ __forceinline__ bool smp_gather(const SmpRow &r, const SmpWork &k, Sm
 }
 
 __global__ __launch_bounds__(SMP_NT) void k_sample_cut(SampleArgs a, SmpWork k) {
-  constexpr int NT = SMP_NT, NP = SMP_GMAX * SMP_PARTS / NT;
+  constexpr int NT = SMP_NT;
   __shared__ SmpLds lds;
-  __shared__ double tab[32];
+  __shared__ double tab[128];
   __shared__ u64 cert[SMP_GMAX];
   __shared__ SmpRed red;
   const int g = blockIdx.x, row = blockIdx.y, gr = k.row0 + row, t = threadIdx.x, G = k.G, np = G * SMP_PARTS;
   const int lo = min(a.V, g * k.len), hi = min(a.V, lo + k.len);
   SmpRow r = smp_row(a, gr);
   const u64 top1 = t < G ? k.top[(long)row * G + t] : ~0ull;
-  unsigned parts[NP];
-#pragma unroll
-  for (int i = 0; i < NP; i++) parts[i] = t + i * NT < np ? k.part[(long)row * np + t + i * NT] : 0xffffffffu;
+  unsigned *keys = (unsigned *)lds.f.run;
+  for (int i = t; i < np; i += NT) keys[i] = k.part[(long)row * np + i];
   const SmpSet s = smp_set(a, gr);
   smp_table(tab);
   const u64 top = smp_least<NT>(top1, red);
@@ -809,8 +871,8 @@ __global__ __launch_bounds__(SMP_NT) void k_sample_cut(SampleArgs a, SmpWork k) 
   }
   r.m = m;
   r.inv_t = 1.0 / s.t;
-  if (s.by_k && s.k <= min(SMP_KMAX, np)) {
-    const unsigned most = smp_kth<NT>(parts, s.k, red);
+  if (s.by_k && s.k <= np * 3 / 4) {
+    const unsigned most = smp_kth<SMP_GMAX * SMP_PARTS / 64>(keys, np, s.k);
     unsigned n;
     if (!smp_gather(r, k, st, row, lo, hi, lds.f, n, [&](float x) { return smp_key(x) <= most; }, [] {})) return;
     if (n <= SMP_LIST) {
@@ -877,7 +939,7 @@ __global__ __launch_bounds__(SMP_NT) void k_sample_cut(SampleArgs a, SmpWork k) 
 __global__ __launch_bounds__(SMP_NT) void k_sample_list(SampleArgs a, SmpWork k) {
   constexpr int NT = SMP_NT;
   __shared__ SmpLds lds;
-  __shared__ double tab[32];
+  __shared__ double tab[128];
   __shared__ u64 chunk[SMP_GMAX];
   __shared__ SmpRed red;
   const int g = blockIdx.x, row = blockIdx.y, gr = k.row0 + row, t = threadIdx.x, G = k.G;
@@ -933,7 +995,7 @@ __global__ __launch_bounds__(SMP_NT) void k_sample_list(SampleArgs a, SmpWork k)
 
 __global__ __launch_bounds__(SMP_NT) void k_sample_probs(SampleArgs a, SmpWork k) {
   constexpr int NT = SMP_NT;
-  __shared__ double tab[32];
+  __shared__ double tab[128];
   __shared__ SmpRed red;
   const int g = blockIdx.x, row = blockIdx.y, gr = k.row0 + row, t = threadIdx.x;
   const int lo = min(a.V, g * k.len), hi = min(a.V, lo + k.len);
