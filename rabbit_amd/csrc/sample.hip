@@ -30,7 +30,7 @@ namespace rbt {
 typedef unsigned long long u64;
 
 constexpr int SMP_NT = 256, SMP_ONE = 1024;  // threads of a chunk's workgroup, of a row's
-constexpr int SMP_NB = 512, SMP_LIST = 2048, SMP_GMAX = 32, SMP_PARTS = 32;
+constexpr int SMP_NB = 512, SMP_LIST = 2048, SMP_GMAX = 32, SMP_PARTS = 64;
 
 // A logit's bits, larger logits first; NaN counts as -inf, and -0 as 0.
 __device__ __forceinline__ uint32_t smp_key(float x) {
@@ -140,6 +140,10 @@ __device__ __forceinline__ double smp_weight(const SmpRow &r, float x, const dou
 __device__ __forceinline__ u64 smp_mass(const SmpRow &r, float x, const double *tab) {
   const double y = ((double)x - r.m) * r.inv_t;
   return y > -34.0 ? (u64)__double_as_longlong(smp_exp(y, r.S, tab) + 0x1p52) & 0xfffffffffffffull : 0;
+}
+
+__device__ __forceinline__ u64 smp_units(const SmpRow &r, double w) {
+  return (u64)__double_as_longlong(ldexp(w, r.S) + 0x1p52) & 0xfffffffffffffull;
 }
 
 // The bucket of a logit: 24ths of (m - x) / t, never falling along the order; the last holds all from 21.3 on.
@@ -270,9 +274,10 @@ __device__ __forceinline__ unsigned smp_kth(const unsigned *key, int n, int k) {
 #pragma unroll 1
     for (int b = 31; b >= 0; b--) {
       const unsigned x = lo | 1u << b;
-      int c = 0;
+      float f = 0.0f;  // (whole numbers)
 #pragma unroll
-      for (int i = 0; i < N; i++) c += __popcll(__ballot(mine[i] < x));
+      for (int i = 0; i < N; i++) f += mine[i] < x ? 1.0f : 0.0f;
+      const int c = (int)__int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(rbt_group_sum<64>(f))));
       if (c >= k && c <= k + k / 4 + 8) {
         lo = x - 1;
         break;
@@ -315,63 +320,75 @@ __device__ __forceinline__ int smp_find(const SmpRow &r, const SmpSet &s, const 
                                         u64 massk, u64 whole, u64 &total, SmpRed &red) {
   __shared__ int ip, im;
   const int t = threadIdx.x, n1 = c.n1;
+  int n2 = 64;
+  while (n2 < n) n2 *= 2;
+#pragma unroll 1
+  for (int i = n + t; i < n2; i += NT) f.ord[i] = ~0ull;
+  if (t == 0) ip = n1, im = n1 - 1;
+  __syncthreads();
   u64 run = 0;
-  if (t == 0) ip = n1, im = -1;
-  if (n <= 256) {
+  if (n2 <= 256) {
     // every entry counts those before it and their masses; NT / n2 threads share an entry's
-    int n2 = 64;
-    while (n2 < n) n2 *= 2;
-    const int i = t % n2, part = t / n2, parts = NT / n2;
+    const int i = t % n2;
     u64 *mass = f.ord + SMP_LIST / 2, *sum = f.run + SMP_LIST / 2, *at = sum + 256;
-    __syncthreads();
-    const u64 o = i < n ? f.ord[i] : ~0ull;
-    if (part == 0) {
-      mass[i] = i < n ? smp_mass(r, smp_value((uint32_t)(o >> 32)), tab) : 0;
+    const u64 o = f.ord[i];
+    const double w = smp_weight(r, i < n ? smp_value((uint32_t)(o >> 32)) : -INFINITY, tab);
+    if (t < n2) {
+      mass[i] = smp_units(r, w);
       sum[i] = at[i] = 0;
-      if (i >= n) f.ord[i] = ~0ull;
     }
     __syncthreads();
-    u64 v = 0;
-    int c = 0;
-    for (int j = part; j < n; j += parts) {
+    u64 v = 0, before = 0;
+#pragma unroll 4
+    for (int j = t / n2; j < n; j += NT / n2) {
       const bool in = f.ord[j] <= o;
       v += in ? mass[j] : 0;
-      c += in;
+      before += in;
     }
-    if (i < n) {
+    if (NT > n2) {
       atomicAdd(&sum[i], v);
-      atomicAdd(&at[i], (u64)c);
+      atomicAdd(&at[i], before);
+      __syncthreads();
+      v = sum[i];
+      before = at[i];
     }
     __syncthreads();
-    if (part == 0 && i < n) {
-      const int to = (int)at[i] - 1;
+    if (t < n) {
+      const int to = (int)before - 1;
       f.ord[to] = o;
-      f.run[to] = sum[i];
-      if (to < n1 && (!s.by_m || smp_weight(r, smp_value((uint32_t)(o >> 32)), tab) >= s.min_p)) atomicMax(&im, to);
+      f.run[to] = v;
+      if (to < n1 && !(w >= s.min_p)) atomicMin(&im, to - 1);
     }
     __syncthreads();
     run = f.run[n - 1];
   } else {
-    int n2 = 512;
-    while (n2 < n) n2 *= 2;
-    for (int i = n + t; i < n2; i += NT) f.ord[i] = ~0ull;
-    __syncthreads();
-    for (int len = 2; len <= n2; len *= 2)  // bitonic, padded to a power of two
+    // bitonic, padded to a power of two; steps of up to 64 stay within a wave's 128 entries
+#pragma unroll 1
+    for (int len = 2; len <= n2; len *= 2)
+#pragma unroll 1
       for (int d = len / 2; d; d /= 2) {
+#pragma unroll 1
         for (int i = t; i < n2 / 2; i += NT) {
           const int x = 2 * i - (i & (d - 1)), y = x + d;
           const u64 p = f.ord[x], q = f.ord[y];
           if ((p > q) == !(x & len)) f.ord[x] = q, f.ord[y] = p;
         }
-        __syncthreads();
+        if (d > 64 || (d == 1 && len > 64))
+          __syncthreads();
+        else
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
       }
+    __syncthreads();
+#pragma unroll 1
     for (int i0 = 0; i0 < n; i0 += NT) {
       const int i = i0 + t;
-      const float x = i < n ? smp_value((uint32_t)(f.ord[i] >> 32)) : -INFINITY;
+      const double w = smp_weight(r, i < n ? smp_value((uint32_t)(f.ord[i] >> 32)) : -INFINITY, tab);
       u64 all;
-      const u64 up = run + smp_scan<NT>(smp_mass(r, x, tab), all, red);
+      const u64 up = run + smp_scan<NT>(smp_units(r, w), all, red);
       if (i < n) f.run[i] = up;
-      if (i < n1 && (!s.by_m || smp_weight(r, x, tab) >= s.min_p)) atomicMax(&im, i);
+      // (weights fall along the order: the first that is too light)
+      if (i < n1 && !(w >= s.min_p) && (i == 0 || smp_value((uint32_t)(f.ord[i] >> 32)) != smp_value((uint32_t)(f.ord[i - 1] >> 32))))
+        atomicMin(&im, i - 1);
       run += all;
     }
     __syncthreads();
@@ -386,8 +403,9 @@ __device__ __forceinline__ int smp_find(const SmpRow &r, const SmpSet &s, const 
   }
   if (s.by_p) {
     const double target = s.top_p * (double)left;
-    for (int i = t; i < n1; i += NT)
-      if ((double)(mass0 + f.run[i]) >= target) atomicMin(&ip, i);
+#pragma unroll 1
+    for (int i = t; i < n1; i += NT)  // (the first that reaches it: one thread's)
+      if ((double)(mass0 + f.run[i]) >= target && (i == 0 || !((double)(mass0 + f.run[i - 1]) >= target))) ip = i;
     __syncthreads();
     last = min(last, ip);
   }
@@ -406,6 +424,7 @@ __device__ __forceinline__ int smp_draw_list(const SmpFind &f, int last, double 
   for (int i = t; i <= last; i += NT) {
     const unsigned at = (unsigned)f.ord[i];
     u64 run = 0, before = 0;
+#pragma unroll 2
     for (int j = 0; j <= last; j++) {
       const u64 up = f.run[j];
       if ((unsigned)f.ord[j] <= at) run += up - before;
@@ -417,49 +436,64 @@ __device__ __forceinline__ int smp_draw_list(const SmpFind &f, int last, double 
   return first == ~0ull ? -1 : (int)first;
 }
 
-// The least index in [lo, hi) at which the running mass of entries up to thr passes `left`: a thread sums 32 in a row,
-// then the one in whose the running mass passes looks for the entry.
+// The least index in [lo, hi) at which the running mass of entries up to thr passes `left`: every wave sums a part of it,
+// then the workgroup looks through the part where it passes, four entries a thread.
 template <int NT>
 __device__ __forceinline__ int smp_draw(const SmpRow &r, const double *tab, int lo, int hi, u64 thr, double left, SmpRed &red) {
   __shared__ int found;
-  constexpr int RUN = 32;
-  const int t = threadIdx.x;
+  constexpr int W = NT / 64, UN = 8;
+  const int t = threadIdx.x, w = t >> 6, lane = t & 63, part = (hi - lo + W - 1) / W;
+  auto kept = [&](float x, int i) { return smp_ord(x, i) <= thr ? smp_mass(r, x, tab) : 0; };
+  u64 sum = 0;
+  const int end = min(hi, lo + (w + 1) * part);
+#pragma unroll 1
+  for (int i = lo + w * part + lane; i < end; i += 64 * UN) {
+    float x[UN];
+#pragma unroll
+    for (int e = 0; e < UN; e++) x[e] = r.at(min(i + 64 * e, hi - 1));
+#pragma unroll
+    for (int e = 0; e < UN; e++)
+      if (i + 64 * e < end) sum += kept(x[e], i + 64 * e);
+  }
+  sum = smp_wave_sum(sum);
+  __syncthreads();
+  if (lane == 0) red.w[w] = sum;
   if (t == 0) found = INT32_MAX;
+  __syncthreads();
   u64 run = 0;
-  for (int i0 = lo; i0 < hi; i0 += RUN * NT) {
-    const int i = i0 + RUN * t;
-    u64 sum = 0, all;
+  int q = -1;
+#pragma unroll
+  for (int i = 0; i < W; i++) {
+    if (q < 0 && (double)(run + red.w[i]) > left) q = i;
+    if (q < 0) run += red.w[i];
+  }
+  if (q < 0) return -1;  // (not reached: u below 1 times the whole is below the whole)
+  const int e1 = min(hi, lo + (q + 1) * part);
 #pragma unroll 1
-    for (int k = 0; k < RUN; k += 8) {
-      float x[8];
+  for (int i0 = lo + q * part; i0 < e1; i0 += 4 * NT) {
+    const int i = i0 + 4 * t;
+    u64 m[4], all;
 #pragma unroll
-      for (int e = 0; e < 8; e++) x[e] = r.at(min(i + k + e, hi - 1));
-#pragma unroll
-      for (int e = 0; e < 8; e++)
-        if (i + k + e < hi && smp_ord(x[e], i + k + e) <= thr) sum += smp_mass(r, x[e], tab);
+    for (int e = 0; e < 4; e++) {
+      const float x = r.at(min(i + e, hi - 1));
+      m[e] = i + e < e1 ? kept(x, i + e) : 0;
     }
-    u64 up = run + smp_scan<NT>(sum, all, red);
-    if ((double)up > left && !((double)(up - sum) > left)) {  // this thread's (one's alone)
-      up -= sum;
-      int at = INT32_MAX;
-#pragma unroll 1
-      for (int k = 0; k < RUN && at == INT32_MAX; k += 8) {
-        float x[8];
+    const u64 mine = (m[0] + m[1]) + (m[2] + m[3]), up = run + smp_scan<NT>(mine, all, red);
+    if ((double)up > left && !((double)(up - mine) > left)) {  // this thread's (one's alone)
+      u64 at = up - mine;
+      int e = 0;
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = r.at(min(i + k + e, hi - 1));
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          if (i + k + e < hi && smp_ord(x[e], i + k + e) <= thr) up += smp_mass(r, x[e], tab);
-          if (at == INT32_MAX && (double)up > left) at = i + k + e;
-        }
+      for (; e < 3; e++) {
+        at += m[e];
+        if ((double)at > left) break;
       }
-      found = at;
+      found = i + e;
     }
     run += all;
     __syncthreads();
     if (found != INT32_MAX) return found;
   }
-  return -1;  // (not reached: u below 1 times the whole is below the whole)
+  return -1;
 }
 
 // ---- digit by digit --------------------------------------------------------------------------------
@@ -572,9 +606,10 @@ __device__ __forceinline__ SmpCut smp_cut(const SmpSet &s, int V, const SmpUnits
   const int kb = kb_s;
   if (s.by_p && in) {  // of the mass that top-k leaves
     const double whole0 = s.by_k ? low(kb) : ldexp((double)all, -un.sh), whole1 = s.by_k ? high(kb + 1) : whole0;
-    for (int e = 0; e < 2; e++) {
-      if (high(2 * t + e + 1) >= s.top_p * whole0) atomicMin(&p0_s, 2 * t + e);
-      if (low(2 * t + e + 1) >= s.top_p * whole1) atomicMin(&p1_s, 2 * t + e);
+    for (int e = 0; e < 2; e++) {  // (the first of those that reach it: one thread's)
+      const int b = 2 * t + e;
+      if (high(b + 1) >= s.top_p * whole0 && (b == 0 || !(high(b) >= s.top_p * whole0))) p0_s = b;
+      if (low(b + 1) >= s.top_p * whole1 && (b == 0 || !(low(b) >= s.top_p * whole1))) p1_s = b;
     }
   }
   __syncthreads();
@@ -765,9 +800,8 @@ __global__ __launch_bounds__(SMP_NT) void k_sample_top(SampleArgs a, SmpWork k) 
   unsigned key = (unsigned)(mine >> 32);
   key = min(key, (unsigned)__shfl_xor((int)key, 1, 64));
   key = min(key, (unsigned)__shfl_xor((int)key, 2, 64));
-  key = min(key, (unsigned)__shfl_xor((int)key, 4, 64));
   const long chunk = (long)row * k.G + g;
-  if (t % 8 == 0) k.part[chunk * SMP_PARTS + t / 8] = key;
+  if (t % 4 == 0) k.part[chunk * SMP_PARTS + t / 4] = key;
   const u64 top = smp_least<SMP_NT>(mine, red);
   if (t == 0) {
     k.top[chunk] = top;
@@ -871,7 +905,7 @@ __global__ __launch_bounds__(SMP_NT) void k_sample_cut(SampleArgs a, SmpWork k) 
   }
   r.m = m;
   r.inv_t = 1.0 / s.t;
-  if (s.by_k && s.k <= np * 3 / 4) {
+  if (s.by_k && s.k <= min(np * 3 / 4, SMP_LIST / 4)) {
     const unsigned most = smp_kth<SMP_GMAX * SMP_PARTS / 64>(keys, np, s.k);
     unsigned n;
     if (!smp_gather(r, k, st, row, lo, hi, lds.f, n, [&](float x) { return smp_key(x) <= most; }, [] {})) return;
