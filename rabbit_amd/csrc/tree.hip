@@ -395,9 +395,9 @@ __device__ __forceinline__ bool tree_group(const TreeArgs &a, int rt, int &g, in
   return false;
 }
 
+// Workgroup (bx, by, bz) of a pass.
 template <int HD, int KV, int KW>
-__global__ __launch_bounds__(tree_wide(KV, KW) ? 512 : 256, tree_wide(KV, KW) ? 1 : 2)
-void k_tree(TreeArgs a) {
+__device__ __forceinline__ void tree_pass(const TreeArgs &a, int bx, int by, int bz) {
   using TT = TreeTile<HD, KV, KW>;
   constexpr bool I8 = KV == KV_I8;
   constexpr bool B16 = KV != KV_F32, PARTS = tree_parts(KV);  // values' tiles of 16 entries; split rows
@@ -412,9 +412,9 @@ void k_tree(TreeArgs a) {
 
   // workgroup -> (row tile, piece, KV head, sequence); with several row tiles the workgroups that share keys are
   // consecutive ones of an XCD (id % 8)
-  int piece = blockIdx.x, rt = 0, kv = blockIdx.y, b = blockIdx.z;
+  int piece = bx, rt = 0, kv = by, b = bz;
   if (a.tiles > 1) {
-    const unsigned id = blockIdx.x, g = id / 8 / a.tiles * 8 + id % 8, KB = a.K * a.seqs;
+    const unsigned id = bx, g = id / 8 / a.tiles * 8 + id % 8, KB = a.K * a.seqs;
     if (g >= a.pieces * KB) return;
     rt = id / 8 % a.tiles;
     piece = g / KB;
@@ -1074,6 +1074,29 @@ void k_tree(TreeArgs a) {
   }
 }
 
+template <int HD, int KV, int KW>
+__global__ __launch_bounds__(tree_wide(KV, KW) ? 512 : 256, tree_wide(KV, KW) ? 1 : 2)
+void k_tree(TreeArgs a) {
+  tree_pass<HD, KV, KW>(a, blockIdx.x, blockIdx.y, blockIdx.z);
+}
+
+// The pass over the prefixes (its first np workgroups) and the sequences' own in one launch: many rows against few, so
+// that the second's trips to memory run beside the first's products where the chip has room for both (8 users behind 1500
+// rows 36.7 -> 27.8 us, 11 trees of five behind 1001 f32 rows 34.6 -> 31.8).
+template <int HD, int KVP, int KV, int KW>
+__global__ __launch_bounds__(512, 1) void k_tree_both(TreeArgs p, TreeArgs a, int np) {
+  const int id = blockIdx.x;
+  if (id < np) {
+    if (p.tiles > 1)
+      tree_pass<HD, KVP, 1>(p, id, 0, 0);
+    else
+      tree_pass<HD, KVP, 1>(p, id % p.pieces, id / p.pieces, 0);
+  } else {
+    const int i = id - np, r = i / a.pieces;
+    tree_pass<HD, KV, KW>(a, i - r * a.pieces, r % a.K, r / a.K);
+  }
+}
+
 // The pieces of 16 rows joined. WP = 1: a workgroup takes 64 entries of the rows, 16 per wave; WP = 4: 16 entries, its
 // waves take every fourth piece each and their sums are added in order. Lane by lane as the partial sums lie.
 template <int WP>
@@ -1438,9 +1461,36 @@ void tree_prefix_args(const TreeArgs &a, TreeArgs &p) {
   p.joined = 1;
 }
 
+// False: two launches are better. (8-bit rows of 192 or 256 at more workgroups than CUs: the prefixes' stages of 128
+// keys leave a CU one workgroup, where a pass over own rows by itself has two. 32 users behind 8000 int8 rows 80 us,
+// 90 in one launch; with bf16 rows of 256, one workgroup a CU in both, 64 behind 4096 86.5 and 84.2, 8 behind
+// 6000 43.8 and 36.7; with rows of 128, 64 behind 4096 54.2 and 49.2, 32 behind 8000 int8 ones 56.2 and 55.5.)
+template <int HD, int KVP, int KV, int KW>
+static bool run_tree_both(const Ctx &c, const TreeArgs &p, const TreeArgs &a) {
+  constexpr int lp = TreeTile<HD, KVP, 1>::LDS, la = TreeTile<HD, KV, KW>::LDS, lds = lp > la ? lp : la;
+  const long groups = (long)p.pieces * p.K, np = p.tiles > 1 ? (groups + 7) / 8 * 8 * p.tiles : groups;
+  const long own = (long)a.pieces * a.K * a.B;
+  if (np + own >= 1L << 22 || (KV == KV_I8 && HD > 128 && np + own > c.num_cu)) return false;
+  const int threads = std::max(tree_threads(p), tree_threads(a));
+  launch_ks(c, k_tree_both<HD, KVP, KV, KW>, dim3((unsigned)(np + own)), dim3(threads), (unsigned)lds, p, a, (int)np);
+  return true;
+}
+template <int HD>
+static bool run_tree_both_hd(const Ctx &c, const TreeArgs &p, const TreeArgs &a) {
+  // (where the prefixes have three row tiles or more, a sequence one, or two in int8 and f32)
+  if (p.kw != 1 || p.four || a.kw != (a.kv16 ? 4 : 2) || a.tiles != 1) return false;
+  return a.kv8    ? run_tree_both<HD, KV_I8, KV_I8, 2>(c, p, a)
+         : a.kv16 ? run_tree_both<HD, KV_BF16, KV_BF16, 4>(c, p, a)
+                  : run_tree_both<HD, KV_PARTS, KV_F32, 2>(c, p, a);
+}
+
 hipError_t launch_prefix(const Ctx &c, const TreeArgs &a, const TreeArgs &p) {
-  hipError_t e = run_tree_pass(c, p);
-  if (e == hipSuccess) e = run_tree_pass(c, a);
+  const bool one = a.hd == 64    ? run_tree_both_hd<64>(c, p, a)
+                   : a.hd == 128 ? run_tree_both_hd<128>(c, p, a)
+                   : a.hd == 192 ? run_tree_both_hd<192>(c, p, a)
+                                 : run_tree_both_hd<256>(c, p, a);
+  hipError_t e = one ? hipGetLastError() : run_tree_pass(c, p);
+  if (!one && e == hipSuccess) e = run_tree_pass(c, a);
   if (e != hipSuccess) return e;
   const int tiles = (a.T * a.R + 15) / 16;
   launch_k(c, k_prefix_join, dim3(tiles * (a.hd / 64), a.K, a.B), dim3(256), a, p);
