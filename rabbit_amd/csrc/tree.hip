@@ -582,9 +582,9 @@ __device__ __forceinline__ void tree_pass(const TreeArgs &a, int bx, int by, int
     if (__builtin_amdgcn_ldexpf(most, 23 - e) > TREE_TOP) e++;
     e = max(e, -100);
     const bool whole = top < 0x7f800000u;
-    // (the scale's sign goes to the query; a scale of 0 is one that makes nothing of any score)
-    qs = whole ? fmaxf(fabsf(a.scale), 1e-30f) * 1.44269504088896341f * __builtin_amdgcn_ldexpf(1.0f, e - 23) : __uint_as_float(0x7fc00000u);
-    const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
+    // (the scale's sign goes to the query, zeros for a scale of 0; the factor stays above 0 for hidden keys' sake)
+    qs = whole ? fmaxf(fabsf(a.scale) * 1.44269504088896341f * __builtin_amdgcn_ldexpf(1.0f, e - 23), 0x1p-126f) : __uint_as_float(0x7fc00000u);
+    const float sign = a.scale < 0.0f ? -1.0f : a.scale > 0.0f ? 1.0f : 0.0f;
 #pragma unroll
     for (int s = 0; s < HD / 64; s++)
 #pragma unroll
@@ -805,11 +805,21 @@ __device__ __forceinline__ void tree_pass(const TreeArgs &a, int bx, int by, int
       m = mt;
     }
     const float ms = m == -INFINITY ? 0.0f : m;
+    // (8-bit rows: m is a rounded product and the fused difference from it is not. Past 2^20 they would be apart by more than
+    // 2^-4, by anything at scores of 2^32: the products there are rounded first)
+    float step = qs;
+    if (I8 && __any(fabsf(ms) > 0x1p20f)) {
+#pragma unroll
+      for (int x = 0; x < NT; x++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) sc[x][i] *= qs;
+      step = 1.0f;
+    }
 #pragma unroll
     for (int x = 0; x < NT; x++)
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        sc[x][i] = __builtin_amdgcn_exp2f(I8 ? fmaf(sc[x][i], qs, -ms) : sc[x][i] - ms);
+        sc[x][i] = __builtin_amdgcn_exp2f(I8 ? fmaf(sc[x][i], step, -ms) : sc[x][i] - ms);
         l += sc[x][i];
       }
 
