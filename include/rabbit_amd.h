@@ -525,10 +525,11 @@ int rbt_kv_dequant_d(rbt_ctx *ctx, const rbt_kv_quant_desc *desc, size_t n_seq, 
  *  - parent NULL: chains (node i hangs from node i - 1).
  *  - n_prefix 0: prefix, prefix_len and prefix_first are not used.
  * Everything else as rbt_gqa_tree_d; entries 16-byte aligned, scales 4-byte. Over 8-bit rows q and the
- * probabilities are taken to 2^-22 of their row's largest (of 64 or 128 keys at a time), products and
+ * probabilities are taken to 2^-22 of their row's largest (of 32 or 128 keys at a time), products and
  * their sums are exact in whole numbers, and sums over all keys f32. n_prefix <= 1024 and
  * n_seq * max_nodes * (query heads per KV head) <= 2^20 (RBT_E_UNSUPPORTED). A row with scale NaN
- * makes every entry NaN of the nodes that see it, and of no other. */
+ * makes every entry NaN of the nodes that see it, and of no other. Scales are as rbt_kv_quant_d writes them, not
+ * negative. */
 typedef struct {
     size_t n_heads, n_kv_heads, head_dim;
     float attn_scale;

@@ -7,6 +7,10 @@
 //                cores, with the running maximum and sum; writes the output, or the piece's partial sums
 //   k_tree_join  the pieces' partial sums joined
 //   k_tree_any   any head dim: fp32 multiply-adds, one workgroup per query head and node
+// Sequences behind shared prefixes (rbt_gqa_prefix_d) take two passes: over each prefix once, its sequences' rows in tiles
+// as one long sequence's, and over the sequences' own rows; both leave partial sums.
+//   k_tree_both    the two passes in one launch, where that is faster
+//   k_prefix_join  a sequence's own pieces and its prefix's joined
 //
 // Bounds and times (64 query heads over 4 KV heads of 256, one MI355X):
 //   64 nodes over 32749 bf16 rows: 292-314 us, of them 280-290 in k_tree: 412 GFLOP of bf16 products, 1.4 PFLOP/s (a
@@ -18,6 +22,11 @@
 //     bf16 of 128, 88 and 189 for f32: the caches at 4.3 to 4.9 TB/s.
 //   one node over 32768 bf16 rows: 35 us, k_tree 26 (134 MB: 5.1 TB/s); over 513 rows: 13.3 us, two launches of one
 //     trip to memory each; five nodes over 4096 f32 rows: 32 us.
+//   64 users, 512 own bf16 rows each, behind 8192 shared: 119-126 us (the products of three bf16 parts at the rate of a large
+//     library product 94); 8 with 300 own behind 1500: 27 us.
+//   32 users, 1000 own int8 rows each, behind 32749 shared: 166-172 us, 121-128 in the pass over the prefix (its int8 products
+//     at the rate of a large library product 118: vector work 66% of the cycles, matrix cores 43%, one after the other);
+//     16 with up to 8192 own rows: 78 us (bytes at a large copy's rate 45).
 #include "rbt_device.h"
 #include "rbt_internal.h"
 
