@@ -9,7 +9,7 @@
 // piece); the largest magnitude is taken over the bit patterns, where infinities and NaN come out on top. Bound by
 // the rows' bytes for prompts and by the launch and two trips to memory for one token. Measured, 4 KV heads of 256: one token
 // written and read back 6.7 to 8.3 us (kernels 2.5 and 1.9); 4 prompts, 12287 bf16 rows inside q, k, v rows, written and
-// read back as f32 50 us: 24 (76 MB: 3.1 TB/s) and 21.5 (126 MB: 5.9 TB/s); 16 caches of 8192 rows read back as
+// read back as f32 47.5 us, by divisions instead of kvq_four 49.6: 22 (76 MB: 3.4 TB/s) and 21.5 (126 MB: 5.9 TB/s); 16 caches of 8192 rows read back as
 // bf16 144 us (810 MB: 5.6 TB/s; a large copy 4.6); 77 rows of 8 heads of 128 read back 3.8 to 4.1 us.
 #include "rbt_device.h"
 #include "rbt_internal.h"
@@ -23,6 +23,24 @@ __device__ __forceinline__ float kvq_ld(const void *p, long i, int b16) {
 __device__ __forceinline__ int kvq_entry(float x, float scale) {
   const float r = rintf(__fdiv_rn(x, scale));
   return (int)fminf(fmaxf(r, -127.0f), 127.0f);
+}
+
+// Four entries, packed, where the scale lies in [2^-60, 2^60] and r = 1 / scale rounded to nearest: x r is within two steps
+// of the quotient, the first correction by its remainder (which an fma gives exactly) brings it within one, and
+// the second one rounds it as a division would (Markstein 1990). A quotient whose remainder underflows is below
+// 2^-40, an entry of 0 either way. Adding 1.5 * 2^23 rounds to the nearest whole number, ties to even, and leaves its
+// last eight bits in the sum's; |x / scale| <= 127 (1 + 2^-23), so nothing has to be cut.
+__device__ __forceinline__ uint32_t kvq_four(const float *x, float scale, float r) {
+  uint32_t o[4];
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    float q = x[e] * r;
+    q = fmaf(fmaf(-q, scale, x[e]), r, q);
+    q = fmaf(fmaf(-q, scale, x[e]), r, q);
+    o[e] = __float_as_uint(q + 12582912.0f);
+  }
+  const uint32_t lo = __builtin_amdgcn_perm(o[1], o[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(o[3], o[2], 0x04000c0cu);
+  return lo | hi;
 }
 
 // What a row's largest magnitude (as bits) makes of it: the scale, and whether its entries are to be formed.
@@ -79,7 +97,11 @@ __global__ __launch_bounds__(256) void k_kv_quant(KvqArgs a, int G) {
       for (int d = 1; d < G; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d, 64));
       const bool form = kvq_scale(top, scale);
       uint32_t o[2] = {0, 0};
-      if (form) {
+      if (form && scale >= 0x1p-60f && scale <= 0x1p60f) {
+        const float r = __fdiv_rn(1.0f, scale);
+        o[0] = kvq_four(x, scale, r);
+        o[1] = kvq_four(x + 4, scale, r);
+      } else if (form) {
 #pragma unroll
         for (int e = 0; e < 8; e++) o[e >> 2] |= ((uint32_t)kvq_entry(x[e], scale) & 0xffu) << (8 * (e & 3));
       }

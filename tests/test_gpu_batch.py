@@ -77,6 +77,24 @@ def test_quant(ctx, B, Tn, K, D, cap, dtype, wide, counts, lens):
                 assert np.array_equal(_np(o)[b, :n[b]], w[b, :n[b]]) and (_np(o)[b, n[b]:] == 5.0).all()
 
 
+def test_quant_halves(ctx):
+    """Quotients at halves and one step beside them, scales on both sides of every rule, bit for bit."""
+    rng = np.random.default_rng(11)
+    R, K, D = 290, 2, 256
+    a = np.ldexp(1 + rng.random((1, R, K, 1)), (np.arange(R) - 145).reshape(1, R, 1, 1) * 4 // 5).astype(np.float32)
+    x = (a / np.float32(127)).astype(np.float64) * (rng.integers(-127, 127, (1, R, K, D)) + 0.5)
+    x = x.astype(np.float32)
+    x[..., 1::3] = np.nextafter(x[..., 1::3], np.float32(np.inf))
+    x[..., 2::3] = np.nextafter(x[..., 2::3], np.float32(-np.inf))
+    x = np.clip(x, -a, a)
+    x[..., :1] = a
+    cache = _cache8(1, R, K, D)
+    ctx.kv_quant(_t(x), _t(-x), cache)
+    q, s = BT.quantise(x)
+    assert np.array_equal(_np(cache[0]), q) and np.array_equal(_np(cache[2]), s)
+    assert np.array_equal(_np(cache[1]), -q) and np.array_equal(_np(cache[3]), s)
+
+
 def test_quant_special_values(ctx):
     """A row with a non-finite entry reads back as NaN, whole; its neighbours do not notice."""
     import torch
