@@ -8,9 +8,10 @@
 // G lanes share a row, eight entries each (8 bytes of the cache a lane: a row of 256 is written by half a wave in one
 // piece); the largest magnitude is taken over the bit patterns, where infinities and NaN come out on top. Bound by
 // the rows' bytes for prompts and by the launch and two trips to memory for one token. Measured, 4 KV heads of 256: one token
-// written and read back 6.7 to 8.3 us (kernels 2.5 and 1.9); 4 prompts, 12287 bf16 rows inside q, k, v rows, written and
-// read back as f32 47.5 us, by divisions instead of kvq_four 49.6: 22 (76 MB: 3.4 TB/s) and 21.5 (126 MB: 5.9 TB/s); 16 caches of 8192 rows read back as
-// bf16 144 us (810 MB: 5.6 TB/s; a large copy 4.6); 77 rows of 8 heads of 128 read back 3.8 to 4.1 us.
+// written and read back 6.7 to 8.3 us (kernels 2.4 and 1.9); 4 prompts, 12287 bf16 rows inside q, k, v rows, written and
+// read back as f32 47.5 us: 19.2 (76 MB: 4.0 TB/s; by divisions instead of kvq_four 24.2) and 21.5 (126 MB: 5.9 TB/s); 16
+// caches of 8192 rows read back as bf16 144 us (810 MB: 5.6 TB/s; a large copy 4.6); 77 rows of 8 heads of 128 read back
+// 3.8 to 4.1 us.
 #include "rbt_device.h"
 #include "rbt_internal.h"
 
