@@ -39,11 +39,15 @@ __device__ __forceinline__ float tree_ld(const void *p, long i, int b16) {
   return b16 ? rbt_bf16_f32(((const uint16_t *)p)[i]) : ((const float *)p)[i];
 }
 
-// Whether the sequence's numbers fit; what does not is reported once per sequence.
+// Whether a sequence of n nodes behind L own rows is one that is attended to: the passes and the joins ask alike.
+__device__ __forceinline__ bool tree_valid(const TreeArgs &a, int n, int L) {
+  return n >= 0 && n <= a.T && L >= 0 && L <= a.cap - (a.in_cache ? n : 0);
+}
+// The sequence's numbers; those that are not valid are reported once per sequence.
 __device__ __forceinline__ bool tree_fits(const TreeArgs &a, int b, int &n, int &L) {
   n = a.n_nodes[b];
   L = a.len[b];
-  if (n >= 0 && n <= a.T && L >= 0 && L <= a.cap - (a.in_cache ? n : 0)) return true;
+  if (tree_valid(a, n, L)) return true;
   if (threadIdx.x == 0) *a.bad = 1;
   return false;
 }
@@ -1141,7 +1145,7 @@ __global__ __launch_bounds__(256) void k_tree_join(TreeArgs a, int TK) {
 #pragma unroll
   for (int k = 0; k < PF; k++) y[k] = *(const float4 *)(po + min(first + k * WP, most) * ps * 16 * a.hd);
   const int n = a.n_nodes[b], L = a.len[b];
-  if (n < 0 || n > a.T || L < 0 || L > a.cap || tile * 16 >= n * a.R) return;
+  if (!tree_valid(a, n, L) || tile * 16 >= n * a.R) return;
   unsigned per, pieces;
   tree_pieces(a, L, TK, per, pieces);
   const int np = (int)pieces;
@@ -1220,7 +1224,7 @@ __global__ __launch_bounds__(256) void k_prefix_join(TreeArgs a, TreeArgs p) {
   const int n = a.n_nodes[b], L = a.len[b];
   int g, f0, P;
   if (!tree_prefix(p, b, g, f0, P)) return;
-  if (n < 0 || n > a.T || L < 0 || L > a.cap - (a.in_cache ? n : 0) || tile * 16 >= n * a.R) return;
+  if (!tree_valid(a, n, L) || tile * 16 >= n * a.R) return;
   unsigned per, u1, u2 = 0;
   tree_pieces(a, L, a.tk, per, u1);
   if (P > 0) tree_pieces(p, P, p.tk, per, u2);

@@ -1,0 +1,43 @@
+"""GPU checks of the batch step's operators at their edges: full caches, padding, ranges of settings, odd memory."""
+import numpy as np
+import pytest
+
+from test_gpu_batch import _both, _kv, _reported
+from test_gpu_drafts import _i, _t
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- attention --------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", ["f32", "bf16", "i8"])
+@pytest.mark.parametrize("B,H,K,D,N,cap", [
+    (4, 8, 2, 64, 1, 4000),      # many pieces of few rows
+    (40, 16, 8, 128, 1, 2000),   # more rows, few pieces
+    (4, 8, 2, 256, 3, 4000),
+    (2, 40, 1, 192, 2, 4000),    # several row tiles
+    (4, 8, 2, 80, 2, 300),       # a head dim off the matrix cores
+])
+def test_full_cache_without_prefixes(own_ctx, kind, B, H, K, D, N, cap):
+    """Nodes' rows in the cache: a sequence whose rows do not fit it is left as it was and reported, whether or not its length
+    alone does; the others' bits stay."""
+    import torch
+    ctx, rng = own_ctx, np.random.default_rng(61)
+    cache = _both(_kv(rng, kind, B, cap, K, D), _kv(rng, kind, B, cap, K, D))
+    q = _t(rng.standard_normal((B, N, H, D)).astype(np.float32))
+    lens = rng.integers(cap // 2, cap - N + 1, B)
+    lens[0] = cap - N  # the last that fits
+
+    def run(at):
+        out = torch.full_like(q, 3.0)
+        ctx.gqa_prefix(q, cache, _i(at), _i([N] * B), D ** -0.5, out, sync=False)
+        return out
+    good = run(lens)
+    ctx.sync()
+    assert torch.isfinite(good).all() and (good != 3.0).any(-1).all()
+    for full in (cap, cap - N + 1):
+        at = lens.copy()
+        at[1] = full
+        out = run(at)
+        _reported(ctx)
+        keep = [b for b in range(B) if b != 1]
+        assert (out[1] == 3.0).all() and torch.equal(out[keep], good[keep])
