@@ -524,6 +524,7 @@ int rbt_kv_dequant_d(rbt_ctx *ctx, const rbt_kv_quant_desc *desc, size_t n_seq, 
  *    whose new row has been written, or a chain. Else as rbt_gqa_tree_d's draft rows, of the cache's type.
  *  - parent NULL: chains (node i hangs from node i - 1).
  *  - n_prefix 0: prefix, prefix_len and prefix_first are not used.
+ *  - Queries and gates of padding nodes may be read here, and change no other node's output.
  * Everything else as rbt_gqa_tree_d; entries 16-byte aligned, scales 4-byte. Over 8-bit rows q and the
  * probabilities are taken to 2^-22 of their row's largest (of 32 or 128 keys at a time), products and
  * their sums are exact in whole numbers, and sums over all keys f32. n_prefix <= 1024 and

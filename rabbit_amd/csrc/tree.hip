@@ -819,14 +819,16 @@ __device__ __forceinline__ void tree_pass(const TreeArgs &a, int bx, int by, int
     }
     const float ms = m == -INFINITY ? 0.0f : m;
     // (8-bit rows: m is a rounded product and the fused difference from it is not. Past 2^20 they would be apart by more than
-    // 2^-4, by anything at scores of 2^32: the products there are rounded first)
+    // 2^-4, by anything at scores of 2^32: the products there are rounded first. Row by row: a wave's rows are of several
+    // users, and of padding nodes)
     float step = qs;
-    if (I8 && __any(fabsf(ms) > 0x1p20f)) {
+    const bool far = I8 && fabsf(ms) > 0x1p20f;
+    if (I8 && __any(far)) {
 #pragma unroll
       for (int x = 0; x < NT; x++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) sc[x][i] *= qs;
-      step = 1.0f;
+        for (int i = 0; i < 4; i++) sc[x][i] = far ? sc[x][i] * qs : sc[x][i];
+      step = far ? 1.0f : qs;
     }
 #pragma unroll
     for (int x = 0; x < NT; x++)

@@ -41,3 +41,31 @@ def test_full_cache_without_prefixes(own_ctx, kind, B, H, K, D, N, cap):
         _reported(ctx)
         keep = [b for b in range(B) if b != 1]
         assert (out[1] == 3.0).all() and torch.equal(out[keep], good[keep])
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "i8"])
+@pytest.mark.parametrize("D", [64, 256, 80])
+@pytest.mark.parametrize("N", [1, 3])
+def test_padding_queries(ctx, kind, D, N):
+    """Queries and gates of padding nodes and of sequences without nodes, behind a prefix they share with others: whatever
+    they hold, the others' bits stay."""
+    import torch
+    rng = np.random.default_rng(62)
+    B, H, K, cap, pcap = 4, 8, 2, 40, 500
+    cache, draft, prefix = [_both(_kv(rng, kind, n, c, K, D), _kv(rng, kind, n, c, K, D)) for n, c in ((B, cap), (B, N), (1, pcap))]
+    counts = [N, 0, N, max(0, N - 2)]
+    q, gate = [_t(rng.standard_normal((B, N, H, D)).astype(np.float32)) for _ in range(2)]
+    live = torch.arange(N, device="cuda")[None] < _i(counts)[:, None]
+
+    def run(qq, gg):
+        out = torch.full_like(q, 3.0)
+        ctx.gqa_prefix(qq, cache, _i([5, 0, 33, 8]), _i(counts), D ** -0.5, out, draft=draft, prefix=prefix, prefix_len=_i([pcap - 1]),
+                       prefix_first=_i([0, B]), gate=gg)
+        return out
+    good = run(q, gate)
+    assert torch.isfinite(good).all() and (good[~live] == 3.0).all()
+    for bad in (1e7, 1e30, float("inf"), float("nan")):
+        qq, gg = q.clone(), gate.clone()
+        qq[~live] *= bad
+        gg[~live] = bad
+        assert torch.equal(run(qq, gg), good), bad
