@@ -2550,6 +2550,9 @@ int rbt_gqa_prefix_d(rbt_ctx *c, const rbt_gqa_prefix_desc *d, size_t n_seq, siz
     if (n_prefix) RBT_TRY(kv_rows_ok(c, "prefix", prefix, d->kv_dtype));
     if (misaligned(q, 16) || misaligned(out, 16) || misaligned(gate, 4))
       return refuse(c, RBT_E_INVALID, "q and out must be 16-byte aligned");
+    if (misaligned(len, 4) || misaligned(n_nodes, 4) || misaligned(parent, 4) ||
+        (n_prefix && (misaligned(prefix_len, 4) || misaligned(prefix_first, 4))))
+      return refuse(c, RBT_E_INVALID, "lengths, counts, parents and prefixes must be aligned to their type");
   }
   if (!c) return refuse(c, RBT_E_INVALID, "null context");
   if (n_seq == 0) return RBT_OK;
