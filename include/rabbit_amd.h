@@ -508,8 +508,8 @@ typedef struct {
 int rbt_kv_quant_d(rbt_ctx *ctx, const rbt_kv_quant_desc *desc, size_t n_seq, size_t max_rows, const void *k, const void *v,
                    const int32_t *len, const int32_t *n_rows, const rbt_kv_rows *cache);
 /* The other way: rows len[b] + j (NULL: j), j < n_rows[b] (NULL: max_rows), of the cache to rows j of k and v,
- * rounded once to their type. Rows of k and v may not overlap each other (RBT_E_INVALID); rows past n_rows[b] stay as
- * they were. */
+ * rounded once to their type. Rows past n_rows[b] stay as they were. No two of the max_rows rows of k's sequences and of v's
+ * may share an entry (RBT_E_INVALID); k's may lie between v's. The cache and its scales overlap neither side. */
 int rbt_kv_dequant_d(rbt_ctx *ctx, const rbt_kv_quant_desc *desc, size_t n_seq, size_t max_rows, const rbt_kv_rows *cache,
                      const int32_t *len, const int32_t *n_rows, void *k, void *v);
 

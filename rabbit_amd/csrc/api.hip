@@ -2444,6 +2444,19 @@ int rbt_kv_commit_d(rbt_ctx *c, const rbt_kv_commit_desc *d, size_t n_seq, size_
 }
 
 // ---- a batch's decode step: 8-bit caches, shared prefixes, sampling -------------------------------
+// Whether rows of one side share an entry with rows of another that begins `delta` entries on. Axes by rising stride; rows
+// of one side lie apart, so what the smaller strides span is less than a stride, and of the largest only the two multiples
+// beside delta come into question.
+static bool sides_meet(const size_t *n, const size_t *stride, const int *axis, int axes, long row, long delta) {
+  if (axes == 0) return delta < row && -delta < row;
+  const int x = axis[axes - 1];
+  if (n[x] <= 1) return sides_meet(n, stride, axis, axes - 1, row, delta);
+  const long s = (long)stride[x], q = delta / s - (delta % s < 0), most = (long)n[x] - 1;
+  for (long d = q; d <= q + 1; d++)
+    if (d <= most && -d <= most && sides_meet(n, stride, axis, axes - 1, row, delta - d * s)) return true;
+  return false;
+}
+
 static int kvq_call(rbt_ctx *c, const rbt_kv_quant_desc *d, size_t n_seq, size_t max_rows, const void *k, const void *v,
                     const int32_t *len, const int32_t *n_rows, const rbt_kv_rows *cache, bool read) {
   if (!d) return refuse(c, RBT_E_INVALID, "null descriptor");
@@ -2456,6 +2469,9 @@ static int kvq_call(rbt_ctx *c, const rbt_kv_quant_desc *d, size_t n_seq, size_t
     return refuse(c, RBT_E_INVALID, "%zu rows of %zu kv heads into a cache of %zu", max_rows, d->n_kv_heads, d->cap);
   const size_t lim = (size_t)1 << 40, hs = d->head_stride, rs = d->row_stride, ss = d->seq_stride, hd = d->head_dim;
   if (hs > lim || rs > lim || ss > lim) return refuse(c, RBT_E_INVALID, "a stride is past 2^40");
+  const size_t n[3] = {d->n_kv_heads, max_rows, n_seq}, st[3] = {hs, rs, ss};
+  int axis[3] = {0, 1, 2};  // by rising stride
+  std::sort(axis, axis + 3, [&](int x, int y) { return st[x] < st[y]; });
   if (n_seq && max_rows) {
     if (!k || !v || !cache || !cache->k || !cache->v || !cache->k_scale || !cache->v_scale)
       return refuse(c, RBT_E_INVALID, "null rows, cache or scales");
@@ -2463,11 +2479,9 @@ static int kvq_call(rbt_ctx *c, const rbt_kv_quant_desc *d, size_t n_seq, size_t
         misaligned(cache->v_scale, 4) || misaligned(len, 4) || misaligned(n_rows, 4))
       return refuse(c, RBT_E_INVALID, "a pointer is not aligned to its type");
     if (read) {
-      // result rows lie apart: sorted by stride, each reaches past what the smaller ones span
-      size_t n[3] = {d->n_kv_heads, max_rows, n_seq}, st[3] = {hs, rs, ss}, span = hd;
-      int o[3] = {0, 1, 2};
-      std::sort(o, o + 3, [&](int x, int y) { return st[x] < st[y]; });
-      for (int i : o) {
+      // result rows lie apart: each stride reaches past what the smaller ones span
+      size_t span = hd;
+      for (int i : axis) {
         if (n[i] <= 1) continue;
         if (st[i] < span) return refuse(c, RBT_E_INVALID, "result rows overlap");
         span += (n[i] - 1) * st[i];
@@ -2476,6 +2490,8 @@ static int kvq_call(rbt_ctx *c, const rbt_kv_quant_desc *d, size_t n_seq, size_t
   }
   if (!c) return refuse(c, RBT_E_INVALID, "null context");
   if (n_seq == 0 || max_rows == 0) return RBT_OK;
+  if (read && sides_meet(n, st, axis, 3, (long)hd, ((long)(uintptr_t)v - (long)(uintptr_t)k) / (long)dtype_size(d->dtype)))
+    return refuse(c, RBT_E_INVALID, "k and v overlap");
   DeviceScope dev(c->device);
   rbt::KvqArgs a{};
   a.k = k;

@@ -2,8 +2,9 @@
 import numpy as np
 import pytest
 
+import batch_truth as BT
 from test_gpu_batch import _both, _kv, _reported
-from test_gpu_drafts import _i, _t
+from test_gpu_drafts import _i, _np, _t
 
 pytestmark = pytest.mark.gpu
 
@@ -69,3 +70,38 @@ def test_padding_queries(ctx, kind, D, N):
         qq[~live] *= bad
         gg[~live] = bad
         assert torch.equal(run(qq, gg), good), bad
+
+
+# ---- 8-bit rows -------------------------------------------------------------------------------------
+def test_read_back_refuses_sides_over_each_other(ctx):
+    """Rows of k and of v that share an entry are refused; sides that lie within each other, between rows, are not."""
+    import torch
+    import rabbit_amd as R
+    rng = np.random.default_rng(63)
+    B, Tn, K, D = 2, 5, 3, 64
+    cache = (_t(rng.integers(-127, 128, (B, Tn, K, D)).astype(np.int8)), _t(rng.integers(-127, 128, (B, Tn, K, D)).astype(np.int8)),
+             _t(rng.random((B, Tn, K)).astype(np.float32)), _t(rng.random((B, Tn, K)).astype(np.float32)))
+    want = [BT.values(_np(cache[i]), _np(cache[2 + i]), np.float32) for i in (0, 1)]
+    n = B * Tn * K * D
+    buf = torch.zeros(4 * n + 512, device="cuda")
+    dense = lambda at: buf[at:at + n].view(B, Tn, K, D)  # noqa: E731
+    wide = lambda at: buf[at:at + 2 * n].view(B, Tn, 2 * K, D)[:, :, :K]  # noqa: E731
+    sides = lambda i: buf[:2 * n].view(K, 2, B, Tn, D)[:, i].permute(1, 2, 0, 3)  # noqa: E731
+    rows = lambda at: buf[at:at + 2 * n].view(B, Tn, K, 2 * D)[..., :D]  # noqa: E731
+    for k, v in ((dense(0), dense(0)), (dense(0), dense(n - 1)), (dense(1), dense(0)), (dense(n - 4), dense(0)), (wide(0), wide(0)),
+                 (wide(0), wide((K - 1) * D)), (wide(0), wide((K + 1) * D)), (wide(0), wide(2 * K * D * 7)), (rows(0), rows(D - 1)),
+                 (rows(0), rows(2 * D * (K * Tn * B - 1))), (rows(3 * D + 1), rows(0)), (sides(0), sides(0))):
+        for a, b in ((k, v), (v, k)):
+            with pytest.raises(R.RbtError, match="overlap"):
+                ctx.kv_dequant(cache, a, b)
+    for k, v in ((dense(0), dense(n)), (wide(0), wide(K * D)), (wide(0), wide(2 * n)), (rows(0), rows(D)), (rows(0), rows(2 * D * K * Tn * B)),
+                 (rows(D), rows(2 * D * 4)), (sides(0), sides(1))):
+        for a, b in ((k, v), (v, k)):
+            ctx.kv_dequant(cache, a, b)
+            assert np.array_equal(_np(a), want[0]) and np.array_equal(_np(b), want[1])
+    # one axis of size 1 has no step; rows that no sequence writes count too
+    one = lambda at: buf[at:at + n].view(B, Tn, K, D)[:, :1]  # noqa: E731
+    ctx.kv_dequant(cache, one(0), one(K * D))
+    assert np.array_equal(_np(one(0)), want[0][:, :1]) and np.array_equal(_np(one(K * D)), want[1][:, :1])
+    with pytest.raises(R.RbtError, match="overlap"):
+        ctx.kv_dequant(cache, dense(0), dense(n - D), n_rows=_i([1, 1]))
