@@ -2480,11 +2480,11 @@ static int kvq_call(rbt_ctx *c, const rbt_kv_quant_desc *d, size_t n_seq, size_t
       return refuse(c, RBT_E_INVALID, "a pointer is not aligned to its type");
     if (read) {
       // result rows lie apart: each stride reaches past what the smaller ones span
-      size_t span = hd;
+      unsigned __int128 span = hd;  // (2^31 rows 2^40 apart pass 64 bits)
       for (int i : axis) {
         if (n[i] <= 1) continue;
         if (st[i] < span) return refuse(c, RBT_E_INVALID, "result rows overlap");
-        span += (n[i] - 1) * st[i];
+        span += (unsigned __int128)(n[i] - 1) * st[i];
       }
     }
   }

@@ -21,3 +21,11 @@ def test_prefix_refuses_misaligned_numbers(rbt_lib, which, off):
     if which in ("plen", "first"):  # not used without prefixes
         rc = rbt_lib.rbt_gqa_prefix_d(None, C.byref(d), *{**a, which: A + off, "G": 0, "prefix": None}.values())
         _refused(rbt_lib, rc, RBT_E_INVALID, "null context")
+
+
+@pytest.mark.parametrize("rows,row,seq", [((1 << 25) + 1, 1 << 39, 1 << 40), ((1 << 24) + 1, 1 << 40, 1 << 40), ((1 << 30) + 1, 1 << 36, 1 << 37)])
+def test_read_back_spans_past_64_bits(rbt_lib, rows, row, seq):
+    """Rows whose span is 2^64 entries and a few: the next sequence begins inside it."""
+    d, r = abi.RbtKvQuantDesc(1, 64, (1 << 31) - 1, 0, seq, row, 64), _rows()
+    _refused(rbt_lib, rbt_lib.rbt_kv_dequant_d(None, C.byref(d), 2, rows, C.byref(r), A, A, A, 2 * A), RBT_E_INVALID, "result rows overlap")
+    _refused(rbt_lib, rbt_lib.rbt_kv_dequant_d(None, C.byref(d), 1, rows, C.byref(r), A, A, A, 2 * A), RBT_E_INVALID, "null context")
