@@ -414,9 +414,13 @@ __device__ __forceinline__ int smp_find(const SmpRow &r, const SmpSet &s, const 
   return last;
 }
 
+// The draw's border: a running mass passes u times the whole where it is above this. In whole numbers, since sums past 2^53
+// are rounded as doubles, and a border that lies in one chunk by rounded sums need not lie in its entries.
+__device__ __forceinline__ u64 smp_left(const SmpSet &s, u64 total) { return (u64)(s.u * (double)total); }
+
 // Where nothing is kept before the list: the draw among its entries up to `last`, in the order of their indexes.
 template <int NT>
-__device__ __forceinline__ int smp_draw_list(const SmpFind &f, int last, double left) {
+__device__ __forceinline__ int smp_draw_list(const SmpFind &f, int last, u64 left) {
   __shared__ u64 first;
   const int t = threadIdx.x;
   if (t == 0) first = ~0ull;
@@ -430,7 +434,7 @@ __device__ __forceinline__ int smp_draw_list(const SmpFind &f, int last, double 
       if ((unsigned)f.ord[j] <= at) run += up - before;
       before = up;
     }
-    if ((double)run > left) atomicMin(&first, (u64)at);
+    if (run > left) atomicMin(&first, (u64)at);
   }
   __syncthreads();
   return first == ~0ull ? -1 : (int)first;
@@ -439,7 +443,7 @@ __device__ __forceinline__ int smp_draw_list(const SmpFind &f, int last, double 
 // The least index in [lo, hi) at which the running mass of entries up to thr passes `left`: every wave sums a part of it,
 // then the workgroup looks through the part where it passes, four entries a thread.
 template <int NT>
-__device__ __forceinline__ int smp_draw(const SmpRow &r, const double *tab, int lo, int hi, u64 thr, double left, SmpRed &red) {
+__device__ __forceinline__ int smp_draw(const SmpRow &r, const double *tab, int lo, int hi, u64 thr, u64 left, SmpRed &red) {
   __shared__ int found;
   constexpr int W = NT / 64, UN = 8;
   const int t = threadIdx.x, w = t >> 6, lane = t & 63, part = (hi - lo + W - 1) / W;
@@ -464,7 +468,7 @@ __device__ __forceinline__ int smp_draw(const SmpRow &r, const double *tab, int 
   int q = -1;
 #pragma unroll
   for (int i = 0; i < W; i++) {
-    if (q < 0 && (double)(run + red.w[i]) > left) q = i;
+    if (q < 0 && run + red.w[i] > left) q = i;
     if (q < 0) run += red.w[i];
   }
   if (q < 0) return -1;  // (not reached: u below 1 times the whole is below the whole)
@@ -479,13 +483,13 @@ __device__ __forceinline__ int smp_draw(const SmpRow &r, const double *tab, int 
       m[e] = i + e < e1 ? kept(x, i + e) : 0;
     }
     const u64 mine = (m[0] + m[1]) + (m[2] + m[3]), up = run + smp_scan<NT>(mine, all, red);
-    if ((double)up > left && !((double)(up - mine) > left)) {  // this thread's (one's alone)
+    if (up > left && up - mine <= left) {  // this thread's (one's alone)
       u64 at = up - mine;
       int e = 0;
 #pragma unroll
       for (; e < 3; e++) {
         at += m[e];
-        if ((double)at > left) break;
+        if (at > left) break;
       }
       found = i + e;
     }
@@ -697,8 +701,8 @@ __global__ __launch_bounds__(SMP_ONE) void k_sample_one(SampleArgs a, SmpUnits u
       if (!slow) {
         const int last = smp_find<NT>(r, s, tab, lds.f, n, smp_cut_all(n), 0, 0, ~0ull, total, red);
         thr = lds.f.ord[last];
-        tok = last < NT ? smp_draw_list<NT>(lds.f, last, s.u * (double)total)
-                        : smp_draw<NT>(r, tab, 0, V, thr, s.u * (double)total, red);
+        tok = last < NT ? smp_draw_list<NT>(lds.f, last, smp_left(s, total))
+                        : smp_draw<NT>(r, tab, 0, V, thr, smp_left(s, total), red);
       }
     } else {
       const bool any = s.by_k || s.by_p || s.by_m;
@@ -735,16 +739,16 @@ __global__ __launch_bounds__(SMP_ONE) void k_sample_one(SampleArgs a, SmpUnits u
           const int last = smp_find<NT>(r, s, tab, lds.f, n, c, sum0, sumk, all, total, red);
           thr = last >= 0 ? lds.f.ord[last] : lds.f.ord[0] - 1;
           if (sum0 == 0 && last < NT) {
-            tok = smp_draw_list<NT>(lds.f, last, s.u * (double)total);
+            tok = smp_draw_list<NT>(lds.f, last, smp_left(s, total));
             drawn = true;
           }
         }
       }
-      if (!slow && !drawn) tok = smp_draw<NT>(r, tab, 0, V, thr, s.u * (double)total, red);
+      if (!slow && !drawn) tok = smp_draw<NT>(r, tab, 0, V, thr, smp_left(s, total), red);
     }
     if (slow) {
       thr = smp_slow<NT>(r, s, tab, lds.slow, total, red);
-      tok = smp_draw<NT>(r, tab, 0, V, thr, s.u * (double)total, red);
+      tok = smp_draw<NT>(r, tab, 0, V, thr, smp_left(s, total), red);
     }
   }
   if (t == 0) {
@@ -810,24 +814,24 @@ __global__ __launch_bounds__(SMP_NT) void k_sample_top(SampleArgs a, SmpWork k) 
 }
 
 // The chunk where the running mass passes `left`, and the mass before it.
-__device__ __forceinline__ int smp_chunk(const u64 *mass, int G, double left, u64 &before) {
+__device__ __forceinline__ int smp_chunk(const u64 *mass, int G, u64 left, u64 &before) {
   before = 0;
   for (int g = 0; g < G; g++) {
-    if ((double)(before + mass[g]) > left) return g;
+    if (before + mass[g] > left) return g;
     before += mass[g];
   }
   return -1;
 }
-__device__ __forceinline__ int smp_draw_chunk(const SmpRow &r, const SmpWork &k, const double *tab, const u64 *mass, u64 thr, double left,
+__device__ __forceinline__ int smp_draw_chunk(const SmpRow &r, const SmpWork &k, const double *tab, const u64 *mass, u64 thr, u64 left,
                                               SmpRed &red) {
   u64 before;
   const int ch = smp_chunk(mass, k.G, left, before);
-  return ch < 0 ? -1 : smp_draw<SMP_NT>(r, tab, ch * k.len, min(r.V, (ch + 1) * k.len), thr, left - (double)before, red);
+  return ch < 0 ? -1 : smp_draw<SMP_NT>(r, tab, ch * k.len, min(r.V, (ch + 1) * k.len), thr, left - before, red);
 }
 // The token: of the list up to `last`, and of what lies before it (mass0, by chunks in `chunk`).
 __device__ __forceinline__ int smp_token(const SmpRow &r, const SmpWork &k, const SmpSet &s, const double *tab, const SmpFind &f, int last,
                                          u64 thr, u64 total, u64 mass0, u64 *chunk, SmpRed &red) {
-  const double left = s.u * (double)total;
+  const u64 left = smp_left(s, total);
   if (mass0 == 0 && last < SMP_NT) return smp_draw_list<SMP_NT>(f, last, left);
   for (int i = threadIdx.x; i <= last; i += SMP_NT) {
     const u64 v = f.run[i] - (i ? f.run[i - 1] : 0);
@@ -958,7 +962,7 @@ __global__ __launch_bounds__(SMP_NT) void k_sample_cut(SampleArgs a, SmpWork k) 
   u64 all = 0;
   for (int j = 0; j < G; j++) all += cert[j];
   if (!any) {
-    smp_finish(a, st, gr, smp_draw_chunk(r, k, tab, cert, ~0ull, s.u * (double)all, red), ~0ull, all);
+    smp_finish(a, st, gr, smp_draw_chunk(r, k, tab, cert, ~0ull, smp_left(s, all), red), ~0ull, all);
     return;
   }
   const SmpCut c = smp_cut<NT>(s, a.V, k.un, v, all, lds.hist, red);
@@ -993,7 +997,7 @@ __global__ __launch_bounds__(SMP_NT) void k_sample_list(SampleArgs a, SmpWork k)
   if (mode == SMP_SLOW) {
     u64 total;
     const u64 thr = smp_slow<NT>(r, s, tab, lds.slow, total, red);
-    smp_finish(a, st, gr, smp_draw<NT>(r, tab, 0, a.V, thr, s.u * (double)total, red), thr, total);
+    smp_finish(a, st, gr, smp_draw<NT>(r, tab, 0, a.V, thr, smp_left(s, total), red), thr, total);
     return;
   }
   const float cf = smp_scale(s.t);

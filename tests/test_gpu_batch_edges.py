@@ -105,3 +105,22 @@ def test_read_back_refuses_sides_over_each_other(ctx):
     assert np.array_equal(_np(one(0)), want[0][:, :1]) and np.array_equal(_np(one(K * D)), want[1][:, :1])
     with pytest.raises(R.RbtError, match="overlap"):
         ctx.kv_dequant(cache, dense(0), dense(n - D), n_rows=_i([1, 1]))
+
+
+# ---- sampling ---------------------------------------------------------------------------------------
+def test_draw_at_a_border_of_chunks(ctx):
+    """A draw that falls between the sums of a row's chunks as doubles round them: weights are whole numbers of 2^-45, whose
+    sums pass 2^53 here. With M = 2^45, the first 8000 entries weigh 4600 M + 16, the next 4000 weigh 2000 M + 32, and all of them
+    13200 M + 64; half of that passes 6600 M + 16 and not 6600 M + 48, at the entry of weight 32."""
+    import torch
+    x = np.full(40000, -np.inf, np.float32)
+    x[:4000] = x[4000:4600] = 0.0
+    x[8000:10000] = 0.0
+    x[12000:18600] = 0.0
+    small = lambda w: np.float32(np.log(w * 2.0 ** -45))  # noqa: E731
+    for i, w in ((7999, 16), (10000, 32), (20000, 16)):
+        x[i] = small(w)
+        assert abs(np.exp(np.float64(x[i])) * 2.0 ** 45 - w) < 0.01
+    tok = torch.full((1,), -9, dtype=torch.int32, device="cuda")
+    ctx.sample(_t(x[None]), _t(np.array([0.5], np.float32)), tok)
+    assert int(tok[0]) == 10000
