@@ -619,9 +619,12 @@ __device__ __forceinline__ SmpCut smp_cut(const SmpSet &s, int V, const SmpUnits
   __syncthreads();
   int b0 = s.by_p ? min(p0_s, kb) : kb, b1 = s.by_p ? min(p1_s, kb) : kb;
   if (s.by_m) {  // the bucket of the least weight, and its neighbours for their rounding
-    const int b = (int)fmin(-log(s.min_p) * 24.0, 600.0);
+    // (temperatures past which buckets do not follow the weights: smp_scale cuts 24 / t, or logits up to 21.3 t apart pass
+    // f32. Any bucket may then hold the least weight)
+    const bool all_of_them = s.t < 0x1p-90 || s.t > 0x1p120;
+    const int b = all_of_them ? 0 : (int)fmin(-log(s.min_p) * 24.0, 600.0);
     b0 = min(b0, max(b - 1, 0));
-    b1 = min(b1, b + 1);
+    b1 = min(b1, all_of_them ? SMP_NB : b + 1);
   }
   b0 = min(b0, SMP_NB - 1);
   b1 = min(b1, SMP_NB - 1);

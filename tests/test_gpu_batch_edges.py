@@ -3,6 +3,7 @@ import numpy as np
 import pytest
 
 import batch_truth as BT
+import draft_truth as T
 from test_gpu_batch import _both, _kv, _reported
 from test_gpu_drafts import _i, _np, _t
 
@@ -124,3 +125,22 @@ def test_draw_at_a_border_of_chunks(ctx):
     tok = torch.full((1,), -9, dtype=torch.int32, device="cuda")
     ctx.sample(_t(x[None]), _t(np.array([0.5], np.float32)), tok)
     assert int(tok[0]) == 10000
+
+
+@pytest.mark.parametrize("V", [3000, 40000])
+def test_min_p_at_extreme_temperatures(ctx, V):
+    """Temperatures below the least normal logit differences and near the largest f32: min-p keeps what the definition does."""
+    import torch
+    x = np.full((2, V), -1.0, np.float32)
+    t, m, u = [1e-35, 1e38], [0.5, 0.001], [0.95, 0.9999]
+    x[0, 3], x[0, 7], x[0, 11] = 0.0, -2e-35, -16.3e-30  # the second's weight is e^-2, the third's e^-1630000
+    x[1] = -np.inf
+    x[1, 5], x[1, 9] = 3e38, -3e38                        # they lie further apart than f32 holds: e^-6
+    tok, pr = torch.zeros(2, dtype=torch.int32, device="cuda"), torch.zeros(2, V, device="cuda")
+    f = lambda a: _t(np.asarray(a, np.float32))  # noqa: E731
+    ctx.sample(_t(x), f(u), tok, temperature=f(t), min_p=f(m), probs=pr)
+    for r, want in ((0, 3), (1, 9)):
+        one = lambda a: float(np.float32(a[r]))  # noqa: E731
+        wt, wp, _ = BT.sample(x[r], one(u), one(t), 0, 1.0, one(m))
+        assert wt == want == int(tok[r])
+        assert (np.abs(_np(pr)[r] - wp) <= (T.U32 + V * 2.0 ** -45) * wp + 1e-45).all()
