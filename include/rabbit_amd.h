@@ -555,7 +555,9 @@ int rbt_gqa_prefix_d(rbt_ctx *ctx, const rbt_gqa_prefix_desc *desc, size_t n_seq
  * int32 [n] may be NULL: 1, 1, 0 and 0. u f32 [n] in [0, 1). NaN and -inf entries are never drawn; a row
  * without an entry above -inf, or with +inf, gives token -1 and zeros. So does one whose settings are out of range
  * (t negative or not finite, top_k < 0, top_p or min_p outside 0..1, u outside [0, 1)), and the next rbt_sync reports it.
- * probs f32 [n, vocab] gets p (what rbt_draft_verify_d takes), or is NULL. vocab <= 2^24; n <= 65535. */
+ * probs f32 [n, vocab] gets p (what rbt_draft_verify_d takes), or is NULL; it may be the logits themselves where those are
+ * dense f32 rows, and shares no other entry with them (RBT_E_INVALID). tokens overlaps none of the others, probs none of
+ * the settings. vocab <= 2^24; n <= 65535. */
 typedef struct {
     size_t vocab, row_stride;
     int32_t logits_dtype;        /* RBT_DT_F32, RBT_DT_BF16 */

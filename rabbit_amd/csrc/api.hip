@@ -2654,6 +2654,14 @@ int rbt_sample_d(rbt_ctx *c, const rbt_sample_desc *d, size_t n, const void *log
   }
   if (!c) return refuse(c, RBT_E_INVALID, "null context");
   if (n == 0) return RBT_OK;
+  // probs over the logits: a workgroup's own entries are read before it writes them, another row's may not be
+  const bool same = probs == logits && d->logits_dtype == RBT_DT_F32 && (n == 1 || d->row_stride == d->vocab);
+  if (probs && !same) {
+    const long es = (long)dtype_size(d->logits_dtype), row = (long)d->vocab * es, step = (long)d->row_stride * es;
+    const long lo = (long)((uintptr_t)probs - (uintptr_t)logits), hi = lo + 4L * (long)(n * d->vocab);  // in the logits' bytes
+    const long r = lo < row ? 0 : (lo - row) / step + 1;  // the first row that ends past lo
+    if (r < (long)n && r * step < hi) return refuse(c, RBT_E_INVALID, "probs overlap the logits");
+  }
   DeviceScope dev(c->device);
   rbt::SampleArgs a{};
   a.x = logits;

@@ -144,3 +144,49 @@ def test_min_p_at_extreme_temperatures(ctx, V):
         wt, wp, _ = BT.sample(x[r], one(u), one(t), 0, 1.0, one(m))
         assert wt == want == int(tok[r])
         assert (np.abs(_np(pr)[r] - wp) <= (T.U32 + V * 2.0 ** -45) * wp + 1e-45).all()
+
+
+@pytest.mark.parametrize("V", [1003, 40003])
+def test_probabilities_over_the_logits(ctx, V):
+    """probs may be the logits' own dense f32 rows; any other overlap is refused."""
+    import torch
+    import rabbit_amd as R
+    rng = np.random.default_rng(V)
+    x = _t((3 * rng.standard_normal((5, V))).astype(np.float32))
+    f = lambda a: _t(np.asarray(a, np.float32))  # noqa: E731
+    sets = dict(temperature=f([1, 0.7, 0, 2, 1]), top_k=_i([0, 40, 0, 0, 0]), top_p=f([1, 0.9, 1, 0.8, 1]), min_p=f([0, 0, 0, 0, 0.01]))
+    u = f(rng.random(5))
+    tok, want, pr = (torch.zeros(5, dtype=torch.int32, device="cuda"), torch.zeros(5, dtype=torch.int32, device="cuda"), torch.zeros_like(x))
+    ctx.sample(x, u, want, probs=pr, **sets)
+    y = x.clone()
+    ctx.sample(y, u, tok, probs=y, **sets)
+    assert torch.equal(tok, want) and torch.equal(y, pr)
+    buf = torch.zeros(6 * V + 8, device="cuda")
+    wide = buf[:5 * (V + 1)].view(5, V + 1)[:, :V]
+    for logits, probs in ((wide, buf[:5 * V].view(5, V)), (buf[:5 * V].view(5, V), buf[4:5 * V + 4].view(5, V)),
+                          (buf.view(torch.bfloat16)[:5 * V].view(5, V), buf[:5 * V].view(5, V)),
+                          (buf[5 * V - 1:6 * V - 1].view(1, V), buf[4 * V:5 * V].view(1, V))):
+        n = logits.shape[0]
+        with pytest.raises(R.RbtError, match="overlap"):
+            ctx.sample(logits, u[:n], tok[:n], probs=probs)
+    wide1 = buf[:V + 1].view(1, V + 1)[:, :V]
+    ctx.sample(wide1, u[:1], tok[:1], probs=wide1.view(1, V))  # one row is dense
+    ctx.sample(buf[:5 * V].view(5, V)[:1], u[:1], tok[:1], probs=buf[V:2 * V].view(1, V))  # beside it
+
+
+def test_probabilities_between_the_logits_rows(ctx):
+    """Logits far apart in a buffer: probabilities between two of their rows overlap none, one entry on or back they do."""
+    import torch
+    import rabbit_amd as R
+    V = 50
+    buf = torch.randn(8 * V, device="cuda")
+    x, u, tok = buf.view(2, 4 * V)[:, :V], torch.full((2,), 0.5, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    want = torch.zeros(2, V, device="cuda")
+    ctx.sample(x, u, tok, probs=want)
+    for at in (V, 2 * V, 5 * V, 6 * V):
+        pr = buf[at:at + 2 * V].view(2, V)
+        ctx.sample(x, u, tok, probs=pr)
+        assert torch.equal(pr, want)
+    for at in (0, V - 1, 2 * V + 1, 4 * V, 5 * V - 1):
+        with pytest.raises(R.RbtError, match="overlap"):
+            ctx.sample(x, u, tok, probs=buf[at:at + 2 * V].view(2, V))
