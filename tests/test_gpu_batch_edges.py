@@ -4,7 +4,7 @@ import pytest
 
 import batch_truth as BT
 import draft_truth as T
-from test_gpu_batch import _both, _kv, _reported
+from test_gpu_batch import _both, _dt, _kv, _reported, _sample_check
 from test_gpu_drafts import _i, _np, _t
 
 pytestmark = pytest.mark.gpu
@@ -190,3 +190,147 @@ def test_probabilities_between_the_logits_rows(ctx):
     for at in (0, V - 1, 2 * V + 1, 4 * V, 5 * V - 1):
         with pytest.raises(R.RbtError, match="overlap"):
             ctx.sample(x, u, tok, probs=buf[at:at + 2 * V].view(2, V))
+
+
+# ---- ranges -----------------------------------------------------------------------------------------
+def _attend_check(ctx, kind, H, K, D, lens, counts, N, plens, first, drafted, gated, tree, rng, rows=None, qf=1.0):
+    """One call against the 64-bit form, by its bound. rows(rng, *shape): other rows than normal ones."""
+    import torch
+    B, G, pcap = len(lens), len(plens), max(plens + [0]) + 2
+    cap = max(lens) + N
+    kv = lambda n, c: [_rows_of(rng, kind, rows, n, c, K, D) for _ in "kv"]  # noqa: E731
+    (kc, vc), (kd, vd) = kv(B, cap), kv(B, N)
+    kp, vp = kv(G, pcap) if G else ((None, None), (None, None))
+    q = (qf * rng.standard_normal((B, N, H, D))).astype(np.float32)
+    gate = rng.standard_normal((B, N, H, D)).astype(np.float32) if gated else None
+    par = T.random_parents(rng, B, N, tree)
+    out, scale = torch.full((B, N, H, D), 3.0, device="cuda"), D ** -0.5
+    ctx.gqa_prefix(_t(q), _both(kc, vc), _i(lens), _i(counts), scale, out, draft=_both(kd, vd) if drafted else None,
+                   parent=None if tree == "chain" else _i(par), prefix=_both(kp, vp) if G else None, prefix_len=_i(plens) if G else None,
+                   prefix_first=_i(first) if G else None, gate=None if gate is None else _t(gate))
+    want, mag, qk, keys = BT.prefix_attention(q, kc[1], vc[1], kd[1] if drafted else None, vd[1] if drafted else None, lens, counts, par,
+                                              scale, kp[1], vp[1], plens, first, gate=gate, out=np.full(q.shape, 3.0))
+    tol = T.tree_attention_bound(mag, qk, keys[:, None, None, None], D)
+    if kind == "i8":
+        # (a score's error is the query's largest entry times the sum of a key's, which for rows of unequal entries is less
+        # than D times the largest: the largest such sum of any key here)
+        some = [x for x in ((kc, vc), (kd, vd) if drafted else None, (kp, vp) if G else None) if x]
+        ksum = max(np.abs(k[1].astype(np.float64)).sum(-1).max() for k, _ in some)
+        vmax = max(np.abs(v[1]).max() for _, v in some)
+        tol = tol + BT.bound8(q, ksum / D, vmax, scale, keys, gate)
+    live = np.arange(N)[None] < np.array(counts)[:, None]
+    got = _np(out)
+    assert (got[~live] == 3.0).all()
+    err = np.abs(got.astype(np.float64) - want)
+    assert (err <= tol)[live].all(), (err[live].max(), (err / tol)[live].max())
+    return np.linalg.norm(err[live]) / np.linalg.norm(want[live])
+
+
+def _rows_of(rng, kind, rows, *shape):
+    if rows is None:
+        return _kv(rng, kind, *shape)
+    x = rows(rng, *shape).astype(np.float32)
+    if kind == "i8":
+        q, s = BT.quantise(x)
+        return (_t(q), _t(s)), BT.values(q, s)
+    return (_t(x),), x
+
+
+@pytest.mark.parametrize("kind", ["i8", "bf16", "f32"])
+@pytest.mark.parametrize("H,K,D,N,lens,counts,plens,first,drafted,tree", [
+    (16, 2, 64, 256, [70, 3], [256, 200], [200], [0, 2], True, "chain"),     # a prompt's chunk: the most nodes, eight row tiles
+    (8, 2, 128, 130, [0, 40, 65], [130, 33, 64], [129, 5], [0, 1, 3], False, "tree"),
+    (12, 1, 192, 40, [100, 31], [40, 17], [], [0], False, "chain"),          # no prefix, the nodes' rows in the cache
+    (8, 2, 256, 70, [33, 20], [70, 65], [90], [0, 2], True, "tree"),
+    (4, 2, 80, 100, [9, 0], [100, 71], [60], [0, 2], False, "tree"),
+])
+def test_attend_many_nodes(ctx, kind, H, K, D, N, lens, counts, plens, first, drafted, tree):
+    """Chunks of a prompt and large trees: drafted rows over several stages and words of the visibility bits."""
+    rel = _attend_check(ctx, kind, H, K, D, lens, counts, N, plens, first, drafted, True, tree, np.random.default_rng(D + N))
+    assert rel <= 4e-6  # test_attend's bound of the whole
+
+
+@pytest.mark.parametrize("D", [64, 256])
+@pytest.mark.parametrize("side", ["q", "kv"])
+def test_attend_8bit_unequal_channels(ctx, D, side):
+    """A channel of the queries, or of the keys and values, 100 times the others: within the bound that the largest entry gives."""
+    rng = np.random.default_rng(71)
+    f = np.ones(D)
+    f[3] = 100.0 if side == "kv" else 0.01
+    rows = lambda r, *s: r.standard_normal(s) * f  # noqa: E731
+    _attend_check(ctx, "i8", 8, 2, D, [40, 300, 0], [1, 1, 1], 1, [700], [0, 3], False, False, "chain", rng, rows=rows,
+                  qf=1.0 / f[3] if side == "kv" else 1.0 / f)
+
+
+@pytest.mark.parametrize("D", [64, 256])
+@pytest.mark.parametrize("kf,vf", [(-53, 65), (65, -53), (65, 65), (-53, -53)])
+def test_attend_8bit_scales(ctx, D, kf, vf):
+    """Scales at both ends of 2^-60 to 2^60, and a little past the upper one: keys' and values' rows times 2^kf and 2^vf (a row's
+    largest of 64 or 256 normal numbers lies between 1 and 6, so scales 4.4 to 7 bits below), queries the other way."""
+    import torch
+    rng = np.random.default_rng(72)
+    H, K, cap, pcap = 8, 2, 60, 500
+    rows = [[BT.quantise(np.ldexp(rng.standard_normal((n, c, K, D)), f).astype(np.float32)) for f in (kf, vf)] for n, c in ((3, cap), (1, pcap))]
+    assert all(2.0 ** -60 <= s.min() and s.max() <= 2.0 ** 60.6 for r in rows for _, s in r)
+    t = [tuple(_t(x) for x in (k[0], v[0], k[1], v[1])) for k, v in rows]
+    q = np.ldexp(rng.standard_normal((3, 1, H, D)), -kf).astype(np.float32)
+    out = torch.zeros(3, 1, H, D, device="cuda")
+    lens = [59, 0, 30]
+    ctx.gqa_prefix(_t(q), t[0], _i(lens), _i([1] * 3), D ** -0.5, out, prefix=t[1], prefix_len=_i([499]), prefix_first=_i([0, 3]))
+    (kc, vc), (kp, vp) = [[BT.values(*x) for x in r] for r in rows]
+    want, mag, qk, keys = BT.prefix_attention(q, kc, vc, None, None, lens, [1] * 3, np.full((3, 1), -1), D ** -0.5, kp, vp, [499], [0, 3])
+    tol = T.tree_attention_bound(mag, qk, keys[:, None, None, None], D) + BT.bound8(
+        q, max(np.abs(kc).max(), np.abs(kp).max()), max(np.abs(vc).max(), np.abs(vp).max()), D ** -0.5, keys)
+    err = np.abs(_np(out) - want)
+    assert (err <= tol).all()
+    assert np.linalg.norm(err) <= 4e-6 * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("V", [5000, 70000])
+def test_sample_small_min_p(ctx, V):
+    """min-p between 0 and e^-21.3, whose bucket is past the last, alone and with the others. What is kept goes by the weights
+    themselves (to 2^-48 of each), not by sums: no weight here is within 2^-44 of its min-p."""
+    import torch
+    rng = np.random.default_rng(V)
+    x = (8 * rng.standard_normal((8, V))).astype(np.float32)
+    t, m = [1, 1, 1, 0.5, 1, 1, 1, 1], [1e-10, 1e-12, 1e-20, 1e-30, 1e-44, 1e-12, 1e-10, 5e-10]
+    k, p, u = [0, 0, 0, 0, 0, 3000, 0, 100], [1, 1, 1, 1, 1, 1, 0.999, 0.9], rng.random(8)
+    f = lambda a: _t(np.asarray(a, np.float32))  # noqa: E731
+    tok, pr = torch.zeros(8, dtype=torch.int32, device="cuda"), torch.full((8, V), 7.0, device="cuda")
+    ctx.sample(_t(x), f(u), tok, temperature=f(t), top_k=_i(k), top_p=f(p), min_p=f(m), probs=pr)
+    for r in range(8):
+        tok_r, wp, off = _small_min_p_row(x[r], u[r], t[r], k[r], p[r], m[r])
+        g = _np(pr)[r].astype(np.float64)
+        assert int(tok[r]) == tok_r
+        assert (g[wp == 0] == 0).all() and (np.abs(g - wp) <= (T.U32 + 2 * off) * wp + 1e-45).all()
+
+
+def _small_min_p_row(x, *a):
+    """(token, p, the sums' error), the answers being certain."""
+    u, t, k, p, m = [float(np.float32(v)) for v in a]
+    off = len(x) * 2.0 ** -46 + 2.0 ** -48
+    w = np.exp((x.astype(np.float64) - x.max()) / t)
+    assert (np.abs(w - m) > 2.0 ** -44 * m).all()
+    tok, wp, _ = BT.sample(x, u, t, int(k), p, m)
+    assert BT.sample(x, u, t, int(k), p, 0.0)[2] > 2 * off or p == 1.0
+    assert np.abs(np.cumsum(wp)[wp > 0] - u).min() > 2 * off
+    return tok, wp, off
+
+
+@pytest.mark.parametrize("V", [20000, 131072])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_sample_masked_and_flat_rows(ctx, V, dtype):
+    """Rows masked to fewer tokens than top-k, by -inf, the type's lowest value and NaN; rows without spikes, whose thresholds lie
+    among thousands of entries."""
+    import torch
+    rng = np.random.default_rng(V)
+    x = np.full((6, V), -np.inf, np.float32)
+    x[1] = float(torch.finfo(_dt(dtype)).min)
+    x[2] = np.nan
+    for r in range(3):
+        x[r, rng.choice(V, 20, replace=False)] = rng.standard_normal(20)
+    x[3:] = rng.standard_normal((3, V))
+    x[4] *= 2.5
+    u = rng.random(6)
+    for k, p, m, t in ((50, 1.0, 0.0, 1.0), (50, 0.9, 0.01, 0.8), (0, 0.9, 0.0, 1.0), (21, 0.5, 0.0, 2.0)):
+        _sample_check(ctx, x, u, dtype, [t] * 6, [k] * 6, [p] * 6, [m] * 6)
