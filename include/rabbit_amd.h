@@ -526,8 +526,10 @@ int rbt_kv_dequant_d(rbt_ctx *ctx, const rbt_kv_quant_desc *desc, size_t n_seq, 
  *  - n_prefix 0: prefix, prefix_len and prefix_first are not used.
  *  - Queries and gates of padding nodes may be read here, and change no other node's output.
  * Everything else as rbt_gqa_tree_d; entries 16-byte aligned, scales 4-byte. Over 8-bit rows q and the
- * probabilities are taken to 2^-22 of their row's largest (of 32 or 128 keys at a time), products and
- * their sums are exact in whole numbers, and sums over all keys f32. n_prefix <= 1024 and
+ * probabilities (times their value's scale) are taken to 2^-22 of their row's largest (of 32 or 128 keys at a time), products
+ * and their sums are exact in whole numbers, and sums over all keys f32: entries far below their row's largest keep
+ * fewer bits, where f32 and bf16 rows keep 24 of each. That holds for scales from 2^-60 to 2^60 (and NaN); past them scores and
+ * sums may pass f32, or lose bits. n_prefix <= 1024 and
  * n_seq * max_nodes * (query heads per KV head) <= 2^20 (RBT_E_UNSUPPORTED). A row with scale NaN
  * makes every entry NaN of the nodes that see it, and of no other. Scales are as rbt_kv_quant_d writes them, not
  * negative. */
@@ -549,8 +551,9 @@ int rbt_gqa_prefix_d(rbt_ctx *ctx, const rbt_gqa_prefix_desc *desc, size_t n_seq
  * lower index. Of these are kept: the first top_k (0: all); of what is left, the shortest run from the front whose
  * sum of w reaches top_p of theirs (1: all; at least one); and those with w >= min_p. p_i = w_i / (the sum of
  * what is kept), 0 elsewhere. tokens[r] is the least index whose running sum of p passes u[r]. t = 0 takes the
- * first of the order alone (greedy). w and its sums are exact to 2^-45 of the largest w (vocabularies up to 2^17; one bit less
- * for each doubling).
+ * first of the order alone (greedy). Each w (itself to 2^-48) counts in the sums as the nearest multiple of 2^-45 of the largest
+ * (vocabularies up to 2^17; one bit less for each doubling), so a sum of n of them is off by n 2^-46 at most, and sums do
+ * not depend on their order. An entry below half a multiple counts as 0: it is never drawn, though probs holds its p.
  * logits [n, vocab] of logits_dtype, row_stride entries apart. temperature, top_p, min_p f32 [n] and top_k
  * int32 [n] may be NULL: 1, 1, 0 and 0. u f32 [n] in [0, 1). NaN and -inf entries are never drawn; a row
  * without an entry above -inf, or with +inf, gives token -1 and zeros. So does one whose settings are out of range
