@@ -14,8 +14,13 @@
 //   else 512 buckets of (m - x) / t, with counts and rounded masses, tell the buckets where the thresholds may lie, and
 //     those buckets' entries go to a list.
 //   The list (at most SMP_LIST) is sorted, summed up, and every threshold found in it. Without thresholds there is none.
-//   A row whose list would be longer (thousands of equal logits; a temperature that leaves all mass in one bucket) is
-//     taken digit by digit of `ord`: 120 to 300 us instead of 12 to 40.
+//   A row whose list would be longer is taken digit by digit of `ord`, by one workgroup: seven passes over the row for top-k,
+//     seven for top-p, and the draw's. Such are thousands of equal logits; rows without spikes, where one bucket at top-p's
+//     threshold holds more than the list (normal logits of deviation 1, top-p 0.9, from some 100000 entries on); and rows with
+//     fewer finite logits than top-k, whose parts' largest run out so that all entries are listed. Right, and slow. Measured, one
+//     row, us, with the list and digit by digit: 32000 entries 18 and 290 (masked to 20 tokens, top-k 50) to 760 (equal
+//     logits, top-k 2500 and top-p), 131072 entries 24 to 76 and 1820 to 3620, 248320 26 to 38 and 3400 to 6540, 2^20 40 and
+//     14200 to 27000; 64 rows of 131072 38 to 128 and 4480 to 9700.
 //
 //   k_sample_one   rows of up to 32768 entries, and any rows where there are enough for the chip: a workgroup of 16 waves
 //                  per row does all of it, and the probabilities, in one launch.
@@ -1049,7 +1054,7 @@ __global__ __launch_bounds__(SMP_NT) void k_sample_probs(SampleArgs a, SmpWork k
   smp_probs<NT>(a, r, gr, lo, hi, thr, total, tab);
 }
 
-// Chunks of a row (1: a workgroup per row): some 1024 workgroups in all, of at least 4096 entries each.
+// Chunks of a row (1: a workgroup per row): some 1024 workgroups in all, of 4096 entries or a little less at the least.
 static int smp_chunks(const Ctx &c, long rows, int V) {
   if (V <= 32 * SMP_ONE || rows >= c.num_cu) return 1;
   return (int)std::max(2L, std::min({(long)SMP_GMAX, (V + 4095L) / 4096, 4L * c.num_cu / rows}));

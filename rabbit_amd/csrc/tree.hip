@@ -24,9 +24,12 @@
 //     trip to memory each; five nodes over 4096 f32 rows: 32 us.
 //   64 users, 512 own bf16 rows each, behind 8192 shared: 119-126 us (the products of three bf16 parts at the rate of a large
 //     library product 94); 8 with 300 own behind 1500: 27 us.
-//   32 users, 1000 own int8 rows each, behind 32749 shared: 166-172 us, 121-128 in the pass over the prefix (its int8 products
-//     at the rate of a large library product 118: vector work 66% of the cycles, matrix cores 43%, one after the other);
-//     16 with up to 8192 own rows: 78 us (bytes at a large copy's rate 45).
+//   32 users, 1000 own int8 rows each, behind 32749 shared: 157-172 us, in the pass over the prefix 117-128 by events around
+//     the launch and 133-137 under a profiler (its int8 products at the rate of a large library product 118; vector
+//     instructions issue in 60% of the busy cycles, the matrix cores work in 37%, mostly one after the other);
+//     16 with up to 8192 own rows: 73-78 us (bytes at a large copy's rate 45), k_tree 63-69: CUs are busy for 65% of the
+//     launch (pieces of one length, sequences of unequal ones), their waves wait 58% of the time (two of four compute).
+//   One chunk of 256 nodes behind 8192 rows: 364 us bf16, 296 int8 (419 GFLOP or GOP: 371 and 237 at a library product's rate).
 #include "rbt_device.h"
 #include "rbt_internal.h"
 
